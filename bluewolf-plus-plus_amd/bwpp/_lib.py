@@ -96,6 +96,36 @@ class ElementwiseParams(Structure):
                 ("op", c_uint32), ("bmode", c_uint32)]
 
 
+class RotaryLayout(enum.IntEnum):
+    HALF = 0
+    INTERLEAVED = 1
+
+
+class RotaryScaling(enum.IntEnum):
+    NONE = 0
+    LINEAR = 1
+    BY_PARTS = 2
+
+
+class RotaryParams(Structure):
+    _fields_ = [("tokens", c_uint32), ("q_heads", c_uint32), ("k_heads", c_uint32), ("dim", c_uint32),
+                ("batch", c_uint32), ("rot_dim", c_uint32), ("layout", c_uint32), ("dtype", c_uint32),
+                ("ldq", c_uint32), ("ldk", c_uint32), ("ldqo", c_uint32), ("ldko", c_uint32),
+                ("q_batch_stride", c_uint64), ("q_head_stride", c_uint64),
+                ("k_batch_stride", c_uint64), ("k_head_stride", c_uint64),
+                ("qo_batch_stride", c_uint64), ("qo_head_stride", c_uint64),
+                ("ko_batch_stride", c_uint64), ("ko_head_stride", c_uint64),
+                ("pos_batch_stride", c_uint64), ("pos_offset", c_int32), ("scaling", c_uint32),
+                ("base", c_float), ("factor", c_float), ("low_turns", c_float), ("high_turns", c_float),
+                ("context", c_uint32), ("magnitude", c_float)]
+
+
+class ResidualNormParams(Structure):
+    _fields_ = [("rows", c_uint32), ("cols", c_uint32), ("ldx", c_uint32), ("ldo", c_uint32),
+                ("ldy", c_uint32), ("ldg", c_uint32), ("post_norm", c_uint32), ("gate_rows", c_uint32),
+                ("eps", c_float), ("stream_scale", c_float), ("branch_scale", c_float), ("dtype", c_uint32)]
+
+
 class Arena(Structure):
     _fields_ = [("buffer", c_void_p), ("capacity", c_size_t),
                 ("offset", c_size_t), ("device", c_int)]
@@ -186,6 +216,10 @@ SIGNATURES = {
     "bwpp_hip_dispatch_mean_square": (c_int, [_P, _P, _P, _P, _P, _P, MeanSquareParams]),
     "bwpp_hip_dispatch_reduce_sum": (c_int, [_P, _P, _P, ReduceParams]),
     "bwpp_hip_dispatch_elementwise": (c_int, [_P, _P, _P, _P, ElementwiseParams]),
+    "bwpp_hip_dispatch_rotary": (c_int, [_P] * 6 + [RotaryParams]),
+    "bwpp_hip_dispatch_rotary_grad": (c_int, [_P] * 6 + [RotaryParams]),
+    "bwpp_hip_dispatch_residual_norm": (c_int, [_P] * 8 + [ResidualNormParams]),
+    "bwpp_hip_dispatch_residual_norm_grad": (c_int, [_P] * 13 + [ResidualNormParams]),
     "bwpp_synth_uniform_f32": (None, [_P, c_uint64, c_uint64, c_uint64, c_float, c_float]),
     "bwpp_synth_normal_f32": (None, [_P, c_uint64, c_uint64, c_uint64, c_float, c_float]),
     "bwpp_synth_ramp_f32": (None, [_P, c_uint32, c_uint32, c_float]),
@@ -229,6 +263,7 @@ def load():
 
 __all__ = ["Status", "DType", "Epilogue", "MatmulParams", "Fusion", "FusionParams", "SoftmaxParams",
            "RmsnormParams", "MeanSquareParams", "AttentionParams", "ReduceParams", "ElementwiseParams", "Arena",
+           "RotaryLayout", "RotaryScaling", "RotaryParams", "ResidualNormParams",
            "CoreDType", "Tensor",
            "SIGNATURES", "load", "LIB_PATH", "LIB_DIR", "HEADER_PATH",
            "LibraryMissing", "byref", "c_void_p", "c_uint16"]

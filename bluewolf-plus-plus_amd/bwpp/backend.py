@@ -189,6 +189,28 @@ class HipBackend:
     def dispatch_reduce_sum(self, x, out, params: ReduceParams):
         self._check(self.lib.bwpp_hip_dispatch_reduce_sum(self._h, _ptr(x), _ptr(out), params))
 
+    # ------------------------------------------- around the block, losses
+    def dispatch_rotary(self, q, k, positions, qo, ko, params):
+        """qo, ko = q, k with rotary positions (in place: qo is q, ko is k)."""
+        self._check(self.lib.bwpp_hip_dispatch_rotary(
+            self._h, _ptr(q), _ptr(k), _ptr(positions), _ptr(qo), _ptr(ko), params))
+
+    def dispatch_rotary_grad(self, dqo, dko, positions, dq, dk, params):
+        """dq, dk from the gradients of qo, ko (q's strides and qo's, as in the forward)."""
+        self._check(self.lib.bwpp_hip_dispatch_rotary_grad(
+            self._h, _ptr(dqo), _ptr(dko), _ptr(positions), _ptr(dq), _ptr(dk), params))
+
+    def dispatch_residual_norm(self, x, o, post_gamma, gate, pre_gamma, r, y, params):
+        """r = stream_scale x + branch_scale gate post_norm(o), y = pre_norm(r)."""
+        self._check(self.lib.bwpp_hip_dispatch_residual_norm(
+            self._h, _ptr(x), _ptr(o), _ptr(post_gamma), _ptr(gate), _ptr(pre_gamma), _ptr(r), _ptr(y), params))
+
+    def dispatch_residual_norm_grad(self, o, r, post_gamma, gate, pre_gamma, dr, dy, dx, dout, dpost_gamma, dgate,
+                                    dpre_gamma, params):
+        self._check(self.lib.bwpp_hip_dispatch_residual_norm_grad(
+            self._h, _ptr(o), _ptr(r), _ptr(post_gamma), _ptr(gate), _ptr(pre_gamma), _ptr(dr), _ptr(dy), _ptr(dx),
+            _ptr(dout), _ptr(dpost_gamma), _ptr(dgate), _ptr(dpre_gamma), params))
+
     # ------------------------------------------------------ tensor forms
     def tensor_matmul(self, a, b, bias, c, epilogue: int = 0):
         ref = lambda t: ctypes.byref(t) if t is not None else None

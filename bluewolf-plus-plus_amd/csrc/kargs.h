@@ -150,4 +150,51 @@ typedef struct {
   uint32_t vec; /* 1: every segment has 16-byte rows (cols, strides, pointers) */
 } BwppCopyArgs;
 
+/* Rotary positions (rotary.hip): rows of `dim` elements, one per (batch,
+ * token, head), q's heads before k's. */
+typedef struct {
+  const void *q;
+  const void *k;
+  void *qo;
+  void *ko;
+  const int32_t *positions; /* [batch][pos_bs], or NULL: pos0 + token */
+  uint64_t q_ts, q_hs, q_bs, k_ts, k_hs, k_bs;       /* token / head / batch strides (elements) */
+  uint64_t qo_ts, qo_hs, qo_bs, ko_ts, ko_hs, ko_bs;
+  uint64_t pos_bs;
+  double log2_step; /* log2 of the ratio of two successive frequencies */
+  double inv_factor;
+  double turns;     /* context / (2 pi): turns of a frequency of 1 over the context */
+  double low, inv_range; /* by parts: share kept = (turns f - low) inv_range in [0, 1] */
+  float cos_scale, sin_scale; /* magnitude; the sine's sign is the direction */
+  int32_t pos0;
+  uint32_t tokens, batch;
+  uint32_t q_heads, heads; /* heads = q's and k's */
+  uint32_t dim, pairs;     /* pairs = rot_dim / 2 */
+  uint32_t scaling;        /* BWPP_HIP_ROTARY_SCALE_* */
+  uint32_t tile;           /* tokens per block */
+  uint32_t hgroup;         /* heads per block (grid y), at most 256 */
+  uint32_t copy;           /* bit 0: copy q's columns past 2 pairs, bit 1: k's */
+  uint32_t tail_chunks;    /* chunks of those columns */
+} BwppRotaryArgs;
+
+/* The join of a branch with the residual stream and its gradient
+ * (resnorm.hip). */
+typedef struct {
+  const void *x, *o, *r;            /* stream in, branch, stream out (gradient: in) */
+  const void *post, *gate, *pre;    /* weights, NULL = 1 */
+  void *ro, *y;                     /* forward outputs */
+  const void *dr, *dy;              /* upstream gradients, either NULL = 0 */
+  void *dx, *dout, *dpost, *dgate, *dpre;
+  float *part_pre, *part_post, *part_gate; /* [workers][cols] sums (NULL: not asked for) */
+  uint64_t ldx, ldo, ldy, ldg;
+  uint32_t rows, cols;
+  uint32_t gate_rows; /* rows per gate row (0: one gate row) */
+  uint32_t post_norm;
+  float eps, stream_scale, branch_scale;
+  /* gradient: workers (blocks, or waves of blocks that hold a row each) take
+   * `span` rows of a group of `group` rows (split > 1 workers a group, whose
+   * gate sums go to part_gate), or whole groups of them (split = 1) */
+  uint32_t workers, group, split, span;
+} BwppResNormArgs;
+
 #endif /* BWPP_KARGS_H */

@@ -33,7 +33,8 @@ thread_local std::string g_create_error;
 
 // Code objects built by the package Makefile, all required.
 const char *const kModules[] = {"bwpp_rowops.hsaco", "bwpp_gemm.hsaco", "bwpp_attention.hsaco",
-                                 "bwpp_attention_f32.hsaco", "bwpp_attention_bwd.hsaco", "bwpp_grad.hsaco"};
+                                 "bwpp_attention_f32.hsaco", "bwpp_attention_bwd.hsaco", "bwpp_grad.hsaco",
+                                 "bwpp_rotary.hsaco", "bwpp_resnorm.hsaco"};
 
 // Row-op kernels: bwpp_row_<op>_v<VPT>_w<WPR>_<f|p>, see rowops.hip.
 enum RowOpId { ROW_SOFTMAX, ROW_RMSNORM, ROW_LAYERNORM, ROW_MAX, ROW_MAXGRAD, ROW_MASK, ROW_NOPS };
@@ -141,6 +142,7 @@ struct BwppHip {
   hipFunction_t silu_grad = nullptr, softmax_grad = nullptr, rmsnorm_grad = nullptr, col_partials_sum = nullptr,
                 reduce_sum_rows = nullptr, reduce_sum_cols = nullptr, elementwise = nullptr,
                 mean_square_part = nullptr, mean_square_final = nullptr, copy_multi = nullptr;
+  std::vector<hipFunction_t> lm;  // bwpp_hip_lm_kernels
   // Library-owned device workspace (column partials), grown on demand and
   // freed by bwpp_hip_destroy.  Calls on one handle are stream-ordered, so
   // reuse across calls is safe.
@@ -329,6 +331,9 @@ BwppHipStatus resolve_all(BwppHip *h) {
   };
   for (auto &e : singles)
     if ((s = resolve(h, e.name, e.slot)) != BWPP_HIP_OK) return s;
+  h->lm.resize((size_t)bwpp_hip_lm_kernel_count);
+  for (int i = 0; i < bwpp_hip_lm_kernel_count; ++i)
+    if ((s = resolve(h, bwpp_hip_lm_kernels[i], &h->lm[(size_t)i])) != BWPP_HIP_OK) return s;
   for (int c = 0; c < kGradNCfg; ++c)
     for (int vec = 0; vec < 2; ++vec) {
       const std::string n = "_v" + std::to_string(kGradCfgs[c].vpt) + "_w" + std::to_string(kGradCfgs[c].wpr) +
@@ -478,9 +483,8 @@ BwppHipStatus enter(BwppHip *h) {
 
 inline bool launchable(uint64_t blocks, uint32_t threads) { return blocks * threads <= 0xffffffffull; }
 
-template <class Args>
-BwppHipStatus launch(BwppHip *h, hipFunction_t f, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bx,
-                     const Args &args, uint32_t shmem = 0) {
+BwppHipStatus launch_block(BwppHip *h, hipFunction_t f, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bx,
+                           const void *args, uint32_t shmem) {
   if (gx == 0 || gy == 0 || gz == 0) return BWPP_HIP_OK;
   // Threads along x are counted in 32 bits: beyond that a launch runs a part
   // of its grid and reports success.
@@ -490,7 +494,7 @@ BwppHipStatus launch(BwppHip *h, hipFunction_t f, uint32_t gx, uint32_t gy, uint
   if (mt == h->max_threads.end() || bx > mt->second)
     return fail(h, BWPP_HIP_ERR_HIP, "launch of %u threads per block exceeds the kernel's limit (%u)", bx,
                 mt == h->max_threads.end() ? 0u : mt->second);
-  void *params[] = {const_cast<Args *>(&args)};
+  void *params[] = {const_cast<void *>(args)};
   hipError_t e = hipModuleLaunchKernel(f, gx, gy, gz, bx, 1, 1, shmem, h->stream, params, nullptr);
   if (e != hipSuccess) return fail(h, BWPP_HIP_ERR_HIP, "hipModuleLaunchKernel: %s", hipGetErrorString(e));
   const auto nm = h->names.find(f);
@@ -498,6 +502,12 @@ BwppHipStatus launch(BwppHip *h, hipFunction_t f, uint32_t gx, uint32_t gy, uint
   for (int i = 3; i > 0; --i) h->recent[i] = h->recent[i - 1];
   h->recent[0] = h->last_kernel;
   return BWPP_HIP_OK;
+}
+
+template <class Args>
+BwppHipStatus launch(BwppHip *h, hipFunction_t f, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bx,
+                     const Args &args, uint32_t shmem = 0) {
+  return launch_block(h, f, gx, gy, gz, bx, &args, shmem);
 }
 
 inline uint32_t eff_ld(uint32_t ld, uint32_t cols) { return ld ? ld : cols; }
@@ -2189,4 +2199,34 @@ BwppHipStatus bwpp_hip_copy_strided_multi(BwppHip *h, uint32_t n, const float *c
   a.row0[n] = (uint32_t)total;
   if (total == 0) return BWPP_HIP_OK;
   return launch(h, h->copy_multi, row_grid(h, (uint32_t)total), 1, 1, 256, a);
+}
+
+// ------------------------------------------- shared with bwpp_lm.cpp
+
+BwppHipStatus bwpp_hip_enter(BwppHip *h) {
+  if (!h) return fail(nullptr, BWPP_HIP_ERR_INVALID_ARG, "NULL handle");
+  return enter(h);
+}
+
+BwppHipStatus bwpp_hip_launch_lm(BwppHip *h, int index, uint64_t gx, uint32_t gy, uint32_t threads, const void *args,
+                                 uint32_t shmem) {
+  if (!launchable(gx, threads))
+    return fail(h, BWPP_HIP_ERR_UNSUPPORTED, "launch of %llu blocks of %u threads: 2^32 threads or more",
+                (unsigned long long)gx, threads);
+  return launch_block(h, h->lm[(size_t)index], (uint32_t)gx, gy, 1, threads, args, shmem);
+}
+
+BwppHipStatus bwpp_hip_take_workspace(BwppHip *h, size_t bytes, void **p) {
+  if (!ws_ready(h, bytes))
+    return fail(h, BWPP_HIP_ERR_OUT_OF_MEMORY,
+                "the workspace (%zu bytes, %zu needed) cannot grow while the stream is recorded: run the call once before",
+                h->ws_bytes, bytes);
+  const BwppHipStatus s = ensure_ws(h, bytes);
+  *p = s == BWPP_HIP_OK ? h->ws : nullptr;
+  return s;
+}
+
+bool bwpp_hip_blocks_overlap(const void *pa, uint64_t ra, uint64_t ca, uint64_t lda, const void *pb, uint64_t rb,
+                             uint64_t cb, uint64_t ldb, uint64_t es) {
+  return blocks_overlap(pa, ra, ca, lda, pb, rb, cb, ldb, es);
 }

@@ -1,0 +1,375 @@
+// Operators of libbwpp_hip around a transformer block: rotary positions and
+// the residual join with its norms, forward and gradient.  Argument checks,
+// launch geometry and the choice of a kernel; the kernels are rotary.hip and
+// resnorm.hip.
+#include "bwpp_hip.h"
+#include "internal.h"
+
+#include <algorithm>
+#include <cmath>
+
+#include "../kargs.h"
+
+namespace {
+
+enum LmKernel {
+  LM_ROTARY_BF16,                      // [interleaved][chunk 8, 4, 1]
+  LM_ROTARY_F32 = LM_ROTARY_BF16 + 6,  // [interleaved][chunk 4, 1]
+  LM_RESNORM = LM_ROTARY_F32 + 4,      // [bf16][kResCfgs, any]
+  LM_RESNORM_GRAD = LM_RESNORM + 14,   // [bf16][kResCfgs - 1, any]
+  LM_RESNORM_FINISH = LM_RESNORM_GRAD + 12,  // [bf16]
+  LM_COUNT = LM_RESNORM_FINISH + 2
+};
+
+// Rows in registers (resnorm.hip): elements a thread and waves a row.
+struct ResCfg {
+  uint32_t elems, waves;
+};
+constexpr int kResNCfg = 6, kResGradNCfg = 5;
+const ResCfg kResCfgs[kResNCfg] = {{8, 1}, {8, 2}, {8, 4}, {8, 8}, {8, 16}, {16, 16}};
+constexpr uint32_t kResAnyThreads = 512;
+
+}  // namespace
+
+const char *const bwpp_hip_lm_kernels[] = {
+    "bwpp_rotary_bf16_half_8",      "bwpp_rotary_bf16_half_4",      "bwpp_rotary_bf16_half_1",
+    "bwpp_rotary_bf16_inter_8",     "bwpp_rotary_bf16_inter_4",     "bwpp_rotary_bf16_inter_1",
+    "bwpp_rotary_f32_half_4",       "bwpp_rotary_f32_half_1",       "bwpp_rotary_f32_inter_4",
+    "bwpp_rotary_f32_inter_1",      "bwpp_resnorm_f32_n8_w1",       "bwpp_resnorm_f32_n8_w2",
+    "bwpp_resnorm_f32_n8_w4",       "bwpp_resnorm_f32_n8_w8",       "bwpp_resnorm_f32_n8_w16",
+    "bwpp_resnorm_f32_n16_w16",     "bwpp_resnorm_f32_any",         "bwpp_resnorm_bf16_n8_w1",
+    "bwpp_resnorm_bf16_n8_w2",      "bwpp_resnorm_bf16_n8_w4",      "bwpp_resnorm_bf16_n8_w8",
+    "bwpp_resnorm_bf16_n8_w16",     "bwpp_resnorm_bf16_n16_w16",    "bwpp_resnorm_bf16_any",
+    "bwpp_resnorm_grad_f32_n8_w1",  "bwpp_resnorm_grad_f32_n8_w2",  "bwpp_resnorm_grad_f32_n8_w4",
+    "bwpp_resnorm_grad_f32_n8_w8",  "bwpp_resnorm_grad_f32_n8_w16", "bwpp_resnorm_grad_f32_any",
+    "bwpp_resnorm_grad_bf16_n8_w1", "bwpp_resnorm_grad_bf16_n8_w2", "bwpp_resnorm_grad_bf16_n8_w4",
+    "bwpp_resnorm_grad_bf16_n8_w8", "bwpp_resnorm_grad_bf16_n8_w16", "bwpp_resnorm_grad_bf16_any",
+    "bwpp_resnorm_finish_f32",      "bwpp_resnorm_finish_bf16",
+};
+const int bwpp_hip_lm_kernel_count = (int)(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]));
+static_assert(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]) == LM_COUNT, "kernel names");
+
+namespace {
+
+uint32_t cus_of(const BwppHip *h) {
+  const int n = bwpp_hip_device_cus(h);
+  return n > 0 ? (uint32_t)n : 256u;
+}
+
+// ---------------------------------------------------------------- rotary
+
+// Rows of one operand of a rotary call: [batch][heads][tokens] rows of dim.
+struct RowSet {
+  const void *p;
+  uint64_t ts, hs, bs;
+  uint64_t batch, heads, tokens, dim;
+
+  // The set as one row-strided block, where its rows are column blocks of
+  // token rows (heads within a token's stride, batches stacked).
+  bool as_block(uint64_t &rows, uint64_t &cols) const {
+    cols = (heads - 1) * hs + dim;
+    if (cols > ts || (batch > 1 && (ts == 0 || bs % ts != 0))) return false;
+    rows = (batch > 1 ? (batch - 1) * (bs / ts) : 0) + tokens;
+    return true;
+  }
+  uint64_t span() const { return (batch - 1) * bs + (heads - 1) * hs + (tokens - 1) * ts + dim; }
+};
+
+// Whether two sets share an element (by byte range, unless both are blocks
+// of one row stride).
+bool meet(const RowSet &a, const RowSet &b, uint64_t es) {
+  if (!a.p || !b.p) return false;
+  uint64_t ra, ca, rb, cb;
+  if (a.ts == b.ts && a.as_block(ra, ca) && b.as_block(rb, cb))
+    return bwpp_hip_blocks_overlap(a.p, ra, ca, a.ts, b.p, rb, cb, b.ts, es);
+  return bwpp_hip_blocks_overlap(a.p, 1, a.span(), 0, b.p, 1, b.span(), 0, es);
+}
+bool same_rows(const RowSet &a, const RowSet &b) {
+  return a.p == b.p && (a.tokens == 1 || a.ts == b.ts) && (a.heads == 1 || a.hs == b.hs) &&
+         (a.batch == 1 || a.bs == b.bs);
+}
+// Whether the rows of an output are disjoint: every stride passes what lies
+// inside it, in some order of the three.
+bool disjoint_rows(const RowSet &s) {
+  struct Axis {
+    uint64_t n, st;
+  } ax[3] = {{s.tokens, s.ts}, {s.heads, s.hs}, {s.batch, s.bs}};
+  std::sort(ax, ax + 3, [](const Axis &a, const Axis &b) { return a.st < b.st; });
+  uint64_t inside = s.dim;
+  for (const Axis &a : ax) {
+    if (a.n == 1) continue;
+    if (a.st < inside) return false;
+    inside += (a.n - 1) * a.st;
+  }
+  return true;
+}
+
+BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k, const int32_t *positions, void *qo,
+                     void *ko, const BwppRotaryParams &p, bool grad) {
+  auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
+  if (p.dtype > BWPP_HIP_BF16) return bad("unknown dtype");
+  if (p.layout > BWPP_HIP_ROTARY_INTERLEAVED) return bad("unknown layout");
+  if (p.scaling > BWPP_HIP_ROTARY_SCALE_BY_PARTS) return bad("unknown scaling");
+  if ((p.q_heads && (!q || !qo)) || (p.k_heads && (!k || !ko))) return bad("NULL q, k or output");
+  const uint32_t rot = p.rot_dim ? p.rot_dim : p.dim;
+  if (rot % 2 || rot > p.dim) return bad("rot_dim must be even and at most dim");
+  const double base = p.base != 0.0f ? p.base : 10000.0, factor = p.factor != 0.0f ? p.factor : 1.0;
+  if (!(base > 0.0) || !(factor > 0.0) || !std::isfinite(base) || !std::isfinite(factor) ||
+      !std::isfinite(p.magnitude))
+    return bad("base and factor must be positive and finite, magnitude finite");
+  if (p.scaling == BWPP_HIP_ROTARY_SCALE_BY_PARTS &&
+      (p.context == 0 || !(p.high_turns > p.low_turns) || !std::isfinite(p.low_turns) || !std::isfinite(p.high_turns)))
+    return bad("scaling by parts needs a context and low_turns < high_turns");
+  const uint64_t B = p.batch ? p.batch : 1, T = p.tokens, d = p.dim;
+  if (p.tokens == 0 || p.dim == 0 || (p.q_heads == 0 && p.k_heads == 0)) return bwpp_hip_enter(h);
+  const uint64_t heads = (uint64_t)p.q_heads + p.k_heads;
+  if (rot > 4096 || heads > (1u << 24) || T > (1u << 31))
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: rot_dim above 4096, or heads or tokens out of range", what);
+  auto rows = [&](const void *ptr, uint32_t heads, uint32_t ld, uint64_t hs, uint64_t bs) {
+    RowSet r = {heads ? ptr : nullptr, ld ? ld : d, 0, 0, B, heads ? heads : 1u, T, d};
+    r.hs = hs ? hs : T * r.ts;
+    r.bs = bs ? bs : r.heads * r.hs;
+    return r;
+  };
+  // The gradient reads with the outputs' strides and writes with the inputs'.
+  RowSet sq = rows(nullptr, p.q_heads, p.ldq, p.q_head_stride, p.q_batch_stride);
+  RowSet sk = rows(nullptr, p.k_heads, p.ldk, p.k_head_stride, p.k_batch_stride);
+  RowSet dq = rows(nullptr, p.q_heads, p.ldqo, p.qo_head_stride, p.qo_batch_stride);
+  RowSet dk = rows(nullptr, p.k_heads, p.ldko, p.ko_head_stride, p.ko_batch_stride);
+  if (grad) {
+    std::swap(sq, dq);
+    std::swap(sk, dk);
+  }
+  sq.p = p.q_heads ? q : nullptr;
+  sk.p = p.k_heads ? k : nullptr;
+  dq.p = p.q_heads ? qo : nullptr;
+  dk.p = p.k_heads ? ko : nullptr;
+  for (const RowSet *r : {&sq, &sk, &dq, &dk})
+    if (r->p && T > 1 && r->ts < d) return bad("token stride smaller than the row");
+  for (const RowSet *r : {&dq, &dk})
+    if (r->p && !disjoint_rows(*r)) return bad("rows of an output overlap");
+  const uint64_t es = p.dtype == BWPP_HIP_BF16 ? 2 : 4;
+  const bool q_in_place = sq.p && same_rows(sq, dq), k_in_place = sk.p && same_rows(sk, dk);
+  if ((!q_in_place && meet(dq, sq, es)) || meet(dq, sk, es) || (!k_in_place && meet(dk, sk, es)) ||
+      meet(dk, sq, es) || meet(dq, dk, es))
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: an output overlaps an input or the other output", what);
+  const BwppHipStatus s = bwpp_hip_enter(h);
+  if (s != BWPP_HIP_OK) return s;
+
+  BwppRotaryArgs a = {};
+  a.q = sq.p;
+  a.k = sk.p;
+  a.qo = const_cast<void *>(dq.p);
+  a.ko = const_cast<void *>(dk.p);
+  a.positions = positions;
+  a.q_ts = sq.ts, a.q_hs = sq.hs, a.q_bs = sq.bs;
+  a.k_ts = sk.ts, a.k_hs = sk.hs, a.k_bs = sk.bs;
+  a.qo_ts = dq.ts, a.qo_hs = dq.hs, a.qo_bs = dq.bs;
+  a.ko_ts = dk.ts, a.ko_hs = dk.hs, a.ko_bs = dk.bs;
+  a.pos_bs = p.pos_batch_stride;
+  a.log2_step = rot ? -2.0 / rot * std::log2(base) : 0.0;
+  a.inv_factor = 1.0 / factor;
+  a.turns = p.context * 0.15915494309189533577;  // 1 / (2 pi)
+  a.low = p.low_turns;
+  a.inv_range = p.scaling == BWPP_HIP_ROTARY_SCALE_BY_PARTS ? 1.0 / ((double)p.high_turns - (double)p.low_turns) : 0.0;
+  a.cos_scale = p.magnitude != 0.0f ? p.magnitude : 1.0f;
+  a.sin_scale = grad ? -a.cos_scale : a.cos_scale;
+  a.pos0 = p.pos_offset;
+  a.tokens = p.tokens;
+  a.batch = (uint32_t)B;
+  a.q_heads = p.q_heads;
+  a.dim = p.dim;
+  a.pairs = rot / 2;
+  a.scaling = p.scaling;
+  a.copy = rot < p.dim ? (sq.p && !q_in_place ? 1u : 0u) | (sk.p && !k_in_place ? 2u : 0u) : 0u;
+  a.heads = (uint32_t)heads;
+  const bool bf16 = p.dtype == BWPP_HIP_BF16, inter = p.layout == BWPP_HIP_ROTARY_INTERLEAVED;
+  const uint32_t pick = bf16 ? (a.pairs % 8 == 0 ? 0u : a.pairs % 4 == 0 ? 1u : 2u) : (a.pairs % 4 == 0 ? 0u : 1u);
+  const uint32_t chunk = bf16 ? (pick == 0 ? 8u : pick == 1 ? 4u : 1u) : (pick == 0 ? 4u : 1u);
+  a.tail_chunks = a.copy ? (p.dim - rot + chunk - 1) / chunk : 0u;
+  if (a.pairs == 0 && a.tail_chunks == 0) return BWPP_HIP_OK;
+  // Tiles of tokens as wide as the angles' LDS allows while eight blocks a CU
+  // remain; where there are few tokens the heads are split over blocks too.
+  const uint64_t want = 8ull * cus_of(h);
+  const uint32_t most = std::max(1u, 2048u / std::max(1u, a.pairs));
+  a.tile = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(most, T), std::max<uint64_t>(1, B * T / want));
+  a.hgroup = std::min(a.heads, 256u);
+  const uint64_t blocks = B * ((T + a.tile - 1) / a.tile);
+  while (a.hgroup > 8 && blocks * ((a.heads + a.hgroup - 1) / a.hgroup) * 2 <= want) a.hgroup = (a.hgroup + 1) / 2;
+  const uint32_t groups = (a.heads + a.hgroup - 1) / a.hgroup;
+  if (groups > 65535) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: too many heads", what);
+  const int index = bf16 ? LM_ROTARY_BF16 + (inter ? 3 : 0) + (int)pick : LM_ROTARY_F32 + (inter ? 2 : 0) + (int)pick;
+  return bwpp_hip_launch_lm(h, index, blocks, groups, 256, &a);
+}
+
+// --------------------------------------------------------- residual norm
+
+// Checks and the arguments both directions share.
+BwppHipStatus resnorm_prepare(BwppHip *h, const char *what, const BwppResidualNormParams &p, BwppResNormArgs &a) {
+  auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
+  if (p.dtype > BWPP_HIP_BF16) return bad("unknown dtype");
+  a.rows = p.rows;
+  a.cols = p.cols;
+  a.ldx = p.ldx ? p.ldx : p.cols;
+  a.ldo = p.ldo ? p.ldo : p.cols;
+  a.ldy = p.ldy ? p.ldy : p.cols;
+  a.ldg = p.ldg ? p.ldg : p.cols;
+  if (a.ldx < p.cols || a.ldo < p.cols || a.ldy < p.cols || a.ldg < p.cols)
+    return bad("row stride smaller than the row");
+  if (!(p.eps >= 0.0f)) return bad("eps must not be negative");
+  a.post_norm = p.post_norm ? 1u : 0u;
+  a.gate_rows = p.gate_rows;
+  a.eps = p.eps;
+  a.stream_scale = p.stream_scale != 0.0f ? p.stream_scale : 1.0f;
+  a.branch_scale = p.branch_scale != 0.0f ? p.branch_scale : 1.0f;
+  return BWPP_HIP_OK;
+}
+
+// Smallest layout whose threads hold a row, or -1: a block reads it again.
+int res_cfg(uint32_t cols, int n) {
+  for (int i = 0; i < n; ++i)
+    if (64u * kResCfgs[i].elems * kResCfgs[i].waves >= cols) return i;
+  return -1;
+}
+
+struct Block {
+  const void *p;
+  uint64_t rows, cols, ld;
+};
+bool meet(const Block &a, const Block &b, uint64_t es) {
+  if (!a.p || !b.p || a.rows == 0 || b.rows == 0) return false;
+  return bwpp_hip_blocks_overlap(a.p, a.rows, a.cols, a.ld, b.p, b.rows, b.cols, b.ld, es);
+}
+
+}  // namespace
+
+extern "C" BwppHipStatus bwpp_hip_dispatch_rotary(BwppHip *h, const void *q, const void *k, const int32_t *positions,
+                                                  void *qo, void *ko, BwppRotaryParams p) {
+  return rotary(h, "rotary", q, k, positions, qo, ko, p, false);
+}
+
+extern "C" BwppHipStatus bwpp_hip_dispatch_rotary_grad(BwppHip *h, const void *dqo, const void *dko,
+                                                       const int32_t *positions, void *dq, void *dk,
+                                                       BwppRotaryParams p) {
+  return rotary(h, "rotary_grad", dqo, dko, positions, dq, dk, p, true);
+}
+
+extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm(BwppHip *h, const void *x, const void *o,
+                                                         const void *post_gamma, const void *gate,
+                                                         const void *pre_gamma, void *r, void *y,
+                                                         BwppResidualNormParams p) {
+  if (!x || !o || !r) return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "residual_norm: NULL x, o or r");
+  BwppResNormArgs a = {};
+  BwppHipStatus s = resnorm_prepare(h, "residual_norm", p, a);
+  if (s != BWPP_HIP_OK) return s;
+  const uint64_t es = p.dtype == BWPP_HIP_BF16 ? 2 : 4, R = p.rows, C = p.cols;
+  const uint64_t gates = p.gate_rows ? (R + p.gate_rows - 1) / p.gate_rows : 1;
+  const Block bx = {x, R, C, a.ldx}, bo = {o, R, C, a.ldo}, br = {r, R, C, a.ldx}, by = {y, R, C, a.ldy};
+  const Block small[3] = {{p.post_norm ? post_gamma : nullptr, 1, C, C}, {gate, gates, C, a.ldg}, {pre_gamma, 1, C, C}};
+  bool alias = (x != r && meet(br, bx, es)) || meet(br, bo, es) || meet(br, by, es) || meet(by, bx, es) || meet(by, bo, es);
+  for (const Block &b : small) alias = alias || meet(br, b, es) || meet(by, b, es);
+  if (alias) return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "residual_norm: an output overlaps another operand");
+  if ((s = bwpp_hip_enter(h)) != BWPP_HIP_OK || R == 0 || C == 0) return s;
+  a.x = x;
+  a.o = o;
+  a.post = post_gamma;
+  a.gate = gate;
+  a.pre = pre_gamma;
+  a.ro = r;
+  a.y = y;
+  const int c = res_cfg(p.cols, kResNCfg), bf16 = p.dtype == BWPP_HIP_BF16;
+  const uint32_t waves = c >= 0 ? kResCfgs[c].waves : 8u, rpb = waves == 1 ? 4u : 1u;
+  // Blocks that keep the weights in registers over several rows.
+  const uint64_t cap = (uint64_t)cus_of(h) * (waves >= 16 ? 2u : waves >= 8 ? 4u : 8u);
+  const uint64_t blocks = std::min<uint64_t>((R + rpb - 1) / rpb, cap);
+  return bwpp_hip_launch_lm(h, LM_RESNORM + bf16 * (kResNCfg + 1) + (c >= 0 ? c : kResNCfg), blocks, 1,
+                            c < 0 ? kResAnyThreads : waves == 1 ? 256u : 64u * waves, &a);
+}
+
+extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const void *o, const void *r,
+                                                              const void *post_gamma, const void *gate,
+                                                              const void *pre_gamma, const void *dr, const void *dy,
+                                                              void *dx, void *dout, void *dpost_gamma, void *dgate,
+                                                              void *dpre_gamma, BwppResidualNormParams p) {
+  const char *what = "residual_norm_grad";
+  auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
+  if (!o || !r || (!dr && !dy)) return bad("NULL o or r, or neither dr nor dy");
+  if (!dx && !dout && !dpost_gamma && !dgate && !dpre_gamma) return bad("no output");
+  if (dpost_gamma && !p.post_norm) return bad("dpost_gamma without a post-norm");
+  BwppResNormArgs a = {};
+  BwppHipStatus s = resnorm_prepare(h, what, p, a);
+  if (s != BWPP_HIP_OK) return s;
+  const uint64_t es = p.dtype == BWPP_HIP_BF16 ? 2 : 4, R = p.rows, C = p.cols;
+  const uint64_t gates = p.gate_rows ? (R + p.gate_rows - 1) / p.gate_rows : 1;
+  const Block in[7] = {{o, R, C, a.ldo}, {r, R, C, a.ldx}, {dr, R, C, a.ldx}, {dy, R, C, a.ldy},
+                       {p.post_norm ? post_gamma : nullptr, 1, C, C}, {gate, gates, C, a.ldg}, {pre_gamma, 1, C, C}};
+  const Block out[5] = {{dx, R, C, a.ldx}, {dout, R, C, a.ldo}, {dpost_gamma, 1, C, C}, {dgate, gates, C, a.ldg},
+                        {dpre_gamma, 1, C, C}};
+  for (int i = 0; i < 5; ++i) {
+    for (int j = 0; j < 7; ++j)
+      if (!(i == 0 && j == 2 && dx == dr) && meet(out[i], in[j], es))
+        return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: an output overlaps an input", what);
+    for (int j = 0; j < i; ++j)
+      if (meet(out[i], out[j], es))
+        return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: two outputs overlap", what);
+  }
+  if ((s = bwpp_hip_enter(h)) != BWPP_HIP_OK || C == 0) return s;
+  if (R == 0 && p.gate_rows) dgate = nullptr;  // no gate rows
+  if (R == 0 && !dgate && !dpost_gamma && !dpre_gamma) return BWPP_HIP_OK;
+  a.o = o;
+  a.r = r;
+  a.post = post_gamma;
+  a.gate = gate;
+  a.pre = pre_gamma;
+  a.dr = dr;
+  a.dy = dy;
+  a.dx = dx;
+  a.dout = dout;
+  a.dpost = dpost_gamma;
+  a.dgate = dgate;
+  a.dpre = dpre_gamma;
+  const int c = res_cfg(p.cols, kResGradNCfg), bf16 = p.dtype == BWPP_HIP_BF16;
+  const uint32_t waves = c >= 0 ? kResCfgs[c].waves : 8u, rpb = waves == 1 ? 4u : 1u;
+  // Workers: about one block a CU of the longest rows, more of shorter ones;
+  // each leaves a partial row of every weight gradient.  A group is what one
+  // row of dgate sums over; it is split over workers or a worker takes several.
+  const uint64_t target = (uint64_t)cus_of(h) * (waves >= 8 ? 1u : waves >= 2 ? 8u / waves : 8u);
+  const uint64_t group = dgate && p.gate_rows ? std::min<uint64_t>(p.gate_rows, std::max<uint64_t>(R, 1)) : std::max<uint64_t>(R, 1);
+  const uint64_t ngroups = std::max<uint64_t>(1, (R + group - 1) / group);
+  uint64_t split = 1, span;
+  if (ngroups < target) {
+    split = std::min<uint64_t>((target + ngroups - 1) / ngroups, std::max<uint64_t>(1, group));
+    span = (group + split - 1) / split;
+    split = (group + span - 1) / span;
+  }
+  uint64_t workers;
+  if (split > 1) {
+    workers = ngroups * split;
+  } else {
+    const uint64_t per = std::max<uint64_t>(1, (ngroups + target - 1) / target);
+    span = per * group;
+    workers = (ngroups + per - 1) / per;
+  }
+  if (span > 0xffffffffull) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: too many rows", what);
+  a.group = (uint32_t)group;
+  a.split = (uint32_t)split;
+  a.span = (uint32_t)span;
+  a.workers = (uint32_t)workers;
+  const bool gate_part = dgate && (split > 1 || c < 0 || R == 0);
+  const uint64_t nparts = (dpre_gamma ? 1 : 0) + (dpost_gamma ? 1 : 0) + (gate_part ? 1 : 0);
+  if (nparts) {
+    void *ws = nullptr;
+    if ((s = bwpp_hip_take_workspace(h, nparts * workers * C * sizeof(float), &ws)) != BWPP_HIP_OK) return s;
+    float *f = static_cast<float *>(ws);
+    if (dpre_gamma) a.part_pre = f, f += workers * C;
+    if (dpost_gamma) a.part_post = f, f += workers * C;
+    if (gate_part) a.part_gate = f;
+  }
+  s = bwpp_hip_launch_lm(h, LM_RESNORM_GRAD + bf16 * (kResGradNCfg + 1) + (c >= 0 ? c : kResGradNCfg),
+                         (workers + rpb - 1) / rpb, 1, c < 0 ? kResAnyThreads : waves == 1 ? 256u : 64u * waves, &a);
+  if (s != BWPP_HIP_OK || !nparts) return s;
+  const bool gate_sum = gate_part && (split > 1 || R == 0);
+  if (!gate_sum) a.part_gate = nullptr;
+  if (!dpre_gamma && !dpost_gamma && !gate_sum) return BWPP_HIP_OK;
+  return bwpp_hip_launch_lm(h, LM_RESNORM_FINISH + bf16, (C + 63) / 64, gate_sum ? 2u + (uint32_t)ngroups : 2u, 256, &a);
+}

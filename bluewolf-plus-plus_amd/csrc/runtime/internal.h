@@ -55,3 +55,25 @@ BwppHipStatus bwpp_hip_copy_strided(BwppHip *h, const float *src, uint32_t ld_sr
 BwppHipStatus bwpp_hip_copy_strided_multi(BwppHip *h, uint32_t n, const float *const *src, const uint32_t *ld_src,
                                           float *const *dst, const uint32_t *ld_dst, const uint32_t *rows,
                                           const uint32_t *cols);
+
+// ---- shared with bwpp_lm.cpp (the operators around a block and the loss)
+
+// Kernels of bwpp_lm.cpp, by name; the handle resolves them at creation.
+extern const char *const bwpp_hip_lm_kernels[];
+extern const int bwpp_hip_lm_kernel_count;
+
+// Clears the last error and makes the handle's device current.
+BwppHipStatus bwpp_hip_enter(BwppHip *h);
+
+// Launches kernel `index` of bwpp_hip_lm_kernels with one argument block.
+BwppHipStatus bwpp_hip_launch_lm(BwppHip *h, int index, uint64_t gx, uint32_t gy, uint32_t threads, const void *args,
+                                 uint32_t shmem = 0);
+
+// `bytes` of the handle's workspace (OUT_OF_MEMORY while the handle's stream
+// is being recorded and the workspace would have to grow).
+BwppHipStatus bwpp_hip_take_workspace(BwppHip *h, size_t bytes, void **p);
+
+// Whether two row-strided blocks of es-byte elements share an element: exact
+// when their row strides are equal, by byte range otherwise.
+bool bwpp_hip_blocks_overlap(const void *pa, uint64_t ra, uint64_t ca, uint64_t lda, const void *pb, uint64_t rb,
+                             uint64_t cb, uint64_t ldb, uint64_t es);

@@ -164,6 +164,69 @@ typedef struct {
   uint32_t bmode; /* BwppHipBroadcast */
 } BwppElementwiseParams;
 
+/* Rotary positions of one attention call's q and k (no reference
+ * counterpart; strides named as BwppAttentionParams names them, the outputs'
+ * with an o).  Row (b, t, h) of q is at b * q_batch_stride + t * ldq + h *
+ * q_head_stride (elements), `dim` long; zero strides mean contiguous [batch,
+ * heads, tokens, dim].  The first rot_dim columns are n/2 = rot_dim/2 pairs:
+ * (i, i + n/2) (HALF) or (2i, 2i + 1) (INTERLEAVED); pair i of a token at
+ * position p turns by p * f_i, f_i = base^(-2i/n), and is multiplied by
+ * `magnitude`; the other columns are copied.  For contexts longer than the
+ * one trained on: LINEAR divides every f_i by `factor`; BY_PARTS divides by
+ * parts, f_i (c + (1 - c) / factor) with c = (r - low_turns) / (high_turns -
+ * low_turns) cut to 0..1 and r = context * f_i / (2 pi), the turns of the pair
+ * over `context` positions: fast pairs keep their frequency. */
+typedef enum { BWPP_HIP_ROTARY_HALF = 0, BWPP_HIP_ROTARY_INTERLEAVED = 1 } BwppHipRotaryLayout;
+typedef enum {
+  BWPP_HIP_ROTARY_SCALE_NONE = 0,
+  BWPP_HIP_ROTARY_SCALE_LINEAR = 1,
+  BWPP_HIP_ROTARY_SCALE_BY_PARTS = 2
+} BwppHipRotaryScaling;
+typedef struct {
+  uint32_t tokens;
+  uint32_t q_heads;
+  uint32_t k_heads;
+  uint32_t dim;
+  uint32_t batch;   /* 0 = 1 */
+  uint32_t rot_dim; /* even, at most dim and 4096; 0 = dim */
+  uint32_t layout;  /* BwppHipRotaryLayout */
+  uint32_t dtype;   /* BwppHipDType, 0 = F32 */
+  uint32_t ldq, ldk, ldqo, ldko; /* token strides; 0 = dim */
+  uint64_t q_batch_stride, q_head_stride;
+  uint64_t k_batch_stride, k_head_stride;
+  uint64_t qo_batch_stride, qo_head_stride;
+  uint64_t ko_batch_stride, ko_head_stride;
+  uint64_t pos_batch_stride; /* positions of a batch; 0 = the same for all */
+  int32_t pos_offset;        /* without positions: token t is at pos_offset + t */
+  uint32_t scaling;          /* BwppHipRotaryScaling */
+  float base;                /* 0 = 10000 */
+  float factor;              /* 0 = 1 */
+  float low_turns, high_turns;
+  uint32_t context;
+  float magnitude;           /* 0 = 1 */
+} BwppRotaryParams;
+
+/* The join of a block's branch o with the residual stream x, and the norms
+ * around it (no reference counterpart).  With v' = v / sqrt(mean(v^2) + eps)
+ * along the rows:
+ *   u = post_gamma o'   (post_norm = 0: u = o)
+ *   r = stream_scale x + branch_scale gate u
+ *   y = pre_gamma r'    (the next block's input)
+ * gate row i / gate_rows applies to row i (0: one gate row for all; 1: a gate
+ * of o's shape).  x, r and their gradients have row stride ldx, o and its
+ * gradient ldo, y and its gradient ldy, gate rows ldg. */
+typedef struct {
+  uint32_t rows;
+  uint32_t cols;
+  uint32_t ldx, ldo, ldy, ldg; /* 0 = cols */
+  uint32_t post_norm;
+  uint32_t gate_rows;
+  float eps;
+  float stream_scale; /* 0 = 1 */
+  float branch_scale; /* 0 = 1 */
+  uint32_t dtype;     /* BwppHipDType of every operand, 0 = F32 */
+} BwppResidualNormParams;
+
 typedef struct BwppHip BwppHip;
 
 /* ---- handle ---- */
@@ -526,6 +589,42 @@ BwppHipStatus bwpp_hip_dispatch_reduce_sum(BwppHip *h, const float *x, float *ou
 /* add / sub / mul / div with broadcasting, and broadcast (op COPY). */
 BwppHipStatus bwpp_hip_dispatch_elementwise(BwppHip *h, const float *a, const float *b, float *out,
                                             BwppElementwiseParams params);
+
+/* ---- around the block: positions, residual joins ----
+ * F32 or BF16 operands; arithmetic and sums in fp32, each output rounded
+ * once.  No reference counterparts. */
+
+/* qo, ko = the rotated q, k.  positions: device int32 [batch][tokens] (row
+ * stride pos_batch_stride) or NULL; any int32 is a position.  k may be NULL
+ * with k_heads 0 (and q with q_heads 0).  qo may be q with the same strides
+ * (in place; columns past rot_dim stay), and ko k; outputs must not meet
+ * inputs or each other otherwise (ALIAS).  Angles are reduced in 64 bits. */
+BwppHipStatus bwpp_hip_dispatch_rotary(BwppHip *h, const void *q, const void *k, const int32_t *positions, void *qo,
+                                       void *ko, BwppRotaryParams params);
+
+/* Its gradient: dq, dk (q's and k's strides) from dqo, dko (qo's and ko's):
+ * the same turn backwards, the same magnitude. */
+BwppHipStatus bwpp_hip_dispatch_rotary_grad(BwppHip *h, const void *dqo, const void *dko, const int32_t *positions,
+                                            void *dq, void *dk, BwppRotaryParams params);
+
+/* r and y of BwppResidualNormParams.  post_gamma, gate, pre_gamma NULL = 1
+ * (gate NULL: no gate); y NULL: no norm after.  r may be x; outputs must not
+ * meet inputs or each other otherwise (ALIAS).  y is taken from r before its
+ * rounding. */
+BwppHipStatus bwpp_hip_dispatch_residual_norm(BwppHip *h, const void *x, const void *o, const void *post_gamma,
+                                              const void *gate, const void *pre_gamma, void *r, void *y,
+                                              BwppResidualNormParams params);
+
+/* Its gradient from the branch o, the stored r, and the upstream dr (of r, by
+ * later blocks) and dy, either NULL = 0: dx (may be dr), dout (of o) and the
+ * sums dpost_gamma [cols], dgate (gate's shape and row stride), dpre_gamma
+ * [cols]; a NULL output is not computed.  Sums over rows are taken in fp32, in
+ * an order that depends on the sizes only; their partial rows lie in the
+ * handle's workspace. */
+BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const void *o, const void *r, const void *post_gamma,
+                                                   const void *gate, const void *pre_gamma, const void *dr,
+                                                   const void *dy, void *dx, void *dout, void *dpost_gamma,
+                                                   void *dgate, void *dpre_gamma, BwppResidualNormParams params);
 
 /* ---- launch plans (compiled graphs) ----
  *
