@@ -6,7 +6,7 @@ if the library or a code object is missing, HipBackend() raises.
 """
 from . import _lib, plan, synth
 from ._lib import (AttentionParams, CoreDType, DType, ElementwiseParams, Epilogue, Fusion,
-                   FusionParams, LibraryMissing, MatmulParams, MeanSquareParams, ReduceParams,
+                   FusionParams, LibraryMissing, LinearXentParams, MatmulParams, MeanSquareParams, ReduceParams,
                    ResidualNormParams, RmsnormParams, RotaryLayout, RotaryParams, RotaryScaling,
                    SoftmaxParams, Status, Tensor)
 from .backend import BwppError, HipBackend, tensor_of
@@ -14,6 +14,7 @@ from .backend import BwppError, HipBackend, tensor_of
 __all__ = ["HipBackend", "BwppError", "LibraryMissing", "Status", "DType",
            "Epilogue", "Fusion", "FusionParams", "MatmulParams", "SoftmaxParams", "RmsnormParams",
            "MeanSquareParams", "RotaryLayout", "RotaryScaling", "RotaryParams", "ResidualNormParams",
+           "LinearXentParams",
            "AttentionParams", "ReduceParams", "ElementwiseParams", "CoreDType", "Tensor",
            "tensor_of", "synth", "plan",
            "load_library"]

@@ -126,6 +126,12 @@ class ResidualNormParams(Structure):
                 ("eps", c_float), ("stream_scale", c_float), ("branch_scale", c_float), ("dtype", c_uint32)]
 
 
+class LinearXentParams(Structure):
+    _fields_ = [("rows", c_uint32), ("vocab", c_uint32), ("dim", c_uint32), ("ldx", c_uint32), ("ldw", c_uint32),
+                ("lddx", c_uint32), ("lddw", c_uint32), ("trans_w", c_uint32), ("dtype", c_uint32),
+                ("dloss_scalar", c_uint32), ("scale", c_float)]
+
+
 class Arena(Structure):
     _fields_ = [("buffer", c_void_p), ("capacity", c_size_t),
                 ("offset", c_size_t), ("device", c_int)]
@@ -220,6 +226,8 @@ SIGNATURES = {
     "bwpp_hip_dispatch_rotary_grad": (c_int, [_P] * 6 + [RotaryParams]),
     "bwpp_hip_dispatch_residual_norm": (c_int, [_P] * 8 + [ResidualNormParams]),
     "bwpp_hip_dispatch_residual_norm_grad": (c_int, [_P] * 13 + [ResidualNormParams]),
+    "bwpp_hip_dispatch_linear_xent": (c_int, [_P] * 7 + [LinearXentParams]),
+    "bwpp_hip_dispatch_linear_xent_grad": (c_int, [_P] * 8 + [LinearXentParams]),
     "bwpp_synth_uniform_f32": (None, [_P, c_uint64, c_uint64, c_uint64, c_float, c_float]),
     "bwpp_synth_normal_f32": (None, [_P, c_uint64, c_uint64, c_uint64, c_float, c_float]),
     "bwpp_synth_ramp_f32": (None, [_P, c_uint32, c_uint32, c_float]),
@@ -264,6 +272,6 @@ def load():
 __all__ = ["Status", "DType", "Epilogue", "MatmulParams", "Fusion", "FusionParams", "SoftmaxParams",
            "RmsnormParams", "MeanSquareParams", "AttentionParams", "ReduceParams", "ElementwiseParams", "Arena",
            "RotaryLayout", "RotaryScaling", "RotaryParams", "ResidualNormParams",
-           "CoreDType", "Tensor",
+           "LinearXentParams", "CoreDType", "Tensor",
            "SIGNATURES", "load", "LIB_PATH", "LIB_DIR", "HEADER_PATH",
            "LibraryMissing", "byref", "c_void_p", "c_uint16"]

@@ -211,6 +211,15 @@ class HipBackend:
             self._h, _ptr(o), _ptr(r), _ptr(post_gamma), _ptr(gate), _ptr(pre_gamma), _ptr(dr), _ptr(dy), _ptr(dx),
             _ptr(dout), _ptr(dpost_gamma), _ptr(dgate), _ptr(dpre_gamma), params))
 
+    def dispatch_linear_xent(self, x, w, targets, loss, lse, sums, params):
+        """loss[t] = lse[t] - z[t][targets[t]], z = scale x W; sums: their sum and how many rows count."""
+        self._check(self.lib.bwpp_hip_dispatch_linear_xent(
+            self._h, _ptr(x), _ptr(w), _ptr(targets), _ptr(loss), _ptr(lse), _ptr(sums), params))
+
+    def dispatch_linear_xent_grad(self, x, w, targets, lse, dloss, dx, dw, params):
+        self._check(self.lib.bwpp_hip_dispatch_linear_xent_grad(
+            self._h, _ptr(x), _ptr(w), _ptr(targets), _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw), params))
+
     # ------------------------------------------------------ tensor forms
     def tensor_matmul(self, a, b, bias, c, epilogue: int = 0):
         ref = lambda t: ctypes.byref(t) if t is not None else None

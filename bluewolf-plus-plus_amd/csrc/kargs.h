@@ -197,4 +197,43 @@ typedef struct {
   uint32_t workers, group, split, span;
 } BwppResNormArgs;
 
+/* Cross entropy of hidden states against a vocabulary (xent.hip).  Logits
+ * z = scale op(W) x: g holds their product (M tokens, N of the columns n_base
+ * .. of the vocabulary, K = dim). */
+typedef struct {
+  BwppGemmArgs g;
+  const int32_t *target;
+  const float *lse;   /* gradient */
+  const float *dloss; /* gradient: NULL = 1 */
+  uint32_t dloss_scalar;
+  uint32_t n_base;
+  uint32_t vocab;
+  float scale;
+  float *part; /* forward: [tiles_n][M] pairs (max, sum of exp(z - max)) */
+  float *zt;   /* forward: [M] target logits */
+  uint16_t *dl; /* gradient: dz scale, [M][ldl] bf16 */
+  uint32_t ldl;
+  uint32_t accumulate; /* sums: add to what is there */
+  float *raw;          /* sums: [ksplit][M][N] */
+} BwppXentArgs;
+
+/* Its row kernels. */
+typedef struct {
+  const void *x;
+  void *y;
+  const float *src;      /* fp32 sums or logits */
+  const int32_t *target;
+  const float *dloss;
+  const float *lse_in;
+  float *part;
+  float *zt;
+  float *loss, *lse, *sums;
+  uint64_t ldx, ldy, lds;
+  uint32_t rows, cols;
+  uint32_t n_base, vocab;
+  uint32_t nparts; /* partials a row, or planes of sums */
+  uint32_t dloss_scalar;
+  float scale;
+} BwppXentRowArgs;
+
 #endif /* BWPP_KARGS_H */

@@ -1,0 +1,398 @@
+// Cross entropy of hidden states against a vocabulary, for gfx950, without
+// keeping the logits:
+//
+//   z = scale x W                        [tokens x vocabulary]
+//   lse_t = log sum_v exp z_tv           loss_t = lse_t - z_t,target
+//   dz_tv = g_t (exp(z_tv - lse_t) - [v = target]),   dx = scale dz W^T,
+//   dW = scale x^T dz
+//
+// A target outside the vocabulary leaves its row out: loss and gradients 0.
+//
+// bf16: the logits' product runs on the matrix cores (gemm_bf16.h's loops)
+// and stays in its accumulators.  The forward's epilogue reduces each tile's
+// rows to (max, sum of exp), a pair per row and tile, and a second kernel
+// joins the pairs.  The gradient's epilogue turns the same product, made
+// again from x and W, into dz, rounded to bf16 as the next two products'
+// operand (each element off by half a step, 2^-9 of it in the mean; dx and dW
+// add thousands of them, and are rounded to bf16 themselves).  It does so for
+// one piece of the vocabulary at a time, small enough to stay in the Infinity
+// Cache between its writer and its readers.  dx is summed over the pieces in
+// fp32 planes (one per K split) and rounded once; each piece's dW is final.
+// fp32: the logits of a piece go through memory once, in fp32 (8 to 16 bytes a
+// logit beside 2 dim FLOPs at a sixteenth of the bf16 rate).
+//
+// Maxima and sums are fp32, the last logarithm 64-bit (once a row): lse is off
+// by a few 2^-24 of itself.  exp(z - max) is taken as exp2 of the rounded
+// difference, which is exact for the logits that count.
+#include "gemm_bf16.h"
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// exp(z - m) with m the maximum of some z's; an infinite maximum (no logit,
+// or an infinite one) counts from 0.
+__device__ __forceinline__ float finite_or_0(float m) { return __builtin_isfinite(m) ? m : 0.0f; }
+__device__ __forceinline__ float exp_diff(float z, float ref) { return __builtin_amdgcn_exp2f((z - ref) * kLog2e); }
+__device__ __forceinline__ void join(float &m, float &s, float m2, float s2) {
+  const float mm = fmaxf(m, m2), ref = finite_or_0(mm);
+  // (a part without logits is (-inf, 0))
+  s = s * exp_diff(m, ref) + s2 * exp_diff(m2, ref);
+  m = mm;
+}
+
+template <int FN, int FM, class F>
+__device__ __forceinline__ void each_column(uint32_t n_first, int lhalf, F f) {
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) f(i, r, n_first + (uint32_t)(i * 32 + 8 * (r / 4) + 4 * lhalf + r % 4));
+}
+
+// Per row of the tile: maximum and sum of exp, and the target's logit.
+struct EpiStats {
+  static constexpr bool kStore = false;
+  const BwppXentArgs &a;
+
+  template <int BM, int BN, int WM, int WN, int FN, int FM>
+  __device__ __forceinline__ void run(f32x16_t (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0,
+                                      uint32_t tn, uint32_t, int tid, int wm, int wn) const {
+    constexpr int TM = BM / WM, TN = BN / WN;
+    const int lane = tid & 63, lrow = lane & 31, lhalf = lane >> 5;
+    float2 *pair = reinterpret_cast<float2 *>(smem);  // [BM][WN]
+    const uint32_t nw = n0 + (uint32_t)(wn * TN);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t ml = (uint32_t)(wm * TM + j * 32 + lrow), m = m0 + ml;
+      const uint32_t t = m < a.g.M ? (uint32_t)a.target[m] : 0xffffffffu;
+      if (n0 + BN > a.g.N)  // the last tile column: no logits past N
+        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t n) {
+          if (n >= a.g.N) acc[i][j][r] = -__builtin_inff();
+          else acc[i][j][r] *= a.scale;
+        });
+      else
+        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { acc[i][j][r] *= a.scale; });
+      const uint32_t tl = t - a.n_base;  // the target's column of this product
+      if (__any(t < a.vocab && tl - nw < (uint32_t)TN))
+        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t n) {
+          if (t < a.vocab && n == tl && n < a.g.N) a.zt[m] = acc[i][j][r];
+        });
+      float mx = -__builtin_inff(), s = 0.0f;
+      each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { mx = fmaxf(mx, acc[i][j][r]); });
+      mx = fmaxf(mx, xor_f32(mx, 32));
+      const float ref = finite_or_0(mx);
+      each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { s += exp_diff(acc[i][j][r], ref); });
+      s += xor_f32(s, 32);
+      if (lhalf == 0) pair[ml * WN + wn] = make_float2(mx, s);
+    }
+    __syncthreads();
+    if (tid < BM && m0 + (uint32_t)tid < a.g.M) {
+      float2 p = pair[tid * WN];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) {
+        const float2 q = pair[tid * WN + w];
+        join(p.x, p.y, q.x, q.y);
+      }
+      reinterpret_cast<float2 *>(a.part)[(size_t)tn * a.g.M + m0 + (uint32_t)tid] = p;
+    }
+  }
+};
+
+// dz scale in bf16.
+struct EpiGrad {
+  static constexpr bool kStore = false;
+  const BwppXentArgs &a;
+
+  template <int BM, int BN, int WM, int WN, int FN, int FM>
+  __device__ __forceinline__ void run(f32x16_t (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0,
+                                      uint32_t, uint32_t, int tid, int wm, int wn) const {
+    constexpr int TM = BM / WM, TN = BN / WN, NT = 64 * WM * WN, kCld = BN + 8;
+    const int lane = tid & 63, lrow = lane & 31, lhalf = lane >> 5;
+    uint16_t *cs = reinterpret_cast<uint16_t *>(smem);  // [BM][BN + 8]
+    const uint32_t nw = n0 + (uint32_t)(wn * TN);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t ml = (uint32_t)(wm * TM + j * 32 + lrow), m = m0 + ml;
+      uint32_t t = 0xffffffffu;
+      float lse = 0.0f, g = 0.0f;
+      if (m < a.g.M) {
+        t = (uint32_t)a.target[m];
+        lse = a.lse[m];
+        g = (a.dloss ? a.dloss[a.dloss_scalar ? 0u : m] : 1.0f) * a.scale;
+      }
+      const bool live = t < a.vocab;
+      each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { acc[i][j][r] = exp_diff(acc[i][j][r] * a.scale, lse); });
+      const uint32_t tl = t - a.n_base;
+      if (__any(live && tl - nw < (uint32_t)TN))
+        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t n) {
+          if (live && n == tl) acc[i][j][r] -= 1.0f;
+        });
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = live ? g * acc[i][j][4 * q + e] : 0.0f;
+          uint2 o;
+          o.x = pack_bf16x2(v[0], v[1]);
+          o.y = pack_bf16x2(v[2], v[3]);
+          *reinterpret_cast<uint2 *>(cs + ml * kCld + wn * TN + i * 32 + q * 8 + lhalf * 4) = o;
+        }
+    }
+    __syncthreads();
+    // ldl is a multiple of 8: whole chunks, columns past N with the values of
+    // the columns that were read again (inside the row, never used).
+#pragma unroll 4
+    for (int it = 0; it < BM * (BN / 8) / NT; ++it) {
+      const int q = tid + it * NT, row = q / (BN / 8), c = q % (BN / 8);
+      const uint32_t m = m0 + (uint32_t)row, n = n0 + 8u * (uint32_t)c;
+      if (m < a.g.M && n < a.ldl)
+        *reinterpret_cast<uint4 *>(a.dl + (size_t)m * a.ldl + n) = *reinterpret_cast<const uint4 *>(cs + row * kCld + c * 8);
+    }
+  }
+};
+
+// fp32 sums, one plane per K split, added to what is there where asked.
+struct EpiSums {
+  static constexpr bool kStore = false;
+  const BwppXentArgs &a;
+
+  template <int BM, int BN, int WM, int WN, int FN, int FM>
+  __device__ __forceinline__ void run(f32x16_t (&acc)[FN][FM], unsigned char *, uint32_t m0, uint32_t n0, uint32_t,
+                                      uint32_t split, int tid, int wm, int wn) const {
+    constexpr int TM = BM / WM, TN = BN / WN;
+    const int lane = tid & 63, lrow = lane & 31, lhalf = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t m = m0 + (uint32_t)(wm * TM + j * 32 + lrow);
+      float *row = a.raw + ((size_t)split * a.g.M + m) * a.g.N;
+      if (m >= a.g.M) continue;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t n = n0 + (uint32_t)(wn * TN + i * 32 + q * 8 + lhalf * 4);
+          float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+          if (n + 4 <= a.g.N) {
+            if (a.accumulate) {
+              const float4 o = load4(row + n);
+              v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+            }
+            store4(row + n, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.g.N) row[n + e] = acc[i][j][4 * q + e] + (a.accumulate ? row[n + e] : 0.0f);
+          }
+        }
+    }
+  }
+};
+
+// ------------------------------------------------------------ row kernels
+
+__device__ __forceinline__ bool live(const BwppXentRowArgs &a, uint32_t row) {
+  return (uint32_t)a.target[row] < a.vocab;
+}
+
+template <class T>
+__device__ __forceinline__ T to(float v);
+template <>
+__device__ __forceinline__ float to<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ uint16_t to<uint16_t>(float v) { return f32_to_bf16_bits(v); }
+
+// y = x, rows that are left out 0 (their values, infinities and NaN among
+// them, stay out of dW's sums).
+template <class T>
+__device__ __forceinline__ void copy_rows(const BwppXentRowArgs &a) {
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const bool on = live(a, row);
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    T *y = static_cast<T *>(a.y) + row * a.ldy;
+    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) y[c] = on ? x[c] : T(0);
+  }
+}
+// Rows that are left out: 0.
+template <class T>
+__device__ __forceinline__ void zero_rows(const BwppXentRowArgs &a) {
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (live(a, row)) continue;
+    T *y = static_cast<T *>(a.y) + row * a.ldy;
+    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) y[c] = T(0);
+  }
+}
+
+}  // namespace
+
+// Joins a row's pairs: 64 rows a block, 16 waves each over a sixteenth of the
+// pairs (coalesced over the rows); then loss and lse, and with a single block
+// the sums over the rows too.
+extern "C" __global__ __launch_bounds__(1024) void bwpp_xent_join(const BwppXentRowArgs a) {
+  __shared__ float2 p[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t row = blockIdx.x * 64 + lane;
+  float m = -__builtin_inff(), s = 0.0f;
+  if (row < a.rows) {
+    const float2 *part = reinterpret_cast<const float2 *>(a.part) + row;
+#pragma unroll 4
+    for (uint32_t i = wave; i < a.nparts; i += 16) {
+      const float2 q = part[(size_t)i * a.rows];
+      join(m, s, q.x, q.y);
+    }
+  }
+  p[wave][lane] = make_float2(m, s);
+  __syncthreads();
+  if (wave != 0) return;
+  double total = 0.0;
+  uint32_t n = 0;
+  if (row < a.rows) {
+    for (int w = 1; w < 16; ++w) join(m, s, p[w][lane].x, p[w][lane].y);
+    const double lse = (double)finite_or_0(m) + log((double)s);
+    const bool on = live(a, row);
+    const float loss = on ? (float)(lse - (double)a.zt[row]) : 0.0f;
+    if (a.lse) a.lse[row] = (float)lse;
+    if (a.loss) a.loss[row] = loss;
+    total = loss;
+    n = on ? 1u : 0u;
+  }
+  if (a.sums && gridDim.x == 1) {
+    for (int d = 1; d < 64; d *= 2) {
+      total += __shfl_xor(total, d, 64);
+      n += (uint32_t)__shfl_xor((int)n, d, 64);
+    }
+    if (lane == 0) {
+      a.sums[0] = (float)total;
+      a.sums[1] = (float)n;
+    }
+  }
+}
+
+// Sum of the losses (64-bit) and number of rows that count, one block.
+extern "C" __global__ __launch_bounds__(1024) void bwpp_xent_sums(const BwppXentRowArgs a) {
+  __shared__ double ts[16];
+  __shared__ uint32_t ns[16];
+  double total = 0.0;
+  uint32_t n = 0;
+  for (uint64_t row = threadIdx.x; row < a.rows; row += 1024) {
+    const bool on = live(a, (uint32_t)row);
+    total += on ? (double)a.loss[row] : 0.0;
+    n += on ? 1u : 0u;
+  }
+  for (int d = 1; d < 64; d *= 2) {
+    total += __shfl_xor(total, d, 64);
+    n += (uint32_t)__shfl_xor((int)n, d, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    ts[threadIdx.x >> 6] = total;
+    ns[threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) {
+      total += ts[w];
+      n += ns[w];
+    }
+    a.sums[0] = (float)total;
+    a.sums[1] = (float)n;
+  }
+}
+
+// fp32 logits of a piece (src, unscaled): one pair per row into part[rows].
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_stats_f32(const BwppXentRowArgs a) {
+  __shared__ float ms[4], ss[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float *z = a.src + (uint64_t)row * a.lds;
+    float m = -__builtin_inff(), s = 0.0f;
+    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
+      const float v = z[c] * a.scale;
+      join(m, s, v, 1.0f);
+    }
+    for (int d = 1; d < 64; d *= 2) join(m, s, xor_f32(m, d), xor_f32(s, d));
+    if (lane == 0) {
+      ms[wave] = m;
+      ss[wave] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 4; ++w) join(m, s, ms[w], ss[w]);
+      reinterpret_cast<float2 *>(a.part)[row] = make_float2(m, s);
+      const uint32_t t = (uint32_t)a.target[row], tl = t - a.n_base;
+      if (t < a.vocab && tl < a.cols) a.zt[row] = z[tl] * a.scale;
+    }
+    __syncthreads();
+  }
+}
+
+// fp32 logits of a piece (y, unscaled) -> dz scale, in place.
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_grad_f32(const BwppXentRowArgs a) {
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    float *z = static_cast<float *>(a.y) + (uint64_t)row * a.ldy;
+    const uint32_t t = (uint32_t)a.target[row], tl = t - a.n_base;
+    const bool on = t < a.vocab;
+    const float lse = a.lse_in[row], g = (a.dloss ? a.dloss[a.dloss_scalar ? 0u : row] : 1.0f) * a.scale;
+    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
+      const float p = exp_diff(z[c] * a.scale, lse);
+      z[c] = on ? g * (c == tl ? p - 1.0f : p) : 0.0f;
+    }
+  }
+}
+
+// Planes of fp32 sums -> bf16 rows, rows that are left out 0.
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_bf16(const BwppXentRowArgs a) {
+  const uint64_t plane = (uint64_t)a.rows * a.cols;
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const bool on = live(a, row);
+    uint16_t *y = static_cast<uint16_t *>(a.y) + row * a.ldy;
+    const float *src = a.src + (uint64_t)row * a.cols;
+    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
+      float v = src[c];
+      for (uint32_t i = 1; i < a.nparts; ++i) v += src[i * plane + c];
+      y[c] = on ? f32_to_bf16_bits(v) : (uint16_t)0;
+    }
+  }
+}
+
+// Zeros (dW of no rows).
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_clear(const BwppXentRowArgs a) {
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    unsigned char *y = static_cast<unsigned char *>(a.y) + row * a.ldy;  // bytes
+    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) y[c] = 0;
+  }
+}
+
+#define BWPP_XENT_ROWS(TN, T)                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void bwpp_xent_copy_##TN(const BwppXentRowArgs a) { copy_rows<T>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void bwpp_xent_zero_##TN(const BwppXentRowArgs a) { zero_rows<T>(a); }
+BWPP_XENT_ROWS(bf16, uint16_t)
+BWPP_XENT_ROWS(f32, float)
+
+// bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 full K tiles, r32 and
+// r128 any size (32 x 64, 128 x 128), _u with operands through registers.
+#define BWPP_XENT_PIPE(KIND, EPI, TB)                                                                     \
+  extern "C" __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) \
+  void bwpp_xent_##KIND##_p_t0##TB(const BwppXentArgs a) {                                                \
+    gemm_bf16_pipe<false, TB != 0, 2, 4, 256, 3, EPI>(a.g, EPI{a});                                       \
+  }
+#define BWPP_XENT_RING(KIND, EPI, TB, NAME, BM, BN, WM, WN, KPS, STAGES, WPE, KPSU, WPEU)                       \
+  extern "C" __global__ __launch_bounds__(64 * WM * WN, WPE) void bwpp_xent_##KIND##_##NAME##_t0##TB(           \
+      const BwppXentArgs a) {                                                                                   \
+    gemm_bf16_ring<false, TB != 0, BM, BN, WM, WN, KPS, STAGES, false, EPI>(a.g, EPI{a});                       \
+  }                                                                                                             \
+  extern "C" __global__ __launch_bounds__(64 * WM * WN, WPEU) void bwpp_xent_##KIND##_##NAME##_t0##TB##_u(      \
+      const BwppXentArgs a) {                                                                                   \
+    gemm_bf16_ring<false, TB != 0, BM, BN, WM, WN, KPSU, 2, true, EPI>(a.g, EPI{a});                            \
+  }
+#define BWPP_XENT_TB(TB)                                                    \
+  BWPP_XENT_PIPE(stats, EpiStats, TB)                                       \
+  BWPP_XENT_PIPE(grad, EpiGrad, TB)                                         \
+  BWPP_XENT_PIPE(sums, EpiSums, TB)                                         \
+  BWPP_XENT_RING(stats, EpiStats, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)     \
+  BWPP_XENT_RING(grad, EpiGrad, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)       \
+  BWPP_XENT_RING(stats, EpiStats, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)  \
+  BWPP_XENT_RING(grad, EpiGrad, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)    \
+  BWPP_XENT_RING(sums, EpiSums, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)
+BWPP_XENT_TB(0)
+BWPP_XENT_TB(1)

@@ -34,7 +34,7 @@ thread_local std::string g_create_error;
 // Code objects built by the package Makefile, all required.
 const char *const kModules[] = {"bwpp_rowops.hsaco", "bwpp_gemm.hsaco", "bwpp_attention.hsaco",
                                  "bwpp_attention_f32.hsaco", "bwpp_attention_bwd.hsaco", "bwpp_grad.hsaco",
-                                 "bwpp_rotary.hsaco", "bwpp_resnorm.hsaco"};
+                                 "bwpp_rotary.hsaco", "bwpp_resnorm.hsaco", "bwpp_xent.hsaco"};
 
 // Row-op kernels: bwpp_row_<op>_v<VPT>_w<WPR>_<f|p>, see rowops.hip.
 enum RowOpId { ROW_SOFTMAX, ROW_RMSNORM, ROW_LAYERNORM, ROW_MAX, ROW_MAXGRAD, ROW_MASK, ROW_NOPS };
@@ -148,6 +148,7 @@ struct BwppHip {
   // reuse across calls is safe.
   void *ws = nullptr;
   size_t ws_bytes = 0;
+  size_t ws_held = 0;  // its first bytes, held by an operator that runs others (bwpp_hip_hold_workspace)
   // Split scratch: partials of operators that also have a path without
   // them.  One fixed allocation of kSplitBytes on first use, never moved
   // (so captured plans stay valid whatever runs later), freed by
@@ -1069,7 +1070,11 @@ BwppHipStatus ensure_ws(BwppHip *h, size_t bytes);
 namespace {
 
 // Whether the handle has, or can be given, a workspace of `bytes`.
-bool ws_ready(BwppHip *h, size_t bytes) { return h->ws_bytes >= bytes || !recording(h); }
+bool ws_ready(BwppHip *h, size_t bytes) {
+  if (h->ws_held) return h->ws_bytes - h->ws_held >= bytes;
+  return h->ws_bytes >= bytes || !recording(h);
+}
+void *ws_ptr(BwppHip *h) { return static_cast<unsigned char *>(h->ws) + h->ws_held; }
 
 // Kernels for any M, N and K (gemm.hip: gemm_bf16_ring, gemm_f32_any) for a
 // product whose operands are set in g: picks the tile and the number of K
@@ -1153,7 +1158,7 @@ BwppHipStatus ring_dispatch(BwppHip *h, BwppGemmArgs g, bool bf16, bool ta, bool
   if (best >= 0 && bestS > 1) {
     const size_t bytes = (size_t)(plane * bestS);
     if (!use_ws) part = split_scratch(h, bytes);
-    else if (ws_ready(h, bytes) && ensure_ws(h, bytes) == BWPP_HIP_OK) part = h->ws;
+    else if (ws_ready(h, bytes) && ensure_ws(h, bytes) == BWPP_HIP_OK) part = ws_ptr(h);
     if (!part) {
       h->err.clear();  // no failure of this call
       search(1);
@@ -1373,7 +1378,7 @@ BwppHipStatus matmul_impl(BwppHip *h, const void *a, const void *b, void *c, con
       if ((s = ensure_ws(h, (size_t)bestS * p.M * p.N * sizeof(float))) != BWPP_HIP_OK) return s;
       g.ksplit = (uint32_t)bestS;
       g.kchunk = bestChunk;
-      g.part = static_cast<float *>(h->ws);
+      g.part = static_cast<float *>(ws_ptr(h));
       if ((s = launch(h, bestKind ? h->gemm_f32p[ring4][ta][tb][1] : h->gemm_f32_split[ta][tb],
                       (uint32_t)(tiles * bestS), 1, 1, 256, g)) != BWPP_HIP_OK)
         return s;
@@ -1910,6 +1915,10 @@ namespace {
 // Ensures the handle's workspace holds `bytes`; waits for queued work on the
 // handle's stream before replacing a smaller buffer.
 BwppHipStatus ensure_ws(BwppHip *h, size_t bytes) {
+  if (h->ws_held) {  // a part of it is in use: it stays as it is
+    if (h->ws_bytes - h->ws_held >= bytes) return BWPP_HIP_OK;
+    return fail(h, BWPP_HIP_ERR_OUT_OF_MEMORY, "workspace of %zu bytes held, %zu more needed", h->ws_bytes, bytes);
+  }
   if (h->ws_bytes >= bytes) return BWPP_HIP_OK;
   if (h->ws) {
     hipError_t e = hipStreamSynchronize(h->stream);
@@ -2225,6 +2234,8 @@ BwppHipStatus bwpp_hip_take_workspace(BwppHip *h, size_t bytes, void **p) {
   *p = s == BWPP_HIP_OK ? h->ws : nullptr;
   return s;
 }
+
+void bwpp_hip_hold_workspace(BwppHip *h, size_t bytes) { h->ws_held = bytes; }
 
 bool bwpp_hip_blocks_overlap(const void *pa, uint64_t ra, uint64_t ca, uint64_t lda, const void *pb, uint64_t rb,
                              uint64_t cb, uint64_t ldb, uint64_t es) {

@@ -1,7 +1,7 @@
-// Operators of libbwpp_hip around a transformer block: rotary positions and
-// the residual join with its norms, forward and gradient.  Argument checks,
-// launch geometry and the choice of a kernel; the kernels are rotary.hip and
-// resnorm.hip.
+// Operators of libbwpp_hip around a transformer block: rotary positions, the
+// residual join with its norms, and the cross entropy against a vocabulary,
+// forward and gradient.  Argument checks, launch geometry and the choice of a
+// kernel; the kernels are rotary.hip, resnorm.hip and xent.hip.
 #include "bwpp_hip.h"
 #include "internal.h"
 
@@ -18,7 +18,18 @@ enum LmKernel {
   LM_RESNORM = LM_ROTARY_F32 + 4,      // [bf16][kResCfgs, any]
   LM_RESNORM_GRAD = LM_RESNORM + 14,   // [bf16][kResCfgs - 1, any]
   LM_RESNORM_FINISH = LM_RESNORM_GRAD + 12,  // [bf16]
-  LM_COUNT = LM_RESNORM_FINISH + 2
+  LM_XENT_JOIN = LM_RESNORM_FINISH + 2,
+  LM_XENT_SUMS,
+  LM_XENT_STATS_F32,
+  LM_XENT_GRAD_F32,
+  LM_XENT_ROUND,
+  LM_XENT_CLEAR,
+  LM_XENT_COPY,                          // [bf16]
+  LM_XENT_ZERO = LM_XENT_COPY + 2,       // [bf16]
+  LM_XENT_STATS = LM_XENT_ZERO + 2,      // [trans_w][XentTile]
+  LM_XENT_GRAD = LM_XENT_STATS + 10,
+  LM_XENT_RAW = LM_XENT_GRAD + 10,
+  LM_COUNT = LM_XENT_RAW + 10
 };
 
 // Rows in registers (resnorm.hip): elements a thread and waves a row.
@@ -45,6 +56,39 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_resnorm_grad_bf16_n8_w1", "bwpp_resnorm_grad_bf16_n8_w2", "bwpp_resnorm_grad_bf16_n8_w4",
     "bwpp_resnorm_grad_bf16_n8_w8", "bwpp_resnorm_grad_bf16_n8_w16", "bwpp_resnorm_grad_bf16_any",
     "bwpp_resnorm_finish_f32",      "bwpp_resnorm_finish_bf16",
+    "bwpp_xent_join", "bwpp_xent_sums", "bwpp_xent_stats_f32", "bwpp_xent_grad_f32",
+    "bwpp_xent_round_bf16", "bwpp_xent_clear", "bwpp_xent_copy_f32", "bwpp_xent_copy_bf16",
+    "bwpp_xent_zero_f32", "bwpp_xent_zero_bf16",
+    "bwpp_xent_stats_p_t00",
+    "bwpp_xent_stats_r32_t00",
+    "bwpp_xent_stats_r32_t00_u",
+    "bwpp_xent_stats_r128_t00",
+    "bwpp_xent_stats_r128_t00_u",
+    "bwpp_xent_stats_p_t01",
+    "bwpp_xent_stats_r32_t01",
+    "bwpp_xent_stats_r32_t01_u",
+    "bwpp_xent_stats_r128_t01",
+    "bwpp_xent_stats_r128_t01_u",
+    "bwpp_xent_grad_p_t00",
+    "bwpp_xent_grad_r32_t00",
+    "bwpp_xent_grad_r32_t00_u",
+    "bwpp_xent_grad_r128_t00",
+    "bwpp_xent_grad_r128_t00_u",
+    "bwpp_xent_grad_p_t01",
+    "bwpp_xent_grad_r32_t01",
+    "bwpp_xent_grad_r32_t01_u",
+    "bwpp_xent_grad_r128_t01",
+    "bwpp_xent_grad_r128_t01_u",
+    "bwpp_xent_sums_p_t00",
+    "bwpp_xent_sums_r128_t00",
+    "bwpp_xent_sums_r128_t00_u",
+    "bwpp_xent_sums_r128_t00",
+    "bwpp_xent_sums_r128_t00_u",
+    "bwpp_xent_sums_p_t01",
+    "bwpp_xent_sums_r128_t01",
+    "bwpp_xent_sums_r128_t01_u",
+    "bwpp_xent_sums_r128_t01",
+    "bwpp_xent_sums_r128_t01_u",
 };
 const int bwpp_hip_lm_kernel_count = (int)(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]));
 static_assert(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]) == LM_COUNT, "kernel names");
@@ -372,4 +416,342 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const 
   if (!gate_sum) a.part_gate = nullptr;
   if (!dpre_gamma && !dpost_gamma && !gate_sum) return BWPP_HIP_OK;
   return bwpp_hip_launch_lm(h, LM_RESNORM_FINISH + bf16, (C + 63) / 64, gate_sum ? 2u + (uint32_t)ngroups : 2u, 256, &a);
+}
+
+// ------------------------------------------- cross entropy, vocabulary in pieces
+
+namespace {
+
+enum XentTile { XT_P, XT_R32, XT_R32U, XT_R128, XT_R128U };
+struct XentShape {
+  uint32_t bm, bn, threads;
+};
+const XentShape kXentShapes[5] = {{256, 256, 512}, {32, 64, 128}, {32, 64, 128}, {128, 128, 256}, {128, 128, 256}};
+
+bool on16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+// The tile for a product A [M x K] op(B) [K x N] in the loops of gemm_bf16.h:
+// the DMA reads whole 16-byte chunks, the 256-wide tiles K in steps of 32.
+XentTile xent_tile(const BwppGemmArgs &g, bool tb, bool few_rows) {
+  const bool dma = on16(g.a) && on16(g.b) && g.lda % 8 == 0 && g.ldb % 8 == 0 && g.K % 8 == 0 && (tb || g.N % 8 == 0) &&
+                   256ull * std::max(g.lda, g.ldb) < (1ull << 31);
+  if (dma && g.K % 32 == 0 && g.M > 128) return XT_P;
+  if (few_rows && g.M <= 32) return dma ? XT_R32 : XT_R32U;
+  return dma ? XT_R128 : XT_R128U;
+}
+
+BwppHipStatus xent_product(BwppHip *h, int first, BwppXentArgs &a, bool tb, XentTile tile, uint32_t split) {
+  const XentShape &sh = kXentShapes[tile];
+  a.g.tiles_m = (uint32_t)((a.g.M + (uint64_t)sh.bm - 1) / sh.bm);
+  a.g.tiles_n = (uint32_t)((a.g.N + (uint64_t)sh.bn - 1) / sh.bn);
+  a.g.group_m = 8;
+  a.g.kchunk = split > 1 ? (uint32_t)up((a.g.K + (uint64_t)split - 1) / split, 128) : a.g.K;
+  split = (a.g.K + a.g.kchunk - 1) / a.g.kchunk;  // no empty range
+  a.g.ksplit = split;
+  const uint64_t tiles = (uint64_t)a.g.tiles_m * a.g.tiles_n;
+  if (tiles > 0xffffffffull)
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "linear_xent: too many tiles");
+  return bwpp_hip_launch_lm(h, first + (tb ? 5 : 0) + tile, tiles * split, 1, sh.threads, &a);
+}
+
+struct XentMatrices {
+  uint64_t ldx, ldw, lddx, lddw, wrows, wcols;
+};
+
+BwppHipStatus xent_prepare(BwppHip *h, const char *what, const BwppLinearXentParams &p, XentMatrices &m) {
+  auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
+  if (p.dtype > BWPP_HIP_BF16) return bad("unknown dtype");
+  if (p.vocab == 0 || p.dim == 0) return bad("empty vocabulary or dim");
+  if (!std::isfinite(p.scale)) return bad("scale must be finite");
+  m.wrows = p.trans_w ? p.vocab : p.dim;
+  m.wcols = p.trans_w ? p.dim : p.vocab;
+  m.ldx = p.ldx ? p.ldx : p.dim;
+  m.ldw = p.ldw ? p.ldw : m.wcols;
+  m.lddx = p.lddx ? p.lddx : p.dim;
+  m.lddw = p.lddw ? p.lddw : m.wcols;
+  if (m.ldx < p.dim || m.ldw < m.wcols || m.lddx < p.dim || m.lddw < m.wcols) return bad("row stride smaller than the row");
+  if (p.rows > 0x7fffffffu || p.vocab > 0x7fffffffu || p.dim > 0x7fffffffu)
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: a size of 2^31 or more", what);
+  if (p.dtype == BWPP_HIP_BF16 && (p.dim < 8 || (!p.trans_w && p.vocab < 8)))
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: bf16 rows of fewer than 8 elements", what);
+  return BWPP_HIP_OK;
+}
+
+// Columns of a piece: dz (bf16) or logits (fp32) of all rows in 256 MiB, which
+// the Infinity Cache holds between the products, in whole tiles; at least 1024.
+constexpr uint64_t kXentPiece = 256ull << 20;
+uint32_t xent_piece(uint64_t rows, uint64_t vocab, uint64_t es) {
+  uint64_t n = std::max<uint64_t>(kXentPiece / (std::max<uint64_t>(rows, 1) * es) / 256 * 256, 1024);
+  if (n >= vocab) return (uint32_t)vocab;
+  while (vocab % n != 0 && vocab % n < 8) n -= 256;  // a last piece has a whole 16-byte chunk
+  return (uint32_t)n;
+}
+
+uint32_t xent_grid(BwppHip *h, uint64_t rows) { return (uint32_t)std::min<uint64_t>(rows, 16ull * cus_of(h)); }
+
+// Ends the hold on the workspace on every way out.
+struct Hold {
+  BwppHip *h;
+  Hold(BwppHip *handle, size_t bytes) : h(handle) { bwpp_hip_hold_workspace(h, bytes); }
+  ~Hold() { bwpp_hip_hold_workspace(h, 0); }
+};
+// Room behind the held part for the fp32 products' K splits.
+constexpr size_t kXentSplitRoom = 64u << 20;
+
+// z (unscaled) of the vocabulary's columns n0 .. n0 + n, fp32.
+BwppHipStatus xent_logits_f32(BwppHip *h, const float *x, const float *w, float *z, uint32_t n0, uint32_t n,
+                              const BwppLinearXentParams &p, const XentMatrices &m) {
+  BwppMatmulParams g = {};
+  g.M = p.rows;
+  g.N = n;
+  g.K = p.dim;
+  g.lda = (uint32_t)m.ldx;
+  g.ldb = (uint32_t)m.ldw;
+  g.ldc = (uint32_t)up(n, 4);
+  g.trans_b = p.trans_w ? 1u : 0u;
+  return bwpp_hip_dispatch_matmul(h, x, w + (p.trans_w ? (uint64_t)n0 * m.ldw : n0), z, nullptr, g);
+}
+
+}  // namespace
+
+extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const void *w,
+                                                       const int32_t *targets, float *loss, float *lse, float *sums,
+                                                       BwppLinearXentParams p) {
+  const char *what = "linear_xent";
+  if (!x || !w || !targets || (!loss && !lse && !sums))
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: NULL x, w or targets, or no output", what);
+  XentMatrices m;
+  BwppHipStatus s = xent_prepare(h, what, p, m);
+  if (s != BWPP_HIP_OK) return s;
+  const uint64_t T = p.rows, es = p.dtype == BWPP_HIP_BF16 ? 2 : 4;
+  {
+    const Block in[3] = {{x, T, p.dim * es, m.ldx * es}, {w, m.wrows, m.wcols * es, m.ldw * es}, {targets, 1, T * 4, T * 4}};
+    const Block out[3] = {{loss, 1, T * 4, T * 4}, {lse, 1, T * 4, T * 4}, {sums, 1, 8, 8}};
+    for (int i = 0; i < 3; ++i) {
+      for (const Block &b : in)
+        if (meet(out[i], b, 1)) return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: an output overlaps an input", what);
+      for (int j = 0; j < i; ++j)
+        if (meet(out[i], out[j], 1)) return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: two outputs overlap", what);
+    }
+  }
+  if ((s = bwpp_hip_enter(h)) != BWPP_HIP_OK) return s;
+  BwppXentRowArgs r = {};
+  r.target = targets;
+  r.rows = p.rows;
+  r.vocab = p.vocab;
+  r.loss = loss;
+  r.lse = lse;
+  r.sums = sums;
+  r.scale = p.scale != 0.0f ? p.scale : 1.0f;
+  if (T == 0) return sums ? bwpp_hip_launch_lm(h, LM_XENT_SUMS, 1, 1, 1024, &r) : BWPP_HIP_OK;
+  // More rows than one block joins: the sums are taken from the losses.
+  const bool own_loss = sums && !loss && T > 64;
+  const uint64_t loss_bytes = own_loss ? up(T * 4, 256) : 0, zt_bytes = up(T * 4, 256);
+  void *ws = nullptr;
+  if (p.dtype == BWPP_HIP_BF16) {
+    BwppXentArgs a = {};
+    a.g.a = x;
+    a.g.b = w;
+    a.g.M = p.rows;
+    a.g.N = p.vocab;
+    a.g.K = p.dim;
+    a.g.lda = (uint32_t)m.ldx;
+    a.g.ldb = (uint32_t)m.ldw;
+    a.target = targets;
+    a.vocab = p.vocab;
+    a.scale = r.scale;
+    const XentTile tile = xent_tile(a.g, p.trans_w != 0, true);
+    r.nparts = (uint32_t)((p.vocab + (uint64_t)kXentShapes[tile].bn - 1) / kXentShapes[tile].bn);
+    if ((s = bwpp_hip_take_workspace(h, zt_bytes + loss_bytes + (uint64_t)r.nparts * T * 8, &ws)) != BWPP_HIP_OK) return s;
+    a.zt = static_cast<float *>(ws);
+    a.part = reinterpret_cast<float *>(static_cast<unsigned char *>(ws) + zt_bytes + loss_bytes);
+    r.zt = a.zt;
+    r.part = a.part;
+    if ((s = xent_product(h, LM_XENT_STATS, a, p.trans_w != 0, tile, 1)) != BWPP_HIP_OK) return s;
+  } else {
+    const uint32_t piece = xent_piece(T, p.vocab, 4);
+    const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece;
+    const uint64_t part_bytes = up(npieces * T * 8, 256), z_bytes = up(T * up(piece, 4) * 4, 256);
+    const uint64_t held = zt_bytes + loss_bytes + part_bytes + z_bytes;
+    if ((s = bwpp_hip_take_workspace(h, held + kXentSplitRoom, &ws)) != BWPP_HIP_OK) return s;
+    Hold hold(h, held);
+    unsigned char *base = static_cast<unsigned char *>(ws);
+    r.zt = reinterpret_cast<float *>(base);
+    float *part = reinterpret_cast<float *>(base + zt_bytes + loss_bytes);
+    float *z = reinterpret_cast<float *>(base + zt_bytes + loss_bytes + part_bytes);
+    for (uint64_t i = 0; i < npieces; ++i) {
+      const uint32_t n0 = (uint32_t)(i * piece), n = std::min(piece, p.vocab - n0);
+      if ((s = xent_logits_f32(h, static_cast<const float *>(x), static_cast<const float *>(w), z, n0, n, p, m)) != BWPP_HIP_OK)
+        return s;
+      r.src = z;
+      r.lds = up(n, 4);
+      r.cols = n;
+      r.n_base = n0;
+      r.part = part + i * T * 2;
+      if ((s = bwpp_hip_launch_lm(h, LM_XENT_STATS_F32, xent_grid(h, T), 1, 256, &r)) != BWPP_HIP_OK) return s;
+    }
+    r.part = part;
+    r.nparts = (uint32_t)npieces;
+  }
+  if (own_loss) r.loss = reinterpret_cast<float *>(static_cast<unsigned char *>(ws) + zt_bytes);
+  if ((s = bwpp_hip_launch_lm(h, LM_XENT_JOIN, (T + 63) / 64, 1, 1024, &r)) != BWPP_HIP_OK) return s;
+  return sums && T > 64 ? bwpp_hip_launch_lm(h, LM_XENT_SUMS, 1, 1, 1024, &r) : BWPP_HIP_OK;
+}
+
+extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const void *x, const void *w,
+                                                            const int32_t *targets, const float *lse,
+                                                            const float *dloss, void *dx, void *dw,
+                                                            BwppLinearXentParams p) {
+  const char *what = "linear_xent_grad";
+  if (!x || !w || !targets || !lse || (!dx && !dw))
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: NULL x, w, targets or lse, or no output", what);
+  XentMatrices m;
+  BwppHipStatus s = xent_prepare(h, what, p, m);
+  if (s != BWPP_HIP_OK) return s;
+  const bool bf16 = p.dtype == BWPP_HIP_BF16, tw = p.trans_w != 0;
+  const uint64_t T = p.rows, es = bf16 ? 2 : 4, D = p.dim;
+  {
+    const uint64_t nd = p.dloss_scalar ? 4 : T * 4;
+    const Block in[5] = {{x, T, D * es, m.ldx * es}, {w, m.wrows, m.wcols * es, m.ldw * es}, {targets, 1, T * 4, T * 4},
+                         {lse, 1, T * 4, T * 4}, {dloss, 1, nd, nd}};
+    const Block out[2] = {{dx, T, D * es, m.lddx * es}, {dw, m.wrows, m.wcols * es, m.lddw * es}};
+    for (const Block &o : out)
+      for (const Block &b : in)
+        if (meet(o, b, 1)) return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: an output overlaps an input", what);
+    if (meet(out[0], out[1], 1)) return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: dx overlaps dw", what);
+  }
+  if ((s = bwpp_hip_enter(h)) != BWPP_HIP_OK) return s;
+  BwppXentRowArgs r = {};
+  r.target = targets;
+  r.rows = p.rows;
+  r.vocab = p.vocab;
+  r.scale = p.scale != 0.0f ? p.scale : 1.0f;
+  r.dloss = dloss;
+  r.dloss_scalar = p.dloss_scalar;
+  r.lse_in = lse;
+  if (T == 0) {
+    if (!dw) return BWPP_HIP_OK;
+    r.y = dw;
+    r.rows = (uint32_t)m.wrows;
+    r.cols = (uint32_t)std::min<uint64_t>(m.wcols * es, 0xffffffffull);
+    if (m.wcols * es > 0xffffffffull) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: rows too long", what);
+    r.ldy = m.lddw * es;
+    return bwpp_hip_launch_lm(h, LM_XENT_CLEAR, xent_grid(h, m.wrows), 1, 256, &r);
+  }
+  // bf16 with several pieces: dx is summed in fp32, over planes of K ranges
+  // where its tiles alone would leave CUs idle.
+  const uint32_t piece = xent_piece(T, p.vocab, es);
+  const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece;
+  const bool sums = bf16 && dx && npieces > 1;
+  uint32_t split = 1;
+  if (sums) {
+    const uint64_t tiles = ((T + 255) / 256) * ((D + 255) / 256);
+    while (split < 8 && tiles * split * 2 <= cus_of(h) && piece / (split * 2) >= 512) split *= 2;
+    const uint32_t range = (uint32_t)up((piece + split - 1) / split, 128);  // as xent_product cuts the first piece
+    split = (piece + range - 1) / range;
+  }
+  const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit);
+  const uint64_t x_bytes = dw ? up(T * ldxc * es, 256) : 0, z_bytes = up(T * ldz * es, 256);
+  const uint64_t sum_bytes = sums ? up(split * T * D * 4, 256) : 0, held = x_bytes + z_bytes + sum_bytes;
+  void *ws = nullptr;
+  if ((s = bwpp_hip_take_workspace(h, held + (bf16 ? 0 : kXentSplitRoom), &ws)) != BWPP_HIP_OK) return s;
+  Hold hold(h, held);
+  unsigned char *base = static_cast<unsigned char *>(ws);
+  void *xc = base, *z = base + x_bytes;
+  float *acc = reinterpret_cast<float *>(base + x_bytes + z_bytes);
+  auto at = [&](const void *ptr, uint64_t elems) {
+    return static_cast<const unsigned char *>(ptr) + elems * es;
+  };
+  if (dw) {
+    r.x = x;
+    r.y = xc;
+    r.ldx = m.ldx;
+    r.ldy = ldxc;
+    r.cols = p.dim;
+    if ((s = bwpp_hip_launch_lm(h, LM_XENT_COPY + bf16, xent_grid(h, T), 1, 256, &r)) != BWPP_HIP_OK) return s;
+  }
+  for (uint64_t i = 0; i < npieces; ++i) {
+    const uint32_t n0 = (uint32_t)(i * piece), n = std::min(piece, p.vocab - n0);
+    const uint64_t ldp = up(n, unit);
+    const void *wp = at(w, tw ? n0 * m.ldw : n0);
+    if (bf16) {
+      BwppXentArgs a = {};
+      a.g.a = x;
+      a.g.b = wp;
+      a.g.M = p.rows;
+      a.g.N = n;
+      a.g.K = p.dim;
+      a.g.lda = (uint32_t)m.ldx;
+      a.g.ldb = (uint32_t)m.ldw;
+      a.target = targets;
+      a.lse = lse;
+      a.dloss = dloss;
+      a.dloss_scalar = p.dloss_scalar;
+      a.n_base = n0;
+      a.vocab = p.vocab;
+      a.scale = r.scale;
+      a.dl = static_cast<uint16_t *>(z);
+      a.ldl = (uint32_t)ldp;
+      if ((s = xent_product(h, LM_XENT_GRAD, a, tw, xent_tile(a.g, tw, true), 1)) != BWPP_HIP_OK) return s;
+    } else {
+      if ((s = xent_logits_f32(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(z), n0,
+                               n, p, m)) != BWPP_HIP_OK)
+        return s;
+      r.y = z;
+      r.ldy = ldp;
+      r.cols = n;
+      r.n_base = n0;
+      if ((s = bwpp_hip_launch_lm(h, LM_XENT_GRAD_F32, xent_grid(h, T), 1, 256, &r)) != BWPP_HIP_OK) return s;
+    }
+    if (dx && sums) {
+      BwppXentArgs a = {};
+      a.g.a = z;
+      a.g.b = wp;
+      a.g.M = p.rows;
+      a.g.N = p.dim;
+      a.g.K = n;
+      a.g.lda = (uint32_t)ldp;
+      a.g.ldb = (uint32_t)m.ldw;
+      a.raw = acc;
+      a.accumulate = i > 0;
+      if ((s = xent_product(h, LM_XENT_RAW, a, !tw, xent_tile(a.g, !tw, false), split)) != BWPP_HIP_OK) return s;
+    } else if (dx) {
+      BwppMatmulParams g = {};
+      g.M = p.rows;
+      g.N = p.dim;
+      g.K = n;
+      g.lda = (uint32_t)ldp;
+      g.ldb = (uint32_t)m.ldw;
+      g.ldc = (uint32_t)m.lddx;
+      g.dtype = p.dtype;
+      g.trans_b = tw ? 0u : 1u;
+      BwppHipFusionParams f = {};
+      f.kind = i > 0 ? BWPP_HIP_FUSE_RESIDUAL : BWPP_HIP_FUSE_NONE;
+      f.ld_aux = g.ldc;
+      s = bwpp_hip_dispatch_matmul_fused(h, z, wp, dx, nullptr, i > 0 ? static_cast<const float *>(dx) : nullptr, nullptr, g, f);
+      if (s != BWPP_HIP_OK) return s;
+    }
+    if (dw) {
+      BwppMatmulParams g = {};
+      g.K = p.rows;
+      g.M = tw ? n : p.dim;
+      g.N = tw ? p.dim : n;
+      g.lda = (uint32_t)(tw ? ldp : ldxc);
+      g.ldb = (uint32_t)(tw ? ldxc : ldp);
+      g.ldc = (uint32_t)m.lddw;
+      g.dtype = p.dtype;
+      g.trans_a = 1;
+      void *dwp = const_cast<unsigned char *>(at(dw, tw ? n0 * m.lddw : n0));
+      if ((s = bwpp_hip_dispatch_matmul(h, tw ? z : xc, tw ? xc : z, dwp, nullptr, g)) != BWPP_HIP_OK) return s;
+    }
+  }
+  if (!dx) return BWPP_HIP_OK;
+  r.y = dx;
+  r.ldy = m.lddx;
+  r.cols = p.dim;
+  if (!sums) return bwpp_hip_launch_lm(h, LM_XENT_ZERO + bf16, xent_grid(h, T), 1, 256, &r);
+  r.src = acc;
+  r.nparts = split;
+  return bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, T), 1, 256, &r);
 }

@@ -77,3 +77,8 @@ BwppHipStatus bwpp_hip_take_workspace(BwppHip *h, size_t bytes, void **p);
 // when their row strides are equal, by byte range otherwise.
 bool bwpp_hip_blocks_overlap(const void *pa, uint64_t ra, uint64_t ca, uint64_t lda, const void *pb, uint64_t rb,
                              uint64_t cb, uint64_t ldb, uint64_t es);
+
+// Keeps the first `bytes` of the workspace for the caller while it runs other
+// operators of the library (matrix products), which then split through what
+// lies behind them and never move the workspace.  0 ends it.
+void bwpp_hip_hold_workspace(BwppHip *h, size_t bytes);

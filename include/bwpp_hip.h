@@ -227,6 +227,21 @@ typedef struct {
   uint32_t dtype;     /* BwppHipDType of every operand, 0 = F32 */
 } BwppResidualNormParams;
 
+/* Cross entropy of hidden states x [rows x dim] against a vocabulary, logits
+ * z = scale x W, W [dim x vocab] (trans_w: stored [vocab x dim]), without the
+ * logits in memory (no reference counterpart; its compiler has no loss). */
+typedef struct {
+  uint32_t rows; /* tokens */
+  uint32_t vocab;
+  uint32_t dim;
+  uint32_t ldx, ldw;   /* row strides of the stored matrices; 0 = contiguous */
+  uint32_t lddx, lddw; /* of the gradients (dW is stored as W is) */
+  uint32_t trans_w;
+  uint32_t dtype;        /* BwppHipDType of x, W and their gradients, 0 = F32 */
+  uint32_t dloss_scalar; /* the upstream gradient is one value for all rows */
+  float scale;           /* 0 = 1 */
+} BwppLinearXentParams;
+
 typedef struct BwppHip BwppHip;
 
 /* ---- handle ---- */
@@ -625,6 +640,28 @@ BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const void *o, co
                                                    const void *gate, const void *pre_gamma, const void *dr,
                                                    const void *dy, void *dx, void *dout, void *dpost_gamma,
                                                    void *dgate, void *dpre_gamma, BwppResidualNormParams params);
+
+/* loss[t] = lse[t] - z[t][targets[t]], lse[t] = log sum_v exp z[t][v] (natural,
+ * fp32) for the logits of BwppLinearXentParams.  A target outside [0, vocab)
+ * leaves its row out (loss 0, no gradient; its lse is still written).  sums
+ * (may be NULL): [0] the sum of the losses, [1] how many rows count.  loss and
+ * lse may be NULL, not all three.  bf16 needs dim >= 8 (and, W not transposed,
+ * vocab >= 8).  Workspace: a pair of floats per row and 64 to 256 columns of
+ * the vocabulary (fp32: the logits of a piece of it, 256 MiB or 1024 columns). */
+BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const void *w, const int32_t *targets,
+                                            float *loss, float *lse, float *sums, BwppLinearXentParams params);
+
+/* Its gradients dx and dw (either may be NULL) for the upstream gradient dloss
+ * of the row losses ([rows], one value with dloss_scalar, NULL = 1) and the
+ * forward's lse.  The logits are made again, a piece of the vocabulary at a
+ * time; bf16 rounds each dz to bf16 for the products that give dx and dw,
+ * whose sums are fp32.  dx rows of left-out tokens are 0, and their x (which
+ * may hold anything) has no part in dw.  Outputs must not meet inputs or each
+ * other (ALIAS).  Workspace: a copy of x, dz of a piece (256 MiB or 1024
+ * columns) and, with more than one piece in bf16, fp32 sums of dx. */
+BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const void *x, const void *w, const int32_t *targets,
+                                                 const float *lse, const float *dloss, void *dx, void *dw,
+                                                 BwppLinearXentParams params);
 
 /* ---- launch plans (compiled graphs) ----
  *

@@ -123,3 +123,42 @@ def test_residual_norm_grad_refusals():
     for kw in (dict(dx=C), dict(dx=None, dout=None, dpre=G), dict(dr=None), dict(dy=None)):
         st, msg = call(**kw)
         assert st == S.INVALID_ARG and "residual_norm_grad" not in msg, kw
+
+
+def _xent(**kw):
+    d = dict(rows=8, vocab=100, dim=64, trans_w=1)
+    d.update(kw)
+    return bwpp.LinearXentParams(**d)
+
+
+def test_linear_xent_refusals():
+    assert ctypes.sizeof(bwpp.LinearXentParams) == 44
+    ok = (A, B, C, D, E, F)
+    for i in (0, 1, 2):
+        args = list(ok)
+        args[i] = None
+        assert _lib_call("linear_xent", *args, _xent())[0] == S.INVALID_ARG
+    assert _lib_call("linear_xent", A, B, C, None, None, None, _xent())[0] == S.INVALID_ARG
+    for kw in (dict(dtype=2), dict(vocab=0), dict(dim=0), dict(ldx=63), dict(ldw=63), dict(trans_w=0, ldw=99),
+               dict(scale=float("nan")), dict(scale=float("inf"))):
+        for name, args in (("linear_xent", ok), ("linear_xent_grad", (A, B, C, D, None, E, F))):
+            st, msg = _lib_call(name, *args, _xent(**kw))
+            assert st == S.INVALID_ARG and name in msg, kw
+    for kw in (dict(dtype=1, dim=7), dict(dtype=1, trans_w=0, vocab=7), dict(rows=1 << 31), dict(vocab=1 << 31)):
+        assert _lib_call("linear_xent", *ok, _xent(**kw))[0] == S.UNSUPPORTED, kw
+    for args in ((A, B, C, A, E, F), (A, B, C, D, D, F), (A, B, C, D, E, E + 28), (A, B, C, C + 4, E, F)):
+        assert _lib_call("linear_xent", *args, _xent())[0] == S.ALIAS, args
+    st, msg = _lib_call("linear_xent", *ok, _xent())
+    assert st == S.INVALID_ARG and "linear_xent" not in msg  # only the handle is missing
+
+
+def test_linear_xent_grad_refusals():
+    for args in ((None, B, C, D, None, E, F), (A, None, C, D, None, E, F), (A, B, None, D, None, E, F),
+                 (A, B, C, None, None, E, F), (A, B, C, D, None, None, None)):
+        assert _lib_call("linear_xent_grad", *args, _xent())[0] == S.INVALID_ARG
+    G = 7 * 0x100000000
+    for args in ((A, B, C, D, None, A, F), (A, B, C, D, None, E, B + 4), (A, B, C, D, G, G, F), (A, B, C, D, None, E, E),
+                 (A, B, C, D, None, E, D)):
+        assert _lib_call("linear_xent_grad", *args, _xent())[0] == S.ALIAS, args
+    st, msg = _lib_call("linear_xent_grad", A, B, C, D, G, E, F, _xent(lddx=70, lddw=65))
+    assert st == S.INVALID_ARG and "linear_xent" not in msg
