@@ -185,16 +185,18 @@ typedef struct {
   void *ro, *y;                     /* forward outputs */
   const void *dr, *dy;              /* upstream gradients, either NULL = 0 */
   void *dx, *dout, *dpost, *dgate, *dpre;
-  float *part_pre, *part_post, *part_gate; /* [workers][cols] sums (NULL: not asked for) */
+  float *part_pre, *part_post, *part_gate; /* [nparts][cols] sums (NULL: not asked for) */
   uint64_t ldx, ldo, ldy, ldg;
   uint32_t rows, cols;
   uint32_t gate_rows; /* rows per gate row (0: one gate row) */
   uint32_t post_norm;
   float eps, stream_scale, branch_scale;
-  /* gradient: workers (blocks, or waves of blocks that hold a row each) take
-   * `span` rows of a group of `group` rows (split > 1 workers a group, whose
-   * gate sums go to part_gate), or whole groups of them (split = 1) */
-  uint32_t workers, group, split, span;
+  /* gradient: a group is the rows of one row of dgate.  split > 1: that many
+   * blocks a group take `span` of its rows each, their gate sums go to
+   * part_gate; split = 1: workers (blocks, or waves of blocks where a wave
+   * holds a row) take `span` rows each, whole groups.  nparts: blocks, one row
+   * of partial sums each. */
+  uint32_t workers, group, split, span, nparts;
 } BwppResNormArgs;
 
 /* Cross entropy of hidden states against a vocabulary (xent.hip).  Logits
@@ -209,9 +211,10 @@ typedef struct {
   uint32_t n_base;
   uint32_t vocab;
   float scale;
-  float *part; /* forward: [tiles_n][M] pairs (max, sum of exp(z - max)) */
+  float *part; /* forward: [tiles][M] pairs (max, sum of exp(z - max)), ... */
+  uint32_t part_base; /* ... of this launch from here */
   float *zt;   /* forward: [M] target logits */
-  uint16_t *dl; /* gradient: dz scale, [M][ldl] bf16 */
+  uint16_t *dl; /* gradient: dz scale, [M][ldl] bf16, ldl a multiple of 8 */
   uint32_t ldl;
   uint32_t accumulate; /* sums: add to what is there */
   float *raw;          /* sums: [ksplit][M][N] */

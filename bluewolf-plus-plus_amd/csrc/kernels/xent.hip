@@ -93,7 +93,7 @@ struct EpiStats {
         const float2 q = pair[tid * WN + w];
         join(p.x, p.y, q.x, q.y);
       }
-      reinterpret_cast<float2 *>(a.part)[(size_t)tn * a.g.M + m0 + (uint32_t)tid] = p;
+      reinterpret_cast<float2 *>(a.part)[(size_t)(a.part_base + tn) * a.g.M + m0 + (uint32_t)tid] = p;
     }
   }
 };
@@ -141,13 +141,13 @@ struct EpiGrad {
         }
     }
     __syncthreads();
-    // ldl is a multiple of 8: whole chunks, columns past N with the values of
-    // the columns that were read again (inside the row, never used).
+    // Whole chunks: the last one's columns past N, which the row has room for,
+    // get values of columns that were read again, and are never used.
 #pragma unroll 4
     for (int it = 0; it < BM * (BN / 8) / NT; ++it) {
       const int q = tid + it * NT, row = q / (BN / 8), c = q % (BN / 8);
       const uint32_t m = m0 + (uint32_t)row, n = n0 + 8u * (uint32_t)c;
-      if (m < a.g.M && n < a.ldl)
+      if (m < a.g.M && n < a.g.N)
         *reinterpret_cast<uint4 *>(a.dl + (size_t)m * a.ldl + n) = *reinterpret_cast<const uint4 *>(cs + row * kCld + c * 8);
     }
   }

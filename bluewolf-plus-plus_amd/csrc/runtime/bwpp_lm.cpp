@@ -17,7 +17,7 @@ enum LmKernel {
   LM_ROTARY_F32 = LM_ROTARY_BF16 + 6,  // [interleaved][chunk 4, 1]
   LM_RESNORM = LM_ROTARY_F32 + 4,      // [bf16][kResCfgs, any]
   LM_RESNORM_GRAD = LM_RESNORM + 14,   // [bf16][kResCfgs - 1, any]
-  LM_RESNORM_FINISH = LM_RESNORM_GRAD + 12,  // [bf16]
+  LM_RESNORM_FINISH = LM_RESNORM_GRAD + 14,  // [bf16]
   LM_XENT_JOIN = LM_RESNORM_FINISH + 2,
   LM_XENT_SUMS,
   LM_XENT_STATS_F32,
@@ -36,8 +36,9 @@ enum LmKernel {
 struct ResCfg {
   uint32_t elems, waves;
 };
-constexpr int kResNCfg = 6, kResGradNCfg = 5;
+constexpr int kResNCfg = 6, kResGradNCfg = 6;
 const ResCfg kResCfgs[kResNCfg] = {{8, 1}, {8, 2}, {8, 4}, {8, 8}, {8, 16}, {16, 16}};
+const ResCfg kResGradCfgs[kResGradNCfg] = {{8, 1}, {16, 1}, {16, 2}, {16, 4}, {8, 8}, {16, 8}};
 constexpr uint32_t kResAnyThreads = 512;
 
 }  // namespace
@@ -51,10 +52,12 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_resnorm_f32_n16_w16",     "bwpp_resnorm_f32_any",         "bwpp_resnorm_bf16_n8_w1",
     "bwpp_resnorm_bf16_n8_w2",      "bwpp_resnorm_bf16_n8_w4",      "bwpp_resnorm_bf16_n8_w8",
     "bwpp_resnorm_bf16_n8_w16",     "bwpp_resnorm_bf16_n16_w16",    "bwpp_resnorm_bf16_any",
-    "bwpp_resnorm_grad_f32_n8_w1",  "bwpp_resnorm_grad_f32_n8_w2",  "bwpp_resnorm_grad_f32_n8_w4",
-    "bwpp_resnorm_grad_f32_n8_w8",  "bwpp_resnorm_grad_f32_n8_w16", "bwpp_resnorm_grad_f32_any",
-    "bwpp_resnorm_grad_bf16_n8_w1", "bwpp_resnorm_grad_bf16_n8_w2", "bwpp_resnorm_grad_bf16_n8_w4",
-    "bwpp_resnorm_grad_bf16_n8_w8", "bwpp_resnorm_grad_bf16_n8_w16", "bwpp_resnorm_grad_bf16_any",
+    "bwpp_resnorm_grad_f32_n8_w1", "bwpp_resnorm_grad_f32_n16_w1", "bwpp_resnorm_grad_f32_n16_w2",
+    "bwpp_resnorm_grad_f32_n16_w4", "bwpp_resnorm_grad_f32_n8_w8", "bwpp_resnorm_grad_f32_n16_w8",
+    "bwpp_resnorm_grad_f32_any",
+    "bwpp_resnorm_grad_bf16_n8_w1", "bwpp_resnorm_grad_bf16_n16_w1", "bwpp_resnorm_grad_bf16_n16_w2",
+    "bwpp_resnorm_grad_bf16_n16_w4", "bwpp_resnorm_grad_bf16_n8_w8", "bwpp_resnorm_grad_bf16_n16_w8",
+    "bwpp_resnorm_grad_bf16_any",
     "bwpp_resnorm_finish_f32",      "bwpp_resnorm_finish_bf16",
     "bwpp_xent_join", "bwpp_xent_sums", "bwpp_xent_stats_f32", "bwpp_xent_grad_f32",
     "bwpp_xent_round_bf16", "bwpp_xent_clear", "bwpp_xent_copy_f32", "bwpp_xent_copy_bf16",
@@ -269,10 +272,12 @@ BwppHipStatus resnorm_prepare(BwppHip *h, const char *what, const BwppResidualNo
   return BWPP_HIP_OK;
 }
 
-// Smallest layout whose threads hold a row, or -1: a block reads it again.
-int res_cfg(uint32_t cols, int n) {
+// Smallest layout whose threads hold a row, or -1: a block reads it again
+// (as it does rows shorter than a chunk).
+int res_cfg(uint32_t cols, const ResCfg *cfgs, int n) {
+  if (cols < 8) return -1;
   for (int i = 0; i < n; ++i)
-    if (64u * kResCfgs[i].elems * kResCfgs[i].waves >= cols) return i;
+    if (64u * cfgs[i].elems * cfgs[i].waves >= cols) return i;
   return -1;
 }
 
@@ -321,7 +326,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm(BwppHip *h, const void 
   a.pre = pre_gamma;
   a.ro = r;
   a.y = y;
-  const int c = res_cfg(p.cols, kResNCfg), bf16 = p.dtype == BWPP_HIP_BF16;
+  const int c = res_cfg(p.cols, kResCfgs, kResNCfg), bf16 = p.dtype == BWPP_HIP_BF16;
   const uint32_t waves = c >= 0 ? kResCfgs[c].waves : 8u, rpb = waves == 1 ? 4u : 1u;
   // Blocks that keep the weights in registers over several rows.
   const uint64_t cap = (uint64_t)cus_of(h) * (waves >= 16 ? 2u : waves >= 8 ? 4u : 8u);
@@ -372,50 +377,50 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const 
   a.dpost = dpost_gamma;
   a.dgate = dgate;
   a.dpre = dpre_gamma;
-  const int c = res_cfg(p.cols, kResGradNCfg), bf16 = p.dtype == BWPP_HIP_BF16;
-  const uint32_t waves = c >= 0 ? kResCfgs[c].waves : 8u, rpb = waves == 1 ? 4u : 1u;
-  // Workers: about one block a CU of the longest rows, more of shorter ones;
-  // each leaves a partial row of every weight gradient.  A group is what one
-  // row of dgate sums over; it is split over workers or a worker takes several.
-  const uint64_t target = (uint64_t)cus_of(h) * (waves >= 8 ? 1u : waves >= 2 ? 8u / waves : 8u);
+  const int c = res_cfg(p.cols, kResGradCfgs, kResGradNCfg), bf16 = p.dtype == BWPP_HIP_BF16;
+  const uint32_t waves = c >= 0 ? kResGradCfgs[c].waves : 8u, rpb = waves == 1 ? 4u : 1u;
+  // About `target` blocks, each of which leaves a partial row of every weight
+  // gradient.  A group is what one row of dgate sums over; it is split over
+  // blocks, or a worker takes whole groups.
+  const uint64_t target = (uint64_t)cus_of(h) * (waves >= 8 ? 1u : waves >= 2 ? 8u / waves : bf16 ? 2u : 1u);
   const uint64_t group = dgate && p.gate_rows ? std::min<uint64_t>(p.gate_rows, std::max<uint64_t>(R, 1)) : std::max<uint64_t>(R, 1);
   const uint64_t ngroups = std::max<uint64_t>(1, (R + group - 1) / group);
-  uint64_t split = 1, span;
+  uint64_t split = 1, span, blocks;
   if (ngroups < target) {
-    split = std::min<uint64_t>((target + ngroups - 1) / ngroups, std::max<uint64_t>(1, group));
+    split = std::min<uint64_t>((target + ngroups - 1) / ngroups, std::max<uint64_t>(1, group / rpb));
     span = (group + split - 1) / split;
     split = (group + span - 1) / span;
   }
-  uint64_t workers;
   if (split > 1) {
-    workers = ngroups * split;
+    a.workers = (uint32_t)(blocks = ngroups * split);
   } else {
-    const uint64_t per = std::max<uint64_t>(1, (ngroups + target - 1) / target);
+    const uint64_t per = std::max<uint64_t>(1, (ngroups + target * rpb - 1) / (target * rpb));
     span = per * group;
-    workers = (ngroups + per - 1) / per;
+    a.workers = (uint32_t)((ngroups + per - 1) / per);
+    blocks = (a.workers + rpb - 1) / rpb;
   }
   if (span > 0xffffffffull) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: too many rows", what);
   a.group = (uint32_t)group;
   a.split = (uint32_t)split;
   a.span = (uint32_t)span;
-  a.workers = (uint32_t)workers;
+  a.nparts = (uint32_t)blocks;
   const bool gate_part = dgate && (split > 1 || c < 0 || R == 0);
   const uint64_t nparts = (dpre_gamma ? 1 : 0) + (dpost_gamma ? 1 : 0) + (gate_part ? 1 : 0);
   if (nparts) {
     void *ws = nullptr;
-    if ((s = bwpp_hip_take_workspace(h, nparts * workers * C * sizeof(float), &ws)) != BWPP_HIP_OK) return s;
+    if ((s = bwpp_hip_take_workspace(h, nparts * blocks * C * sizeof(float), &ws)) != BWPP_HIP_OK) return s;
     float *f = static_cast<float *>(ws);
-    if (dpre_gamma) a.part_pre = f, f += workers * C;
-    if (dpost_gamma) a.part_post = f, f += workers * C;
+    if (dpre_gamma) a.part_pre = f, f += blocks * C;
+    if (dpost_gamma) a.part_post = f, f += blocks * C;
     if (gate_part) a.part_gate = f;
   }
   s = bwpp_hip_launch_lm(h, LM_RESNORM_GRAD + bf16 * (kResGradNCfg + 1) + (c >= 0 ? c : kResGradNCfg),
-                         (workers + rpb - 1) / rpb, 1, c < 0 ? kResAnyThreads : waves == 1 ? 256u : 64u * waves, &a);
+                         blocks, 1, c < 0 ? kResAnyThreads : waves == 1 ? 256u : 64u * waves, &a);
   if (s != BWPP_HIP_OK || !nparts) return s;
   const bool gate_sum = gate_part && (split > 1 || R == 0);
   if (!gate_sum) a.part_gate = nullptr;
   if (!dpre_gamma && !dpost_gamma && !gate_sum) return BWPP_HIP_OK;
-  return bwpp_hip_launch_lm(h, LM_RESNORM_FINISH + bf16, (C + 63) / 64, gate_sum ? 2u + (uint32_t)ngroups : 2u, 256, &a);
+  return bwpp_hip_launch_lm(h, LM_RESNORM_FINISH + bf16, (C + 63) / 64, gate_sum ? 2u + (uint32_t)ngroups : 2u, 1024, &a);
 }
 
 // ------------------------------------------- cross entropy, vocabulary in pieces
@@ -453,6 +458,37 @@ BwppHipStatus xent_product(BwppHip *h, int first, BwppXentArgs &a, bool tb, Xent
   if (tiles > 0xffffffffull)
     return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "linear_xent: too many tiles");
   return bwpp_hip_launch_lm(h, first + (tb ? 5 : 0) + tile, tiles * split, 1, sh.threads, &a);
+}
+
+// Columns of a product on 256-wide tiles that smaller ones take instead: where
+// the last round of tiles would leave half of the CUs idle or more, its tile
+// columns (128 x 128 tiles, four for one, finish it in 0.4 to 0.7 of a round's
+// time: 2048 tokens x 4096 x 50001, 6.1 rounds, 790 -> 739 us).
+uint32_t xent_main_columns(const BwppHip *h, const BwppGemmArgs &g, XentTile tile) {
+  const uint64_t tm = (g.M + 255ull) / 256, tn = (g.N + 255ull) / 256, cus = cus_of(h);
+  if (tile != XT_P || tm * tn <= cus) return g.N;
+  const uint64_t left = tm * tn % cus, columns = (left + tm - 1) / tm;
+  return left == 0 || columns * tm * 2 > cus || columns >= tn ? g.N : (uint32_t)((tn - columns) * 256);
+}
+
+// The logits' product with the statistics' or the gradient's epilogue, in one
+// launch or two.
+uint32_t xent_tiles_n(const BwppHip *h, const BwppGemmArgs &g, XentTile tile) {
+  const uint32_t n = xent_main_columns(h, g, tile);
+  const uint32_t bn = kXentShapes[tile].bn;
+  return (uint32_t)((n + (uint64_t)bn - 1) / bn) + (uint32_t)((g.N - n + 127ull) / 128);
+}
+BwppHipStatus xent_logits(BwppHip *h, int first, BwppXentArgs a, bool tb, XentTile tile) {
+  const uint32_t n = xent_main_columns(h, a.g, tile), rest = a.g.N - n;
+  a.g.N = n;
+  const BwppHipStatus s = xent_product(h, first, a, tb, tile, 1);
+  if (s != BWPP_HIP_OK || rest == 0) return s;
+  a.part_base = a.g.tiles_n;
+  a.g.b = static_cast<const uint16_t *>(a.g.b) + (tb ? (uint64_t)n * a.g.ldb : n);
+  a.n_base += n;
+  if (a.dl) a.dl += n;
+  a.g.N = rest;
+  return xent_product(h, first, a, tb, XT_R128, 1);
 }
 
 struct XentMatrices {
@@ -562,13 +598,13 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x
     a.vocab = p.vocab;
     a.scale = r.scale;
     const XentTile tile = xent_tile(a.g, p.trans_w != 0, true);
-    r.nparts = (uint32_t)((p.vocab + (uint64_t)kXentShapes[tile].bn - 1) / kXentShapes[tile].bn);
+    r.nparts = xent_tiles_n(h, a.g, tile);
     if ((s = bwpp_hip_take_workspace(h, zt_bytes + loss_bytes + (uint64_t)r.nparts * T * 8, &ws)) != BWPP_HIP_OK) return s;
     a.zt = static_cast<float *>(ws);
     a.part = reinterpret_cast<float *>(static_cast<unsigned char *>(ws) + zt_bytes + loss_bytes);
     r.zt = a.zt;
     r.part = a.part;
-    if ((s = xent_product(h, LM_XENT_STATS, a, p.trans_w != 0, tile, 1)) != BWPP_HIP_OK) return s;
+    if ((s = xent_logits(h, LM_XENT_STATS, a, p.trans_w != 0, tile)) != BWPP_HIP_OK) return s;
   } else {
     const uint32_t piece = xent_piece(T, p.vocab, 4);
     const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece;
@@ -639,18 +675,19 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     r.ldy = m.lddw * es;
     return bwpp_hip_launch_lm(h, LM_XENT_CLEAR, xent_grid(h, m.wrows), 1, 256, &r);
   }
-  // bf16 with several pieces: dx is summed in fp32, over planes of K ranges
-  // where its tiles alone would leave CUs idle.
+  // bf16: dx is summed in fp32 over several pieces, and in planes of K ranges
+  // where its 256-wide tiles alone would leave half of the CUs idle (4096 x 2048
+  // from 32768 columns: 645 us as one product on smaller tiles, 515 so).
   const uint32_t piece = xent_piece(T, p.vocab, es);
-  const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece;
-  const bool sums = bf16 && dx && npieces > 1;
+  const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece, dx_tiles = ((T + 255) / 256) * ((D + 255) / 256);
   uint32_t split = 1;
-  if (sums) {
-    const uint64_t tiles = ((T + 255) / 256) * ((D + 255) / 256);
-    while (split < 8 && tiles * split * 2 <= cus_of(h) && piece / (split * 2) >= 512) split *= 2;
+  if (bf16 && dx && T > 128) {
+    while (split < 8 && dx_tiles * split * 2 <= cus_of(h) && piece / (split * 2) >= 2048) split *= 2;
     const uint32_t range = (uint32_t)up((piece + split - 1) / split, 128);  // as xent_product cuts the first piece
     split = (piece + range - 1) / range;
   }
+  const bool sums = bf16 && dx && (npieces > 1 || (split > 1 && dx_tiles * split >= 128));
+  if (!sums) split = 1;
   const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit);
   const uint64_t x_bytes = dw ? up(T * ldxc * es, 256) : 0, z_bytes = up(T * ldz * es, 256);
   const uint64_t sum_bytes = sums ? up(split * T * D * 4, 256) : 0, held = x_bytes + z_bytes + sum_bytes;
@@ -693,7 +730,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.scale = r.scale;
       a.dl = static_cast<uint16_t *>(z);
       a.ldl = (uint32_t)ldp;
-      if ((s = xent_product(h, LM_XENT_GRAD, a, tw, xent_tile(a.g, tw, true), 1)) != BWPP_HIP_OK) return s;
+      if ((s = xent_logits(h, LM_XENT_GRAD, a, tw, xent_tile(a.g, tw, true))) != BWPP_HIP_OK) return s;
     } else {
       if ((s = xent_logits_f32(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(z), n0,
                                n, p, m)) != BWPP_HIP_OK)

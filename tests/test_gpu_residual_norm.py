@@ -16,6 +16,13 @@ import bwpp
 from lm64 import HALF_STEP, resnorm64, resnorm_grad64, strided, untouched
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(1234)
+
+
 F32, BF16 = torch.float32, torch.bfloat16
 U = 2.0 ** -24
 EPS = 1e-6

@@ -11,6 +11,13 @@ import bwpp
 from lm64 import HALF_STEP, rotary64, strided, untouched
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(1234)
+
+
 F32, BF16 = torch.float32, torch.bfloat16
 PARTS = dict(scaling=2, factor=16.0, context=8192, low_turns=1.0, high_turns=32.0, magnitude=1.25)
 
