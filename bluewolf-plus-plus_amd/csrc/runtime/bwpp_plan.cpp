@@ -13,7 +13,8 @@
 // Text format (one statement per line, '#' starts a comment):
 //   bwpp.plan 1
 //   dim NAME EXPR                     EXPR: product of integers / dims, e.g. B*T
-//   value NAME f32 [EXPR,...] KIND    KIND: input | param | temp | output | const=<float>
+//   value NAME DTYPE [EXPR,...] KIND  DTYPE: f32 | bf16 | i32 (input or param only);
+//                                     KIND: input | param | temp | output | const=<float>
 //   view NAME of=BASE offset=EXPR ld=EXPR shape=[EXPR,EXPR]
 //   op KIND out=A[,B..] in=X[,Y..] [key=value ...]
 // Op kinds: matmul (ta, tb, epi, fuse), softmax, rmsnorm, layernorm,
@@ -21,7 +22,17 @@
 // in/out pairs, one launch), reduce_sum, reduce_max,
 // reduce_max_mask (axis), mean_square, silu_grad, softmax_grad,
 // rmsnorm_grad, attention, attention_grad (batch, heads, causal, scale,
-// layout).
+// layout); and, with optional operands named in order by with= (inputs behind
+// the fixed ones) and gives= (outputs):
+//   rotary, rotary_grad   in=Q[,K][,POSITIONS] out=QO[,KO]  (batch, heads,
+//                         k_heads, layout as attention; rot, pairs=half|interleaved,
+//                         base, offset, scaling=none|linear|parts, factor, context,
+//                         low, high, magnitude); out may be in
+//   residual_norm         in=X,O with=post,gate,pre out=R[,Y]  (post_norm,
+//                         gate_rows, eps, stream_scale, branch_scale)
+//   residual_norm_grad    in=O,R with=post,gate,pre,dr,dy gives=dx,do,dpost,dgate,dpre
+//   linear_xent           in=X,W,TARGETS gives=loss,lse,sums  (trans_w, scale)
+//   linear_xent_grad      in=X,W,TARGETS,LSE[,DLOSS] gives=dx,dw
 // Tensors are row-major; row operators see [rows, cols] with cols the last
 // dim and rows the product of the others; a view is a 2-D strided window
 // (offset and row stride ld in elements) into another tensor's storage.
@@ -34,6 +45,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <sstream>
 #include <string>
@@ -42,6 +54,9 @@
 #include <hip/hip_runtime_api.h>
 
 namespace {
+
+// Plan-only dtype beside BwppHipDType: 32-bit integers (positions, targets).
+constexpr uint32_t kI32 = 2;
 
 enum class Kind { kInput, kParam, kTemp, kOutput, kConst, kView };
 
@@ -227,7 +242,8 @@ BwppHipStatus parse(BwppHipPlan &p, const char *text) {
       v.name = t[1];
       if (t[2] == "f32") v.dtype = BWPP_HIP_F32;
       else if (t[2] == "bf16") v.dtype = BWPP_HIP_BF16;
-      else return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d: dtype f32 or bf16", ln);
+      else if (t[2] == "i32") v.dtype = kI32;
+      else return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d: dtype f32, bf16 or i32", ln);
       BwppHipStatus s = parse_dims(p, t[3], v, ln);
       if (s != BWPP_HIP_OK) return s;
       const std::string &k = t[4];
@@ -251,6 +267,8 @@ BwppHipStatus parse(BwppHipPlan &p, const char *text) {
       } else {
         return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d: unknown kind '%s'", ln, k.c_str());
       }
+      if (v.dtype == kI32 && v.kind != Kind::kInput && v.kind != Kind::kParam)
+        return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d: an i32 value is an input or a param", ln);
       p.by_name[v.name] = (int)p.values.size();
       p.values.push_back(v);
     } else if (t[0] == "view") {
@@ -546,16 +564,236 @@ extern "C" void *bwpp_hip_plan_value_ptr(const BwppHipPlan *p, const char *name)
 
 namespace {
 
-const char *dtype_name(uint32_t dt) { return dt == BWPP_HIP_BF16 ? "bf16" : "f32"; }
+const char *dtype_name(uint32_t dt) { return dt == BWPP_HIP_BF16 ? "bf16" : dt == kI32 ? "i32" : "f32"; }
 
 std::string attr(const Op &op, const char *k, const char *dflt) {
   auto it = op.attrs.find(k);
   return it == op.attrs.end() ? std::string(dflt) : it->second;
 }
 
+// The names in a comma-separated attribute, in order (none where absent).
+std::vector<std::string> name_list(const Op &op, const char *k) {
+  const std::string v = attr(op, k, "");
+  return v.empty() ? std::vector<std::string>() : split(v, ',');
+}
+// Operand `name` of a with= / gives= list whose first entry is operand
+// `first`; -1 where it is not in the list.
+int listed(const std::vector<int> &ops, const std::vector<std::string> &names, size_t first, const char *name) {
+  for (size_t i = 0; i < names.size() && first + i < ops.size(); ++i)
+    if (names[i] == name) return ops[first + i];
+  return -1;
+}
+
+bool checks_own_dtypes(const std::string &k) {
+  return k == "rotary" || k == "rotary_grad" || k == "residual_norm" || k == "residual_norm_grad" ||
+         k == "linear_xent" || k == "linear_xent_grad";
+}
+
 // In check-only mode (plan creation) each op validates its arguments and
 // shapes and launches nothing.
 #define BWPP_PLAN_CALL(expr) (p.check_only ? BWPP_HIP_OK : (expr))
+
+// rotary, residual_norm, linear_xent and their gradients.
+BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
+  BwppHip *h = p.h;
+  const std::string &k = op.kind;
+  auto val = [&](int i) -> const Value & { return p.values[i]; };
+  auto ptr = [&](int i) { return i < 0 ? nullptr : bwpp_hip_plan_value_ptr(&p, p.values[i].name.c_str()); };
+  auto f32 = [&](int i) { return static_cast<float *>(ptr(i)); };
+  auto i32 = [&](int i) { return static_cast<const int32_t *>(ptr(i)); };
+  auto bad = [&](const char *what) {
+    return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d (%s): %s", op.line, k.c_str(), what);
+  };
+  auto num = [&](const char *key, double dflt) {
+    auto it = op.attrs.find(key);
+    if (it == op.attrs.end()) return dflt;
+    uint64_t n = 0;
+    if (eval_expr(p, it->second, n) && it->second.find('.') == std::string::npos) return (double)n;
+    return strtod(it->second.c_str(), nullptr);
+  };
+  auto shape = [&](int i, uint64_t rows, uint64_t cols) { return i < 0 || (val(i).rows() == rows && val(i).cols() == cols); };
+  auto elems = [&](int i, uint64_t n) { return i < 0 || (val(i).kind != Kind::kView && val(i).elems() == n); };
+  auto dtype = [&](std::initializer_list<int> list, uint32_t dt) {
+    for (int i : list)
+      if (i >= 0 && val(i).dtype != dt) return false;
+    return true;
+  };
+  auto known = [&](const std::vector<std::string> &names, std::initializer_list<const char *> all, size_t count) {
+    if (names.size() != count) return false;
+    for (size_t i = 0; i < names.size(); ++i) {
+      bool ok = false;
+      for (const char *a : all) ok = ok || names[i] == a;
+      for (size_t j = 0; j < i; ++j) ok = ok && names[i] != names[j];
+      if (!ok) return false;
+    }
+    return true;
+  };
+  const bool grad = k.size() > 5 && k.compare(k.size() - 5, 5, "_grad") == 0;
+  if (op.ins.empty()) return bad("no operands");
+  const uint32_t dt = val(op.ins[0]).dtype;
+  if (dt > BWPP_HIP_BF16) return bad("operands must be f32 or bf16");
+  BwppHipStatus s = BWPP_HIP_OK;
+  if (k == "rotary" || k == "rotary_grad") {
+    // [batch*seq, heads*dim] row blocks or, layout=bhsd, [batch, heads, seq,
+    // dim], as attention's q and k.
+    const int pos = val(op.ins.back()).dtype == kI32 ? op.ins.back() : -1;
+    const size_t n = op.outs.size();
+    if (n < 1 || n > 2 || op.ins.size() != n + (pos >= 0 ? 1 : 0)) return bad("in=Q[,K][,positions] out=QO[,KO]");
+    const uint64_t B = (uint64_t)num("batch", 1), H = (uint64_t)num("heads", 1);
+    const uint64_t Hk = n > 1 ? (uint64_t)num("k_heads", (double)H) : 0;
+    const std::string lay = attr(op, "layout", "bshd"), pairs = attr(op, "pairs", "half"), sc = attr(op, "scaling", "none");
+    if (lay != "bshd" && lay != "bhsd") return bad("layout must be bshd or bhsd");
+    if (pairs != "half" && pairs != "interleaved") return bad("pairs must be half or interleaved");
+    if (sc != "none" && sc != "linear" && sc != "parts") return bad("scaling must be none, linear or parts");
+    const bool bhsd = lay == "bhsd";
+    if (!B || !H || (n > 1 && !Hk)) return bad("bad batch / heads");
+    uint64_t seq = 0, dim = 0;
+    for (size_t i = 0; i < n; ++i) {
+      const Value &X = val(op.ins[i]), &Y = val(op.outs[i]);
+      const uint64_t hh = i ? Hk : H, blocks = bhsd ? B * hh : B;
+      if (X.rows() != Y.rows() || X.cols() != Y.cols()) return bad("out must have in's shape");
+      if (X.rows() % blocks || (!bhsd && X.cols() % hh)) return bad("bad batch / heads");
+      const uint64_t sq = X.rows() / blocks, d = bhsd ? X.cols() : X.cols() / hh;
+      if (i && (sq != seq || d != dim)) return bad("K must have Q's sequence and head dim");
+      seq = sq;
+      dim = d;
+      if (!dtype({op.ins[i], op.outs[i]}, dt)) return bad("operands of different dtypes");
+    }
+    if (pos >= 0 && !elems(pos, B * seq) && !elems(pos, seq)) return bad("positions need batch*seq or seq elements");
+    BwppRotaryParams r = {};
+    r.tokens = (uint32_t)seq;
+    r.q_heads = (uint32_t)H;
+    r.k_heads = (uint32_t)Hk;
+    r.dim = (uint32_t)dim;
+    r.batch = (uint32_t)B;
+    r.rot_dim = (uint32_t)num("rot", 0);
+    r.layout = pairs == "half" ? BWPP_HIP_ROTARY_HALF : BWPP_HIP_ROTARY_INTERLEAVED;
+    r.dtype = dt;
+    r.pos_batch_stride = pos >= 0 && val(pos).elems() == B * seq ? seq : 0;
+    r.pos_offset = (int32_t)num("offset", 0);
+    r.scaling = sc == "none" ? BWPP_HIP_ROTARY_SCALE_NONE : sc == "linear" ? BWPP_HIP_ROTARY_SCALE_LINEAR
+                                                                       : BWPP_HIP_ROTARY_SCALE_BY_PARTS;
+    r.base = (float)num("base", 0);
+    r.factor = (float)num("factor", 0);
+    r.context = (uint32_t)num("context", 0);
+    r.low_turns = (float)num("low", 0);
+    r.high_turns = (float)num("high", 0);
+    r.magnitude = (float)num("magnitude", 0);
+    auto strides = [&](int v, uint64_t hh, uint32_t &ld, uint64_t &hs, uint64_t &bs) {
+      const uint64_t st = val(v).row_stride();
+      ld = (uint32_t)st;
+      hs = bhsd ? seq * st : dim;
+      bs = bhsd ? hh * seq * st : seq * st;
+    };
+    // The gradient's inputs have the outputs' strides.
+    strides(grad ? op.outs[0] : op.ins[0], H, r.ldq, r.q_head_stride, r.q_batch_stride);
+    strides(grad ? op.ins[0] : op.outs[0], H, r.ldqo, r.qo_head_stride, r.qo_batch_stride);
+    if (n > 1) {
+      strides(grad ? op.outs[1] : op.ins[1], Hk, r.ldk, r.k_head_stride, r.k_batch_stride);
+      strides(grad ? op.ins[1] : op.outs[1], Hk, r.ldko, r.ko_head_stride, r.ko_batch_stride);
+    }
+    const int ki = n > 1 ? op.ins[1] : -1, ko = n > 1 ? op.outs[1] : -1;
+    s = BWPP_PLAN_CALL(grad ? bwpp_hip_dispatch_rotary_grad(h, ptr(op.ins[0]), ptr(ki), i32(pos), ptr(op.outs[0]), ptr(ko), r)
+                            : bwpp_hip_dispatch_rotary(h, ptr(op.ins[0]), ptr(ki), i32(pos), ptr(op.outs[0]), ptr(ko), r));
+  } else if (k == "residual_norm" || k == "residual_norm_grad") {
+    const std::vector<std::string> with = name_list(op, "with"), gives = name_list(op, "gives");
+    if (op.ins.size() < 2 || !(grad ? known(with, {"post", "gate", "pre", "dr", "dy"}, op.ins.size() - 2)
+                                    : known(with, {"post", "gate", "pre"}, op.ins.size() - 2)))
+      return bad(grad ? "in=O,R,.. with=post,gate,pre,dr,dy (those given, in order)"
+                      : "in=X,O,.. with=post,gate,pre (those given, in order)");
+    if (grad ? !known(gives, {"dx", "do", "dpost", "dgate", "dpre"}, op.outs.size()) : op.outs.size() > 2)
+      return bad(grad ? "out=.. gives=dx,do,dpost,dgate,dpre (those given, in order)" : "out=R[,Y]");
+    const int a0 = op.ins[0], a1 = op.ins[1], o = grad ? a0 : a1;
+    const int post = listed(op.ins, with, 2, "post"), gate = listed(op.ins, with, 2, "gate"),
+              pre = listed(op.ins, with, 2, "pre");
+    const uint64_t rows = val(o).rows(), cols = val(o).cols();
+    BwppResidualNormParams r = {};
+    r.rows = (uint32_t)rows;
+    r.cols = (uint32_t)cols;
+    r.ldo = (uint32_t)val(o).row_stride();
+    r.post_norm = (uint32_t)num("post_norm", post >= 0 ? 1 : 0);
+    r.gate_rows = (uint32_t)num("gate_rows", 0);
+    r.eps = (float)num("eps", 1e-5);
+    r.stream_scale = (float)num("stream_scale", 0);
+    r.branch_scale = (float)num("branch_scale", 0);
+    r.dtype = dt;
+    const uint64_t gates = r.gate_rows ? (rows + r.gate_rows - 1) / r.gate_rows : 1;
+    for (const std::vector<int> *list : {&op.ins, &op.outs})
+      for (int v : *list)
+        if (val(v).dtype != dt) return bad("operands of different dtypes");
+    if (!elems(post, cols) || !elems(pre, cols) || !shape(gate, gates, cols)) return bad("weight or gate shape does not match");
+    if (gate >= 0) r.ldg = (uint32_t)val(gate).row_stride();
+    if (!grad) {
+      const int y = op.outs.size() > 1 ? op.outs[1] : -1;
+      if (!shape(a0, rows, cols) || !shape(op.outs[0], rows, cols) || !shape(y, rows, cols)) return bad("operand shapes do not match");
+      r.ldx = (uint32_t)val(a0).row_stride();
+      if (val(op.outs[0]).row_stride() != r.ldx) return bad("R needs X's row stride");
+      if (y >= 0) r.ldy = (uint32_t)val(y).row_stride();
+      s = BWPP_PLAN_CALL(bwpp_hip_dispatch_residual_norm(h, ptr(a0), ptr(a1), ptr(post), ptr(gate), ptr(pre), ptr(op.outs[0]),
+                                                         ptr(y), r));
+    } else {
+      const int dr = listed(op.ins, with, 2, "dr"), dy = listed(op.ins, with, 2, "dy");
+      const int dx = listed(op.outs, gives, 0, "dx"), dout = listed(op.outs, gives, 0, "do"),
+                dpost = listed(op.outs, gives, 0, "dpost"), dgate = listed(op.outs, gives, 0, "dgate"),
+                dpre = listed(op.outs, gives, 0, "dpre");
+      if (dr < 0 && dy < 0) return bad("needs dr or dy");
+      if (!shape(a1, rows, cols) || !shape(dr, rows, cols) || !shape(dy, rows, cols) || !shape(dx, rows, cols) ||
+          !shape(dout, rows, cols) || !shape(dgate, gates, cols) || !elems(dpost, cols) || !elems(dpre, cols))
+        return bad("operand shapes do not match");
+      r.ldx = (uint32_t)val(a1).row_stride();
+      if (dy >= 0) r.ldy = (uint32_t)val(dy).row_stride();
+      if ((dr >= 0 && val(dr).row_stride() != r.ldx) || (dx >= 0 && val(dx).row_stride() != r.ldx) ||
+          (dout >= 0 && val(dout).row_stride() != r.ldo))
+        return bad("dr and dx need R's row stride, do O's");
+      if (dgate >= 0) {
+        if (gate >= 0 && val(dgate).row_stride() != r.ldg) return bad("dgate needs the gate's row stride");
+        r.ldg = (uint32_t)val(dgate).row_stride();
+      }
+      s = BWPP_PLAN_CALL(bwpp_hip_dispatch_residual_norm_grad(h, ptr(a0), ptr(a1), ptr(post), ptr(gate), ptr(pre), ptr(dr),
+                                                              ptr(dy), ptr(dx), ptr(dout), ptr(dpost), ptr(dgate), ptr(dpre), r));
+    }
+  } else {
+    const std::vector<std::string> gives = name_list(op, "gives");
+    if (grad ? op.ins.size() != 4 && op.ins.size() != 5 : op.ins.size() != 3)
+      return bad(grad ? "in=X,W,targets,LSE[,dloss]" : "in=X,W,targets");
+    if (!(grad ? known(gives, {"dx", "dw"}, op.outs.size()) : known(gives, {"loss", "lse", "sums"}, op.outs.size())))
+      return bad(grad ? "out=.. gives=dx,dw (those given, in order)" : "out=.. gives=loss,lse,sums (those given, in order)");
+    const int x = op.ins[0], w = op.ins[1], t = op.ins[2];
+    const uint64_t rows = val(x).rows(), dim = val(x).cols();
+    BwppLinearXentParams r = {};
+    r.trans_w = (uint32_t)num("trans_w", 0);
+    r.rows = (uint32_t)rows;
+    r.dim = (uint32_t)dim;
+    r.vocab = (uint32_t)(r.trans_w ? val(w).rows() : val(w).cols());
+    r.ldx = (uint32_t)val(x).row_stride();
+    r.ldw = (uint32_t)val(w).row_stride();
+    r.dtype = dt;
+    r.scale = (float)num("scale", 0);
+    if ((r.trans_w ? val(w).cols() : val(w).rows()) != dim) return bad("W does not have X's columns");
+    if (!dtype({w}, dt) || !dtype({t}, kI32)) return bad("W must have X's dtype, targets i32");
+    if (!elems(t, rows)) return bad("targets need one element a row");
+    if (!grad) {
+      const int loss = listed(op.outs, gives, 0, "loss"), lse = listed(op.outs, gives, 0, "lse"),
+                sums = listed(op.outs, gives, 0, "sums");
+      if (!dtype({loss, lse, sums}, BWPP_HIP_F32)) return bad("loss, lse and sums are f32");
+      if (!elems(loss, rows) || !elems(lse, rows) || !elems(sums, 2)) return bad("output shapes do not match");
+      s = BWPP_PLAN_CALL(bwpp_hip_dispatch_linear_xent(h, ptr(x), ptr(w), i32(t), f32(loss), f32(lse), f32(sums), r));
+    } else {
+      const int lse = op.ins[3], dloss = op.ins.size() > 4 ? op.ins[4] : -1;
+      const int dx = listed(op.outs, gives, 0, "dx"), dw = listed(op.outs, gives, 0, "dw");
+      if (!dtype({lse, dloss}, BWPP_HIP_F32) || !dtype({dx, dw}, dt)) return bad("lse and dloss are f32, gradients of X's dtype");
+      if (!elems(lse, rows) || (!elems(dloss, rows) && !elems(dloss, 1)) || !shape(dx, rows, dim) ||
+          !shape(dw, val(w).rows(), val(w).cols()))
+        return bad("operand shapes do not match");
+      r.dloss_scalar = dloss >= 0 && val(dloss).elems() == 1 ? 1 : 0;
+      if (dx >= 0) r.lddx = (uint32_t)val(dx).row_stride();
+      if (dw >= 0) r.lddw = (uint32_t)val(dw).row_stride();
+      s = BWPP_PLAN_CALL(bwpp_hip_dispatch_linear_xent_grad(h, ptr(x), ptr(w), i32(t), f32(lse), f32(dloss), ptr(dx), ptr(dw), r));
+    }
+  }
+  if (s != BWPP_HIP_OK) return perr(&p, s, "line %d (%s): %s", op.line, k.c_str(), bwpp_hip_last_error(h));
+  return BWPP_HIP_OK;
+}
 
 BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
   BwppHip *h = p.h;
@@ -582,8 +820,10 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
   {
     auto dt = [&](int i) { return val(i).dtype; };
     if (k == "matmul" || k == "attention" || k == "attention_grad") {
+      if (op.ins.empty()) return bad("no operands");
       const uint32_t d0 = dt(op.ins[0]);
       const bool att = k != "matmul";
+      if (d0 == kI32) return bad("operands must be f32 or bf16");
       for (size_t j = 0; j < op.ins.size(); ++j)
         if (!(k == "attention_grad" && j == 5) && dt(op.ins[j]) != d0) return bad("operands of different dtypes");
       for (size_t j = 0; j < op.outs.size(); ++j) {
@@ -591,7 +831,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
         if (dt(op.outs[j]) != (lse ? (uint32_t)BWPP_HIP_F32 : d0)) return bad("output dtype does not match");
       }
       if (k == "attention_grad" && op.ins.size() > 5 && dt(op.ins[5]) != BWPP_HIP_F32) return bad("lse must be f32");
-    } else {
+    } else if (!checks_own_dtypes(k)) {
       for (const std::vector<int> *list : {&op.ins, &op.outs})
         for (int v : *list)
           if (dt(v) != BWPP_HIP_F32) return bad("this operator takes f32 values only");
@@ -813,6 +1053,8 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
                                           ptr(op.ins[4]), f32(op.ins[5]), ptr(op.outs[0]), ptr(op.outs[1]),
                                           ptr(op.outs[2]), ap));
     }
+  } else if (checks_own_dtypes(k)) {
+    return run_lm_op(p, op);
   } else {
     return bad("unknown op");
   }
