@@ -1,5 +1,5 @@
-// The bf16 matrix products' main loops (gemm.hip, xent.hip): full 256-row
-// tiles and tiles for any M, N and K, each with an epilogue of the caller's:
+// The bf16 matrix products' main loops: full 256-row tiles (gemm.hip), and tiles
+// for any M, N and K (gemm.hip, xent.hip), these with an epilogue of the caller's:
 // EpiStore stores C = acc (+ bias) (-> SiLU) in bf16, or a K split's raw sums;
 // any other gets the accumulators.
 #pragma once
@@ -40,10 +40,15 @@ __device__ __forceinline__ float silu(float x) {
 }
 
 // A caller's epilogue has kStore = false and
-//   run<BM, BN, WM, WN>(acc, smem, m0, n0, tn, split, tid, wm, wn)
+//   run<Frag32, BM, BN, WM, WN>(acc, smem, m0, n0, tn, split, tid, wm, wn)
 // with f32x16_t acc[FN][FM]: register r of acc[i][j] in lane l is row m0 + wm TM
-// + 32 j + l % 32 and column n0 + wn TN + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4
-// (TM = BM / WM, TN = BN / WN).  smem is free (BM (BN + 8) bf16 at least).
+// + 32 j + Frag32::row(l) and column n0 + wn TN + 32 i + Frag32::col(l, r) (TM =
+// BM / WM, TN = BN / WN).  smem is free (BM (BN + 8) bf16 at least).
+struct Frag32 {  // v_mfma_f32_32x32x16_bf16
+  static constexpr int kSize = 32, kRegs = 16;
+  static __device__ __forceinline__ uint32_t row(int lane) { return (uint32_t)(lane & 31); }
+  static __device__ __forceinline__ uint32_t col(int lane, int r) { return (uint32_t)(8 * (r / 4) + 4 * (lane >> 5) + r % 4); }
+};
 struct EpiStore {
   static constexpr bool kStore = true;
 };
@@ -204,12 +209,8 @@ using bool_tag = std::integral_constant<bool, V>;
 // stages fit three deep, the epilogue stages C through LDS in two halves
 // of 128 rows, and N need only be a multiple of 8 -- a tile column that
 // overhangs N re-reads B's last columns (or rows) and stores only n < N.
-//
-// With an epilogue of the caller's (256 x 256): M and N are any, as long as an
-// operand's 16-byte chunks are whole (rows past them re-read the last ones;
-// the epilogue leaves them out), and K may be split as in gemm_bf16_ring.
-template <bool TA, bool TB, int WM, int WN, int BN = 256, int STAGES = 4, class EPI = EpiStore>
-__device__ __forceinline__ void gemm_bf16_pipe(const BwppGemmArgs &a, const EPI &epi = EPI{}) {
+template <bool TA, bool TB, int WM, int WN, int BN = 256, int STAGES = 4>
+__device__ __forceinline__ void gemm_bf16_pipe(const BwppGemmArgs &a) {
   constexpr int BM = 256;
   constexpr int NW = WM * WN, NT = 64 * NW;
   constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
@@ -218,7 +219,6 @@ __device__ __forceinline__ void gemm_bf16_pipe(const BwppGemmArgs &a, const EPI 
   static_assert(LPA * NW * 1024 == kTileA && LPB * NW * 1024 == kTileB, "DMA blocks split evenly over the waves");
   static_assert(TN % 32 == 0 && TM % 32 == 0 && STAGES >= 2 && STAGES <= 4, "tile shape");
   constexpr bool kEdgeN = BN != 256;
-  constexpr bool kClamp = !EPI::kStore;
   // Lean register use (the 8-wave 384-wide tile holds 192 accumulator
   // VGPRs): DMA sources as 32-bit offsets from wave-uniform tile origins,
   // and one set of A operands, each re-read for the next k-step as soon as
@@ -237,24 +237,12 @@ __device__ __forceinline__ void gemm_bf16_pipe(const BwppGemmArgs &a, const EPI 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  uint32_t tm, tn, split = 0, klen = a.K;
+  uint32_t tm, tn;
+  tile_coords(a, tm, tn);
+  const uint32_t m0 = tm * BM, n0 = tn * BN;
   const uint16_t *A = static_cast<const uint16_t *>(a.a);
   const uint16_t *B = static_cast<const uint16_t *>(a.b);
-  if constexpr (EPI::kStore) {
-    tile_coords(a, tm, tn);
-  } else {
-    const uint32_t tiles = a.tiles_m * a.tiles_n;
-    split = a.ksplit > 1 ? blockIdx.x / tiles : 0u;
-    tile_coords(a, tm, tn, blockIdx.x - split * tiles);
-    if (a.ksplit > 1) {
-      const uint32_t kbeg = split * a.kchunk;
-      klen = min(a.K - kbeg, a.kchunk);
-      A += TA ? (size_t)kbeg * a.lda : (size_t)kbeg;
-      B += TB ? (size_t)kbeg : (size_t)kbeg * a.ldb;
-    }
-  }
-  const uint32_t m0 = tm * BM, n0 = tn * BN;
-  const uint32_t nk = klen / kPipeBK;
+  const uint32_t nk = a.K / kPipeBK;
   const uint16_t *bias = static_cast<const uint16_t *>(a.bias);
   const bool add = (a.epilogue & kEpiAdd) && bias;
   const bool act = (a.epilogue & kEpiSilu) != 0;
@@ -269,12 +257,12 @@ __device__ __forceinline__ void gemm_bf16_pipe(const BwppGemmArgs &a, const EPI 
 #pragma unroll
   for (int i = 0; i < LPA; ++i) {
     if constexpr (kLean) offA[i] = tile_off<TA, BM>(a.lda, m0, (uint32_t)(wave * LPA + i), lane);
-    else srcA[i] = tile_src<TA, BM, kClamp>(A, a.lda, m0, (uint32_t)(wave * LPA + i), lane, a.M);
+    else srcA[i] = tile_src<TA, BM>(A, a.lda, m0, (uint32_t)(wave * LPA + i), lane);
   }
 #pragma unroll
   for (int i = 0; i < LPB; ++i) {
     if constexpr (kLean) offB[i] = tile_off<!TB, BN, kEdgeN>(a.ldb, n0, (uint32_t)(wave * LPB + i), lane, a.N);
-    else srcB[i] = tile_src<!TB, BN, kClamp>(B, a.ldb, n0, (uint32_t)(wave * LPB + i), lane, a.N);
+    else srcB[i] = tile_src<!TB, BN>(B, a.ldb, n0, (uint32_t)(wave * LPB + i), lane);
   }
   const size_t stepA = TA ? (size_t)kPipeBK * a.lda : (size_t)kPipeBK;
   const size_t stepB = TB ? (size_t)kPipeBK : (size_t)kPipeBK * a.ldb;
@@ -422,10 +410,6 @@ __device__ __forceinline__ void gemm_bf16_pipe(const BwppGemmArgs &a, const EPI 
   for (; kt + 1 < nk; ++kt) ktile(kt, bool_tag<false>{}, bool_tag<true>{});
   if (kt < nk) ktile(kt, bool_tag<false>{}, bool_tag<false>{});
   __syncthreads();
-  if constexpr (!EPI::kStore) {
-    epi.template run<BM, BN, WM, WN>(acc, smem, m0, n0, tn, split, tid, wm, wn);
-    return;
-  }
 
   // Epilogue through LDS (see gemm_bf16), in kHalves passes of kHR rows.
   uint16_t *cs = reinterpret_cast<uint16_t *>(smem);
@@ -745,7 +729,7 @@ __device__ __forceinline__ void gemm_bf16_ring(const BwppGemmArgs &a, const EPI 
 
   if constexpr (!EPI::kStore) {
     __syncthreads();
-    epi.template run<BM, BN, WM, WN>(acc, smem, m0, n0, tn, split, tid, wm, wn);
+    epi.template run<Frag32, BM, BN, WM, WN>(acc, smem, m0, n0, tn, split, tid, wm, wn);
     return;
   }
   const int lrow = lane & 31, lhalf = lane >> 5;

@@ -8,7 +8,8 @@
 //
 // A target outside the vocabulary leaves its row out: loss and gradients 0.
 //
-// bf16: the logits' product runs on the matrix cores (gemm_bf16.h's loops)
+// bf16: the logits' product runs on the matrix cores (gemm_bf16_k32.h's loop, and
+// gemm_bf16.h's for any sizes)
 // and stays in its accumulators.  The forward's epilogue reduces each tile's
 // rows to (max, sum of exp), a pair per row and tile, and a second kernel
 // joins the pairs.  The gradient's epilogue turns the same product, made
@@ -24,7 +25,7 @@
 // Maxima and sums are fp32, the last logarithm 64-bit (once a row): lse is off
 // by a few 2^-24 of itself.  exp(z - max) is taken as exp2 of the rounded
 // difference, which is exact for the logits that count.
-#include "gemm_bf16.h"
+#include "gemm_bf16_k32.h"
 
 namespace {
 
@@ -41,12 +42,24 @@ __device__ __forceinline__ void join(float &m, float &s, float m2, float s2) {
   m = mm;
 }
 
-template <int FN, int FM, class F>
-__device__ __forceinline__ void each_column(uint32_t n_first, int lhalf, F f) {
+// f(i, r, n) for the registers of a wave's fragments in one row, n its column.
+template <class FR, int FN, class F>
+__device__ __forceinline__ void each_column(uint32_t n_first, int lane, F f) {
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) f(i, r, n_first + (uint32_t)(i * 32 + 8 * (r / 4) + 4 * lhalf + r % 4));
+    for (int r = 0; r < FR::kRegs; ++r) f(i, r, n_first + (uint32_t)(i * FR::kSize) + FR::col(lane, r));
+}
+// Over the lanes that share a row.
+template <class FR>
+__device__ __forceinline__ float row_max(float v) {
+  if constexpr (FR::kSize == 16) v = fmaxf(v, xor_f32(v, 16));
+  return fmaxf(v, xor_f32(v, 32));
+}
+template <class FR>
+__device__ __forceinline__ float row_sum(float v) {
+  if constexpr (FR::kSize == 16) v += xor_f32(v, 16);
+  return v + xor_f32(v, 32);
 }
 
 // Per row of the tile: maximum and sum of exp, and the target's logit.
@@ -54,36 +67,35 @@ struct EpiStats {
   static constexpr bool kStore = false;
   const BwppXentArgs &a;
 
-  template <int BM, int BN, int WM, int WN, int FN, int FM>
-  __device__ __forceinline__ void run(f32x16_t (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0,
-                                      uint32_t tn, uint32_t, int tid, int wm, int wn) const {
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t tn,
+                                      uint32_t, int tid, int wm, int wn) const {
     constexpr int TM = BM / WM, TN = BN / WN;
-    const int lane = tid & 63, lrow = lane & 31, lhalf = lane >> 5;
+    const int lane = tid & 63;
     float2 *pair = reinterpret_cast<float2 *>(smem);  // [BM][WN]
     const uint32_t nw = n0 + (uint32_t)(wn * TN);
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const uint32_t ml = (uint32_t)(wm * TM + j * 32 + lrow), m = m0 + ml;
+      const uint32_t ml = (uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane), m = m0 + ml;
       const uint32_t t = m < a.g.M ? (uint32_t)a.target[m] : 0xffffffffu;
       if (n0 + BN > a.g.N)  // the last tile column: no logits past N
-        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t n) {
-          if (n >= a.g.N) acc[i][j][r] = -__builtin_inff();
-          else acc[i][j][r] *= a.scale;
+        each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t n) {
+          acc[i][j][r] = n < a.g.N ? acc[i][j][r] * a.scale : -__builtin_inff();
         });
       else
-        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { acc[i][j][r] *= a.scale; });
+        each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t) { acc[i][j][r] *= a.scale; });
       const uint32_t tl = t - a.n_base;  // the target's column of this product
       if (__any(t < a.vocab && tl - nw < (uint32_t)TN))
-        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t n) {
+        each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t n) {
           if (t < a.vocab && n == tl && n < a.g.N) a.zt[m] = acc[i][j][r];
         });
       float mx = -__builtin_inff(), s = 0.0f;
-      each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { mx = fmaxf(mx, acc[i][j][r]); });
-      mx = fmaxf(mx, xor_f32(mx, 32));
+      each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t) { mx = fmaxf(mx, acc[i][j][r]); });
+      mx = row_max<FR>(mx);
       const float ref = finite_or_0(mx);
-      each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { s += exp_diff(acc[i][j][r], ref); });
-      s += xor_f32(s, 32);
-      if (lhalf == 0) pair[ml * WN + wn] = make_float2(mx, s);
+      each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t) { s += exp_diff(acc[i][j][r], ref); });
+      s = row_sum<FR>(s);
+      if (lane < FR::kSize) pair[ml * WN + wn] = make_float2(mx, s);
     }
     __syncthreads();
     if (tid < BM && m0 + (uint32_t)tid < a.g.M) {
@@ -103,16 +115,16 @@ struct EpiGrad {
   static constexpr bool kStore = false;
   const BwppXentArgs &a;
 
-  template <int BM, int BN, int WM, int WN, int FN, int FM>
-  __device__ __forceinline__ void run(f32x16_t (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0,
-                                      uint32_t, uint32_t, int tid, int wm, int wn) const {
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t, uint32_t,
+                                      int tid, int wm, int wn) const {
     constexpr int TM = BM / WM, TN = BN / WN, NT = 64 * WM * WN, kCld = BN + 8;
-    const int lane = tid & 63, lrow = lane & 31, lhalf = lane >> 5;
+    const int lane = tid & 63;
     uint16_t *cs = reinterpret_cast<uint16_t *>(smem);  // [BM][BN + 8]
     const uint32_t nw = n0 + (uint32_t)(wn * TN);
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const uint32_t ml = (uint32_t)(wm * TM + j * 32 + lrow), m = m0 + ml;
+      const uint32_t ml = (uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane), m = m0 + ml;
       uint32_t t = 0xffffffffu;
       float lse = 0.0f, g = 0.0f;
       if (m < a.g.M) {
@@ -121,23 +133,23 @@ struct EpiGrad {
         g = (a.dloss ? a.dloss[a.dloss_scalar ? 0u : m] : 1.0f) * a.scale;
       }
       const bool live = t < a.vocab;
-      each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t) { acc[i][j][r] = exp_diff(acc[i][j][r] * a.scale, lse); });
+      each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t) { acc[i][j][r] = exp_diff(acc[i][j][r] * a.scale, lse); });
       const uint32_t tl = t - a.n_base;
       if (__any(live && tl - nw < (uint32_t)TN))
-        each_column<FN, FM>(nw, lhalf, [&](int i, int r, uint32_t n) {
+        each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t n) {
           if (live && n == tl) acc[i][j][r] -= 1.0f;
         });
 #pragma unroll
       for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int r = 0; r < FR::kRegs; r += 4) {  // four columns
           float v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = live ? g * acc[i][j][4 * q + e] : 0.0f;
+          for (int e = 0; e < 4; ++e) v[e] = live ? g * acc[i][j][r + e] : 0.0f;
           uint2 o;
           o.x = pack_bf16x2(v[0], v[1]);
           o.y = pack_bf16x2(v[2], v[3]);
-          *reinterpret_cast<uint2 *>(cs + ml * kCld + wn * TN + i * 32 + q * 8 + lhalf * 4) = o;
+          *reinterpret_cast<uint2 *>(cs + ml * kCld + wn * TN + i * FR::kSize + FR::col(lane, r)) = o;
         }
     }
     __syncthreads();
@@ -158,22 +170,22 @@ struct EpiSums {
   static constexpr bool kStore = false;
   const BwppXentArgs &a;
 
-  template <int BM, int BN, int WM, int WN, int FN, int FM>
-  __device__ __forceinline__ void run(f32x16_t (&acc)[FN][FM], unsigned char *, uint32_t m0, uint32_t n0, uint32_t,
-                                      uint32_t split, int tid, int wm, int wn) const {
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *, uint32_t m0, uint32_t n0, uint32_t, uint32_t split,
+                                      int tid, int wm, int wn) const {
     constexpr int TM = BM / WM, TN = BN / WN;
-    const int lane = tid & 63, lrow = lane & 31, lhalf = lane >> 5;
+    const int lane = tid & 63;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const uint32_t m = m0 + (uint32_t)(wm * TM + j * 32 + lrow);
+      const uint32_t m = m0 + (uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane);
       float *row = a.raw + ((size_t)split * a.g.M + m) * a.g.N;
       if (m >= a.g.M) continue;
 #pragma unroll
       for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t n = n0 + (uint32_t)(wn * TN + i * 32 + q * 8 + lhalf * 4);
-          float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        for (int r = 0; r < FR::kRegs; r += 4) {
+          const uint32_t n = n0 + (uint32_t)(wn * TN + i * FR::kSize) + FR::col(lane, r);
+          float4 v = make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]);
           if (n + 4 <= a.g.N) {
             if (a.accumulate) {
               const float4 o = load4(row + n);
@@ -183,7 +195,7 @@ struct EpiSums {
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (n + e < a.g.N) row[n + e] = acc[i][j][4 * q + e] + (a.accumulate ? row[n + e] : 0.0f);
+              if (n + e < a.g.N) row[n + e] = acc[i][j][r + e] + (a.accumulate ? row[n + e] : 0.0f);
           }
         }
     }
@@ -369,12 +381,12 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_clear(const BwppXent
 BWPP_XENT_ROWS(bf16, uint16_t)
 BWPP_XENT_ROWS(f32, float)
 
-// bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 full K tiles, r32 and
+// bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 (K in steps of 32), r32 and
 // r128 any size (32 x 64, 128 x 128), _u with operands through registers.
 #define BWPP_XENT_PIPE(KIND, EPI, TB)                                                                     \
   extern "C" __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) \
   void bwpp_xent_##KIND##_p_t0##TB(const BwppXentArgs a) {                                                \
-    gemm_bf16_pipe<false, TB != 0, 2, 4, 256, 3, EPI>(a.g, EPI{a});                                       \
+    gemm_bf16_k32<false, TB != 0, TB != 0, EPI>(a.g, EPI{a});                                             \
   }
 #define BWPP_XENT_RING(KIND, EPI, TB, NAME, BM, BN, WM, WN, KPS, STAGES, WPE, KPSU, WPEU)                       \
   extern "C" __global__ __launch_bounds__(64 * WM * WN, WPE) void bwpp_xent_##KIND##_##NAME##_t0##TB(           \
