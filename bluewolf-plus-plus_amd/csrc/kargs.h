@@ -216,6 +216,8 @@ typedef struct {
   float *zt;   /* forward: [M] target logits */
   uint16_t *dl; /* gradient: dz scale, [M][ldl] bf16, ldl a multiple of 8 */
   uint32_t ldl;
+  uint32_t rows_up; /* gradient: dl's rows, M and zeros behind (at most 31) */
+  uint32_t rows_out, cols_out; /* rows product: what is stored of g.M x g.N */
   uint32_t accumulate; /* sums: add to what is there */
   float *raw;          /* sums: [ksplit][M][N] */
 } BwppXentArgs;
@@ -232,7 +234,7 @@ typedef struct {
   float *zt;
   float *loss, *lse, *sums;
   uint64_t ldx, ldy, lds;
-  uint32_t rows, cols;
+  uint32_t rows, cols, rows_up; /* rows_up: the copy's */
   uint32_t n_base, vocab;
   uint32_t nparts; /* partials a row, or planes of sums */
   uint32_t dloss_scalar;

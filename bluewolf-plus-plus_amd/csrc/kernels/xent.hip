@@ -159,8 +159,49 @@ struct EpiGrad {
     for (int it = 0; it < BM * (BN / 8) / NT; ++it) {
       const int q = tid + it * NT, row = q / (BN / 8), c = q % (BN / 8);
       const uint32_t m = m0 + (uint32_t)row, n = n0 + 8u * (uint32_t)c;
-      if (m < a.g.M && n < a.g.N)
+      if (m < a.rows_up && n < a.g.N)  // rows past M: zeros
         *reinterpret_cast<uint4 *>(a.dl + (size_t)m * a.ldl + n) = *reinterpret_cast<const uint4 *>(cs + row * kCld + c * 8);
+    }
+  }
+};
+
+// bf16 rows (dW), at any address and row stride.
+struct EpiRows {
+  static constexpr bool kStore = false;
+  const BwppXentArgs &a;
+
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t, uint32_t,
+                                      int tid, int wm, int wn) const {
+    constexpr int TM = BM / WM, TN = BN / WN, NT = 64 * WM * WN, kCld = BN + 8;
+    const int lane = tid & 63;
+    uint16_t *cs = reinterpret_cast<uint16_t *>(smem);  // [BM][BN + 8]
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int r = 0; r < FR::kRegs; r += 4) {
+          uint2 o;
+          o.x = pack_bf16x2(acc[i][j][r], acc[i][j][r + 1]);
+          o.y = pack_bf16x2(acc[i][j][r + 2], acc[i][j][r + 3]);
+          *reinterpret_cast<uint2 *>(cs + ((uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane)) * kCld + wn * TN +
+                                     i * FR::kSize + FR::col(lane, r)) = o;
+        }
+    __syncthreads();
+    uint16_t *C = static_cast<uint16_t *>(a.g.c);
+#pragma unroll 4
+    for (int it = 0; it < BM * (BN / 8) / NT; ++it) {
+      const int q = tid + it * NT, row = q / (BN / 8), c = q % (BN / 8);
+      const uint32_t m = m0 + (uint32_t)row, n = n0 + 8u * (uint32_t)c;
+      if (m >= a.rows_out || n >= a.cols_out) continue;
+      const uint16_t *h = cs + row * kCld + c * 8;
+      uint16_t *dst = C + (size_t)m * a.g.ldc + n;
+      if (n + 8 <= a.cols_out) {
+        *reinterpret_cast<u32x4a2_t *>(dst) = *reinterpret_cast<const u32x4_t *>(h);
+      } else {
+        for (uint32_t e = 0; e < 8 && n + e < a.cols_out; ++e) dst[e] = h[e];
+      }
     }
   }
 };
@@ -216,14 +257,15 @@ template <>
 __device__ __forceinline__ uint16_t to<uint16_t>(float v) { return f32_to_bf16_bits(v); }
 
 // y = x, rows that are left out 0 (their values, infinities and NaN among
-// them, stay out of dW's sums).
+// them, stay out of dW's sums), and so rows past the last (rows_up) and columns
+// (ldy).
 template <class T>
 __device__ __forceinline__ void copy_rows(const BwppXentRowArgs &a) {
-  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const bool on = live(a, row);
+  for (uint32_t row = blockIdx.x; row < a.rows_up; row += gridDim.x) {
+    const bool on = row < a.rows && live(a, row);
     const T *x = static_cast<const T *>(a.x) + row * a.ldx;
     T *y = static_cast<T *>(a.y) + row * a.ldy;
-    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) y[c] = on ? x[c] : T(0);
+    for (uint32_t c = threadIdx.x; c < a.ldy; c += 256) y[c] = on && c < a.cols ? x[c] : T(0);
   }
 }
 // Rows that are left out: 0.
@@ -388,6 +430,10 @@ BWPP_XENT_ROWS(f32, float)
   void bwpp_xent_##KIND##_p_t0##TB(const BwppXentArgs a) {                                                \
     gemm_bf16_k32<false, TB != 0, TB != 0, EPI>(a.g, EPI{a});                                             \
   }
+extern "C" __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
+void bwpp_xent_rows_p_t10(const BwppXentArgs a) {
+  gemm_bf16_k32<true, false, false, EpiRows>(a.g, EpiRows{a});
+}
 #define BWPP_XENT_RING(KIND, EPI, TB, NAME, BM, BN, WM, WN, KPS, STAGES, WPE, KPSU, WPEU)                       \
   extern "C" __global__ __launch_bounds__(64 * WM * WN, WPE) void bwpp_xent_##KIND##_##NAME##_t0##TB(           \
       const BwppXentArgs a) {                                                                                   \

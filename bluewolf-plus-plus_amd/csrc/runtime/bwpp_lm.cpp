@@ -29,7 +29,8 @@ enum LmKernel {
   LM_XENT_STATS = LM_XENT_ZERO + 2,      // [trans_w][XentTile]
   LM_XENT_GRAD = LM_XENT_STATS + 10,
   LM_XENT_RAW = LM_XENT_GRAD + 10,
-  LM_COUNT = LM_XENT_RAW + 10
+  LM_XENT_ROWS = LM_XENT_RAW + 10,
+  LM_COUNT
 };
 
 // Rows in registers (resnorm.hip): elements a thread and waves a row.
@@ -92,6 +93,7 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_xent_sums_r128_t01_u",
     "bwpp_xent_sums_r128_t01",
     "bwpp_xent_sums_r128_t01_u",
+    "bwpp_xent_rows_p_t10",
 };
 const int bwpp_hip_lm_kernel_count = (int)(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]));
 static_assert(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]) == LM_COUNT, "kernel names");
@@ -675,21 +677,25 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     r.ldy = m.lddw * es;
     return bwpp_hip_launch_lm(h, LM_XENT_CLEAR, xent_grid(h, m.wrows), 1, 256, &r);
   }
-  // bf16: dx is summed in fp32 over several pieces, and in planes of K ranges
-  // where its 256-wide tiles alone would leave half of the CUs idle (4096 x 2048
-  // from 32768 columns: 645 us as one product on smaller tiles, 515 so).
+  // bf16: dx is summed in fp32 over several pieces, and over planes of K ranges
+  // where its 256-wide tiles alone would leave half of the CUs idle; with fewer
+  // than half of them even so, it is one product on the tiles dispatch_matmul
+  // finds (4096 x 2048 from 32768 columns: 645 us as such a product, 515 so).
   const uint32_t piece = xent_piece(T, p.vocab, es);
   const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece, dx_tiles = ((T + 255) / 256) * ((D + 255) / 256);
+  const bool wide = bf16 && dx && T > 128 && piece >= 32 && on16(w) && m.ldw % 8 == 0 && (!tw || D % 8 == 0) &&
+                    256ull * std::max<uint64_t>(piece + 8ull, m.ldw) < (1ull << 31);
   uint32_t split = 1;
-  if (bf16 && dx && T > 128) {
+  if (wide) {
     while (split < 8 && dx_tiles * split * 2 <= cus_of(h) && piece / (split * 2) >= 2048) split *= 2;
-    const uint32_t range = (uint32_t)up((piece + split - 1) / split, 128);  // as xent_product cuts the first piece
-    split = (piece + range - 1) / range;
+    const uint32_t k = piece / 32 * 32, range = (uint32_t)up((k + split - 1) / split, 128);  // as xent_product cuts it
+    split = (k + range - 1) / range;
   }
-  const bool sums = bf16 && dx && (npieces > 1 || (split > 1 && dx_tiles * split >= 128));
+  const bool sums = bf16 && dx && (npieces > 1 || (wide && dx_tiles * split * 2 >= cus_of(h)));
   if (!sums) split = 1;
-  const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit);
-  const uint64_t x_bytes = dw ? up(T * ldxc * es, 256) : 0, z_bytes = up(T * ldz * es, 256);
+  // (rows of x's copy and of dz up to a multiple of 32, zeros: dW's K)
+  const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit), Tu = bf16 ? up(T, 32) : T;
+  const uint64_t x_bytes = dw ? up(Tu * ldxc * es, 256) : 0, z_bytes = up(Tu * ldz * es, 256);
   const uint64_t sum_bytes = sums ? up(split * T * D * 4, 256) : 0, held = x_bytes + z_bytes + sum_bytes;
   void *ws = nullptr;
   if ((s = bwpp_hip_take_workspace(h, held + (bf16 ? 0 : kXentSplitRoom), &ws)) != BWPP_HIP_OK) return s;
@@ -706,7 +712,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     r.ldx = m.ldx;
     r.ldy = ldxc;
     r.cols = p.dim;
-    if ((s = bwpp_hip_launch_lm(h, LM_XENT_COPY + bf16, xent_grid(h, T), 1, 256, &r)) != BWPP_HIP_OK) return s;
+    r.rows_up = (uint32_t)Tu;
+    if ((s = bwpp_hip_launch_lm(h, LM_XENT_COPY + bf16, xent_grid(h, Tu), 1, 256, &r)) != BWPP_HIP_OK) return s;
   }
   for (uint64_t i = 0; i < npieces; ++i) {
     const uint32_t n0 = (uint32_t)(i * piece), n = std::min(piece, p.vocab - n0);
@@ -730,6 +737,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.scale = r.scale;
       a.dl = static_cast<uint16_t *>(z);
       a.ldl = (uint32_t)ldp;
+      a.rows_up = (uint32_t)Tu;
       if ((s = xent_logits(h, LM_XENT_GRAD, a, tw, xent_tile(a.g, tw, true))) != BWPP_HIP_OK) return s;
     } else {
       if ((s = xent_logits_f32(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(z), n0,
@@ -752,7 +760,20 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.g.ldb = (uint32_t)m.ldw;
       a.raw = acc;
       a.accumulate = i > 0;
-      if ((s = xent_product(h, LM_XENT_RAW, a, !tw, xent_tile(a.g, !tw, false), split)) != BWPP_HIP_OK) return s;
+      // K in steps of 32 on the wide tiles, what is left of it on others.
+      BwppXentArgs rest = a;
+      a.g.K = n / 32 * 32;
+      const bool main = wide && n >= 32;
+      if (main && (s = xent_product(h, LM_XENT_RAW, a, !tw, XT_P, split)) != BWPP_HIP_OK) return s;
+      if (!main || n % 32) {
+        if (main) {
+          rest.g.K = n % 32;
+          rest.g.a = static_cast<const uint16_t *>(rest.g.a) + a.g.K;
+          rest.g.b = static_cast<const uint16_t *>(rest.g.b) + (tw ? (uint64_t)a.g.K * m.ldw : a.g.K);
+          rest.accumulate = 1;
+        }
+        if ((s = xent_product(h, LM_XENT_RAW, rest, !tw, xent_tile(rest.g, !tw, false), 1)) != BWPP_HIP_OK) return s;
+      }
     } else if (dx) {
       BwppMatmulParams g = {};
       g.M = p.rows;
@@ -769,7 +790,23 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       s = bwpp_hip_dispatch_matmul_fused(h, z, wp, dx, nullptr, i > 0 ? static_cast<const float *>(dx) : nullptr, nullptr, g, f);
       if (s != BWPP_HIP_OK) return s;
     }
-    if (dw) {
+    void *dwp = dw ? const_cast<unsigned char *>(at(dw, tw ? n0 * m.lddw : n0)) : nullptr;
+    const uint64_t dw_tiles = ((n + 255ull) / 256) * ((D + 255) / 256);
+    if (dw && bf16 && dw_tiles * 2 >= cus_of(h) && 256ull * std::max(ldp, ldxc) < (1ull << 31)) {
+      BwppXentArgs a = {};
+      a.g.a = tw ? z : xc;
+      a.g.b = tw ? xc : z;
+      a.g.c = dwp;
+      a.g.M = (uint32_t)(tw ? ldp : ldxc);
+      a.g.N = (uint32_t)(tw ? ldxc : ldp);
+      a.g.K = (uint32_t)Tu;
+      a.g.lda = a.g.M;
+      a.g.ldb = a.g.N;
+      a.g.ldc = (uint32_t)m.lddw;
+      a.rows_out = tw ? n : p.dim;
+      a.cols_out = tw ? p.dim : n;
+      if ((s = xent_product(h, LM_XENT_ROWS, a, false, XT_P, 1)) != BWPP_HIP_OK) return s;
+    } else if (dw) {
       BwppMatmulParams g = {};
       g.K = p.rows;
       g.M = tw ? n : p.dim;
@@ -779,7 +816,6 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       g.ldc = (uint32_t)m.lddw;
       g.dtype = p.dtype;
       g.trans_a = 1;
-      void *dwp = const_cast<unsigned char *>(at(dw, tw ? n0 * m.lddw : n0));
       if ((s = bwpp_hip_dispatch_matmul(h, tw ? z : xc, tw ? xc : z, dwp, nullptr, g)) != BWPP_HIP_OK) return s;
     }
   }

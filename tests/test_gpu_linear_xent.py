@@ -201,6 +201,20 @@ def test_last_round_and_planes(be, wide, T, D, V):
     _gradient(be, x, w, t, lse, None, BF16, wide)
 
 
+@pytest.mark.parametrize("wide", ["vd", "dv"])
+@pytest.mark.parametrize("T,D,V", [(2048, 1024, 8205), (2050, 1040, 8200), (1500, 2056, 4100)])
+def test_ragged_wide_products(be, wide, T, D, V):
+    """Products on the wide tiles with ragged sizes on every side: tokens and
+    vocabulary that are no multiple of 32 (dx in two products, dW's K filled up
+    with zero rows), rows of dW that start anywhere."""
+    x, w, t = _case(T, D, V, BF16, wide, 14, (0, 8 - (V % 8) if wide == "dv" else 0))
+    t[::11] = -1
+    _, lse, _ = _forward(be, x, w, t, BF16, wide)
+    _gradient(be, x, w, t, lse, None, BF16, wide)
+    _gradient(be, x, w, t, lse, None, BF16, wide, pads=(3, 1))
+    assert be.recent_kernel(1) == "bwpp_xent_rows_p_t10" or be.recent_kernel(0) == "bwpp_xent_round_bf16"
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("wide", ["vd", "dv"])
 def test_left_out_rows_hold_anything(be, dtype, wide):
