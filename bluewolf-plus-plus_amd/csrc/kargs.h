@@ -150,7 +150,7 @@ typedef struct {
   uint32_t vec; /* 1: every segment has 16-byte rows (cols, strides, pointers) */
 } BwppCopyArgs;
 
-/* Rotary positions (rotary.hip): rows of `dim` elements, one per (batch,
+/* Rotary positions (rotary.h): rows of `dim` elements, one per (batch,
  * token, head), q's heads before k's. */
 typedef struct {
   const void *q;
@@ -178,7 +178,7 @@ typedef struct {
 } BwppRotaryArgs;
 
 /* The join of a branch with the residual stream and its gradient
- * (resnorm.hip). */
+ * (resnorm.h). */
 typedef struct {
   const void *x, *o, *r;            /* stream in, branch, stream out (gradient: in) */
   const void *post, *gate, *pre;    /* weights, NULL = 1 */
@@ -199,7 +199,7 @@ typedef struct {
   uint32_t workers, group, split, span, nparts;
 } BwppResNormArgs;
 
-/* Cross entropy of hidden states against a vocabulary (xent.hip).  Logits
+/* Cross entropy of hidden states against a vocabulary (xent.h).  Logits
  * z = scale op(W) x: g holds their product (M tokens, N of the columns n_base
  * .. of the vocabulary, K = dim). */
 typedef struct {
@@ -238,6 +238,7 @@ typedef struct {
   uint32_t n_base, vocab;
   uint32_t nparts; /* partials a row, or planes of sums */
   uint32_t dloss_scalar;
+  uint32_t lanes; /* join: rows a block */
   float scale;
 } BwppXentRowArgs;
 

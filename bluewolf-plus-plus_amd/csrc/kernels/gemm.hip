@@ -1286,3 +1286,5 @@ BWPP_GEMM_F32_PIPE(0, 0)
 BWPP_GEMM_F32_PIPE(0, 1)
 BWPP_GEMM_F32_PIPE(1, 0)
 BWPP_GEMM_F32_PIPE(1, 1)
+
+#include "xent.h"  // the cross entropy's kernels share this code object

@@ -1,5 +1,5 @@
 // The bf16 matrix products' main loops: full 256-row tiles (gemm.hip), and tiles
-// for any M, N and K (gemm.hip, xent.hip), these with an epilogue of the caller's:
+// for any M, N and K (gemm.hip, xent.h), these with an epilogue of the caller's:
 // EpiStore stores C = acc (+ bias) (-> SiLU) in bf16, or a K split's raw sums;
 // any other gets the accumulators.
 #pragma once

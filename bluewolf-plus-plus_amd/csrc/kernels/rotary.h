@@ -22,12 +22,14 @@
 // half for bf16 with C = 8 and fp32 with C = 4 (any address), two 16-byte
 // loads side by side when interleaved; C = 4 of bf16 and C = 1 are for
 // rotated widths those do not divide.
+#pragma once
+
 #include "common.h"
 #include "../kargs.h"
 
 using namespace bwpp;
 
-namespace {
+namespace rotary_pos {
 
 constexpr int kMaxAngles = 2048;  // (token, pair) angles of a block: 16 KiB of LDS
 
@@ -198,8 +200,6 @@ __device__ __forceinline__ void rotary(const BwppRotaryArgs &a) {
   }
 }
 
-}  // namespace
-
 #define BWPP_ROTARY(NAME, T, INTER, C) \
   extern "C" __global__ __launch_bounds__(256) void bwpp_rotary_##NAME(const BwppRotaryArgs a) { rotary<T, INTER, C>(a); }
 BWPP_ROTARY(bf16_half_8, uint16_t, false, 8)
@@ -212,3 +212,5 @@ BWPP_ROTARY(f32_half_4, float, false, 4)
 BWPP_ROTARY(f32_half_1, float, false, 1)
 BWPP_ROTARY(f32_inter_4, float, true, 4)
 BWPP_ROTARY(f32_inter_1, float, true, 1)
+
+}  // namespace rotary_pos

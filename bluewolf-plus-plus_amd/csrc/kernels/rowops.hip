@@ -829,3 +829,7 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_col_mask(const BwppRowArg
     a.y[o] = (a.x[o] == m) ? 1.0f : 0.0f;
   }
 }
+
+// Row kernels of the operators around a block share this code object.
+#include "resnorm.h"
+#include "rotary.h"

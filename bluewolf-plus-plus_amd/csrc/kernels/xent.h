@@ -25,9 +25,11 @@
 // Maxima and sums are fp32, the last logarithm 64-bit (once a row): lse is off
 // by a few 2^-24 of itself.  exp(z - max) is taken as exp2 of the rounded
 // difference, which is exact for the logits that count.
+#pragma once
+
 #include "gemm_bf16_k32.h"
 
-namespace {
+namespace xent {
 
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -278,30 +280,31 @@ __device__ __forceinline__ void zero_rows(const BwppXentRowArgs &a) {
   }
 }
 
-}  // namespace
-
-// Joins a row's pairs: 64 rows a block, 16 waves each over a sixteenth of the
-// pairs (coalesced over the rows); then loss and lse, and with a single block
-// the sums over the rows too.
+// Joins a row's pairs: `lanes` (a power of two, 64 at most) rows a block, its 16
+// waves each over a part of the pairs, a wave's lanes beyond the rows over parts of
+// that (4 rows with 256 pairs: one load a lane); then loss and lse, and with a
+// single block the sums over the rows too.
 extern "C" __global__ __launch_bounds__(1024) void bwpp_xent_join(const BwppXentRowArgs a) {
   __shared__ float2 p[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t row = blockIdx.x * 64 + lane;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t row = blockIdx.x * a.lanes + (lane & (a.lanes - 1)), subs = 64u / a.lanes;
   float m = -__builtin_inff(), s = 0.0f;
   if (row < a.rows) {
     const float2 *part = reinterpret_cast<const float2 *>(a.part) + row;
 #pragma unroll 4
-    for (uint32_t i = wave; i < a.nparts; i += 16) {
+    for (uint32_t i = wave * subs + lane / a.lanes; i < a.nparts; i += 16 * subs) {
       const float2 q = part[(size_t)i * a.rows];
       join(m, s, q.x, q.y);
     }
   }
+  for (uint32_t d = a.lanes; d < 64; d *= 2) join(m, s, xor_f32(m, (int)d), xor_f32(s, (int)d));
   p[wave][lane] = make_float2(m, s);
   __syncthreads();
   if (wave != 0) return;
   double total = 0.0;
   uint32_t n = 0;
-  if (row < a.rows) {
+  if (row < a.rows && lane < a.lanes) {
+#pragma unroll
     for (int w = 1; w < 16; ++w) join(m, s, p[w][lane].x, p[w][lane].y);
     const double lse = (double)finite_or_0(m) + log((double)s);
     const bool on = live(a, row);
@@ -353,16 +356,39 @@ extern "C" __global__ __launch_bounds__(1024) void bwpp_xent_sums(const BwppXent
   }
 }
 
-// fp32 logits of a piece (src, unscaled): one pair per row into part[rows].
+// fp32 logits of a piece (src, unscaled; 16-byte rows with room up to 4 columns):
+// one pair per row into part[rows].  A thread keeps up to 8 chunks of four logits
+// at a time: their maximum first, then their sum (one exp a logit).
 extern "C" __global__ __launch_bounds__(256) void bwpp_xent_stats_f32(const BwppXentRowArgs a) {
   __shared__ float ms[4], ss[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t chunks = (a.cols + 3) / 4;
   for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float *z = a.src + (uint64_t)row * a.lds;
     float m = -__builtin_inff(), s = 0.0f;
-    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
-      const float v = z[c] * a.scale;
-      join(m, s, v, 1.0f);
+    for (uint32_t c0 = threadIdx.x; c0 < chunks; c0 += 256 * 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t c = min(c0 + 256 * k, chunks - 1);
+        v[k] = *reinterpret_cast<const float4 *>(z + 4 * (uint64_t)c);
+      }
+      float mc = -__builtin_inff();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t c = c0 + 256 * k, n = 4 * c;
+        float *e = &v[k].x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = c < chunks && n + i < a.cols ? e[i] * a.scale : -__builtin_inff();
+          mc = fmaxf(mc, e[i]);
+        }
+      }
+      const float ref = finite_or_0(mc);
+      float sc = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sc += (exp_diff(v[k].x, ref) + exp_diff(v[k].y, ref)) + (exp_diff(v[k].z, ref) + exp_diff(v[k].w, ref));
+      join(m, s, mc, sc);
     }
     for (int d = 1; d < 64; d *= 2) join(m, s, xor_f32(m, d), xor_f32(s, d));
     if (lane == 0) {
@@ -380,16 +406,24 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_stats_f32(const Bwpp
   }
 }
 
-// fp32 logits of a piece (y, unscaled) -> dz scale, in place.
+// fp32 logits of a piece (y, unscaled; rows as above) -> dz scale, in place.
 extern "C" __global__ __launch_bounds__(256) void bwpp_xent_grad_f32(const BwppXentRowArgs a) {
+  const uint32_t chunks = (a.cols + 3) / 4;
   for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float *z = static_cast<float *>(a.y) + (uint64_t)row * a.ldy;
     const uint32_t t = (uint32_t)a.target[row], tl = t - a.n_base;
     const bool on = t < a.vocab;
     const float lse = a.lse_in[row], g = (a.dloss ? a.dloss[a.dloss_scalar ? 0u : row] : 1.0f) * a.scale;
-    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
-      const float p = exp_diff(z[c] * a.scale, lse);
-      z[c] = on ? g * (c == tl ? p - 1.0f : p) : 0.0f;
+#pragma unroll 4
+    for (uint32_t c = threadIdx.x; c < chunks; c += 256) {
+      float4 v = *reinterpret_cast<const float4 *>(z + 4 * (uint64_t)c);
+      float *e = &v.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = exp_diff(e[i] * a.scale, lse);
+        e[i] = on ? g * (4 * c + i == tl ? p - 1.0f : p) : 0.0f;
+      }
+      *reinterpret_cast<float4 *>(z + 4 * (uint64_t)c) = v;
     }
   }
 }
@@ -454,3 +488,5 @@ void bwpp_xent_rows_p_t10(const BwppXentArgs a) {
   BWPP_XENT_RING(sums, EpiSums, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)
 BWPP_XENT_TB(0)
 BWPP_XENT_TB(1)
+
+}  // namespace xent

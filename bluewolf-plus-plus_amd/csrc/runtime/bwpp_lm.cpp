@@ -1,7 +1,7 @@
 // Operators of libbwpp_hip around a transformer block: rotary positions, the
 // residual join with its norms, and the cross entropy against a vocabulary,
 // forward and gradient.  Argument checks, launch geometry and the choice of a
-// kernel; the kernels are rotary.hip, resnorm.hip and xent.hip.
+// kernel; the kernels are rotary.h, resnorm.h and xent.h.
 #include "bwpp_hip.h"
 #include "internal.h"
 
@@ -33,7 +33,7 @@ enum LmKernel {
   LM_COUNT
 };
 
-// Rows in registers (resnorm.hip): elements a thread and waves a row.
+// Rows in registers (resnorm.h): elements a thread and waves a row.
 struct ResCfg {
   uint32_t elems, waves;
 };
@@ -198,6 +198,12 @@ BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k,
   for (const RowSet *r : {&dq, &dk})
     if (r->p && !disjoint_rows(*r)) return bad("rows of an output overlap");
   const uint64_t es = p.dtype == BWPP_HIP_BF16 ? 2 : 4;
+  if (positions) {
+    const uint64_t bytes = ((B - 1) * p.pos_batch_stride + T) * 4;
+    for (const RowSet *r : {&dq, &dk})
+      if (r->p && bwpp_hip_blocks_overlap(r->p, 1, r->span() * es, 0, positions, 1, bytes, 0, 1))
+        return bwpp_hip_set_error(h, BWPP_HIP_ERR_ALIAS, "%s: an output overlaps the positions", what);
+  }
   const bool q_in_place = sq.p && same_rows(sq, dq), k_in_place = sk.p && same_rows(sk, dk);
   if ((!q_in_place && meet(dq, sq, es)) || meet(dq, sk, es) || (!k_in_place && meet(dk, sk, es)) ||
       meet(dk, sq, es) || meet(dq, dk, es))
@@ -509,8 +515,8 @@ BwppHipStatus xent_prepare(BwppHip *h, const char *what, const BwppLinearXentPar
   m.lddx = p.lddx ? p.lddx : p.dim;
   m.lddw = p.lddw ? p.lddw : m.wcols;
   if (m.ldx < p.dim || m.ldw < m.wcols || m.lddx < p.dim || m.lddw < m.wcols) return bad("row stride smaller than the row");
-  if (p.rows > 0x7fffffffu || p.vocab > 0x7fffffffu || p.dim > 0x7fffffffu)
-    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: a size of 2^31 or more", what);
+  if (p.rows >= (1u << 27) || p.vocab > 0x7fffffffu || p.dim > 0x7fffffffu)
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: 2^27 rows, or another size of 2^31, or more", what);
   if (p.dtype == BWPP_HIP_BF16 && (p.dim < 8 || (!p.trans_w && p.vocab < 8)))
     return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: bf16 rows of fewer than 8 elements", what);
   return BWPP_HIP_OK;
@@ -633,7 +639,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x
     r.nparts = (uint32_t)npieces;
   }
   if (own_loss) r.loss = reinterpret_cast<float *>(static_cast<unsigned char *>(ws) + zt_bytes);
-  if ((s = bwpp_hip_launch_lm(h, LM_XENT_JOIN, (T + 63) / 64, 1, 1024, &r)) != BWPP_HIP_OK) return s;
+  r.lanes = 1;
+  while (r.lanes < 64 && r.lanes < T) r.lanes *= 2;
+  if ((s = bwpp_hip_launch_lm(h, LM_XENT_JOIN, (T + r.lanes - 1) / r.lanes, 1, 1024, &r)) != BWPP_HIP_OK) return s;
   return sums && T > 64 ? bwpp_hip_launch_lm(h, LM_XENT_SUMS, 1, 1, 1024, &r) : BWPP_HIP_OK;
 }
 

@@ -231,7 +231,7 @@ typedef struct {
  * z = scale x W, W [dim x vocab] (trans_w: stored [vocab x dim]), without the
  * logits in memory (no reference counterpart; its compiler has no loss). */
 typedef struct {
-  uint32_t rows; /* tokens */
+  uint32_t rows; /* tokens, fewer than 2^27 */
   uint32_t vocab;
   uint32_t dim;
   uint32_t ldx, ldw;   /* row strides of the stored matrices; 0 = contiguous */

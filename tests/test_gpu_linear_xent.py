@@ -267,6 +267,20 @@ def test_extreme_logits(be, dtype):
     assert bool(torch.isposinf(lse).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [1, 17, 64, 65, 300])
+def test_outputs_left_out(be, dtype, T):
+    x, w, t = _case(T, 64, 200, dtype, "vd", 2)
+    t[T // 2] = -1
+    p = _params(T, 64, 200, dtype, "vd", x, w)
+    full = torch.empty(T, device="cuda"), torch.empty(T, device="cuda"), torch.empty(2, device="cuda")
+    be.dispatch_linear_xent(x, w, t, *full, p)
+    for keep in (0, 1, 2):
+        got = [torch.empty_like(v) if i == keep else None for i, v in enumerate(full)]
+        be.dispatch_linear_xent(x, w, t, *got, p)
+        assert torch.equal(got[keep], full[keep])
+
+
 def test_no_rows(be):
     w = torch.ones(20, 16, device="cuda")
     t = torch.zeros(1, device="cuda", dtype=torch.int32)

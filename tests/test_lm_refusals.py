@@ -71,6 +71,7 @@ def test_rotary_aliases():
     for q, k, qo, ko, kw in alias:
         st, msg = _lib_call("rotary", q, k, None, qo, ko, _rot(**kw))
         assert st == S.ALIAS, (st, msg, kw)
+    assert _lib_call("rotary", A, B, C + n - 4, C, D, _rot())[0] == S.ALIAS  # positions on qo's last element
     # in place, and q, k side by side in one fused row: taken (the handle is missing)
     fused = dict(ldq=512, ldk=512, ldqo=512, ldko=512, q_head_stride=64, k_head_stride=64, qo_head_stride=64,
                  ko_head_stride=64, q_batch_stride=4096, k_batch_stride=4096, qo_batch_stride=4096,
@@ -144,7 +145,7 @@ def test_linear_xent_refusals():
         for name, args in (("linear_xent", ok), ("linear_xent_grad", (A, B, C, D, None, E, F))):
             st, msg = _lib_call(name, *args, _xent(**kw))
             assert st == S.INVALID_ARG and name in msg, kw
-    for kw in (dict(dtype=1, dim=7), dict(dtype=1, trans_w=0, vocab=7), dict(rows=1 << 31), dict(vocab=1 << 31)):
+    for kw in (dict(dtype=1, dim=7), dict(dtype=1, trans_w=0, vocab=7), dict(rows=1 << 27), dict(vocab=1 << 31)):
         assert _lib_call("linear_xent", *ok, _xent(**kw))[0] == S.UNSUPPORTED, kw
     for args in ((A, B, C, A, E, F), (A, B, C, D, D, F), (A, B, C, D, E, E + 28), (A, B, C, C + 4, E, F)):
         assert _lib_call("linear_xent", *args, _xent())[0] == S.ALIAS, args
