@@ -457,8 +457,9 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_clear(const BwppXent
 BWPP_XENT_ROWS(bf16, uint16_t)
 BWPP_XENT_ROWS(f32, float)
 
-// bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 (K in steps of 32), r32 and
-// r128 any size (32 x 64, 128 x 128), _u with operands through registers.
+// bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 (K in steps of 32); any
+// sizes: r32 = 32 x 64, r64 = 64 x 64, r128 = 128 x 128, _u with operands through
+// registers.
 #define BWPP_XENT_PIPE(KIND, EPI, TB)                                                                     \
   extern "C" __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) \
   void bwpp_xent_##KIND##_p_t0##TB(const BwppXentArgs a) {                                                \
@@ -483,6 +484,8 @@ void bwpp_xent_rows_p_t10(const BwppXentArgs a) {
   BWPP_XENT_PIPE(sums, EpiSums, TB)                                         \
   BWPP_XENT_RING(stats, EpiStats, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)     \
   BWPP_XENT_RING(grad, EpiGrad, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)       \
+  BWPP_XENT_RING(stats, EpiStats, TB, r64, 64, 64, 2, 2, 2, 4, 2, 4, 2)     \
+  BWPP_XENT_RING(grad, EpiGrad, TB, r64, 64, 64, 2, 2, 2, 4, 2, 4, 2)       \
   BWPP_XENT_RING(stats, EpiStats, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)  \
   BWPP_XENT_RING(grad, EpiGrad, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)    \
   BWPP_XENT_RING(sums, EpiSums, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)

@@ -27,9 +27,9 @@ enum LmKernel {
   LM_XENT_COPY,                          // [bf16]
   LM_XENT_ZERO = LM_XENT_COPY + 2,       // [bf16]
   LM_XENT_STATS = LM_XENT_ZERO + 2,      // [trans_w][XentTile]
-  LM_XENT_GRAD = LM_XENT_STATS + 10,
-  LM_XENT_RAW = LM_XENT_GRAD + 10,
-  LM_XENT_ROWS = LM_XENT_RAW + 10,
+  LM_XENT_GRAD = LM_XENT_STATS + 14,
+  LM_XENT_RAW = LM_XENT_GRAD + 14,
+  LM_XENT_ROWS = LM_XENT_RAW + 14,
   LM_COUNT
 };
 
@@ -66,21 +66,29 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_xent_stats_p_t00",
     "bwpp_xent_stats_r32_t00",
     "bwpp_xent_stats_r32_t00_u",
+    "bwpp_xent_stats_r64_t00",
+    "bwpp_xent_stats_r64_t00_u",
     "bwpp_xent_stats_r128_t00",
     "bwpp_xent_stats_r128_t00_u",
     "bwpp_xent_stats_p_t01",
     "bwpp_xent_stats_r32_t01",
     "bwpp_xent_stats_r32_t01_u",
+    "bwpp_xent_stats_r64_t01",
+    "bwpp_xent_stats_r64_t01_u",
     "bwpp_xent_stats_r128_t01",
     "bwpp_xent_stats_r128_t01_u",
     "bwpp_xent_grad_p_t00",
     "bwpp_xent_grad_r32_t00",
     "bwpp_xent_grad_r32_t00_u",
+    "bwpp_xent_grad_r64_t00",
+    "bwpp_xent_grad_r64_t00_u",
     "bwpp_xent_grad_r128_t00",
     "bwpp_xent_grad_r128_t00_u",
     "bwpp_xent_grad_p_t01",
     "bwpp_xent_grad_r32_t01",
     "bwpp_xent_grad_r32_t01_u",
+    "bwpp_xent_grad_r64_t01",
+    "bwpp_xent_grad_r64_t01_u",
     "bwpp_xent_grad_r128_t01",
     "bwpp_xent_grad_r128_t01_u",
     "bwpp_xent_sums_p_t00",
@@ -88,7 +96,11 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_xent_sums_r128_t00_u",
     "bwpp_xent_sums_r128_t00",
     "bwpp_xent_sums_r128_t00_u",
+    "bwpp_xent_sums_r128_t00",
+    "bwpp_xent_sums_r128_t00_u",
     "bwpp_xent_sums_p_t01",
+    "bwpp_xent_sums_r128_t01",
+    "bwpp_xent_sums_r128_t01_u",
     "bwpp_xent_sums_r128_t01",
     "bwpp_xent_sums_r128_t01_u",
     "bwpp_xent_sums_r128_t01",
@@ -435,23 +447,47 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const 
 
 namespace {
 
-enum XentTile { XT_P, XT_R32, XT_R32U, XT_R128, XT_R128U };
+enum XentTile { XT_P, XT_R32, XT_R32U, XT_R64, XT_R64U, XT_R128, XT_R128U, XT_COUNT };
 struct XentShape {
   uint32_t bm, bn, threads;
+  double lat, inc, more;  // see xent_tile
 };
-const XentShape kXentShapes[5] = {{256, 256, 512}, {32, 64, 128}, {32, 64, 128}, {128, 128, 256}, {128, 128, 256}};
+const XentShape kXentShapes[XT_COUNT] = {
+    {256, 256, 512, 0.0247, 0.0247, 3.0},  {32, 64, 128, 0.0039, 0.0032, 1.5},   {32, 64, 128, 0.0085, 0.0021, 1.5},
+    {64, 64, 256, 0.0046, 0.0031, 0.6},    {64, 64, 256, 0.0088, 0.0040, 0.6},   {128, 128, 256, 0.0114, 0.0074, 1.4},
+    {128, 128, 256, 0.0185, 0.0099, 1.4}};
 
 bool on16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
-// The tile for a product A [M x K] op(B) [K x N] in the loops of gemm_bf16.h:
-// the DMA reads whole 16-byte chunks, the 256-wide tiles K in steps of 32.
-XentTile xent_tile(const BwppGemmArgs &g, bool tb, bool few_rows) {
+// The tile for a product A [M x K] op(B) [K x N] in the loops of gemm_bf16.h and
+// gemm_bf16_k32.h: the DMA reads whole 16-byte chunks, the 256-wide tiles K in
+// steps of 32; among those that can run, the one with the least modelled time.  n
+// blocks on a CU take lat + (n - 1) inc us per K element and `more` each beyond the
+// first (the constants that dispatch_matmul's choice was fitted with; 0.0247 for a
+// round of 256-wide tiles, 8192^3 in 790 us), and no product runs faster than its
+// operands arrive (5.6 TB/s).  Without small tiles (RAW sums) 128 x 128.
+XentTile xent_tile(const BwppHip *h, const BwppGemmArgs &g, bool tb, bool small) {
   const bool dma = on16(g.a) && on16(g.b) && g.lda % 8 == 0 && g.ldb % 8 == 0 && g.K % 8 == 0 && (tb || g.N % 8 == 0) &&
                    256ull * std::max(g.lda, g.ldb) < (1ull << 31);
-  if (dma && g.K % 32 == 0 && g.M > 128) return XT_P;
-  if (few_rows && g.M <= 32) return dma ? XT_R32 : XT_R32U;
-  return dma ? XT_R128 : XT_R128U;
+  const uint64_t cus = cus_of(h);
+  const double mem = ((double)g.M * g.K + (double)g.K * g.N) * 2.0 / 5.6e6;
+  XentTile best = dma ? XT_R128 : XT_R128U;
+  double best_us = 1e300;
+  for (int t = 0; t < XT_COUNT; ++t) {
+    const bool wide = t == XT_P, direct = wide || t == XT_R32 || t == XT_R64 || t == XT_R128;
+    if (direct != dma || (wide && (g.K % 32 != 0 || g.M <= 128)) || (!small && t >= XT_R32 && t <= XT_R64U)) continue;
+    const XentShape &sh = kXentShapes[t];
+    const uint64_t tiles = ((g.M + (uint64_t)sh.bm - 1) / sh.bm) * ((g.N + (uint64_t)sh.bn - 1) / sh.bn);
+    if (tiles * sh.threads > 0xffffffffull) continue;
+    const double n = (double)((tiles + cus - 1) / cus);
+    const double us = std::max(mem, (n - 1.0) * sh.more + g.K * (sh.lat + (n - 1.0) * sh.inc));
+    if (us < best_us * 0.999) {
+      best_us = us;
+      best = (XentTile)t;
+    }
+  }
+  return best;
 }
 
 BwppHipStatus xent_product(BwppHip *h, int first, BwppXentArgs &a, bool tb, XentTile tile, uint32_t split) {
@@ -465,7 +501,7 @@ BwppHipStatus xent_product(BwppHip *h, int first, BwppXentArgs &a, bool tb, Xent
   const uint64_t tiles = (uint64_t)a.g.tiles_m * a.g.tiles_n;
   if (tiles > 0xffffffffull)
     return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "linear_xent: too many tiles");
-  return bwpp_hip_launch_lm(h, first + (tb ? 5 : 0) + tile, tiles * split, 1, sh.threads, &a);
+  return bwpp_hip_launch_lm(h, first + (tb ? XT_COUNT : 0) + tile, tiles * split, 1, sh.threads, &a);
 }
 
 // Columns of a product on 256-wide tiles that smaller ones take instead: where
@@ -605,7 +641,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x
     a.target = targets;
     a.vocab = p.vocab;
     a.scale = r.scale;
-    const XentTile tile = xent_tile(a.g, p.trans_w != 0, true);
+    const XentTile tile = xent_tile(h, a.g, p.trans_w != 0, true);
     r.nparts = xent_tiles_n(h, a.g, tile);
     if ((s = bwpp_hip_take_workspace(h, zt_bytes + loss_bytes + (uint64_t)r.nparts * T * 8, &ws)) != BWPP_HIP_OK) return s;
     a.zt = static_cast<float *>(ws);
@@ -746,7 +782,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.dl = static_cast<uint16_t *>(z);
       a.ldl = (uint32_t)ldp;
       a.rows_up = (uint32_t)Tu;
-      if ((s = xent_logits(h, LM_XENT_GRAD, a, tw, xent_tile(a.g, tw, true))) != BWPP_HIP_OK) return s;
+      if ((s = xent_logits(h, LM_XENT_GRAD, a, tw, xent_tile(h, a.g, tw, true))) != BWPP_HIP_OK) return s;
     } else {
       if ((s = xent_logits_f32(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(z), n0,
                                n, p, m)) != BWPP_HIP_OK)
@@ -780,7 +816,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
           rest.g.b = static_cast<const uint16_t *>(rest.g.b) + (tw ? (uint64_t)a.g.K * m.ldw : a.g.K);
           rest.accumulate = 1;
         }
-        if ((s = xent_product(h, LM_XENT_RAW, rest, !tw, xent_tile(rest.g, !tw, false), 1)) != BWPP_HIP_OK) return s;
+        if ((s = xent_product(h, LM_XENT_RAW, rest, !tw, xent_tile(h, rest.g, !tw, false), 1)) != BWPP_HIP_OK) return s;
       }
     } else if (dx) {
       BwppMatmulParams g = {};
