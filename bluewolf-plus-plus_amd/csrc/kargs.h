@@ -199,6 +199,13 @@ typedef struct {
   uint32_t workers, group, split, span, nparts;
 } BwppResNormArgs;
 
+/* Planes of bf16 terms of fp32 operands (gemm_bf16_k32.h): nibble t of *_planes
+ * is the plane of the t-th of six products, planes are *_stride elements apart. */
+typedef struct {
+  uint32_t a_planes, b_planes;
+  uint64_t a_stride, b_stride;
+} BwppSplitTerms;
+
 /* Cross entropy of hidden states against a vocabulary (xent.h).  Logits
  * z = scale op(W) x: g holds their product (M tokens, N of the columns n_base
  * .. of the vocabulary, K = dim). */
@@ -220,6 +227,9 @@ typedef struct {
   uint32_t rows_out, cols_out; /* rows product: what is stored of g.M x g.N */
   uint32_t accumulate; /* sums: add to what is there */
   float *raw;          /* sums: [ksplit][M][N] */
+  BwppSplitTerms terms; /* fp32 operands in bf16 terms */
+  uint64_t dl_stride;   /* gradient in terms: its three planes' distance; ... */
+  uint32_t cols_up;     /* ... its columns, zeros behind N */
 } BwppXentArgs;
 
 /* Its row kernels. */
@@ -238,7 +248,8 @@ typedef struct {
   uint32_t n_base, vocab;
   uint32_t nparts; /* partials a row, or planes of sums */
   uint32_t dloss_scalar;
-  uint32_t lanes; /* join: rows a block */
+  uint32_t lanes; /* join: rows a block; terms: threads a row */
+  uint64_t plane; /* terms: distance of the planes */
   float scale;
 } BwppXentRowArgs;
 

@@ -8,8 +8,8 @@
 //
 // A target outside the vocabulary leaves its row out: loss and gradients 0.
 //
-// bf16: the logits' product runs on the matrix cores (gemm_bf16_k32.h's loop, and
-// gemm_bf16.h's for any sizes)
+// bf16: the logits' product runs on the matrix cores (gemm_bf16_k32.h's loop on 256 x
+// 256 tiles, gemm_bf16.h's on 32 x 64 to 128 x 128 and for any sizes)
 // and stays in its accumulators.  The forward's epilogue reduces each tile's
 // rows to (max, sum of exp), a pair per row and tile, and a second kernel
 // joins the pairs.  The gradient's epilogue turns the same product, made
@@ -19,8 +19,14 @@
 // one piece of the vocabulary at a time, small enough to stay in the Infinity
 // Cache between its writer and its readers.  dx is summed over the pieces in
 // fp32 planes (one per K split) and rounded once; each piece's dW is final.
-// fp32: the logits of a piece go through memory once, in fp32 (8 to 16 bytes a
-// logit beside 2 dim FLOPs at a sixteenth of the bf16 rate).
+// fp32, few tokens: the logits of a piece go through memory once, in fp32 (8 to 16
+// bytes a logit beside 2 dim FLOPs at a sixteenth of the bf16 rate).  More: x, W and
+// dz as three bf16 terms each (gemm_bf16_k32.h), and all as in bf16; the gradient's
+// epilogue leaves dz's terms, and dW is fp32.  What it costs beside the products is
+// a pass over W a call (4 bytes read and 8 written an element, 17 us for 8003 x
+// 1021).  777 x 1021 x 8003 train: 604 us on fp32 matrix instructions, 428 so, and
+// off by 3e-7 of the result; 4096 x 2048 x 8000 4450 and 2630.  A dz that overflows
+// to an infinity leaves NaN where fp32 products could leave the infinity.
 //
 // Maxima and sums are fp32, the last logarithm 64-bit (once a row): lse is off
 // by a few 2^-24 of itself.  exp(z - max) is taken as exp2 of the rounded
@@ -204,6 +210,99 @@ struct EpiRows {
       } else {
         for (uint32_t e = 0; e < 8 && n + e < a.cols_out; ++e) dst[e] = h[e];
       }
+    }
+  }
+};
+
+// dz scale in three bf16 planes (v1 + v2 + v3 = dz to 24 bits).
+struct EpiGradTerms {
+  static constexpr bool kStore = false;
+  const BwppXentArgs &a;
+
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t, uint32_t,
+                                      int tid, int wm, int wn) const {
+    constexpr int TM = BM / WM, TN = BN / WN, NT = 64 * WM * WN, kCld = BN + 8;
+    const int lane = tid & 63;
+    uint16_t *cs = reinterpret_cast<uint16_t *>(smem);  // [BM][BN + 8]
+    const uint32_t nw = n0 + (uint32_t)(wn * TN);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t m = m0 + (uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane);
+      uint32_t t = 0xffffffffu;
+      float lse = 0.0f, g = 0.0f;
+      if (m < a.g.M) {
+        t = (uint32_t)a.target[m];
+        lse = a.lse[m];
+        g = (a.dloss ? a.dloss[a.dloss_scalar ? 0u : m] : 1.0f) * a.scale;
+      }
+      const bool live = t < a.vocab;
+      const uint32_t tl = t - a.n_base;
+      each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t n) {
+        const float p = exp_diff(acc[i][j][r] * a.scale, lse);
+        acc[i][j][r] = live && n < a.g.N ? g * (n == tl ? p - 1.0f : p) : 0.0f;
+      });
+    }
+#pragma unroll 1
+    for (int plane = 0; plane < 3; ++plane) {
+      if (plane > 0) __syncthreads();  // the plane before has left LDS
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int r = 0; r < FR::kRegs; r += 4) {
+            uint2 o;
+            o.x = pack_bf16x2(acc[i][j][r], acc[i][j][r + 1]);
+            o.y = pack_bf16x2(acc[i][j][r + 2], acc[i][j][r + 3]);
+            *reinterpret_cast<uint2 *>(cs + ((uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane)) * kCld + wn * TN +
+                                       i * FR::kSize + FR::col(lane, r)) = o;
+            acc[i][j][r] -= __uint_as_float(o.x << 16);  // exact
+            acc[i][j][r + 1] -= __uint_as_float(o.x & 0xffff0000u);
+            acc[i][j][r + 2] -= __uint_as_float(o.y << 16);
+            acc[i][j][r + 3] -= __uint_as_float(o.y & 0xffff0000u);
+          }
+      __syncthreads();
+      uint16_t *dl = a.dl + plane * a.dl_stride;
+#pragma unroll 4
+      for (int it = 0; it < BM * (BN / 8) / NT; ++it) {
+        const int q = tid + it * NT, row = q / (BN / 8), c = q % (BN / 8);
+        const uint32_t m = m0 + (uint32_t)row, n = n0 + 8u * (uint32_t)c;
+        if (m < a.rows_up && n < a.cols_up)
+          *reinterpret_cast<uint4 *>(dl + (size_t)m * a.ldl + n) = *reinterpret_cast<const uint4 *>(cs + row * kCld + c * 8);
+      }
+    }
+  }
+};
+
+// fp32 rows (dW), at any address and row stride.
+struct EpiRowsF32 {
+  static constexpr bool kStore = false;
+  const BwppXentArgs &a;
+
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *, uint32_t m0, uint32_t n0, uint32_t, uint32_t,
+                                      int tid, int wm, int wn) const {
+    constexpr int TM = BM / WM, TN = BN / WN;
+    const int lane = tid & 63;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t m = m0 + (uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane);
+      if (m >= a.rows_out) continue;
+      float *row = static_cast<float *>(a.g.c) + (size_t)m * a.g.ldc;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int r = 0; r < FR::kRegs; r += 4) {
+          const uint32_t n = n0 + (uint32_t)(wn * TN + i * FR::kSize) + FR::col(lane, r);
+          if (n + 4 <= a.cols_out) {
+            store4(row + n, make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.cols_out) row[n + e] = acc[i][j][r + e];
+          }
+        }
     }
   }
 };
@@ -428,17 +527,64 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_grad_f32(const BwppX
   }
 }
 
-// Planes of fp32 sums -> bf16 rows, rows that are left out 0.
-extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_bf16(const BwppXentRowArgs a) {
+// Planes of fp32 sums -> rows of T, rows that are left out 0.
+template <class T>
+__device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
   const uint64_t plane = (uint64_t)a.rows * a.cols;
   for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const bool on = live(a, row);
-    uint16_t *y = static_cast<uint16_t *>(a.y) + row * a.ldy;
+    const bool on = !a.target || live(a, row);
+    T *y = static_cast<T *>(a.y) + row * a.ldy;
     const float *src = a.src + (uint64_t)row * a.cols;
     for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
       float v = src[c];
       for (uint32_t i = 1; i < a.nparts; ++i) v += src[i * plane + c];
-      y[c] = on ? f32_to_bf16_bits(v) : (uint16_t)0;
+      y[c] = to<T>(on ? v : 0.0f);
+    }
+  }
+}
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_bf16(const BwppXentRowArgs a) { sum_planes<uint16_t>(a); }
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_f32(const BwppXentRowArgs a) { sum_planes<float>(a); }
+
+// fp32 rows (x, any strides) -> four bf16 planes [rows_up][ldy]: v1, v1 where it
+// is finite, v2, v3 (gemm_bf16_k32.h); zeros past the rows and columns and, with
+// targets, in rows that are left out.
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_terms(const BwppXentRowArgs a) {
+  const uint32_t step = 256u / a.lanes, c0 = (threadIdx.x & (a.lanes - 1u)) * 8u;  // `lanes` threads a row
+  for (uint32_t row = blockIdx.x * step + threadIdx.x / a.lanes; row < a.rows_up; row += gridDim.x * step) {
+    const bool on = row < a.rows && (!a.target || live(a, row));
+    const float *x = static_cast<const float *>(a.x) + row * a.ldx;
+    uint16_t *y = static_cast<uint16_t *>(a.y) + row * a.ldy;
+    for (uint32_t c = c0; c < a.ldy; c += a.lanes * 8u) {
+      float v[8];
+      if (on && c + 8 <= a.cols) {
+        const float4 p = load4(x + c), q = load4(x + c + 4);
+        v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w, v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = on && c + e < a.cols ? x[c + e] : 0.0f;
+      }
+      uint16_t t1[8], tf[8], t2[8], t3[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool fin = __builtin_isfinite(v[e]);
+        uint16_t h = f32_to_bf16_bits(v[e]);
+        if (fin && !__builtin_isfinite(bf16_bits_to_f32(h))) h = (uint16_t)(__float_as_uint(v[e]) >> 16);  // no overflow
+        const float r = fin ? v[e] - bf16_bits_to_f32(h) : 0.0f;
+        t1[e] = h;
+        tf[e] = fin ? h : 0;
+        t2[e] = f32_to_bf16_bits(r);
+        t3[e] = f32_to_bf16_bits(r - bf16_bits_to_f32(t2[e]));
+      }
+      auto store = [&](int plane, const uint16_t (&t)[8]) {
+        uint4 o;
+        o.x = t[0] | (uint32_t)t[1] << 16, o.y = t[2] | (uint32_t)t[3] << 16;
+        o.z = t[4] | (uint32_t)t[5] << 16, o.w = t[6] | (uint32_t)t[7] << 16;
+        *reinterpret_cast<uint4 *>(y + plane * a.plane + c) = o;
+      };
+      store(0, t1);
+      store(1, tf);
+      store(2, t2);
+      store(3, t3);
     }
   }
 }
@@ -457,18 +603,14 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_clear(const BwppXent
 BWPP_XENT_ROWS(bf16, uint16_t)
 BWPP_XENT_ROWS(f32, float)
 
-// bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 (K in steps of 32); any
-// sizes: r32 = 32 x 64, r64 = 64 x 64, r128 = 128 x 128, _u with operands through
-// registers.
-#define BWPP_XENT_PIPE(KIND, EPI, TB)                                                                     \
+// bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 (K in steps of
+// 32), sp and sh = 256 x 256 and 128 x 256 for fp32 in terms; any sizes: r32 = 32 x 64, r64 = 64 x 64,
+// r128 = 128 x 128, _u with operands through registers.
+#define BWPP_XENT_K32(NAME, EPI, TA, TB, BM, SPLIT)                                                       \
   extern "C" __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) \
-  void bwpp_xent_##KIND##_p_t0##TB(const BwppXentArgs a) {                                                \
-    gemm_bf16_k32<false, TB != 0, TB != 0, EPI>(a.g, EPI{a});                                             \
+  void bwpp_xent_##NAME(const BwppXentArgs a) {                                                           \
+    gemm_bf16_k32<TA != 0, TB != 0, BM, TB != 0, SPLIT, EPI>(a.g, EPI{a}, a.terms);                       \
   }
-extern "C" __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2)))
-void bwpp_xent_rows_p_t10(const BwppXentArgs a) {
-  gemm_bf16_k32<true, false, false, EpiRows>(a.g, EpiRows{a});
-}
 #define BWPP_XENT_RING(KIND, EPI, TB, NAME, BM, BN, WM, WN, KPS, STAGES, WPE, KPSU, WPEU)                       \
   extern "C" __global__ __launch_bounds__(64 * WM * WN, WPE) void bwpp_xent_##KIND##_##NAME##_t0##TB(           \
       const BwppXentArgs a) {                                                                                   \
@@ -479,9 +621,15 @@ void bwpp_xent_rows_p_t10(const BwppXentArgs a) {
     gemm_bf16_ring<false, TB != 0, BM, BN, WM, WN, KPSU, 2, true, EPI>(a.g, EPI{a});                            \
   }
 #define BWPP_XENT_TB(TB)                                                    \
-  BWPP_XENT_PIPE(stats, EpiStats, TB)                                       \
-  BWPP_XENT_PIPE(grad, EpiGrad, TB)                                         \
-  BWPP_XENT_PIPE(sums, EpiSums, TB)                                         \
+  BWPP_XENT_K32(stats_p_t0##TB, EpiStats, 0, TB, 256, false)                \
+  BWPP_XENT_K32(grad_p_t0##TB, EpiGrad, 0, TB, 256, false)                  \
+  BWPP_XENT_K32(sums_p_t0##TB, EpiSums, 0, TB, 256, false)                  \
+  BWPP_XENT_K32(stats_sp_t0##TB, EpiStats, 0, TB, 256, true)                \
+  BWPP_XENT_K32(grad_sp_t0##TB, EpiGradTerms, 0, TB, 256, true)             \
+  BWPP_XENT_K32(sums_sp_t0##TB, EpiSums, 0, TB, 256, true)                  \
+  BWPP_XENT_K32(stats_sh_t0##TB, EpiStats, 0, TB, 128, true)                \
+  BWPP_XENT_K32(grad_sh_t0##TB, EpiGradTerms, 0, TB, 128, true)             \
+  BWPP_XENT_K32(sums_sh_t0##TB, EpiSums, 0, TB, 128, true)                  \
   BWPP_XENT_RING(stats, EpiStats, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)     \
   BWPP_XENT_RING(grad, EpiGrad, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)       \
   BWPP_XENT_RING(stats, EpiStats, TB, r64, 64, 64, 2, 2, 2, 4, 2, 4, 2)     \
@@ -491,5 +639,10 @@ void bwpp_xent_rows_p_t10(const BwppXentArgs a) {
   BWPP_XENT_RING(sums, EpiSums, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)
 BWPP_XENT_TB(0)
 BWPP_XENT_TB(1)
+BWPP_XENT_K32(rows_p_t10, EpiRows, 1, 0, 256, false)
+BWPP_XENT_K32(rows_sp_t10, EpiRowsF32, 1, 0, 256, true)
+BWPP_XENT_K32(rows_sh_t10, EpiRowsF32, 1, 0, 128, true)
+BWPP_XENT_K32(sums_sp_t10, EpiSums, 1, 0, 256, true)
+BWPP_XENT_K32(sums_sh_t10, EpiSums, 1, 0, 128, true)
 
 }  // namespace xent

@@ -22,15 +22,21 @@ enum LmKernel {
   LM_XENT_SUMS,
   LM_XENT_STATS_F32,
   LM_XENT_GRAD_F32,
-  LM_XENT_ROUND,
-  LM_XENT_CLEAR,
+  LM_XENT_TERMS,
+  LM_XENT_ROUND,                         // [bf16]
+  LM_XENT_CLEAR = LM_XENT_ROUND + 2,
   LM_XENT_COPY,                          // [bf16]
   LM_XENT_ZERO = LM_XENT_COPY + 2,       // [bf16]
   LM_XENT_STATS = LM_XENT_ZERO + 2,      // [trans_w][XentTile]
   LM_XENT_GRAD = LM_XENT_STATS + 14,
   LM_XENT_RAW = LM_XENT_GRAD + 14,
   LM_XENT_ROWS = LM_XENT_RAW + 14,
-  LM_COUNT
+  LM_TERMS_STATS,                        // [trans_w][TermsTile]
+  LM_TERMS_GRAD = LM_TERMS_STATS + 4,
+  LM_TERMS_RAW = LM_TERMS_GRAD + 4,
+  LM_TERMS_ROWS = LM_TERMS_RAW + 4,      // [TermsTile]
+  LM_TERMS_RAW_T = LM_TERMS_ROWS + 2,    // [TermsTile]
+  LM_COUNT = LM_TERMS_RAW_T + 2
 };
 
 // Rows in registers (resnorm.h): elements a thread and waves a row.
@@ -61,7 +67,7 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_resnorm_grad_bf16_any",
     "bwpp_resnorm_finish_f32",      "bwpp_resnorm_finish_bf16",
     "bwpp_xent_join", "bwpp_xent_sums", "bwpp_xent_stats_f32", "bwpp_xent_grad_f32",
-    "bwpp_xent_round_bf16", "bwpp_xent_clear", "bwpp_xent_copy_f32", "bwpp_xent_copy_bf16",
+    "bwpp_xent_terms", "bwpp_xent_round_f32", "bwpp_xent_round_bf16", "bwpp_xent_clear", "bwpp_xent_copy_f32", "bwpp_xent_copy_bf16",
     "bwpp_xent_zero_f32", "bwpp_xent_zero_bf16",
     "bwpp_xent_stats_p_t00",
     "bwpp_xent_stats_r32_t00",
@@ -106,6 +112,22 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_xent_sums_r128_t01",
     "bwpp_xent_sums_r128_t01_u",
     "bwpp_xent_rows_p_t10",
+    "bwpp_xent_stats_sp_t00",
+    "bwpp_xent_stats_sh_t00",
+    "bwpp_xent_stats_sp_t01",
+    "bwpp_xent_stats_sh_t01",
+    "bwpp_xent_grad_sp_t00",
+    "bwpp_xent_grad_sh_t00",
+    "bwpp_xent_grad_sp_t01",
+    "bwpp_xent_grad_sh_t01",
+    "bwpp_xent_sums_sp_t00",
+    "bwpp_xent_sums_sh_t00",
+    "bwpp_xent_sums_sp_t01",
+    "bwpp_xent_sums_sh_t01",
+    "bwpp_xent_rows_sp_t10",
+    "bwpp_xent_rows_sh_t10",
+    "bwpp_xent_sums_sp_t10",
+    "bwpp_xent_sums_sh_t10",
 };
 const int bwpp_hip_lm_kernel_count = (int)(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]));
 static_assert(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]) == LM_COUNT, "kernel names");
@@ -466,7 +488,9 @@ uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 // blocks on a CU take lat + (n - 1) inc us per K element and `more` each beyond the
 // first (the constants that dispatch_matmul's choice was fitted with; 0.0247 for a
 // round of 256-wide tiles, 8192^3 in 790 us), and no product runs faster than its
-// operands arrive (5.6 TB/s).  Without small tiles (RAW sums) 128 x 128.
+// operands arrive (5.6 TB/s; four fifths of it in the 128-byte pieces that 64
+// columns take of row-major B: 42 x 704 x 69376 train 140 us on 64 x 64 tiles, 135
+// on 128 x 128).  Without small tiles (RAW sums) 128 x 128.
 XentTile xent_tile(const BwppHip *h, const BwppGemmArgs &g, bool tb, bool small) {
   const bool dma = on16(g.a) && on16(g.b) && g.lda % 8 == 0 && g.ldb % 8 == 0 && g.K % 8 == 0 && (tb || g.N % 8 == 0) &&
                    256ull * std::max(g.lda, g.ldb) < (1ull << 31);
@@ -481,7 +505,8 @@ XentTile xent_tile(const BwppHip *h, const BwppGemmArgs &g, bool tb, bool small)
     const uint64_t tiles = ((g.M + (uint64_t)sh.bm - 1) / sh.bm) * ((g.N + (uint64_t)sh.bn - 1) / sh.bn);
     if (tiles * sh.threads > 0xffffffffull) continue;
     const double n = (double)((tiles + cus - 1) / cus);
-    const double us = std::max(mem, (n - 1.0) * sh.more + g.K * (sh.lat + (n - 1.0) * sh.inc));
+    const double fetch = !tb && sh.bn == 64 ? mem * 1.25 : mem;
+    const double us = std::max(fetch, (n - 1.0) * sh.more + g.K * (sh.lat + (n - 1.0) * sh.inc));
     if (us < best_us * 0.999) {
       best_us = us;
       best = (XentTile)t;
@@ -593,6 +618,263 @@ BwppHipStatus xent_logits_f32(BwppHip *h, const float *x, const float *w, float 
   return bwpp_hip_dispatch_matmul(h, x, w + (p.trans_w ? (uint64_t)n0 * m.ldw : n0), z, nullptr, g);
 }
 
+// ---- fp32 operands in bf16 terms (gemm_bf16_k32.h)
+
+enum TermsTile { TT_P, TT_H };
+struct TermsShape {
+  uint32_t bm;
+  double us;  // a round of tiles, per K element of one of the six products
+};
+constexpr TermsShape kTermsShapes[2] = {{256, 0.0252}, {128, 0.0163}};
+
+// Terms of a matrix: four planes, or dz's three, of rows x cols up to multiples
+// of 32.
+struct Terms {
+  uint16_t *p;
+  uint64_t rows, cols;
+  uint64_t plane() const { return up(rows * cols, 128); }
+};
+Terms terms_of(void *p, uint64_t rows, uint64_t cols) { return {static_cast<uint16_t *>(p), up(rows, 32), up(cols, 32)}; }
+uint64_t terms_bytes(uint64_t rows, uint64_t cols, int planes) { return terms_of(nullptr, rows, cols).plane() * 2 * planes; }
+
+// Modelled time of a product M x N x K in terms, and the tile that has it.
+double terms_us(const BwppHip *h, uint64_t M, uint64_t N, uint64_t K, uint32_t split, TermsTile &tile) {
+  double best = 1e300;
+  for (int t = TT_P; t <= TT_H; ++t) {
+    const uint64_t tiles = ((M + kTermsShapes[t].bm - 1) / kTermsShapes[t].bm) * ((N + 255) / 256) * split, cus = cus_of(h);
+    const double us = 5.0 + (double)((tiles + cus - 1) / cus) * (3.0 + 6.0 * (double)((K + split - 1) / split) * kTermsShapes[t].us);
+    if (us < best) best = us, tile = (TermsTile)t;
+  }
+  return std::max(best, (double)(M + N) * K * 12.0 / 3e6);  // six planes of each, from the Infinity Cache
+}
+
+// The same with K in ranges, summed in planes, where that is modelled faster by
+// more than the planes cost.
+double terms_split_us(const BwppHip *h, uint64_t M, uint64_t N, uint64_t K, uint32_t &split, TermsTile &tile, bool planes) {
+  double best = terms_us(h, M, N, K, 1, tile) + (planes ? 5.0 + (double)M * N * 8.0 / 5e6 : 0.0);
+  split = 1;
+  for (uint32_t k = 2; k <= 8 && K / k >= 256; k *= 2) {
+    TermsTile t;
+    const double us = terms_us(h, M, N, K, k, t) + 5.0 + (double)k * M * N * 8.0 / 5e6;
+    if (us < best) best = us, split = k, tile = t;
+  }
+  const uint64_t range = split > 1 ? up((K + split - 1) / split, 128) : K;  // as terms_product cuts it
+  split = (uint32_t)((K + range - 1) / range);
+  return best;
+}
+
+// Columns of a piece: its terms and dz's (gradient) in 256 MiB, and whole rounds of
+// tiles of the logits, for few rows in up to 1 GiB.
+uint32_t terms_piece(const BwppHip *h, const BwppLinearXentParams &p, bool grad) {
+  const uint64_t bytes = 256 * (8 * up(p.dim, 32) + (grad ? 6 * up(p.rows, 32) : 0)), fits = kXentPiece / bytes;
+  TermsTile tile;
+  terms_us(h, p.rows, p.vocab, up(p.dim, 32), 1, tile);
+  const uint64_t tm = (p.rows + kTermsShapes[tile].bm - 1) / kTermsShapes[tile].bm;
+  const uint64_t round = std::min(std::max<uint64_t>(cus_of(h) / tm, 1), std::max<uint64_t>(4 * fits, 4));
+  const uint64_t n = std::min<uint64_t>(std::max<uint64_t>(fits / round, 1) * round * 256, 1u << 22);
+  return (uint32_t)std::min<uint64_t>(n, p.vocab);
+}
+
+// Whether a call's products go in terms: all of them as modelled, with the passes
+// that make x's and W's (12 bytes an element), against fp32 matrix products at what
+// they reach on such sizes (less where rows are no whole 16 bytes), logits through
+// memory.  Loss and gradient, us, fp32 against terms: 1024 x 2048 x 8000 302 + 858
+// against 248 + 599, 4096 x 2048 x 8000 1150 + 3295 against 683 + 1917; but 512 x 512
+// x 4000 40 + 95 against 74 + 152, 256 x 2048 x 32000 280 + 803 against 464 + 1095.
+bool xent_in_terms(const BwppHip *h, const BwppLinearXentParams &p, const XentMatrices &m, bool grad) {
+  const uint64_t K = up(p.dim, 32), T = p.rows;
+  if (T <= 128 || K > (1u << 22)) return false;
+  const uint32_t piece = terms_piece(h, p, grad);
+  const double D = p.dim, V = p.vocab, rate = m.ldx % 4 == 0 && m.ldw % 4 == 0 ? 105e6 : 80e6;
+  const double fp32 = 2.0 * T * D * V / rate + 10.0;
+  double us = ((double)T + V) * D * 12.0 / 5e6 + 8.0;
+  const double old = T * V * 8.0 / 4.5e6 + (grad ? 3.0 : 1.0) * fp32;
+  for (uint64_t n0 = 0; n0 < p.vocab && us < old; n0 += piece) {
+    const uint64_t n = std::min<uint64_t>(piece, p.vocab - n0);
+    TermsTile tile;
+    uint32_t split;
+    us += 5.0 + terms_us(h, T, n, K, 1, tile);
+    if (grad) us += terms_split_us(h, T, p.dim, up(n, 32), split, tile, true) + terms_split_us(h, p.dim, n, up(T, 32), split, tile, false);
+  }
+  return us < old;
+}
+
+BwppHipStatus make_terms(BwppHip *h, const float *src, uint64_t ld, uint64_t rows, uint64_t cols, const Terms &t,
+                         const int32_t *targets, uint32_t vocab) {
+  BwppXentRowArgs r = {};
+  r.x = src;
+  r.y = t.p;
+  r.ldx = ld;
+  r.ldy = t.cols;
+  r.rows = (uint32_t)rows;
+  r.cols = (uint32_t)cols;
+  r.rows_up = (uint32_t)t.rows;
+  r.plane = t.plane();
+  r.target = targets;
+  r.vocab = vocab;
+  r.lanes = 4;
+  while (r.lanes < 256 && r.lanes * 8 < t.cols) r.lanes *= 2;
+  const uint64_t blocks = (t.rows + 256 / r.lanes - 1) / (256 / r.lanes);
+  return bwpp_hip_launch_lm(h, LM_XENT_TERMS, std::min<uint64_t>(blocks, 32ull * cus_of(h)), 1, 256, &r);
+}
+
+// Six products as one.  Planes, smallest first: 3 = third, 2 = second, 1 = first
+// where finite, 0 = first; of dz 2, 1, 0.
+constexpr uint32_t kTermsA = 0x012213, kTermsAz = 0x001102, kTermsB = 0x021231, kTermsBz = 0x010120;
+BwppHipStatus terms_product(BwppHip *h, int first, BwppXentArgs &a, bool tb, const Terms &A, const Terms &B, bool za, bool zb,
+                            TermsTile tile, uint32_t split) {
+  a.g.a = A.p;
+  a.g.b = B.p;
+  a.g.lda = (uint32_t)A.cols;
+  a.g.ldb = (uint32_t)B.cols;
+  a.terms.a_planes = za ? kTermsAz : kTermsA;
+  a.terms.b_planes = zb ? kTermsBz : kTermsB;
+  a.terms.a_stride = A.plane();
+  a.terms.b_stride = B.plane();
+  a.g.tiles_m = (uint32_t)((a.g.M + (uint64_t)kTermsShapes[tile].bm - 1) / kTermsShapes[tile].bm);
+  a.g.tiles_n = (uint32_t)((a.g.N + 255ull) / 256);
+  a.g.group_m = 8;
+  a.g.kchunk = split > 1 ? (uint32_t)up((a.g.K + (uint64_t)split - 1) / split, 128) : a.g.K;
+  a.g.ksplit = (a.g.K + a.g.kchunk - 1) / a.g.kchunk;
+  const uint64_t tiles = (uint64_t)a.g.tiles_m * a.g.tiles_n * a.g.ksplit;
+  if (tiles * 512 > 0xffffffffull) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "linear_xent: too many tiles");
+  return bwpp_hip_launch_lm(h, first + (tb ? 2 : 0) + tile, tiles, 1, 512, &a);
+}
+
+// One piece of the vocabulary: W's rows or columns n0 .. n0 + n in terms.
+BwppHipStatus piece_terms(BwppHip *h, const float *w, const BwppLinearXentParams &p, const XentMatrices &m, uint32_t n0,
+                          uint32_t n, Terms &wt, void *room) {
+  wt = p.trans_w ? terms_of(room, n, p.dim) : terms_of(room, p.dim, n);
+  return make_terms(h, w + (p.trans_w ? (uint64_t)n0 * m.ldw : n0), m.ldw, p.trans_w ? n : p.dim, p.trans_w ? p.dim : n, wt,
+                    nullptr, 0);
+}
+
+BwppHipStatus terms_stats(BwppHip *h, const float *x, const float *w, const BwppLinearXentParams &p, const XentMatrices &m,
+                          uint64_t front, BwppXentRowArgs &r, void *&ws) {
+  const bool tw = p.trans_w != 0;
+  const uint64_t T = p.rows, K = up(p.dim, 32);
+  const uint32_t piece = terms_piece(h, p, false);
+  const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece;
+  // (a piece is a multiple of 256 columns, or the only one)
+  r.nparts = (uint32_t)((p.vocab + 255ull) / 256);
+  const uint64_t part_bytes = up((uint64_t)r.nparts * T * 8, 256), x_bytes = terms_bytes(T, p.dim, 4);
+  const uint64_t w_bytes = terms_bytes(piece, p.dim, 4);
+  BwppHipStatus s = bwpp_hip_take_workspace(h, front + part_bytes + x_bytes + w_bytes, &ws);
+  if (s != BWPP_HIP_OK) return s;
+  unsigned char *base = static_cast<unsigned char *>(ws) + front;
+  r.zt = static_cast<float *>(ws);
+  r.part = reinterpret_cast<float *>(base);
+  const Terms xt = terms_of(base + part_bytes, T, p.dim);
+  if ((s = make_terms(h, x, m.ldx, T, p.dim, xt, nullptr, 0)) != BWPP_HIP_OK) return s;
+  for (uint64_t i = 0; i < npieces; ++i) {
+    const uint32_t n0 = (uint32_t)(i * piece), n = std::min(piece, p.vocab - n0);
+    Terms wt;
+    if ((s = piece_terms(h, w, p, m, n0, n, wt, base + part_bytes + x_bytes)) != BWPP_HIP_OK) return s;
+    BwppXentArgs a = {};
+    a.g.M = p.rows;
+    a.g.N = n;
+    a.g.K = (uint32_t)K;
+    a.target = r.target;
+    a.vocab = p.vocab;
+    a.scale = r.scale;
+    a.n_base = n0;
+    a.part_base = n0 / 256;
+    a.zt = r.zt;
+    a.part = r.part;
+    TermsTile tile;
+    terms_us(h, a.g.M, a.g.N, K, 1, tile);
+    if ((s = terms_product(h, LM_TERMS_STATS, a, tw, xt, wt, false, false, tile, 1)) != BWPP_HIP_OK) return s;
+  }
+  return BWPP_HIP_OK;
+}
+
+BwppHipStatus terms_grad(BwppHip *h, const float *x, const float *w, float *dx, float *dw, const BwppLinearXentParams &p,
+                         const XentMatrices &m, BwppXentRowArgs &r) {
+  const bool tw = p.trans_w != 0;
+  const uint64_t T = p.rows, D = p.dim, K = up(D, 32);
+  const uint32_t piece = terms_piece(h, p, true);
+  const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece;
+  uint32_t split = 1, dw_split = 1;
+  TermsTile dx_tile, dw_tile;
+  terms_split_us(h, T, D, up(piece, 32), split, dx_tile, true);
+  terms_split_us(h, tw ? piece : D, tw ? D : piece, up(T, 32), dw_split, dw_tile, false);
+  const uint64_t x_bytes = terms_bytes(T, D, 4), w_bytes = terms_bytes(piece, D, 4), z_bytes = terms_bytes(T, piece, 3);
+  const uint64_t sum_bytes = dx ? up(split * T * D * 4, 256) : 0, dw_bytes = dw && dw_split > 1 ? dw_split * piece * D * 4 : 0;
+  void *ws = nullptr;
+  BwppHipStatus s = bwpp_hip_take_workspace(h, x_bytes + w_bytes + z_bytes + sum_bytes + dw_bytes, &ws);
+  if (s != BWPP_HIP_OK) return s;
+  unsigned char *base = static_cast<unsigned char *>(ws);
+  float *acc = reinterpret_cast<float *>(base + x_bytes + w_bytes + z_bytes);
+  const Terms xt = terms_of(base, T, D);
+  if ((s = make_terms(h, x, m.ldx, T, D, xt, r.target, p.vocab)) != BWPP_HIP_OK) return s;
+  for (uint64_t i = 0; i < npieces; ++i) {
+    const uint32_t n0 = (uint32_t)(i * piece), n = std::min(piece, p.vocab - n0);
+    Terms wt;
+    if ((s = piece_terms(h, w, p, m, n0, n, wt, base + x_bytes)) != BWPP_HIP_OK) return s;
+    const Terms zt = terms_of(base + x_bytes + w_bytes, T, n);
+    BwppXentArgs a = {};
+    TermsTile tile;
+    a.g.M = p.rows;
+    a.g.N = n;
+    a.g.K = (uint32_t)K;
+    a.target = r.target;
+    a.lse = r.lse_in;
+    a.dloss = r.dloss;
+    a.dloss_scalar = r.dloss_scalar;
+    a.vocab = p.vocab;
+    a.scale = r.scale;
+    a.n_base = n0;
+    a.dl = zt.p;
+    a.ldl = (uint32_t)zt.cols;
+    a.rows_up = (uint32_t)zt.rows;
+    a.cols_up = (uint32_t)zt.cols;
+    a.dl_stride = zt.plane();
+    terms_us(h, T, n, K, 1, tile);
+    if ((s = terms_product(h, LM_TERMS_GRAD, a, tw, xt, wt, false, false, tile, 1)) != BWPP_HIP_OK) return s;
+    if (dx) {
+      BwppXentArgs q = {};
+      q.g.M = p.rows;
+      q.g.N = p.dim;
+      q.g.K = (uint32_t)zt.cols;
+      q.raw = acc;
+      q.accumulate = i > 0;
+      // A last piece with fewer ranges leaves the others' sums as they are.
+      if ((s = terms_product(h, LM_TERMS_RAW, q, !tw, zt, wt, true, false, dx_tile, split)) != BWPP_HIP_OK) return s;
+    }
+    if (dw) {
+      BwppXentArgs q = {};
+      q.g.M = tw ? n : p.dim;
+      q.g.N = tw ? p.dim : n;
+      q.g.K = (uint32_t)xt.rows;
+      q.g.c = dw + (tw ? (uint64_t)n0 * m.lddw : n0);
+      q.g.ldc = (uint32_t)m.lddw;
+      q.rows_out = q.g.M;
+      q.cols_out = q.g.N;
+      q.raw = acc + sum_bytes / 4;
+      s = terms_product(h, dw_split > 1 ? LM_TERMS_RAW_T : LM_TERMS_ROWS, q, false, tw ? zt : xt, tw ? xt : zt, tw, !tw, dw_tile,
+                        dw_split);
+      if (s != BWPP_HIP_OK) return s;
+      if (dw_split > 1) {
+        BwppXentRowArgs f = {};
+        f.src = q.raw;
+        f.nparts = dw_split;
+        f.rows = q.g.M;
+        f.cols = q.g.N;
+        f.y = q.g.c;
+        f.ldy = m.lddw;
+        if ((s = bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, f.rows), 1, 256, &f)) != BWPP_HIP_OK) return s;
+      }
+    }
+  }
+  if (!dx) return BWPP_HIP_OK;
+  r.y = dx;
+  r.ldy = m.lddx;
+  r.cols = p.dim;
+  r.src = acc;
+  r.nparts = split;
+  return bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, T), 1, 256, &r);
+}
+
 }  // namespace
 
 extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const void *w,
@@ -649,6 +931,10 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x
     r.zt = a.zt;
     r.part = a.part;
     if ((s = xent_logits(h, LM_XENT_STATS, a, p.trans_w != 0, tile)) != BWPP_HIP_OK) return s;
+  } else if (xent_in_terms(h, p, m, false)) {
+    if ((s = terms_stats(h, static_cast<const float *>(x), static_cast<const float *>(w), p, m, zt_bytes + loss_bytes, r, ws)) !=
+        BWPP_HIP_OK)
+      return s;
   } else {
     const uint32_t piece = xent_piece(T, p.vocab, 4);
     const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece;
@@ -721,6 +1007,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     r.ldy = m.lddw * es;
     return bwpp_hip_launch_lm(h, LM_XENT_CLEAR, xent_grid(h, m.wrows), 1, 256, &r);
   }
+  if (!bf16 && xent_in_terms(h, p, m, true))
+    return terms_grad(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(dx),
+                      static_cast<float *>(dw), p, m, r);
   // bf16: dx is summed in fp32 over several pieces, and over planes of K ranges
   // where its 256-wide tiles alone would leave half of the CUs idle; with fewer
   // than half of them even so, it is one product on the tiles dispatch_matmul
@@ -870,5 +1159,5 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
   if (!sums) return bwpp_hip_launch_lm(h, LM_XENT_ZERO + bf16, xent_grid(h, T), 1, 256, &r);
   r.src = acc;
   r.nparts = split;
-  return bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, T), 1, 256, &r);
+  return bwpp_hip_launch_lm(h, LM_XENT_ROUND + 1, xent_grid(h, T), 1, 256, &r);
 }

@@ -370,3 +370,78 @@ def test_recording_never_grows_the_workspace():
     torch.cuda.synchronize()
     assert bool((loss == 0).all())
     b.close()
+
+
+# ------------------------------------------- fp32 in bf16 terms (the matrix cores)
+TERMS = [("vd", 300, 520, 3000, None), ("dv", 300, 520, 3001, None), ("vd", 777, 1021, 8003, True),
+         ("dv", 777, 1021, 8003, True), ("dv", 1025, 33, 20000, None), ("vd", 2048, 1024, 4100, True),
+         ("dv", 260, 2048, 33001, None), ("vd", 260, 2048, 33001, None), ("vd", 20011, 72, 7001, None),
+         ("vd", 4100, 1024, 9001, True), ("dv", 4100, 1024, 9001, True), ("vd", 1025, 4100, 9001, True),
+         ("dv", 1025, 4100, 9001, True)]
+
+
+@pytest.mark.parametrize("wide,T,D,V,terms", TERMS)
+def test_fp32_in_terms(be, wide, T, D, V, terms):
+    """The same bounds hold: three bf16 terms are an fp32 number, the products of
+    terms that are left out are 2^-26 of theirs.  Ragged on every side, in pieces
+    (9001 columns, of the gradient for 4100 rows, of the loss too for 4100 dim),
+    dx and dW in planes; and sizes near the choice's border."""
+    x, w, t = _case(T, D, V, F32, wide, 15, (1, 3))
+    t[::13] = -1
+    t[3], t[4] = V - 1, 0
+    _, lse, _ = _forward(be, x, w, t, F32, wide, 1.25)
+    full = _gradient(be, x, w, t, lse, torch.randn(T, device="cuda"), F32, wide, 1.25, (3, 1))
+    assert terms is None or any(be.recent_kernel(i).startswith("bwpp_xent_sums_s") for i in range(1, 5))
+    assert full[0].isfinite().all()
+
+
+@pytest.mark.parametrize("wide", ["vd", "dv"])
+def test_fp32_terms_scale_exactly(be, wide):
+    """Scaling x by 2^60 and W by 2^-60 changes no bit of the loss: the terms of a
+    number are as large as it allows, none is lost."""
+    T, D, V = 1200, 512, 8000
+    x, w, t = _case(T, D, V, F32, wide, 16)
+    x1, w1 = x * 2.0 ** 60, w * 2.0 ** -60
+    out = []
+    for a, b in ((x, w), (x1, w1)):
+        p = _params(T, D, V, F32, wide, a, b)
+        loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+        be.dispatch_linear_xent(a, b, t, loss, lse, None, p)
+        dx, dw = torch.empty_like(a), torch.empty_like(b)
+        be.dispatch_linear_xent_grad(a, b, t, lse, None, dx, dw, p)
+        out.append((loss, lse, dx, dw))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    assert torch.equal(out[0][2] * 2.0 ** -60, out[1][2]) and torch.equal(out[0][3] * 2.0 ** 60, out[1][3])
+
+
+@pytest.mark.parametrize("wide", ["vd", "dv"])
+def test_fp32_terms_infinities(be, wide):
+    """As the formula's: a vocabulary row of -inf logits vanishes, an infinite or
+    NaN token spoils its own row alone, a left-out one nothing."""
+    T, D, V = 1200, 256, 8000
+    x, w, t = _case(T, D, V, F32, wide, 17)
+    wv = _vd(w, wide)
+    x[:, 0] = 1.0
+    wv[7, 0] = -float("inf")
+    t[t == 7] = 8
+    x[11, 5], x[12, 5], x[13, 5] = float("inf"), float("nan"), float("inf")
+    t[13] = -1
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    p = _params(T, D, V, F32, wide, x, w)
+    be.dispatch_linear_xent(x, w, t, loss, lse, None, p)
+    assert any(be.recent_kernel(i).startswith("bwpp_xent_stats_s") for i in range(1, 3))
+    keep = torch.ones(T, dtype=torch.bool, device="cuda")
+    keep[11:14] = False
+    rest = torch.arange(V, device="cuda") != 7
+    want, want_lse = xent64(x[keep].contiguous(), wv[rest].contiguous(), torch.where(t[keep] > 7, t[keep] - 1, t[keep]))[:2]
+    e = _logit_error(x[keep], wv[rest], 1.0)
+    tol = e + (V / 64 + 48) * U + U * want_lse.abs()
+    assert bool(((lse[keep].double() - want_lse).abs() <= tol).all())
+    assert bool(((loss[keep].double() - want).abs() <= tol + e).all())
+    assert float(loss[13]) == 0.0 and not bool(loss[11:13].isfinite().any())
+    wv[7, 0] = 1.0
+    t[11] = t[12] = -1
+    be.dispatch_linear_xent(x, w, t, loss, lse, None, p)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    be.dispatch_linear_xent_grad(x, w, t, lse, None, dx, dw, p)
+    assert bool((dx[11:14] == 0).all()) and bool(dx.isfinite().all()) and bool(dw.isfinite().all())
