@@ -230,6 +230,9 @@ typedef struct {
   BwppSplitTerms terms; /* fp32 operands in bf16 terms */
   uint64_t dl_stride;   /* gradient in terms: its three planes' distance; ... */
   uint32_t cols_up;     /* ... its columns, zeros behind N */
+  float *rest;          /* gradient: [rows] what rounding left of the targets' dz scale */
+  uint32_t rows;        /* rows product: tokens, and whether x is its A */
+  uint32_t x_is_a;
 } BwppXentArgs;
 
 /* Its row kernels. */
@@ -250,6 +253,9 @@ typedef struct {
   uint32_t dloss_scalar;
   uint32_t lanes; /* join: rows a block; terms: threads a row */
   uint64_t plane; /* terms: distance of the planes */
+  const float *rest; /* bf16 sums: see BwppXentArgs, and W */
+  const void *w;
+  uint64_t ldw;
   float scale;
 } BwppXentRowArgs;
 

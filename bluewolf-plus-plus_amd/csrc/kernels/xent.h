@@ -6,6 +6,12 @@
 //   dz_tv = g_t (exp(z_tv - lse_t) - [v = target]),   dx = scale dz W^T,
 //   dW = scale x^T dz
 //
+// Measured: 4 x 1024 x 16384 loss 11.5 us (W at 2.9 TB/s, and two launches), 2048 x
+// 4096 x 50001 loss 679 (1235 TFLOP/s), 4096 x 2048 x 32768 train 1797 and 4096 x 4096
+// x 131072 12.8 ms (1224 and 1374 TFLOP/s of the four products a call that does not
+// keep the logits makes); the wide products run at the rate that the chip's power
+// allows (gemm_bf16_k32.h).
+//
 // A target outside the vocabulary leaves its row out: loss and gradients 0.
 //
 // bf16: the logits' product runs on the matrix cores (gemm_bf16_k32.h's loop on 256 x
@@ -14,8 +20,10 @@
 // rows to (max, sum of exp), a pair per row and tile, and a second kernel
 // joins the pairs.  The gradient's epilogue turns the same product, made
 // again from x and W, into dz, rounded to bf16 as the next two products'
-// operand (each element off by half a step, 2^-9 of it in the mean; dx and dW
-// add thousands of them, and are rounded to bf16 themselves).  It does so for
+// operand (each element off by at most half a step, 2^-8 of it; dx and dW add
+// thousands of them, and are rounded to bf16 themselves).  A row's largest element
+// by far is its target's p - 1: what its rounding leaves is kept, a float a token,
+// and added by the kernels that sum dx's planes and dW's wide tiles.  It does so for
 // one piece of the vocabulary at a time, small enough to stay in the Infinity
 // Cache between its writer and its readers.  dx is summed over the pieces in
 // fp32 planes (one per K split) and rounded once; each piece's dW is final.
@@ -145,7 +153,11 @@ struct EpiGrad {
       const uint32_t tl = t - a.n_base;
       if (__any(live && tl - nw < (uint32_t)TN))
         each_column<FR, FN>(nw, lane, [&](int i, int r, uint32_t n) {
-          if (live && n == tl) acc[i][j][r] -= 1.0f;
+          if (live && n == tl) {
+            acc[i][j][r] -= 1.0f;
+            const float v = g * acc[i][j][r], rest = v - bf16_bits_to_f32(f32_to_bf16_bits(v));
+            if (a.rest) a.rest[m] = __builtin_isfinite(rest) ? rest : 0.0f;
+          }
         });
 #pragma unroll
       for (int i = 0; i < FN; ++i)
@@ -178,12 +190,95 @@ struct EpiRows {
   static constexpr bool kStore = false;
   const BwppXentArgs &a;
 
+  // dW += x^T (what rounding left of the targets' dz): of a row of dz the target's
+  // p - 1 is by far the largest element, and its rounding nearly all of the error
+  // that dz's brings (dx and dW off by 0.0025 of their norm with it, 0.0017, their
+  // own rounding, without).  The tokens whose target is in the tile, in order, 32 at
+  // a time as one more K step: a one-hot operand of the remainders (bf16: 2^-9 of
+  // 2^-9) and the rows of x.  T / V of a step's 32 x 256 / 32 a tile on average.
+  template <class FR, int BM, int BN, int TM, int TN, class V, int FN, int FM>
+  __device__ __forceinline__ void add_rest(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, int tid,
+                                           int wm, int wn) const {
+    asm volatile("" : "+v"(tid));  // nothing below is computed ahead of the main loop, whose registers are full
+    static_assert(FR::kSize == 16 && BM == 256 && BN == 256, "one layout for both operands");
+    constexpr uint32_t kEach = 8, kWindow = 512 * kEach;  // tokens a thread, and the block, looks at
+    unsigned char *hot = smem, *xs = smem + 16384;        // [32][256] each
+    uint16_t *list = reinterpret_cast<uint16_t *>(smem + 32768);            // [kWindow] tokens of the window
+    uint32_t *totals = reinterpret_cast<uint32_t *>(smem + 32768 + 2 * kWindow);  // [8 waves]
+    const int lane = tid & 63, wave = tid >> 6;
+    const uint32_t v0 = a.n_base + (a.x_is_a ? n0 : m0), d0 = a.x_is_a ? m0 : n0;
+    const uint32_t lim = (a.x_is_a ? a.g.M : a.g.N) - d0;
+    const uint16_t *x = static_cast<const uint16_t *>(a.x_is_a ? a.g.a : a.g.b);
+    const uint64_t ldx = a.x_is_a ? a.g.lda : a.g.ldb;
+    unsigned char *ta = a.x_is_a ? xs : hot, *tb = a.x_is_a ? hot : xs;
+    for (uint32_t w0 = 0; w0 < a.rows; w0 += kWindow) {
+      uint32_t mine = 0;  // bit e: token w0 + kEach tid + e
+#pragma unroll
+      for (uint32_t e = 0; e < kEach; ++e) {
+        const uint32_t m = w0 + kEach * (uint32_t)tid + e;
+        const uint32_t t = m < a.rows ? (uint32_t)a.target[m] : 0xffffffffu;
+        if (t < a.vocab && t - v0 < 256u) mine |= 1u << e;
+      }
+      const uint32_t n = (uint32_t)__popc(mine);
+      uint32_t before = n;  // of the wave's lanes up to this one
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const uint32_t o = (uint32_t)__shfl_up((int)before, d);
+        if (lane >= d) before += o;
+      }
+      if (lane == 63) totals[wave] = before;
+      __syncthreads();
+      uint32_t at = before - n, count = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const uint32_t c = totals[w];
+        if (w < wave) at += c;
+        count += c;
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < kEach; ++e)
+        if (mine >> e & 1u) list[at++] = (uint16_t)(kEach * (uint32_t)tid + e);
+      __syncthreads();
+      for (uint32_t b = 0; b < count; b += 32) {
+#pragma unroll 1
+        for (int q = tid; q < 1024; q += 512) {
+          const uint32_t k = (uint32_t)q >> 5, c = (uint32_t)q & 31u;
+          u32x4_t v = {0u, 0u, 0u, 0u};
+          *reinterpret_cast<u32x4_t *>(hot + 16 * q) = v;
+          if (b + k < count)
+            v = *reinterpret_cast<const u32x4_t *>(x + (uint64_t)(w0 + list[b + k]) * ldx + d0 + min(8u * c, lim - 8u));
+          *reinterpret_cast<u32x4_t *>(xs + k * 512u + 16u * (c ^ mnc16_swz(k))) = v;
+        }
+        __syncthreads();
+        if (tid < 32 && b + (uint32_t)tid < count) {
+          const uint32_t k = (uint32_t)tid, m = w0 + list[b + k], v = (uint32_t)a.target[m] - v0;
+          *reinterpret_cast<uint16_t *>(hot + k * 512u + 16u * ((v >> 3) ^ mnc16_swz(k)) + 2u * (v & 7u)) =
+              f32_to_bf16_bits(a.rest[m]);
+        }
+        __syncthreads();
+        bf16x8_t fb[FN];
+#pragma unroll
+        for (int i = 0; i < FN; ++i) fb[i] = read16<true, 256>(tb, (uint32_t)(wn * TN + i * 16), lane);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          const bf16x8_t fa = read16<true, 256>(ta, (uint32_t)(wm * TM + j * 16), lane);
+#pragma unroll
+          for (int i = 0; i < FN; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa, acc[i][j], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);  // one operand in registers at a time
+        }
+        __syncthreads();
+      }
+    }
+    __syncthreads();
+  }
+
   template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
   __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t, uint32_t,
                                       int tid, int wm, int wn) const {
     constexpr int TM = BM / WM, TN = BN / WN, NT = 64 * WM * WN, kCld = BN + 8;
     const int lane = tid & 63;
     uint16_t *cs = reinterpret_cast<uint16_t *>(smem);  // [BM][BN + 8]
+    add_rest<FR, BM, BN, TM, TN>(acc, smem, m0, n0, tid, wm, wn);
 #pragma unroll
     for (int j = 0; j < FM; ++j)
 #pragma unroll
@@ -527,7 +622,8 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_grad_f32(const BwppX
   }
 }
 
-// Planes of fp32 sums -> rows of T, rows that are left out 0.
+// Planes of fp32 sums -> rows of T, rows that are left out 0; bf16: with W's row of
+// the target times what rounding left of its dz (EpiRows::add_rest).
 template <class T>
 __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
   const uint64_t plane = (uint64_t)a.rows * a.cols;
@@ -535,15 +631,42 @@ __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
     const bool on = !a.target || live(a, row);
     T *y = static_cast<T *>(a.y) + row * a.ldy;
     const float *src = a.src + (uint64_t)row * a.cols;
+    const float rest = sizeof(T) == 2 && on ? a.rest[row] : 0.0f;
+    const uint16_t *w = static_cast<const uint16_t *>(a.w) + (sizeof(T) == 2 && on ? (uint32_t)a.target[row] * a.ldw : 0u);
     for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
       float v = src[c];
       for (uint32_t i = 1; i < a.nparts; ++i) v += src[i * plane + c];
+      if (sizeof(T) == 2 && on) v += rest * bf16_bits_to_f32(w[c]);
       y[c] = to<T>(on ? v : 0.0f);
     }
   }
 }
 extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_bf16(const BwppXentRowArgs a) { sum_planes<uint16_t>(a); }
 extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_f32(const BwppXentRowArgs a) { sum_planes<float>(a); }
+// W [dim][vocab]: its columns are gathered, every element from a line of its own.
+// An XCD takes 32 columns of dx at a time for all tokens: those 32 rows of W stay in
+// its L2 (4096 x 2048 from two planes: 90 us, 83 with 16 columns, 20 without the
+// gather).  blockIdx: XCD, then 64 tokens, then the XCD's next columns.
+extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_bf16_dv(const BwppXentRowArgs a) {
+  const uint64_t plane = (uint64_t)a.rows * a.cols;
+  const uint32_t groups = (a.rows + 63u) / 64u, q = blockIdx.x >> 3;
+  const uint32_t chunk = (blockIdx.x & 7u) + 8u * (q / groups), c = chunk * 32u + (threadIdx.x & 31u);
+  if (c >= a.cols) return;
+  const uint16_t *w = static_cast<const uint16_t *>(a.w) + c * a.ldw;
+#pragma unroll
+  for (uint32_t i = 0; i < 64; i += 8) {
+    const uint32_t row = q % groups * 64u + i + threadIdx.x / 32u;
+    if (row >= a.rows) continue;
+    const uint32_t t = (uint32_t)a.target[row];
+    float v = 0.0f;
+    if (t < a.vocab) {
+      const float *src = a.src + (uint64_t)row * a.cols + c;
+      v = a.rest[row] * bf16_bits_to_f32(w[t]);
+      for (uint32_t p = 0; p < a.nparts; ++p) v += src[p * plane];
+    }
+    static_cast<uint16_t *>(a.y)[row * a.ldy + c] = to<uint16_t>(v);
+  }
+}
 
 // fp32 rows (x, any strides) -> four bf16 planes [rows_up][ldy]: v1, v1 where it
 // is finite, v2, v3 (gemm_bf16_k32.h); zeros past the rows and columns and, with

@@ -23,8 +23,8 @@ enum LmKernel {
   LM_XENT_STATS_F32,
   LM_XENT_GRAD_F32,
   LM_XENT_TERMS,
-  LM_XENT_ROUND,                         // [bf16]
-  LM_XENT_CLEAR = LM_XENT_ROUND + 2,
+  LM_XENT_ROUND,                         // fp32, bf16, bf16 with row-major W
+  LM_XENT_CLEAR = LM_XENT_ROUND + 3,
   LM_XENT_COPY,                          // [bf16]
   LM_XENT_ZERO = LM_XENT_COPY + 2,       // [bf16]
   LM_XENT_STATS = LM_XENT_ZERO + 2,      // [trans_w][XentTile]
@@ -67,7 +67,8 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_resnorm_grad_bf16_any",
     "bwpp_resnorm_finish_f32",      "bwpp_resnorm_finish_bf16",
     "bwpp_xent_join", "bwpp_xent_sums", "bwpp_xent_stats_f32", "bwpp_xent_grad_f32",
-    "bwpp_xent_terms", "bwpp_xent_round_f32", "bwpp_xent_round_bf16", "bwpp_xent_clear", "bwpp_xent_copy_f32", "bwpp_xent_copy_bf16",
+    "bwpp_xent_terms", "bwpp_xent_round_f32", "bwpp_xent_round_bf16", "bwpp_xent_round_bf16_dv",
+    "bwpp_xent_clear", "bwpp_xent_copy_f32", "bwpp_xent_copy_bf16",
     "bwpp_xent_zero_f32", "bwpp_xent_zero_bf16",
     "bwpp_xent_stats_p_t00",
     "bwpp_xent_stats_r32_t00",
@@ -589,6 +590,8 @@ constexpr uint64_t kXentPiece = 256ull << 20;
 uint32_t xent_piece(uint64_t rows, uint64_t vocab, uint64_t es) {
   uint64_t n = std::max<uint64_t>(kXentPiece / (std::max<uint64_t>(rows, 1) * es) / 256 * 256, 1024);
   if (n >= vocab) return (uint32_t)vocab;
+  const uint64_t pieces = (vocab + n - 1) / n;
+  n = up((vocab + pieces - 1) / pieces, 256);
   while (vocab % n != 0 && vocab % n < 8) n -= 256;  // a last piece has a whole 16-byte chunk
   return (uint32_t)n;
 }
@@ -1024,18 +1027,24 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     const uint32_t k = piece / 32 * 32, range = (uint32_t)up((k + split - 1) / split, 128);  // as xent_product cuts it
     split = (k + range - 1) / range;
   }
+  const bool dw_wide = bf16 && ((piece + 255ull) / 256) * ((D + 255) / 256) * 2 >= cus_of(h) &&
+                       256ull * std::max<uint64_t>(piece + 8ull, D + 8) < (1ull << 31);
   const bool sums = bf16 && dx && (npieces > 1 || (wide && dx_tiles * split * 2 >= cus_of(h)));
   if (!sums) split = 1;
   // (rows of x's copy and of dz up to a multiple of 32, zeros: dW's K)
   const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit), Tu = bf16 ? up(T, 32) : T;
   const uint64_t x_bytes = dw ? up(Tu * ldxc * es, 256) : 0, z_bytes = up(Tu * ldz * es, 256);
-  const uint64_t sum_bytes = sums ? up(split * T * D * 4, 256) : 0, held = x_bytes + z_bytes + sum_bytes;
+  const uint64_t sum_bytes = sums ? up(split * T * D * 4, 256) : 0, rest_bytes = bf16 ? up(T * 4, 256) : 0;
+  const uint64_t held = x_bytes + z_bytes + sum_bytes + rest_bytes;
   void *ws = nullptr;
   if ((s = bwpp_hip_take_workspace(h, held + (bf16 ? 0 : kXentSplitRoom), &ws)) != BWPP_HIP_OK) return s;
   Hold hold(h, held);
   unsigned char *base = static_cast<unsigned char *>(ws);
   void *xc = base, *z = base + x_bytes;
   float *acc = reinterpret_cast<float *>(base + x_bytes + z_bytes);
+  // What rounding leaves of the targets' dz, for the kernels that add it: dx from
+  // planes, dW on the wide tiles.
+  float *rest = reinterpret_cast<float *>(base + x_bytes + z_bytes + sum_bytes);
   auto at = [&](const void *ptr, uint64_t elems) {
     return static_cast<const unsigned char *>(ptr) + elems * es;
   };
@@ -1071,6 +1080,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.dl = static_cast<uint16_t *>(z);
       a.ldl = (uint32_t)ldp;
       a.rows_up = (uint32_t)Tu;
+      a.rest = rest;
       if ((s = xent_logits(h, LM_XENT_GRAD, a, tw, xent_tile(h, a.g, tw, true))) != BWPP_HIP_OK) return s;
     } else {
       if ((s = xent_logits_f32(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(z), n0,
@@ -1124,8 +1134,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       if (s != BWPP_HIP_OK) return s;
     }
     void *dwp = dw ? const_cast<unsigned char *>(at(dw, tw ? n0 * m.lddw : n0)) : nullptr;
-    const uint64_t dw_tiles = ((n + 255ull) / 256) * ((D + 255) / 256);
-    if (dw && bf16 && dw_tiles * 2 >= cus_of(h) && 256ull * std::max(ldp, ldxc) < (1ull << 31)) {
+    if (dw && dw_wide) {
       BwppXentArgs a = {};
       a.g.a = tw ? z : xc;
       a.g.b = tw ? xc : z;
@@ -1138,6 +1147,12 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.g.ldc = (uint32_t)m.lddw;
       a.rows_out = tw ? n : p.dim;
       a.cols_out = tw ? p.dim : n;
+      a.target = targets;
+      a.vocab = p.vocab;
+      a.n_base = n0;
+      a.rest = rest;
+      a.rows = p.rows;
+      a.x_is_a = !tw;
       if ((s = xent_product(h, LM_XENT_ROWS, a, false, XT_P, 1)) != BWPP_HIP_OK) return s;
     } else if (dw) {
       BwppMatmulParams g = {};
@@ -1159,5 +1174,11 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
   if (!sums) return bwpp_hip_launch_lm(h, LM_XENT_ZERO + bf16, xent_grid(h, T), 1, 256, &r);
   r.src = acc;
   r.nparts = split;
-  return bwpp_hip_launch_lm(h, LM_XENT_ROUND + 1, xent_grid(h, T), 1, 256, &r);
+  r.rest = rest;
+  r.w = w;
+  r.ldw = m.ldw;
+  if (tw) return bwpp_hip_launch_lm(h, LM_XENT_ROUND + 1, xent_grid(h, T), 1, 256, &r);
+  const uint64_t blocks = up((D + 31) / 32, 8) * ((T + 63) / 64);
+  if (blocks * 256 > 0xffffffffull) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: too many elements", what);
+  return bwpp_hip_launch_lm(h, LM_XENT_ROUND + 2, blocks, 1, 256, &r);
 }

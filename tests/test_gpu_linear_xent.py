@@ -445,3 +445,43 @@ def test_fp32_terms_infinities(be, wide):
     dx, dw = torch.empty_like(x), torch.empty_like(w)
     be.dispatch_linear_xent_grad(x, w, t, lse, None, dx, dw, p)
     assert bool((dx[11:14] == 0).all()) and bool(dx.isfinite().all()) and bool(dw.isfinite().all())
+
+
+@pytest.mark.parametrize("wide,T,D,V,dw_too", [
+    ("vd", 2048, 1024, 8205, True), ("dv", 2048, 1024, 8200, True), ("vd", 9000, 512, 16400, False),
+    ("dv", 9000, 520, 16400, False), ("vd", 9000, 1032, 16400, True), ("dv", 9000, 1032, 16400, True)])
+def test_targets_keep_their_bits(be, wide, T, D, V, dw_too):
+    """On the wide products the targets' dz, the largest of their rows, counts with
+    its rounding's remainder (rounded to bf16 for dW): two half steps of it are off,
+    one after the other.  A log-sum-exp 7 above the logits' leaves little else in a
+    row, so that one half step of dz would show in the elements' bound.  One target
+    of many tokens (more than a step of the matrix instructions takes), the last of
+    the vocabulary, and some left out; two pieces for 9000 tokens.  dW with few tiles
+    (dim 512) is another kernel's, and has dz's half step."""
+    x, w, t = _case(T, D, V, BF16, wide, 18, lean=0.0)
+    t[100:180], t[200:203], t[4000:] = 5, V - 1, torch.where(t[4000:] < 600, 600, t[4000:])
+    t[::11] = -1
+    wv, live = _vd(w, wide), t >= 0
+    z = x.double() @ wv.double().t().contiguous()
+    lse = (torch.logsumexp(z, dim=1) + 7.0).float()
+    g = torch.rand(T, device="cuda") + 0.5
+    p = torch.exp(z - lse.double()[:, None]) * torch.where(live, g.double(), 0.0)[:, None]
+    rel = (_logit_error(x, wv, 1.0) + 20 * U)[:, None]
+    err = p * (rel + HALF_STEP[BF16])
+    rows = torch.arange(T, device="cuda")[live]
+    cols = t[live].long()
+    dz = p.clone()
+    dz[rows, cols] -= g.double()[live]
+    err[rows, cols] = p[rows, cols] * rel[live, 0] + dz[rows, cols].abs() * (HALF_STEP[BF16] ** 2 + 4 * U)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    be.dispatch_linear_xent_grad(x, w, t, lse, g, dx, dw, _params(T, D, V, BF16, wide, x, w))
+    assert be.recent_kernel(0).startswith("bwpp_xent_round_bf16")
+    assert (be.recent_kernel(1) == "bwpp_xent_rows_p_t10") == dw_too
+    dw_err = err.clone()
+    if not dw_too:
+        dw_err[rows, cols] += dz[rows, cols].abs() * HALF_STEP[BF16]
+    x64 = torch.where(live[:, None], x.double(), 0.0)
+    for got, want, e, size, terms in (
+            (dx, dz @ wv.double(), err @ wv.double().abs(), dz.abs() @ wv.double().abs(), V),
+            (_vd(dw, wide), dz.t().contiguous() @ x64, dw_err.t().contiguous() @ x64.abs(), dz.t().contiguous().abs() @ x64.abs(), T)):
+        assert bool(((got.double() - want).abs() <= e + (terms + 8) * U * size + HALF_STEP[BF16] * want.abs()).all())
