@@ -251,7 +251,7 @@ typedef struct {
   uint32_t n_base, vocab;
   uint32_t nparts; /* partials a row, or planes of sums */
   uint32_t dloss_scalar;
-  uint32_t lanes; /* join: rows a block; terms: threads a row */
+  uint32_t lanes; /* join: rows a block; terms: threads a row; dx: tokens a block */
   uint64_t plane; /* terms: distance of the planes */
   const float *rest; /* bf16 sums: see BwppXentArgs, and W */
   const void *w;

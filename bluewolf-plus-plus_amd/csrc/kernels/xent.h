@@ -23,7 +23,8 @@
 // operand (each element off by at most half a step, 2^-8 of it; dx and dW add
 // thousands of them, and are rounded to bf16 themselves).  A row's largest element
 // by far is its target's p - 1: what its rounding leaves is kept, a float a token,
-// and added by the kernels that sum dx's planes and dW's wide tiles.  It does so for
+// and added by the kernels that sum dx's planes and dW's wide tiles (a small dW
+// keeps it).  It does so for
 // one piece of the vocabulary at a time, small enough to stay in the Infinity
 // Cache between its writer and its readers.  dx is summed over the pieces in
 // fp32 planes (one per K split) and rounded once; each piece's dW is final.
@@ -195,7 +196,8 @@ struct EpiRows {
   // that dz's brings (dx and dW off by 0.0025 of their norm with it, 0.0017, their
   // own rounding, without).  The tokens whose target is in the tile, in order, 32 at
   // a time as one more K step: a one-hot operand of the remainders (bf16: 2^-9 of
-  // 2^-9) and the rows of x.  T / V of a step's 32 x 256 / 32 a tile on average.
+  // 2^-9) and the rows of x.  256 T / V tokens a tile on average.  No longer at 4096 x
+  // 2048 x 32768 (440 us), 2 to 6 us at 120 x 1216 x 19298 (19 -> 24) and the like.
   template <class FR, int BM, int BN, int TM, int TN, class V, int FN, int FM>
   __device__ __forceinline__ void add_rest(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, int tid,
                                            int wm, int wn) const {
@@ -203,8 +205,8 @@ struct EpiRows {
     static_assert(FR::kSize == 16 && BM == 256 && BN == 256, "one layout for both operands");
     constexpr uint32_t kEach = 8, kWindow = 512 * kEach;  // tokens a thread, and the block, looks at
     unsigned char *hot = smem, *xs = smem + 16384;        // [32][256] each
-    uint16_t *list = reinterpret_cast<uint16_t *>(smem + 32768);            // [kWindow] tokens of the window
-    uint32_t *totals = reinterpret_cast<uint32_t *>(smem + 32768 + 2 * kWindow);  // [8 waves]
+    uint32_t *list = reinterpret_cast<uint32_t *>(smem + 32768);  // [kWindow] tokens of the window, and their columns
+    uint32_t *totals = reinterpret_cast<uint32_t *>(smem + 32768 + 4 * kWindow);  // [8 waves]
     const int lane = tid & 63, wave = tid >> 6;
     const uint32_t v0 = a.n_base + (a.x_is_a ? n0 : m0), d0 = a.x_is_a ? m0 : n0;
     const uint32_t lim = (a.x_is_a ? a.g.M : a.g.N) - d0;
@@ -212,12 +214,13 @@ struct EpiRows {
     const uint64_t ldx = a.x_is_a ? a.g.lda : a.g.ldb;
     unsigned char *ta = a.x_is_a ? xs : hot, *tb = a.x_is_a ? hot : xs;
     for (uint32_t w0 = 0; w0 < a.rows; w0 += kWindow) {
-      uint32_t mine = 0;  // bit e: token w0 + kEach tid + e
+      uint32_t mine = 0, column[kEach];  // bit e: token w0 + kEach tid + e
 #pragma unroll
       for (uint32_t e = 0; e < kEach; ++e) {
         const uint32_t m = w0 + kEach * (uint32_t)tid + e;
         const uint32_t t = m < a.rows ? (uint32_t)a.target[m] : 0xffffffffu;
-        if (t < a.vocab && t - v0 < 256u) mine |= 1u << e;
+        column[e] = t - v0;
+        if (t < a.vocab && column[e] < 256u) mine |= 1u << e;
       }
       const uint32_t n = (uint32_t)__popc(mine);
       uint32_t before = n;  // of the wave's lanes up to this one
@@ -237,23 +240,27 @@ struct EpiRows {
       }
 #pragma unroll
       for (uint32_t e = 0; e < kEach; ++e)
-        if (mine >> e & 1u) list[at++] = (uint16_t)(kEach * (uint32_t)tid + e);
+        if (mine >> e & 1u) list[at++] = column[e] << 16 | (kEach * (uint32_t)tid + e);
       __syncthreads();
       for (uint32_t b = 0; b < count; b += 32) {
+        const bool one = tid < 32 && b + (uint32_t)tid < count;
+        const uint32_t entry = one ? list[b + (uint32_t)tid] : 0u;
+        const float rest = one ? a.rest[w0 + (entry & 0xffffu)] : 0.0f;
 #pragma unroll 1
         for (int q = tid; q < 1024; q += 512) {
           const uint32_t k = (uint32_t)q >> 5, c = (uint32_t)q & 31u;
           u32x4_t v = {0u, 0u, 0u, 0u};
           *reinterpret_cast<u32x4_t *>(hot + 16 * q) = v;
           if (b + k < count)
-            v = *reinterpret_cast<const u32x4_t *>(x + (uint64_t)(w0 + list[b + k]) * ldx + d0 + min(8u * c, lim - 8u));
+            v = *reinterpret_cast<const u32x4_t *>(x + (uint64_t)(w0 + (list[b + k] & 0xffffu)) * ldx + d0 +
+                                                   min(8u * c, lim - 8u));
           *reinterpret_cast<u32x4_t *>(xs + k * 512u + 16u * (c ^ mnc16_swz(k))) = v;
         }
         __syncthreads();
-        if (tid < 32 && b + (uint32_t)tid < count) {
-          const uint32_t k = (uint32_t)tid, m = w0 + list[b + k], v = (uint32_t)a.target[m] - v0;
+        if (one) {
+          const uint32_t k = (uint32_t)tid, v = entry >> 16;
           *reinterpret_cast<uint16_t *>(hot + k * 512u + 16u * ((v >> 3) ^ mnc16_swz(k)) + 2u * (v & 7u)) =
-              f32_to_bf16_bits(a.rest[m]);
+              f32_to_bf16_bits(rest);
         }
         __syncthreads();
         bf16x8_t fb[FN];
@@ -633,11 +640,26 @@ __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
     const float *src = a.src + (uint64_t)row * a.cols;
     const float rest = sizeof(T) == 2 && on ? a.rest[row] : 0.0f;
     const uint16_t *w = static_cast<const uint16_t *>(a.w) + (sizeof(T) == 2 && on ? (uint32_t)a.target[row] * a.ldw : 0u);
-    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) {
-      float v = src[c];
-      for (uint32_t i = 1; i < a.nparts; ++i) v += src[i * plane + c];
-      if (sizeof(T) == 2 && on) v += rest * bf16_bits_to_f32(w[c]);
-      y[c] = to<T>(on ? v : 0.0f);
+    for (uint32_t c = (blockIdx.y * 256u + threadIdx.x) * 4u; c < a.cols; c += gridDim.y * 1024u) {
+      const uint32_t n = min(4u, a.cols - c);
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (n == 4) {
+#pragma unroll 4
+        for (uint32_t i = 0; i < a.nparts; ++i) {
+          const float4 o = load4(src + i * plane + c);
+          v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+        }
+      } else {
+        for (uint32_t i = 0; i < a.nparts; ++i)
+#pragma unroll
+          for (uint32_t e = 0; e < 3; ++e) v[e] += e < n ? src[i * plane + c + e] : 0.0f;
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        if (e >= n) break;
+        if (sizeof(T) == 2 && on) v[e] += rest * bf16_bits_to_f32(w[c + e]);
+        y[c + e] = to<T>(on ? v[e] : 0.0f);
+      }
     }
   }
 }
@@ -646,22 +668,24 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_f32(const Bwpp
 // W [dim][vocab]: its columns are gathered, every element from a line of its own.
 // An XCD takes 32 columns of dx at a time for all tokens: those 32 rows of W stay in
 // its L2 (4096 x 2048 from two planes: 90 us, 83 with 16 columns, 20 without the
-// gather).  blockIdx: XCD, then 64 tokens, then the XCD's next columns.
+// gather).  blockIdx: XCD, then `lanes` tokens (a multiple of 8), then the
+// XCD's next columns.
 extern "C" __global__ __launch_bounds__(256) void bwpp_xent_round_bf16_dv(const BwppXentRowArgs a) {
   const uint64_t plane = (uint64_t)a.rows * a.cols;
-  const uint32_t groups = (a.rows + 63u) / 64u, q = blockIdx.x >> 3;
+  const uint32_t groups = (a.rows + a.lanes - 1u) / a.lanes, q = blockIdx.x >> 3;
   const uint32_t chunk = (blockIdx.x & 7u) + 8u * (q / groups), c = chunk * 32u + (threadIdx.x & 31u);
   if (c >= a.cols) return;
   const uint16_t *w = static_cast<const uint16_t *>(a.w) + c * a.ldw;
-#pragma unroll
-  for (uint32_t i = 0; i < 64; i += 8) {
-    const uint32_t row = q % groups * 64u + i + threadIdx.x / 32u;
+#pragma unroll 8
+  for (uint32_t i = 0; i < a.lanes; i += 8) {
+    const uint32_t row = q % groups * a.lanes + i + threadIdx.x / 32u;
     if (row >= a.rows) continue;
     const uint32_t t = (uint32_t)a.target[row];
     float v = 0.0f;
     if (t < a.vocab) {
       const float *src = a.src + (uint64_t)row * a.cols + c;
       v = a.rest[row] * bf16_bits_to_f32(w[t]);
+#pragma unroll 8
       for (uint32_t p = 0; p < a.nparts; ++p) v += src[p * plane];
     }
     static_cast<uint16_t *>(a.y)[row * a.ldy + c] = to<uint16_t>(v);
@@ -755,8 +779,10 @@ BWPP_XENT_ROWS(f32, float)
   BWPP_XENT_K32(sums_sh_t0##TB, EpiSums, 0, TB, 128, true)                  \
   BWPP_XENT_RING(stats, EpiStats, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)     \
   BWPP_XENT_RING(grad, EpiGrad, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)       \
+  BWPP_XENT_RING(sums, EpiSums, TB, r32, 32, 64, 1, 2, 4, 4, 1, 4, 1)       \
   BWPP_XENT_RING(stats, EpiStats, TB, r64, 64, 64, 2, 2, 2, 4, 2, 4, 2)     \
   BWPP_XENT_RING(grad, EpiGrad, TB, r64, 64, 64, 2, 2, 2, 4, 2, 4, 2)       \
+  BWPP_XENT_RING(sums, EpiSums, TB, r64, 64, 64, 2, 2, 2, 4, 2, 4, 2)       \
   BWPP_XENT_RING(stats, EpiStats, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)  \
   BWPP_XENT_RING(grad, EpiGrad, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)    \
   BWPP_XENT_RING(sums, EpiSums, TB, r128, 128, 128, 2, 2, 1, 3, 2, 2, 2)

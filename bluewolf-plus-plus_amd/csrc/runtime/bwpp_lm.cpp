@@ -99,17 +99,17 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_xent_grad_r128_t01",
     "bwpp_xent_grad_r128_t01_u",
     "bwpp_xent_sums_p_t00",
-    "bwpp_xent_sums_r128_t00",
-    "bwpp_xent_sums_r128_t00_u",
-    "bwpp_xent_sums_r128_t00",
-    "bwpp_xent_sums_r128_t00_u",
+    "bwpp_xent_sums_r32_t00",
+    "bwpp_xent_sums_r32_t00_u",
+    "bwpp_xent_sums_r64_t00",
+    "bwpp_xent_sums_r64_t00_u",
     "bwpp_xent_sums_r128_t00",
     "bwpp_xent_sums_r128_t00_u",
     "bwpp_xent_sums_p_t01",
-    "bwpp_xent_sums_r128_t01",
-    "bwpp_xent_sums_r128_t01_u",
-    "bwpp_xent_sums_r128_t01",
-    "bwpp_xent_sums_r128_t01_u",
+    "bwpp_xent_sums_r32_t01",
+    "bwpp_xent_sums_r32_t01_u",
+    "bwpp_xent_sums_r64_t01",
+    "bwpp_xent_sums_r64_t01_u",
     "bwpp_xent_sums_r128_t01",
     "bwpp_xent_sums_r128_t01_u",
     "bwpp_xent_rows_p_t10",
@@ -491,8 +491,9 @@ uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 // round of 256-wide tiles, 8192^3 in 790 us), and no product runs faster than its
 // operands arrive (5.6 TB/s; four fifths of it in the 128-byte pieces that 64
 // columns take of row-major B: 42 x 704 x 69376 train 140 us on 64 x 64 tiles, 135
-// on 128 x 128).  Without small tiles (RAW sums) 128 x 128.
-XentTile xent_tile(const BwppHip *h, const BwppGemmArgs &g, bool tb, bool small) {
+// on 128 x 128).  Sums: in planes of K ranges, as modelled; the 256-wide tiles' are
+// chosen by the caller.
+XentTile xent_tile(const BwppHip *h, const BwppGemmArgs &g, bool tb, bool sums, uint32_t *splits = nullptr) {
   const bool dma = on16(g.a) && on16(g.b) && g.lda % 8 == 0 && g.ldb % 8 == 0 && g.K % 8 == 0 && (tb || g.N % 8 == 0) &&
                    256ull * std::max(g.lda, g.ldb) < (1ull << 31);
   const uint64_t cus = cus_of(h);
@@ -501,16 +502,22 @@ XentTile xent_tile(const BwppHip *h, const BwppGemmArgs &g, bool tb, bool small)
   double best_us = 1e300;
   for (int t = 0; t < XT_COUNT; ++t) {
     const bool wide = t == XT_P, direct = wide || t == XT_R32 || t == XT_R64 || t == XT_R128;
-    if (direct != dma || (wide && (g.K % 32 != 0 || g.M <= 128)) || (!small && t >= XT_R32 && t <= XT_R64U)) continue;
+    if (direct != dma || (wide && (sums || g.K % 32 != 0 || g.M <= 128))) continue;
     const XentShape &sh = kXentShapes[t];
     const uint64_t tiles = ((g.M + (uint64_t)sh.bm - 1) / sh.bm) * ((g.N + (uint64_t)sh.bn - 1) / sh.bn);
-    if (tiles * sh.threads > 0xffffffffull) continue;
-    const double n = (double)((tiles + cus - 1) / cus);
-    const double fetch = !tb && sh.bn == 64 ? mem * 1.25 : mem;
-    const double us = std::max(fetch, (n - 1.0) * sh.more + g.K * (sh.lat + (n - 1.0) * sh.inc));
-    if (us < best_us * 0.999) {
-      best_us = us;
-      best = (XentTile)t;
+    // One range, or as many as fill 1 to 4 rounds of blocks.
+    for (uint32_t rounds = 0; rounds <= (splits ? 4u : 0u); ++rounds) {
+      const uint64_t fill = rounds ? std::min<uint64_t>(rounds * cus / tiles, std::min<uint64_t>(g.K / 256, 32)) : 1;
+      if (rounds && fill < 2) continue;
+      const uint32_t k = (uint32_t)fill;
+      const double n = (double)((tiles * k + cus - 1) / cus);
+      const double fetch = !tb && sh.bn == 64 ? mem * 1.25 : mem, planes = sums ? (double)k * g.M * g.N * 8.0 / 4e6 : 0.0;
+      const double us = std::max(fetch, (n - 1.0) * sh.more + (double)g.K / k * (sh.lat + (n - 1.0) * sh.inc)) + planes;
+      if (us < best_us * 0.999) {
+        best_us = us;
+        best = (XentTile)t;
+        if (splits) *splits = k;
+      }
     }
   }
   return best;
@@ -596,6 +603,8 @@ uint32_t xent_piece(uint64_t rows, uint64_t vocab, uint64_t es) {
   return (uint32_t)n;
 }
 
+// Few rows: a block for every 1024 columns of one.
+uint32_t xent_columns(uint64_t rows, uint64_t cols) { return rows >= 1024 ? 1u : (uint32_t)std::min<uint64_t>((cols + 1023) / 1024, 256); }
 uint32_t xent_grid(BwppHip *h, uint64_t rows) { return (uint32_t)std::min<uint64_t>(rows, 16ull * cus_of(h)); }
 
 // Ends the hold on the workspace on every way out.
@@ -865,7 +874,7 @@ BwppHipStatus terms_grad(BwppHip *h, const float *x, const float *w, float *dx, 
         f.cols = q.g.N;
         f.y = q.g.c;
         f.ldy = m.lddw;
-        if ((s = bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, f.rows), 1, 256, &f)) != BWPP_HIP_OK) return s;
+        if ((s = bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, f.rows), xent_columns(f.rows, f.cols), 256, &f)) != BWPP_HIP_OK) return s;
       }
     }
   }
@@ -875,7 +884,7 @@ BwppHipStatus terms_grad(BwppHip *h, const float *x, const float *w, float *dx, 
   r.cols = p.dim;
   r.src = acc;
   r.nparts = split;
-  return bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, T), 1, 256, &r);
+  return bwpp_hip_launch_lm(h, LM_XENT_ROUND, xent_grid(h, T), xent_columns(T, p.dim), 256, &r);
 }
 
 }  // namespace
@@ -926,7 +935,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x
     a.target = targets;
     a.vocab = p.vocab;
     a.scale = r.scale;
-    const XentTile tile = xent_tile(h, a.g, p.trans_w != 0, true);
+    const XentTile tile = xent_tile(h, a.g, p.trans_w != 0, false);
     r.nparts = xent_tiles_n(h, a.g, tile);
     if ((s = bwpp_hip_take_workspace(h, zt_bytes + loss_bytes + (uint64_t)r.nparts * T * 8, &ws)) != BWPP_HIP_OK) return s;
     a.zt = static_cast<float *>(ws);
@@ -1013,24 +1022,35 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
   if (!bf16 && xent_in_terms(h, p, m, true))
     return terms_grad(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(dx),
                       static_cast<float *>(dw), p, m, r);
-  // bf16: dx is summed in fp32 over several pieces, and over planes of K ranges
-  // where its 256-wide tiles alone would leave half of the CUs idle; with fewer
-  // than half of them even so, it is one product on the tiles dispatch_matmul
-  // finds (4096 x 2048 from 32768 columns: 645 us as such a product, 515 so).
+  // bf16: dx is summed in fp32 over pieces, and over planes of K ranges: on 256-wide
+  // tiles where they keep half of the CUs busy with a few planes, else on the tiles
+  // and ranges that are modelled fastest (4096 x 2048 from 32768 columns: 645 us as
+  // one product, 515 on 256-wide tiles and two planes).
   const uint32_t piece = xent_piece(T, p.vocab, es);
   const uint64_t npieces = (p.vocab + (uint64_t)piece - 1) / piece, dx_tiles = ((T + 255) / 256) * ((D + 255) / 256);
-  const bool wide = bf16 && dx && T > 128 && piece >= 32 && on16(w) && m.ldw % 8 == 0 && (!tw || D % 8 == 0) &&
-                    256ull * std::max<uint64_t>(piece + 8ull, m.ldw) < (1ull << 31);
+  bool wide = bf16 && dx && T > 128 && piece >= 32 && on16(w) && m.ldw % 8 == 0 && (!tw || D % 8 == 0) &&
+              256ull * std::max<uint64_t>(piece + 8ull, m.ldw) < (1ull << 31);
   uint32_t split = 1;
-  if (wide) {
-    while (split < 8 && dx_tiles * split * 2 <= cus_of(h) && piece / (split * 2) >= 2048) split *= 2;
-    const uint32_t k = piece / 32 * 32, range = (uint32_t)up((k + split - 1) / split, 128);  // as xent_product cuts it
+  while (wide && split < 8 && dx_tiles * split * 2 <= cus_of(h) && piece / (split * 2) >= 2048) split *= 2;
+  wide = wide && dx_tiles * split * 2 >= cus_of(h);
+  const bool sums = bf16 && dx && piece >= 8;  // (a chunk of dz)
+  XentTile dx_tile = XT_P;
+  if (sums && !wide) {
+    BwppGemmArgs g = {};
+    g.b = w;
+    g.M = p.rows;
+    g.N = p.dim;
+    g.K = piece;
+    g.lda = (uint32_t)up(piece, 8);
+    g.ldb = (uint32_t)m.ldw;
+    dx_tile = xent_tile(h, g, !tw, true, &split);
+  }
+  if (split > 1) {  // as xent_product cuts the ranges
+    const uint32_t k = wide ? piece / 32 * 32 : piece, range = (uint32_t)up((k + split - 1) / split, 128);
     split = (k + range - 1) / range;
   }
   const bool dw_wide = bf16 && ((piece + 255ull) / 256) * ((D + 255) / 256) * 2 >= cus_of(h) &&
                        256ull * std::max<uint64_t>(piece + 8ull, D + 8) < (1ull << 31);
-  const bool sums = bf16 && dx && (npieces > 1 || (wide && dx_tiles * split * 2 >= cus_of(h)));
-  if (!sums) split = 1;
   // (rows of x's copy and of dz up to a multiple of 32, zeros: dW's K)
   const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit), Tu = bf16 ? up(T, 32) : T;
   const uint64_t x_bytes = dw ? up(Tu * ldxc * es, 256) : 0, z_bytes = up(Tu * ldz * es, 256);
@@ -1081,7 +1101,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.ldl = (uint32_t)ldp;
       a.rows_up = (uint32_t)Tu;
       a.rest = rest;
-      if ((s = xent_logits(h, LM_XENT_GRAD, a, tw, xent_tile(h, a.g, tw, true))) != BWPP_HIP_OK) return s;
+      if ((s = xent_logits(h, LM_XENT_GRAD, a, tw, xent_tile(h, a.g, tw, false))) != BWPP_HIP_OK) return s;
     } else {
       if ((s = xent_logits_f32(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(z), n0,
                                n, p, m)) != BWPP_HIP_OK)
@@ -1103,19 +1123,21 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.g.ldb = (uint32_t)m.ldw;
       a.raw = acc;
       a.accumulate = i > 0;
-      // K in steps of 32 on the wide tiles, what is left of it on others.
-      BwppXentArgs rest = a;
-      a.g.K = n / 32 * 32;
-      const bool main = wide && n >= 32;
-      if (main && (s = xent_product(h, LM_XENT_RAW, a, !tw, XT_P, split)) != BWPP_HIP_OK) return s;
-      if (!main || n % 32) {
-        if (main) {
+      if (!wide) {
+        // (the last piece may be cut for other loads, never for more ranges)
+        const XentTile tile = n == piece ? dx_tile : xent_tile(h, a.g, !tw, true);
+        if ((s = xent_product(h, LM_XENT_RAW, a, !tw, tile, split)) != BWPP_HIP_OK) return s;
+      } else {  // K in steps of 32, what is left of it on other tiles
+        BwppXentArgs rest = a;
+        a.g.K = n / 32 * 32;
+        if (a.g.K && (s = xent_product(h, LM_XENT_RAW, a, !tw, XT_P, split)) != BWPP_HIP_OK) return s;
+        if (n % 32) {
           rest.g.K = n % 32;
           rest.g.a = static_cast<const uint16_t *>(rest.g.a) + a.g.K;
           rest.g.b = static_cast<const uint16_t *>(rest.g.b) + (tw ? (uint64_t)a.g.K * m.ldw : a.g.K);
-          rest.accumulate = 1;
+          rest.accumulate = i > 0 || a.g.K;
+          if ((s = xent_product(h, LM_XENT_RAW, rest, !tw, xent_tile(h, rest.g, !tw, true), 1)) != BWPP_HIP_OK) return s;
         }
-        if ((s = xent_product(h, LM_XENT_RAW, rest, !tw, xent_tile(h, rest.g, !tw, false), 1)) != BWPP_HIP_OK) return s;
       }
     } else if (dx) {
       BwppMatmulParams g = {};
@@ -1177,8 +1199,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
   r.rest = rest;
   r.w = w;
   r.ldw = m.ldw;
-  if (tw) return bwpp_hip_launch_lm(h, LM_XENT_ROUND + 1, xent_grid(h, T), 1, 256, &r);
-  const uint64_t blocks = up((D + 31) / 32, 8) * ((T + 63) / 64);
+  if (tw) return bwpp_hip_launch_lm(h, LM_XENT_ROUND + 1, xent_grid(h, T), xent_columns(T, p.dim), 256, &r);
+  r.lanes = T >= 1024 ? 64 : 8;
+  const uint64_t blocks = up((D + 31) / 32, 8) * ((T + r.lanes - 1) / r.lanes);
   if (blocks * 256 > 0xffffffffull) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: too many elements", what);
   return bwpp_hip_launch_lm(h, LM_XENT_ROUND + 2, blocks, 1, 256, &r);
 }
