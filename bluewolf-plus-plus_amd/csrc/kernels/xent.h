@@ -654,11 +654,24 @@ __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
 #pragma unroll
           for (uint32_t e = 0; e < 3; ++e) v[e] += e < n ? src[i * plane + c + e] : 0.0f;
       }
+      if (n == 4) {
+        typedef uint16_t H4 __attribute__((ext_vector_type(4), aligned(2)));
+        if constexpr (sizeof(T) == 2) {
+          if (on) {
+            const H4 h = *reinterpret_cast<const H4 *>(w + c);
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) {
-        if (e >= n) break;
-        if (sizeof(T) == 2 && on) v[e] += rest * bf16_bits_to_f32(w[c + e]);
-        y[c + e] = to<T>(on ? v[e] : 0.0f);
+            for (uint32_t e = 0; e < 4; ++e) v[e] += rest * bf16_bits_to_f32(h[e]);
+          }
+          const H4 o = {to<T>(on ? v[0] : 0.0f), to<T>(on ? v[1] : 0.0f), to<T>(on ? v[2] : 0.0f), to<T>(on ? v[3] : 0.0f)};
+          *reinterpret_cast<H4 *>(y + c) = o;
+        } else {
+          store4(y + c, on ? make_float4(v[0], v[1], v[2], v[3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        }
+      } else {
+        for (uint32_t e = 0; e < n; ++e) {
+          const float add = sizeof(T) == 2 && on ? rest * bf16_bits_to_f32(w[c + e]) : 0.0f;
+          y[c + e] = to<T>(on ? (e == 0 ? v[0] : e == 1 ? v[1] : v[2]) + add : 0.0f);
+        }
       }
     }
   }
