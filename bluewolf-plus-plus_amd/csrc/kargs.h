@@ -192,8 +192,7 @@ typedef struct {
   uint32_t post_norm;
   float eps, stream_scale, branch_scale;
   /* gradient: a group is the rows of one row of dgate.  split > 1: that many
-   * blocks a group take `span` of its rows each, their gate sums go to
-   * part_gate; split = 1: workers (blocks, or waves of blocks where a wave
+   * blocks a group take its rows in turn, their gate sums go to part_gate; split = 1: workers (blocks, or waves of blocks where a wave
    * holds a row) take `span` rows each, whole groups.  nparts: blocks, one row
    * of partial sums each. */
   uint32_t workers, group, split, span, nparts;

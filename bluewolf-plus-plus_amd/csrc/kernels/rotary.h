@@ -22,6 +22,10 @@
 // half for bf16 with C = 8 and fp32 with C = 4 (any address), two 16-byte
 // loads side by side when interleaved; C = 4 of bf16 and C = 1 are for
 // rotated widths those do not divide.
+//
+// 4 x 4096 tokens of 32 + 8 heads of 128, bf16: 71 us (335 MB, 4.7 TB/s; a copy of as
+// many bytes, not in the caches, 65).  8 x 1 tokens: 4.5 us, a launch.  3 x 1001 x 24
+// heads of 80, 40 turned, fp32: 11.9 us (46 MB, 3.9 TB/s).
 #pragma once
 
 #include "common.h"

@@ -255,7 +255,7 @@ BwppHipStatus bwpp_hip_create(BwppHip **out, int device,
 void bwpp_hip_destroy(BwppHip *h);
 /* Stream for subsequent launches (a hipStream_t); NULL = the null stream.
  * The handle's workspace (split-K partials of fp32 products, attention-
- * backward row sums, column partials) is ordered on the handle's stream: when
+ * backward row sums, column partials, pieces of a cross entropy's logits) is ordered on the handle's stream: when
  * the stream changes, the new stream first waits for the work queued on the
  * old one.
  *
@@ -646,19 +646,26 @@ BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const void *o, co
  * leaves its row out (loss 0, no gradient; its lse is still written).  sums
  * (may be NULL): [0] the sum of the losses, [1] how many rows count.  loss and
  * lse may be NULL, not all three.  bf16 needs dim >= 8 (and, W not transposed,
- * vocab >= 8).  Workspace: a pair of floats per row and 64 to 256 columns of
- * the vocabulary (fp32: the logits of a piece of it, 256 MiB or 1024 columns). */
+ * vocab >= 8).  fp32 products run on fp32 matrix instructions or, for more
+ * tokens, on bf16 ones with each operand as three bf16 terms (24 bits).
+ * Workspace: a pair of floats per row and 64 to 256 columns of the vocabulary;
+ * fp32: the logits of a piece of it (256 MiB or 1024 columns), or terms of x and
+ * of a piece of W (8 bytes an element; the piece in 256 MiB, up to 1 GiB for few
+ * rows). */
 BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const void *w, const int32_t *targets,
                                             float *loss, float *lse, float *sums, BwppLinearXentParams params);
 
 /* Its gradients dx and dw (either may be NULL) for the upstream gradient dloss
  * of the row losses ([rows], one value with dloss_scalar, NULL = 1) and the
  * forward's lse.  The logits are made again, a piece of the vocabulary at a
- * time; bf16 rounds each dz to bf16 for the products that give dx and dw,
- * whose sums are fp32.  dx rows of left-out tokens are 0, and their x (which
- * may hold anything) has no part in dw.  Outputs must not meet inputs or each
- * other (ALIAS).  Workspace: a copy of x, dz of a piece (256 MiB or 1024
- * columns) and, with more than one piece in bf16, fp32 sums of dx. */
+ * time; bf16 rounds each dz to bf16 for the products that give dx and dw, whose
+ * sums are fp32, and adds to dx (and to a large dw) what that took from the
+ * targets' dz.  A dz that overflows to an infinity may come out as NaN.  dx rows
+ * of left-out tokens are 0, and their x (which may hold anything) has no part in
+ * dw.  Outputs must not meet inputs or each other (ALIAS).  Workspace: a copy of
+ * x, dz of a piece (256 MiB or 1024 columns) and fp32 sums of dx, 1 to 32 planes;
+ * fp32 in terms: those of x, W's and dz's piece, sums of dx and, up to 8 planes,
+ * of dw's piece. */
 BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const void *x, const void *w, const int32_t *targets,
                                                  const float *lse, const float *dloss, void *dx, void *dw,
                                                  BwppLinearXentParams params);
