@@ -510,6 +510,7 @@ XentTile xent_tile(const BwppHip *h, const BwppGemmArgs &g, bool tb, bool sums, 
       const uint64_t fill = rounds ? std::min<uint64_t>(rounds * cus / tiles, std::min<uint64_t>(g.K / 256, 32)) : 1;
       if (rounds && fill < 2) continue;
       const uint32_t k = (uint32_t)fill;
+      if (tiles * k * sh.threads > 0xffffffffull) continue;
       const double n = (double)((tiles * k + cus - 1) / cus);
       const double fetch = !tb && sh.bn == 64 ? mem * 1.25 : mem, planes = sums ? (double)k * g.M * g.N * 8.0 / 4e6 : 0.0;
       const double us = std::max(fetch, (n - 1.0) * sh.more + (double)g.K / k * (sh.lat + (n - 1.0) * sh.inc)) + planes;
@@ -599,8 +600,8 @@ uint32_t xent_piece(uint64_t rows, uint64_t vocab, uint64_t es) {
   if (n >= vocab) return (uint32_t)vocab;
   const uint64_t pieces = (vocab + n - 1) / n;
   n = up((vocab + pieces - 1) / pieces, 256);
-  while (vocab % n != 0 && vocab % n < 8) n -= 256;  // a last piece has a whole 16-byte chunk
-  return (uint32_t)n;
+  while (n < vocab && vocab % n != 0 && vocab % n < 8) n += 256;  // a last piece has a whole 16-byte chunk
+  return (uint32_t)std::min(n, vocab);
 }
 
 // Few rows: a block for every 1024 columns of one.
@@ -701,12 +702,16 @@ bool xent_in_terms(const BwppHip *h, const BwppLinearXentParams &p, const XentMa
   const double fp32 = 2.0 * T * D * V / rate + 10.0;
   double us = ((double)T + V) * D * 12.0 / 5e6 + 8.0;
   const double old = T * V * 8.0 / 4.5e6 + (grad ? 3.0 : 1.0) * fp32;
-  for (uint64_t n0 = 0; n0 < p.vocab && us < old; n0 += piece) {
-    const uint64_t n = std::min<uint64_t>(piece, p.vocab - n0);
+  const uint64_t count[2] = {p.vocab / piece, p.vocab % piece ? 1u : 0u}, size[2] = {piece, p.vocab % piece};
+  for (int i = 0; i < 2; ++i) {
+    if (!count[i]) continue;
     TermsTile tile;
     uint32_t split;
-    us += 5.0 + terms_us(h, T, n, K, 1, tile);
-    if (grad) us += terms_split_us(h, T, p.dim, up(n, 32), split, tile, true) + terms_split_us(h, p.dim, n, up(T, 32), split, tile, false);
+    double one = 5.0 + terms_us(h, T, size[i], K, 1, tile);
+    if (grad)
+      one += terms_split_us(h, T, p.dim, up(size[i], 32), split, tile, true) +
+             terms_split_us(h, p.dim, size[i], up(T, 32), split, tile, false);
+    us += (double)count[i] * one;
   }
   return us < old;
 }

@@ -486,3 +486,15 @@ def test_targets_keep_their_bits(be, wide, T, D, V, dw_too):
             (dx, dz @ wv.double(), err @ wv.double().abs(), dz.abs() @ wv.double().abs(), V),
             (_vd(dw, wide), dz.t().contiguous() @ x64, dw_err.t().contiguous() @ x64.abs(), dz.t().contiguous().abs() @ x64.abs(), T)):
         assert bool(((got.double() - want).abs() <= e + (terms + 8) * U * size + HALF_STEP[BF16] * want.abs()).all())
+
+
+def test_piece_with_a_short_rest(be):
+    """A vocabulary one past a multiple of every narrower piece: pieces grow until
+    the last has a chunk of 8 columns (stepping down would end at none)."""
+    T, D, V = 131072, 8, 6145
+    x, w, t = _case(T, D, V, BF16, "vd", 20)
+    t[::5] = -1
+    lse = torch.empty(T, device="cuda")
+    p = _params(T, D, V, BF16, "vd", x, w)
+    be.dispatch_linear_xent(x, w, t, None, lse, None, p)
+    _gradient(be, x, w, t, lse, None, BF16, "vd")
