@@ -23,8 +23,8 @@
 // operand (each element off by at most half a step, 2^-8 of it; dx and dW add
 // thousands of them, and are rounded to bf16 themselves).  A row's largest element
 // by far is its target's p - 1: what its rounding leaves is kept, a float a token,
-// and added by the kernels that sum dx's planes and dW's wide tiles (a small dW
-// keeps it).  It does so for
+// and added by the kernels that sum dx's planes and dW's wide tiles (a dW of few tiles
+// and many tokens keeps it).  It does so for
 // one piece of the vocabulary at a time, small enough to stay in the Infinity
 // Cache between its writer and its readers.  dx is summed over the pieces in
 // fp32 planes (one per K split) and rounded once; each piece's dW is final.

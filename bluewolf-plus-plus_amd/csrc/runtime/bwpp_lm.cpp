@@ -1054,7 +1054,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     const uint32_t k = wide ? piece / 32 * 32 : piece, range = (uint32_t)up((k + split - 1) / split, 128);
     split = (k + range - 1) / range;
   }
-  const bool dw_wide = bf16 && ((piece + 255ull) / 256) * ((D + 255) / 256) * 2 >= cus_of(h) &&
+  // dW on 256-wide tiles where they keep half of the CUs busy, or its K (tokens) is
+  // short; else K in ranges on dispatch_matmul's.
+  const bool dw_wide = bf16 && (T <= 256 || ((piece + 255ull) / 256) * ((D + 255) / 256) * 2 >= cus_of(h)) &&
                        256ull * std::max<uint64_t>(piece + 8ull, D + 8) < (1ull << 31);
   // (rows of x's copy and of dz up to a multiple of 32, zeros: dW's K)
   const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit), Tu = bf16 ? up(T, 32) : T;

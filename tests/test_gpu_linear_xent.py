@@ -450,7 +450,7 @@ def test_fp32_terms_infinities(be, wide):
 @pytest.mark.parametrize("wide,T,D,V,dw_too", [
     ("vd", 2048, 1024, 8205, True), ("dv", 2048, 1024, 8200, True), ("vd", 9000, 512, 16400, False),
     ("dv", 9000, 520, 16400, False), ("vd", 9000, 1032, 16400, True), ("dv", 9000, 1032, 16400, True),
-    ("vd", 300, 72, 2001, False), ("dv", 300, 72, 2000, False), ("vd", 210, 201, 9001, False), ("dv", 230, 600, 33000, True)])
+    ("vd", 300, 72, 2001, False), ("dv", 300, 72, 2000, False), ("vd", 210, 201, 9001, True), ("dv", 230, 600, 33000, True)])
 def test_targets_keep_their_bits(be, wide, T, D, V, dw_too):
     """In dx and in dW of the wide products the targets' dz, the largest of their rows,
     counts with its rounding's remainder (rounded to bf16 for dW): two half steps of it are off,
@@ -458,7 +458,7 @@ def test_targets_keep_their_bits(be, wide, T, D, V, dw_too):
     row, so that one half step of dz would show in the elements' bound.  One target
     of many tokens (more than a step of the matrix instructions takes), the last of
     the vocabulary, and some left out; two pieces for 9000 tokens.  dW with few tiles
-    (dim 512) is another kernel's, and has dz's half step."""
+    for many tokens is another kernel's, and has dz's half step."""
     x, w, t = _case(T, D, V, BF16, wide, 18, lean=0.0)
     t[100:180], t[200:203], t[4000:] = 5, V - 1, torch.where(t[4000:] < 600, 600, t[4000:])
     t[::11] = -1
