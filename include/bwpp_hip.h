@@ -660,10 +660,11 @@ BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const voi
  * forward's lse.  The logits are made again, a piece of the vocabulary at a
  * time; bf16 rounds each dz to bf16 for the products that give dx and dw, whose
  * sums are fp32, and adds to dx (and to dw, but for a small one of more than
- * 256 rows) what that took from the targets' dz.  A dz that overflows to an infinity may come out as NaN.  dx rows
- * of left-out tokens are 0, and their x (which may hold anything) has no part in
- * dw.  Outputs must not meet inputs or each other (ALIAS).  Workspace: a copy of
- * x, dz of a piece (256 MiB or 1024 columns) and fp32 sums of dx, 1 to 32 planes;
+ * 256 rows) what that took from the targets' dz.  A dz that overflows to an
+ * infinity may come out as NaN.  dx rows of left-out tokens are 0, and their x
+ * (which may hold anything) has no part in dw.  Outputs must not meet inputs or
+ * each other (ALIAS).  Workspace: a copy of x, dz of a piece (256 MiB or 1024
+ * columns, in some cases as many again) and fp32 sums of dx, 1 to 32 planes;
  * fp32 in terms: those of x, W's and dz's piece, sums of dx and, up to 8 planes,
  * of dw's piece. */
 BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const void *x, const void *w, const int32_t *targets,
