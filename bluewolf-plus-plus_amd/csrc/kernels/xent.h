@@ -23,8 +23,7 @@
 // operand (each element off by at most half a step, 2^-8 of it; dx and dW add
 // thousands of them, and are rounded to bf16 themselves).  A row's largest element
 // by far is its target's p - 1: what its rounding leaves is kept, a float a token,
-// and added by the kernels that sum dx's planes and dW's wide tiles (a dW of few tiles
-// and many tokens keeps it).  It does so for
+// and added by the kernels that sum dx's planes and make dW.  It does so for
 // one piece of the vocabulary at a time, small enough to stay in the Infinity
 // Cache between its writer and its readers.  dx is summed over the pieces in
 // fp32 planes (one per K split) and rounded once; each piece's dW is final.
@@ -186,41 +185,49 @@ struct EpiGrad {
   }
 };
 
-// bf16 rows (dW), at any address and row stride.
-struct EpiRows {
-  static constexpr bool kStore = false;
+// What dW's epilogues share.
+struct DwRest {
   const BwppXentArgs &a;
 
   // dW += x^T (what rounding left of the targets' dz): of a row of dz the target's
   // p - 1 is by far the largest element, and its rounding nearly all of the error
   // that dz's brings (dx and dW off by 0.0025 of their norm with it, 0.0017, their
-  // own rounding, without).  The tokens whose target is in the tile, in order, 32 at
-  // a time as one more K step: a one-hot operand of the remainders (bf16: 2^-9 of
-  // 2^-9) and the rows of x.  256 T / V tokens a tile on average.  No longer at 4096 x
-  // 2048 x 32768 (440 us), 2 to 6 us at 120 x 1216 x 19298 (19 -> 24) and the like.
-  template <class FR, int BM, int BN, int TM, int TN, class V, int FN, int FM>
-  __device__ __forceinline__ void add_rest(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, int tid,
-                                           int wm, int wn) const {
+  // own rounding, without).  Of the tokens first .. end - 1 those whose target is in
+  // the tile, in order, 32 at a time as one more K step: a one-hot operand of the
+  // remainders (bf16: 2^-9 of 2^-9) and the rows of x, both laid out as the main
+  // loop's K tiles.  256 T / V tokens a tile on average.  No longer at 4096 x 2048 x
+  // 32768 (440 us), 2 to 6 us at 120 x 1216 x 19298 (19 -> 24) and the like.
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void add_rest(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t first,
+                                           uint32_t end, int tid, int wm, int wn) const {
     asm volatile("" : "+v"(tid));  // nothing below is computed ahead of the main loop, whose registers are full
-    static_assert(FR::kSize == 16 && BM == 256 && BN == 256, "one layout for both operands");
-    constexpr uint32_t kEach = 8, kWindow = 512 * kEach;  // tokens a thread, and the block, looks at
-    unsigned char *hot = smem, *xs = smem + 16384;        // [32][256] each
-    uint32_t *list = reinterpret_cast<uint32_t *>(smem + 32768);  // [kWindow] tokens of the window, and their columns
-    uint32_t *totals = reinterpret_cast<uint32_t *>(smem + 32768 + 4 * kWindow);  // [8 waves]
+    static_assert(FR::kSize == 32 || (BM == 256 && BN == 256), "as the main loops lay out their tiles");
+    constexpr int TM = BM / WM, TN = BN / WN, NW = WM * WN, NT = 64 * NW;
+    constexpr uint32_t kEach = 8, kWindow = NT * kEach;  // tokens a thread, and the block, looks at
+    unsigned char *ta = smem, *tb = smem + BM * 64;       // K tiles of 32
+    uint32_t *list = reinterpret_cast<uint32_t *>(smem + (BM + BN) * 64);  // [kWindow] tokens of the window, and their columns
+    uint32_t *totals = list + kWindow;                                     // [NW]
     const int lane = tid & 63, wave = tid >> 6;
-    const uint32_t v0 = a.n_base + (a.x_is_a ? n0 : m0), d0 = a.x_is_a ? m0 : n0;
-    const uint32_t lim = (a.x_is_a ? a.g.M : a.g.N) - d0;
-    const uint16_t *x = static_cast<const uint16_t *>(a.x_is_a ? a.g.a : a.g.b);
-    const uint64_t ldx = a.x_is_a ? a.g.lda : a.g.ldb;
-    unsigned char *ta = a.x_is_a ? xs : hot, *tb = a.x_is_a ? hot : xs;
-    for (uint32_t w0 = 0; w0 < a.rows; w0 += kWindow) {
+    const bool xa = a.x_is_a;
+    const uint32_t v0 = a.n_base + (xa ? n0 : m0), d0 = xa ? m0 : n0;
+    const uint32_t lim = (xa ? a.g.M : a.g.N) - d0;
+    const uint16_t *x = static_cast<const uint16_t *>(xa ? a.g.a : a.g.b);
+    const uint64_t ldx = xa ? a.g.lda : a.g.ldb;
+    unsigned char *xs = xa ? ta : tb, *hot = xa ? tb : ta;
+    const uint32_t wx = xa ? BM : BN, wh = xa ? BN : BM;
+    // Byte offset of chunk c of k-row k in a tile of that width.
+    auto pos = [&](bool in_a, uint32_t k, uint32_t c) {
+      if constexpr (FR::kSize == 16) return k * 512u + 16u * (c ^ mnc16_swz(k));
+      else return in_a ? mnc_off<BM>(k, c) : mnc_off<BN>(k, c);
+    };
+    for (uint32_t w0 = first; w0 < end; w0 += kWindow) {
       uint32_t mine = 0, column[kEach];  // bit e: token w0 + kEach tid + e
 #pragma unroll
       for (uint32_t e = 0; e < kEach; ++e) {
         const uint32_t m = w0 + kEach * (uint32_t)tid + e;
-        const uint32_t t = m < a.rows ? (uint32_t)a.target[m] : 0xffffffffu;
+        const uint32_t t = m < end ? (uint32_t)a.target[m] : 0xffffffffu;
         column[e] = t - v0;
-        if (t < a.vocab && column[e] < 256u) mine |= 1u << e;
+        if (t < a.vocab && column[e] < wh) mine |= 1u << e;
       }
       const uint32_t n = (uint32_t)__popc(mine);
       uint32_t before = n;  // of the wave's lanes up to this one
@@ -233,7 +240,7 @@ struct EpiRows {
       __syncthreads();
       uint32_t at = before - n, count = 0;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const uint32_t c = totals[w];
         if (w < wave) at += c;
         count += c;
@@ -247,37 +254,56 @@ struct EpiRows {
         const uint32_t entry = one ? list[b + (uint32_t)tid] : 0u;
         const float rest = one ? a.rest[w0 + (entry & 0xffffu)] : 0.0f;
 #pragma unroll 1
-        for (int q = tid; q < 1024; q += 512) {
-          const uint32_t k = (uint32_t)q >> 5, c = (uint32_t)q & 31u;
+        for (uint32_t q = (uint32_t)tid; q < 4u * wh; q += NT) *reinterpret_cast<u32x4_t *>(hot + 16u * q) = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll 1
+        for (uint32_t q = (uint32_t)tid; q < 4u * wx; q += NT) {
+          const uint32_t k = q / (wx / 8u), c = q % (wx / 8u);
           u32x4_t v = {0u, 0u, 0u, 0u};
-          *reinterpret_cast<u32x4_t *>(hot + 16 * q) = v;
           if (b + k < count)
             v = *reinterpret_cast<const u32x4_t *>(x + (uint64_t)(w0 + (list[b + k] & 0xffffu)) * ldx + d0 +
                                                    min(8u * c, lim - 8u));
-          *reinterpret_cast<u32x4_t *>(xs + k * 512u + 16u * (c ^ mnc16_swz(k))) = v;
+          *reinterpret_cast<u32x4_t *>(xs + pos(xa, k, c)) = v;
         }
         __syncthreads();
         if (one) {
-          const uint32_t k = (uint32_t)tid, v = entry >> 16;
-          *reinterpret_cast<uint16_t *>(hot + k * 512u + 16u * ((v >> 3) ^ mnc16_swz(k)) + 2u * (v & 7u)) =
-              f32_to_bf16_bits(rest);
+          const uint32_t v = entry >> 16;
+          *reinterpret_cast<uint16_t *>(hot + pos(!xa, (uint32_t)tid, v >> 3) + 2u * (v & 7u)) = f32_to_bf16_bits(rest);
         }
         __syncthreads();
-        bf16x8_t fb[FN];
+        if constexpr (FR::kSize == 16) {
+          bf16x8_t fb[FN];
 #pragma unroll
-        for (int i = 0; i < FN; ++i) fb[i] = read16<true, 256>(tb, (uint32_t)(wn * TN + i * 16), lane);
+          for (int i = 0; i < FN; ++i) fb[i] = read16<true, BN>(tb, (uint32_t)(wn * TN + i * 16), lane);
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-          const bf16x8_t fa = read16<true, 256>(ta, (uint32_t)(wm * TM + j * 16), lane);
+          for (int j = 0; j < FM; ++j) {
+            const bf16x8_t fa = read16<true, BM>(ta, (uint32_t)(wm * TM + j * 16), lane);
 #pragma unroll
-          for (int i = 0; i < FN; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa, acc[i][j], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);  // one operand in registers at a time
+            for (int i = 0; i < FN; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa, acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);  // one operand in registers at a time
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+              const bf16x8_t fa = read_operand<true, BM>(ta, (uint32_t)(wm * TM + j * 32), ks, lane);
+#pragma unroll
+              for (int i = 0; i < FN; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    read_operand<true, BN>(tb, (uint32_t)(wn * TN + i * 32), ks, lane), fa, acc[i][j], 0, 0, 0);
+            }
         }
         __syncthreads();
       }
     }
     __syncthreads();
   }
+};
+
+// bf16 rows (dW), at any address and row stride: on 256-wide tiles, or where those
+// are few (T > 256) on the smaller ones.
+struct EpiRows : DwRest {
+  static constexpr bool kStore = false;
 
   template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
   __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t, uint32_t,
@@ -285,7 +311,7 @@ struct EpiRows {
     constexpr int TM = BM / WM, TN = BN / WN, NT = 64 * WM * WN, kCld = BN + 8;
     const int lane = tid & 63;
     uint16_t *cs = reinterpret_cast<uint16_t *>(smem);  // [BM][BN + 8]
-    add_rest<FR, BM, BN, TM, TN>(acc, smem, m0, n0, tid, wm, wn);
+    add_rest<FR, BM, BN, WM, WN>(acc, smem, m0, n0, 0, a.rows, tid, wm, wn);
 #pragma unroll
     for (int j = 0; j < FM; ++j)
 #pragma unroll
@@ -312,6 +338,45 @@ struct EpiRows {
       } else {
         for (uint32_t e = 0; e < 8 && n + e < a.cols_out; ++e) dst[e] = h[e];
       }
+    }
+  }
+};
+
+// dW where those are few too: K (tokens) in ranges, each an fp32 plane [rows_out]
+// [cols_out] with the remainders of its own tokens, so that a batch with one target
+// brings a tile as many steps as the main loop has, not a block T / 32.  Beside
+// dispatch_matmul without remainders (dW off by 0.0021 to 0.0028 of its norm, 0.0017
+// so), us a pass of loss and gradients: 300 x 256 x 1000 29.5 -> 31, 1505 x 1024 x
+// 3144 104 -> 106, 8000 x 512 x 1000 99 -> 104, 20000 x 64 x 15400 742 -> 770, 635 x
+// 2560 x 2240 104 -> 103.  (256-wide tiles in ranges: 48, 122, 112, 809, 122.)
+struct EpiRowSums : DwRest {
+  static constexpr bool kStore = false;
+
+  template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
+  __device__ __forceinline__ void run(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t, uint32_t split,
+                                      int tid, int wm, int wn) const {
+    constexpr int TM = BM / WM, TN = BN / WN;
+    const int lane = tid & 63;
+    const uint32_t first = split * a.g.kchunk;
+    add_rest<FR, BM, BN, WM, WN>(acc, smem, m0, n0, first, min(a.rows, first + a.g.kchunk), tid, wm, wn);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t m = m0 + (uint32_t)(wm * TM + j * FR::kSize) + FR::row(lane);
+      if (m >= a.rows_out) continue;
+      float *row = a.raw + ((size_t)split * a.rows_out + m) * a.cols_out;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int r = 0; r < FR::kRegs; r += 4) {
+          const uint32_t n = n0 + (uint32_t)(wn * TN + i * FR::kSize) + FR::col(lane, r);
+          if (n + 4 <= a.cols_out) {
+            store4(row + n, make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.cols_out) row[n + e] = acc[i][j][r + e];
+          }
+        }
     }
   }
 };
@@ -629,8 +694,9 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_grad_f32(const BwppX
   }
 }
 
-// Planes of fp32 sums -> rows of T, rows that are left out 0; bf16: with W's row of
-// the target times what rounding left of its dz (EpiRows::add_rest).
+// Planes of fp32 sums -> rows of T, rows that are left out 0 (no targets: every row
+// counts); bf16 dx: with W's row of the target times what rounding left of its dz
+// (DwRest::add_rest).
 template <class T>
 __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
   const uint64_t plane = (uint64_t)a.rows * a.cols;
@@ -638,8 +704,9 @@ __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
     const bool on = !a.target || live(a, row);
     T *y = static_cast<T *>(a.y) + row * a.ldy;
     const float *src = a.src + (uint64_t)row * a.cols;
-    const float rest = sizeof(T) == 2 && on ? a.rest[row] : 0.0f;
-    const uint16_t *w = static_cast<const uint16_t *>(a.w) + (sizeof(T) == 2 && on ? (uint32_t)a.target[row] * a.ldw : 0u);
+    const bool add = sizeof(T) == 2 && on && a.rest;
+    const float rest = add ? a.rest[row] : 0.0f;
+    const uint16_t *w = static_cast<const uint16_t *>(a.w) + (add ? (uint32_t)a.target[row] * a.ldw : 0u);
     for (uint32_t c = (blockIdx.y * 256u + threadIdx.x) * 4u; c < a.cols; c += gridDim.y * 1024u) {
       const uint32_t n = min(4u, a.cols - c);
       float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -657,7 +724,7 @@ __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
       if (n == 4) {
         typedef uint16_t H4 __attribute__((ext_vector_type(4), aligned(2)));
         if constexpr (sizeof(T) == 2) {
-          if (on) {
+          if (add) {
             const H4 h = *reinterpret_cast<const H4 *>(w + c);
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) v[e] += rest * bf16_bits_to_f32(h[e]);
@@ -669,8 +736,8 @@ __device__ __forceinline__ void sum_planes(const BwppXentRowArgs &a) {
         }
       } else {
         for (uint32_t e = 0; e < n; ++e) {
-          const float add = sizeof(T) == 2 && on ? rest * bf16_bits_to_f32(w[c + e]) : 0.0f;
-          y[c + e] = to<T>(on ? (e == 0 ? v[0] : e == 1 ? v[1] : v[2]) + add : 0.0f);
+          const float more = add ? rest * bf16_bits_to_f32(w[c + e]) : 0.0f;
+          y[c + e] = to<T>(on ? (e == 0 ? v[0] : e == 1 ? v[1] : v[2]) + more : 0.0f);
         }
       }
     }
@@ -765,7 +832,8 @@ BWPP_XENT_ROWS(f32, float)
 
 // bwpp_xent_<stats|grad|sums>_<tile>_t0<TB>: p = 256 x 256 (K in steps of
 // 32), sp and sh = 256 x 256 and 128 x 256 for fp32 in terms; any sizes: r32 = 32 x 64, r64 = 64 x 64,
-// r128 = 128 x 128, _u with operands through registers.
+// r128 = 128 x 128, _u with operands through registers.  bwpp_xent_rows_<tile>_t10 and
+// rowsums: dW.
 #define BWPP_XENT_K32(NAME, EPI, TA, TB, BM, SPLIT)                                                       \
   extern "C" __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) \
   void bwpp_xent_##NAME(const BwppXentArgs a) {                                                           \
@@ -779,6 +847,12 @@ BWPP_XENT_ROWS(f32, float)
   extern "C" __global__ __launch_bounds__(64 * WM * WN, WPEU) void bwpp_xent_##KIND##_##NAME##_t0##TB##_u(      \
       const BwppXentArgs a) {                                                                                   \
     gemm_bf16_ring<false, TB != 0, BM, BN, WM, WN, KPSU, 2, true, EPI>(a.g, EPI{a});                            \
+  }
+// A transposed (dW: both operands are rows of tokens in the workspace, whole chunks).
+#define BWPP_XENT_RING_T(KIND, EPI, NAME, BM, BN, WM, WN, KPS, STAGES, WPE)                                     \
+  extern "C" __global__ __launch_bounds__(64 * WM * WN, WPE) void bwpp_xent_##KIND##_##NAME##_t10(              \
+      const BwppXentArgs a) {                                                                                   \
+    gemm_bf16_ring<true, false, BM, BN, WM, WN, KPS, STAGES, false, EPI>(a.g, EPI{a});                          \
   }
 #define BWPP_XENT_TB(TB)                                                    \
   BWPP_XENT_K32(stats_p_t0##TB, EpiStats, 0, TB, 256, false)                \
@@ -802,6 +876,12 @@ BWPP_XENT_ROWS(f32, float)
 BWPP_XENT_TB(0)
 BWPP_XENT_TB(1)
 BWPP_XENT_K32(rows_p_t10, EpiRows, 1, 0, 256, false)
+BWPP_XENT_RING_T(rows, EpiRows, r32, 32, 64, 1, 2, 4, 4, 1)
+BWPP_XENT_RING_T(rows, EpiRows, r64, 64, 64, 2, 2, 2, 4, 2)
+BWPP_XENT_RING_T(rows, EpiRows, r128, 128, 128, 2, 2, 1, 3, 2)
+BWPP_XENT_RING_T(rowsums, EpiRowSums, r32, 32, 64, 1, 2, 4, 4, 1)
+BWPP_XENT_RING_T(rowsums, EpiRowSums, r64, 64, 64, 2, 2, 2, 4, 2)
+BWPP_XENT_RING_T(rowsums, EpiRowSums, r128, 128, 128, 2, 2, 1, 3, 2)
 BWPP_XENT_K32(rows_sp_t10, EpiRowsF32, 1, 0, 256, true)
 BWPP_XENT_K32(rows_sh_t10, EpiRowsF32, 1, 0, 128, true)
 BWPP_XENT_K32(sums_sp_t10, EpiSums, 1, 0, 256, true)

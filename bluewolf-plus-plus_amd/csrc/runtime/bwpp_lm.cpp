@@ -31,7 +31,9 @@ enum LmKernel {
   LM_XENT_GRAD = LM_XENT_STATS + 14,
   LM_XENT_RAW = LM_XENT_GRAD + 14,
   LM_XENT_ROWS = LM_XENT_RAW + 14,
-  LM_TERMS_STATS,                        // [trans_w][TermsTile]
+  LM_XENT_ROWS_RING,                     // XT_R32, XT_R64, XT_R128
+  LM_XENT_ROW_SUMS = LM_XENT_ROWS_RING + 3,  // the same
+  LM_TERMS_STATS = LM_XENT_ROW_SUMS + 3,                        // [trans_w][TermsTile]
   LM_TERMS_GRAD = LM_TERMS_STATS + 4,
   LM_TERMS_RAW = LM_TERMS_GRAD + 4,
   LM_TERMS_ROWS = LM_TERMS_RAW + 4,      // [TermsTile]
@@ -113,6 +115,12 @@ const char *const bwpp_hip_lm_kernels[] = {
     "bwpp_xent_sums_r128_t01",
     "bwpp_xent_sums_r128_t01_u",
     "bwpp_xent_rows_p_t10",
+    "bwpp_xent_rows_r32_t10",
+    "bwpp_xent_rows_r64_t10",
+    "bwpp_xent_rows_r128_t10",
+    "bwpp_xent_rowsums_r32_t10",
+    "bwpp_xent_rowsums_r64_t10",
+    "bwpp_xent_rowsums_r128_t10",
     "bwpp_xent_stats_sp_t00",
     "bwpp_xent_stats_sh_t00",
     "bwpp_xent_stats_sp_t01",
@@ -1054,15 +1062,32 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     const uint32_t k = wide ? piece / 32 * 32 : piece, range = (uint32_t)up((k + split - 1) / split, 128);
     split = (k + range - 1) / range;
   }
-  // dW on 256-wide tiles where they keep half of the CUs busy, or its K (tokens) is
-  // short; else K in ranges on dispatch_matmul's.
-  const bool dw_wide = bf16 && (T <= 256 || ((piece + 255ull) / 256) * ((D + 255) / 256) * 2 >= cus_of(h)) &&
-                       256ull * std::max<uint64_t>(piece + 8ull, D + 8) < (1ull << 31);
+  // dW on 256-wide tiles where they keep half of the CUs busy or its K (tokens) is
+  // short; else on the tiles and K ranges that are modelled fastest, several ranges
+  // summed from planes.  (Rows that 32-bit offsets do not span: dispatch_matmul's,
+  // without the targets' remainders.)
+  const bool dw_fits = bf16 && 256ull * std::max<uint64_t>(piece + 8ull, D + 8) < (1ull << 31);
+  const bool dw_wide = dw_fits && (T <= 256 || ((piece + 255ull) / 256) * ((D + 255) / 256) * 2 >= cus_of(h));
+  const bool dw_ring = dw && dw_fits && !dw_wide;
+  uint32_t dw_split = 1;
+  XentTile dw_tile = XT_P;
+  if (dw_ring) {
+    BwppGemmArgs g = {};
+    g.M = (uint32_t)(tw ? up(piece, 8) : up(D, 8));
+    g.N = (uint32_t)(tw ? up(D, 8) : up(piece, 8));
+    g.K = (uint32_t)up(T, 32);
+    g.lda = g.M;
+    g.ldb = g.N;
+    dw_tile = xent_tile(h, g, false, true, &dw_split);
+    const uint32_t range = dw_split > 1 ? (uint32_t)up((g.K + (uint64_t)dw_split - 1) / dw_split, 128) : g.K;
+    dw_split = (g.K + range - 1) / range;  // as xent_product cuts them
+  }
   // (rows of x's copy and of dz up to a multiple of 32, zeros: dW's K)
   const uint64_t unit = bf16 ? 8 : 4, ldxc = up(D, unit), ldz = up(piece, unit), Tu = bf16 ? up(T, 32) : T;
   const uint64_t x_bytes = dw ? up(Tu * ldxc * es, 256) : 0, z_bytes = up(Tu * ldz * es, 256);
   const uint64_t sum_bytes = sums ? up(split * T * D * 4, 256) : 0, rest_bytes = bf16 ? up(T * 4, 256) : 0;
-  const uint64_t held = x_bytes + z_bytes + sum_bytes + rest_bytes;
+  const uint64_t dw_bytes = dw_split > 1 ? dw_split * (uint64_t)piece * D * 4 : 0;
+  const uint64_t held = x_bytes + z_bytes + sum_bytes + rest_bytes + dw_bytes;
   void *ws = nullptr;
   if ((s = bwpp_hip_take_workspace(h, held + (bf16 ? 0 : kXentSplitRoom), &ws)) != BWPP_HIP_OK) return s;
   Hold hold(h, held);
@@ -1163,7 +1188,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       if (s != BWPP_HIP_OK) return s;
     }
     void *dwp = dw ? const_cast<unsigned char *>(at(dw, tw ? n0 * m.lddw : n0)) : nullptr;
-    if (dw && dw_wide) {
+    if (dw && (dw_wide || dw_ring)) {
       BwppXentArgs a = {};
       a.g.a = tw ? z : xc;
       a.g.b = tw ? xc : z;
@@ -1182,7 +1207,21 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
       a.rest = rest;
       a.rows = p.rows;
       a.x_is_a = !tw;
-      if ((s = xent_product(h, LM_XENT_ROWS, a, false, XT_P, 1)) != BWPP_HIP_OK) return s;
+      a.raw = reinterpret_cast<float *>(base + x_bytes + z_bytes + sum_bytes + rest_bytes);
+      const int ring = (dw_tile - XT_R32) / 2 - dw_tile;  // XT_R32, XT_R64, XT_R128 as 0, 1, 2
+      s = xent_product(h, !dw_ring ? LM_XENT_ROWS : (dw_split > 1 ? LM_XENT_ROW_SUMS : LM_XENT_ROWS_RING) + ring, a, false,
+                       dw_tile, dw_split);
+      if (s != BWPP_HIP_OK) return s;
+      if (dw_split > 1) {
+        BwppXentRowArgs f = {};
+        f.src = a.raw;
+        f.nparts = dw_split;
+        f.rows = a.rows_out;
+        f.cols = a.cols_out;
+        f.y = dwp;
+        f.ldy = m.lddw;
+        if ((s = bwpp_hip_launch_lm(h, LM_XENT_ROUND + 1, xent_grid(h, f.rows), xent_columns(f.rows, f.cols), 256, &f)) != BWPP_HIP_OK) return s;
+      }
     } else if (dw) {
       BwppMatmulParams g = {};
       g.K = p.rows;

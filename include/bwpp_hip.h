@@ -659,9 +659,9 @@ BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const voi
  * of the row losses ([rows], one value with dloss_scalar, NULL = 1) and the
  * forward's lse.  The logits are made again, a piece of the vocabulary at a
  * time; bf16 rounds each dz to bf16 for the products that give dx and dw, whose
- * sums are fp32, and adds to dx (and to dw, but for a small one of more than
- * 256 rows) what that took from the targets' dz.  A dz that overflows to an
- * infinity may come out as NaN.  dx rows of left-out tokens are 0, and their x
+ * sums are fp32, and adds to them what that took from the targets' dz (not to
+ * dx for a vocab below 8, nor to dw for a dim or a vocab of 2^23 and more).  A
+ * dz that overflows to an infinity may come out as NaN.  dx rows of left-out tokens are 0, and their x
  * (which may hold anything) has no part in dw.  Outputs must not meet inputs or
  * each other (ALIAS).  Workspace: a copy of x, dz of a piece (256 MiB or 1024
  * columns, in some cases as many again) and fp32 sums of dx, 1 to 32 planes;

@@ -1,0 +1,54 @@
+"""dW of few tiles from many tokens (K in ranges, summed in planes): the targets'
+dz counts with what its rounding to bf16 left, as in dW of many tiles.
+
+A log-sum-exp 7 above the logits' leaves p small, so that a half step of the
+targets' p - 1 alone would pass the elements' bound: each other dz is off by
+rel, its exp's error, and a half step; a target's by rel of p, and by two half
+steps of p - 1 one after the other (its remainder is rounded to bf16) and fp32's
+own; sums add (terms + planes) 2^-24 of the terms' magnitudes, the result half a
+step of itself."""
+import pytest
+import torch
+
+from lm64 import HALF_STEP, strided, untouched
+from test_gpu_linear_xent import BF16, U, _case, _logit_error, _params, _vd
+
+pytestmark = pytest.mark.gpu
+H = HALF_STEP[BF16]
+
+
+@pytest.mark.parametrize("wide,T,D,V,targets,pads", [
+    ("vd", 257, 8, 9, "any", (0, 0)), ("dv", 257, 9, 8, "any", (0, 0)), ("vd", 300, 72, 2001, "any", (3, 1)),
+    ("dv", 300, 72, 2000, "any", (3, 1)), ("vd", 1505, 1024, 3144, "any", (0, 0)), ("dv", 1505, 1024, 3144, "any", (0, 5)),
+    ("vd", 4500, 130, 515, "one", (0, 0)), ("dv", 4500, 130, 515, "one", (0, 0)), ("vd", 9000, 512, 16400, "any", (0, 0)),
+    ("dv", 9000, 520, 16400, "few", (0, 0)), ("vd", 8191, 264, 300, "few", (8, 8))])
+def test_targets_keep_their_bits(be, wide, T, D, V, targets, pads):
+    g = torch.Generator(device="cuda").manual_seed(77)
+    x, w, t = _case(T, D, V, BF16, wide, 21, lean=0.0)
+    if targets == "one":  # every token's
+        t[:] = V - 1
+    if targets == "few":
+        t %= 7
+    t[::11] = -1
+    wv, live = _vd(w, wide), t >= 0
+    z = x.double() @ wv.double().t().contiguous()
+    lse = (torch.logsumexp(z, dim=1) + 7.0).float()
+    up = torch.rand(T, device="cuda", generator=g) + 0.5
+    p = torch.exp(z - lse.double()[:, None]) * torch.where(live, up.double(), 0.0)[:, None]
+    rel = (_logit_error(x, wv, 1.0) + 20 * U)[:, None]
+    rows = torch.arange(T, device="cuda")[live]
+    cols = t[live].long()
+    dz, err = p.clone(), p * (rel + H)
+    dz[rows, cols] -= up.double()[live]
+    err[rows, cols] = p[rows, cols] * rel[live, 0] + dz[rows, cols].abs() * (H ** 2 + 4 * U)
+    x64 = torch.where(live[:, None], x.double(), 0.0)
+    want = dz.t().contiguous() @ x64
+    tol = err.t().contiguous() @ x64.abs() + (T + 40) * U * (dz.t().contiguous().abs() @ x64.abs()) + H * want.abs()
+    for only in (False, True):
+        dx = None if only else torch.empty_like(x)
+        dw, buf = strided(tuple(w.shape), (w.shape[1] + pads[1], 1), BF16)
+        be.dispatch_linear_xent_grad(x, w, t, lse, up, dx, dw, _params(T, D, V, BF16, wide, x, w, lddw=dw.stride(0)))
+        recent = [be.recent_kernel(i) for i in range(3)]
+        assert any(k.startswith(("bwpp_xent_rowsums_r", "bwpp_xent_rows_r")) for k in recent), recent
+        assert bool(((_vd(dw, wide).double() - want).abs() <= tol).all()), only
+        assert untouched(dw, buf)
