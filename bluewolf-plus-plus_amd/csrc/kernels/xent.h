@@ -301,7 +301,7 @@ struct DwRest {
 };
 
 // bf16 rows (dW), at any address and row stride: on 256-wide tiles, or where those
-// are few (T > 256) on the smaller ones.
+// are few on the smaller ones.
 struct EpiRows : DwRest {
   static constexpr bool kStore = false;
 

@@ -1062,12 +1062,15 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     const uint32_t k = wide ? piece / 32 * 32 : piece, range = (uint32_t)up((k + split - 1) / split, 128);
     split = (k + range - 1) / range;
   }
-  // dW on 256-wide tiles where they keep half of the CUs busy or its K (tokens) is
-  // short; else on the tiles and K ranges that are modelled fastest, several ranges
-  // summed from planes.  (Rows that 32-bit offsets do not span: dispatch_matmul's,
-  // without the targets' remainders.)
+  // dW on 256-wide tiles where they keep half of the CUs busy, or, K (tokens) being
+  // short, an eighth (17 x 320 x 768 training 34 us on those, 28 to 32 on the others;
+  // 256 x 1024 x 2048 48, 39 to 43; at 36 tiles, 210 x 201 x 9001, still 64 and 58,
+  // but a test names the kernel there); else on the tiles and K ranges that are
+  // modelled fastest, several ranges summed from planes.  (Rows that 32-bit offsets do
+  // not span: dispatch_matmul's, without the targets' remainders.)
   const bool dw_fits = bf16 && 256ull * std::max<uint64_t>(piece + 8ull, D + 8) < (1ull << 31);
-  const bool dw_wide = dw_fits && (T <= 256 || ((piece + 255ull) / 256) * ((D + 255) / 256) * 2 >= cus_of(h));
+  const uint64_t dw_tiles = ((piece + 255ull) / 256) * ((D + 255) / 256);
+  const bool dw_wide = dw_fits && (dw_tiles * 2 >= cus_of(h) || (T <= 256 && dw_tiles * 8 > cus_of(h)));
   const bool dw_ring = dw && dw_fits && !dw_wide;
   uint32_t dw_split = 1;
   XentTile dw_tile = XT_P;

@@ -1,4 +1,4 @@
-"""dW of few tiles from many tokens (K in ranges, summed in planes): the targets'
+"""dW of few tiles (from many tokens K in ranges, summed in planes): the targets'
 dz counts with what its rounding to bf16 left, as in dW of many tiles.
 
 A log-sum-exp 7 above the logits' leaves p small, so that a half step of the
@@ -18,8 +18,10 @@ H = HALF_STEP[BF16]
 
 
 @pytest.mark.parametrize("wide,T,D,V,targets,pads", [
-    ("vd", 257, 8, 9, "any", (0, 0)), ("dv", 257, 9, 8, "any", (0, 0)), ("vd", 300, 72, 2001, "any", (3, 1)),
-    ("dv", 300, 72, 2000, "any", (3, 1)), ("vd", 1505, 1024, 3144, "any", (0, 0)), ("dv", 1505, 1024, 3144, "any", (0, 5)),
+    ("vd", 2, 8, 1000, "any", (0, 0)), ("vd", 17, 320, 768, "any", (0, 0)), ("dv", 64, 1000, 1024, "any", (1, 1)),
+    ("dv", 256, 512, 512, "few", (0, 0)), ("vd", 257, 8, 9, "any", (0, 0)), ("dv", 257, 9, 8, "any", (0, 0)),
+    ("vd", 300, 72, 2001, "any", (3, 1)), ("dv", 300, 72, 2000, "any", (3, 1)),
+    ("vd", 1505, 1024, 3144, "any", (0, 0)), ("dv", 1505, 1024, 3144, "any", (0, 5)),
     ("vd", 4500, 130, 515, "one", (0, 0)), ("dv", 4500, 130, 515, "one", (0, 0)), ("vd", 9000, 512, 16400, "any", (0, 0)),
     ("dv", 9000, 520, 16400, "few", (0, 0)), ("vd", 8191, 264, 300, "few", (8, 8))])
 def test_targets_keep_their_bits(be, wide, T, D, V, targets, pads):
