@@ -16,7 +16,7 @@
 //   value NAME DTYPE [EXPR,...] KIND  DTYPE: f32 | bf16 | i32 (input or param only);
 //                                     KIND: input | param | temp | output | const=<float>
 //   view NAME of=BASE offset=EXPR ld=EXPR shape=[EXPR,EXPR]
-//   op KIND out=A[,B..] in=X[,Y..] [key=value ...]
+//   op KIND out=A[,B..] in=X[,Y..] [key=value ...]   numbers: an EXPR, or one decimal number
 // Op kinds: matmul (ta, tb, epi, fuse), softmax, rmsnorm, layernorm,
 // add / sub / mul / div / copy / silu (bcast; copy may take up to 4
 // in/out pairs, one launch), reduce_sum, reduce_max,
@@ -157,7 +157,7 @@ BwppHipStatus perr(BwppHipPlan *p, BwppHipStatus st, const char *fmt, ...) {
 bool eval_expr(const BwppHipPlan &p, const std::string &e, uint64_t &out) {
   out = 1;
   for (const std::string &t : split(e, '*')) {
-    if (t.empty()) return false;
+    if (t.empty() || t[0] == '-') return false;  // (strtoull takes a minus, modulo 2^64)
     char *end = nullptr;
     unsigned long long v = strtoull(t.c_str(), &end, 10);
     if (end && *end == '\0') {
@@ -571,6 +571,39 @@ std::string attr(const Op &op, const char *k, const char *dflt) {
   return it == op.attrs.end() ? std::string(dflt) : it->second;
 }
 
+// An op's numeric attributes: a product of integers and dims, or one decimal
+// number.  `wrong` becomes the first one that is neither, or out of its range;
+// the op's default is used for it until the op reports that.
+struct Numbers {
+  const BwppHipPlan &p;
+  const Op &op;
+  std::string wrong;
+
+  double num(const char *key, double dflt) {
+    auto it = op.attrs.find(key);
+    if (it == op.attrs.end()) return dflt;
+    uint64_t n = 0;
+    if (eval_expr(p, it->second, n)) return (double)n;
+    char *end = nullptr;
+    const double v = strtod(it->second.c_str(), &end);
+    if (end != it->second.c_str() && *end == '\0' && std::isfinite(v)) return v;
+    return refuse(key, dflt);
+  }
+  // A whole number from lo to hi.
+  double whole(const char *key, double dflt, double lo, double hi) {
+    const double v = num(key, dflt);
+    return v >= lo && v <= hi && v == std::floor(v) ? v : refuse(key, dflt);
+  }
+  uint32_t count(const char *key, uint32_t dflt) { return (uint32_t)whole(key, dflt, 0.0, 4294967295.0); }
+  int32_t integer(const char *key, int32_t dflt) { return (int32_t)whole(key, dflt, -2147483648.0, 2147483647.0); }
+
+ private:
+  double refuse(const char *key, double dflt) {
+    if (wrong.empty()) wrong = std::string(key) + "=" + op.attrs.find(key)->second + " is no number that it takes";
+    return dflt;
+  }
+};
+
 // The names in a comma-separated attribute, in order (none where absent).
 std::vector<std::string> name_list(const Op &op, const char *k) {
   const std::string v = attr(op, k, "");
@@ -601,15 +634,9 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
   auto ptr = [&](int i) { return i < 0 ? nullptr : bwpp_hip_plan_value_ptr(&p, p.values[i].name.c_str()); };
   auto f32 = [&](int i) { return static_cast<float *>(ptr(i)); };
   auto i32 = [&](int i) { return static_cast<const int32_t *>(ptr(i)); };
-  auto bad = [&](const char *what) {
-    return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d (%s): %s", op.line, k.c_str(), what);
-  };
-  auto num = [&](const char *key, double dflt) {
-    auto it = op.attrs.find(key);
-    if (it == op.attrs.end()) return dflt;
-    uint64_t n = 0;
-    if (eval_expr(p, it->second, n) && it->second.find('.') == std::string::npos) return (double)n;
-    return strtod(it->second.c_str(), nullptr);
+  Numbers at{p, op, {}};
+  auto bad = [&](const char *what) {  // (a wrong number is named before what followed from its default)
+    return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d (%s): %s", op.line, k.c_str(), at.wrong.empty() ? what : at.wrong.c_str());
   };
   auto shape = [&](int i, uint64_t rows, uint64_t cols) { return i < 0 || (val(i).rows() == rows && val(i).cols() == cols); };
   auto elems = [&](int i, uint64_t n) { return i < 0 || (val(i).kind != Kind::kView && val(i).elems() == n); };
@@ -639,8 +666,8 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     const int pos = val(op.ins.back()).dtype == kI32 ? op.ins.back() : -1;
     const size_t n = op.outs.size();
     if (n < 1 || n > 2 || op.ins.size() != n + (pos >= 0 ? 1 : 0)) return bad("in=Q[,K][,positions] out=QO[,KO]");
-    const uint64_t B = (uint64_t)num("batch", 1), H = (uint64_t)num("heads", 1);
-    const uint64_t Hk = n > 1 ? (uint64_t)num("k_heads", (double)H) : 0;
+    const uint64_t B = at.count("batch", 1), H = at.count("heads", 1);
+    const uint64_t Hk = n > 1 ? at.count("k_heads", (uint32_t)H) : 0;
     const std::string lay = attr(op, "layout", "bshd"), pairs = attr(op, "pairs", "half"), sc = attr(op, "scaling", "none");
     if (lay != "bshd" && lay != "bhsd") return bad("layout must be bshd or bhsd");
     if (pairs != "half" && pairs != "interleaved") return bad("pairs must be half or interleaved");
@@ -666,19 +693,19 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     r.k_heads = (uint32_t)Hk;
     r.dim = (uint32_t)dim;
     r.batch = (uint32_t)B;
-    r.rot_dim = (uint32_t)num("rot", 0);
+    r.rot_dim = at.count("rot", 0);
     r.layout = pairs == "half" ? BWPP_HIP_ROTARY_HALF : BWPP_HIP_ROTARY_INTERLEAVED;
     r.dtype = dt;
     r.pos_batch_stride = pos >= 0 && val(pos).elems() == B * seq ? seq : 0;
-    r.pos_offset = (int32_t)num("offset", 0);
+    r.pos_offset = at.integer("offset", 0);
     r.scaling = sc == "none" ? BWPP_HIP_ROTARY_SCALE_NONE : sc == "linear" ? BWPP_HIP_ROTARY_SCALE_LINEAR
                                                                        : BWPP_HIP_ROTARY_SCALE_BY_PARTS;
-    r.base = (float)num("base", 0);
-    r.factor = (float)num("factor", 0);
-    r.context = (uint32_t)num("context", 0);
-    r.low_turns = (float)num("low", 0);
-    r.high_turns = (float)num("high", 0);
-    r.magnitude = (float)num("magnitude", 0);
+    r.base = (float)at.num("base", 0);
+    r.factor = (float)at.num("factor", 0);
+    r.context = at.count("context", 0);
+    r.low_turns = (float)at.num("low", 0);
+    r.high_turns = (float)at.num("high", 0);
+    r.magnitude = (float)at.num("magnitude", 0);
     auto strides = [&](int v, uint64_t hh, uint32_t &ld, uint64_t &hs, uint64_t &bs) {
       const uint64_t st = val(v).row_stride();
       ld = (uint32_t)st;
@@ -711,11 +738,11 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     r.rows = (uint32_t)rows;
     r.cols = (uint32_t)cols;
     r.ldo = (uint32_t)val(o).row_stride();
-    r.post_norm = (uint32_t)num("post_norm", post >= 0 ? 1 : 0);
-    r.gate_rows = (uint32_t)num("gate_rows", 0);
-    r.eps = (float)num("eps", 1e-5);
-    r.stream_scale = (float)num("stream_scale", 0);
-    r.branch_scale = (float)num("branch_scale", 0);
+    r.post_norm = at.count("post_norm", post >= 0 ? 1 : 0);
+    r.gate_rows = at.count("gate_rows", 0);
+    r.eps = (float)at.num("eps", 1e-5);
+    r.stream_scale = (float)at.num("stream_scale", 0);
+    r.branch_scale = (float)at.num("branch_scale", 0);
     r.dtype = dt;
     const uint64_t gates = r.gate_rows ? (rows + r.gate_rows - 1) / r.gate_rows : 1;
     for (const std::vector<int> *list : {&op.ins, &op.outs})
@@ -761,14 +788,14 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     const int x = op.ins[0], w = op.ins[1], t = op.ins[2];
     const uint64_t rows = val(x).rows(), dim = val(x).cols();
     BwppLinearXentParams r = {};
-    r.trans_w = (uint32_t)num("trans_w", 0);
+    r.trans_w = at.count("trans_w", 0);
     r.rows = (uint32_t)rows;
     r.dim = (uint32_t)dim;
     r.vocab = (uint32_t)(r.trans_w ? val(w).rows() : val(w).cols());
     r.ldx = (uint32_t)val(x).row_stride();
     r.ldw = (uint32_t)val(w).row_stride();
     r.dtype = dt;
-    r.scale = (float)num("scale", 0);
+    r.scale = (float)at.num("scale", 0);
     if ((r.trans_w ? val(w).cols() : val(w).rows()) != dim) return bad("W does not have X's columns");
     if (!dtype({w}, dt) || !dtype({t}, kI32)) return bad("W must have X's dtype, targets i32");
     if (!elems(t, rows)) return bad("targets need one element a row");
@@ -791,6 +818,7 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
       s = BWPP_PLAN_CALL(bwpp_hip_dispatch_linear_xent_grad(h, ptr(x), ptr(w), i32(t), f32(lse), f32(dloss), ptr(dx), ptr(dw), r));
     }
   }
+  if (!at.wrong.empty()) return bad("");
   if (s != BWPP_HIP_OK) return perr(&p, s, "line %d (%s): %s", op.line, k.c_str(), bwpp_hip_last_error(h));
   return BWPP_HIP_OK;
 }
@@ -802,17 +830,11 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
   auto need = [&](size_t nin, size_t nout) {
     return op.ins.size() >= nin && op.outs.size() >= nout;
   };
+  Numbers at{p, op, {}};
   auto bad = [&](const char *what) {
-    return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d (%s): %s", op.line, op.kind.c_str(), what);
+    return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d (%s): %s", op.line, op.kind.c_str(), at.wrong.empty() ? what : at.wrong.c_str());
   };
   auto f32 = [&](int i) { return static_cast<float *>(ptr(i)); };
-  auto num = [&](const char *k, double dflt) {
-    auto it = op.attrs.find(k);
-    if (it == op.attrs.end()) return dflt;
-    uint64_t n = 0;
-    if (eval_expr(p, it->second, n) && it->second.find('.') == std::string::npos) return (double)n;
-    return strtod(it->second.c_str(), nullptr);
-  };
   const std::string &k = op.kind;
   BwppHipStatus s = BWPP_HIP_OK;
   // dtypes: matmul and attention take f32 or bf16 operands of one dtype
@@ -840,7 +862,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
   if (k == "matmul") {
     if (op.ins.size() < 2 || op.outs.empty()) return bad("in=A,B[,bias][,aux] out=C[,C2]");
     const Value &A = val(op.ins[0]), &B = val(op.ins[1]), &C = val(op.outs[0]);
-    const uint32_t ta = (uint32_t)num("ta", 0), tb = (uint32_t)num("tb", 0);
+    const uint32_t ta = at.count("ta", 0), tb = at.count("tb", 0);
     const uint64_t M = C.rows(), N = C.cols();
     const uint64_t K = ta ? A.rows() : A.cols();
     if ((ta ? A.cols() : A.rows()) != M || (tb ? B.cols() : B.rows()) != K || (tb ? B.rows() : B.cols()) != N)
@@ -883,7 +905,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
   } else if (k == "softmax" || k == "rmsnorm" || k == "layernorm") {
     if (!need(1, 1)) return bad("in=X[,gamma[,beta]] out=Y");
     const Value &X = val(op.ins[0]);
-    const float eps = (float)num("eps", 1e-5);
+    const float eps = (float)at.num("eps", 1e-5);
     if (k == "softmax") {
       BwppSoftmaxParams sp = {(uint32_t)X.rows(), (uint32_t)X.cols(), (uint32_t)X.row_stride()};
       s = BWPP_PLAN_CALL(bwpp_hip_dispatch_softmax(h, f32(op.ins[0]), f32(op.outs[0]), sp));
@@ -946,7 +968,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
     if (!need(1, 1)) return bad("in=X out=Y");
     const Value &X = val(op.ins[0]);
     BwppReduceParams rp = {(uint32_t)X.rows(), (uint32_t)X.cols(), (uint32_t)X.row_stride(),
-                           (int32_t)num("axis", 1)};
+                           at.integer("axis", 1)};
     s = BWPP_PLAN_CALL(bwpp_hip_dispatch_reduce_sum(h, f32(op.ins[0]), f32(op.outs[0]), rp));
   } else if (k == "mean_square") {
     // loss = loss_scale * sum(X^2) (one element) and dX = grad_scale * X;
@@ -969,7 +991,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
     if (!need(1, 1)) return bad("in=X out=Y");
     const Value &X = val(op.ins[0]);
     BwppReduceParams rp = {(uint32_t)X.rows(), (uint32_t)X.cols(), (uint32_t)X.row_stride(),
-                           (int32_t)num("axis", 1)};
+                           at.integer("axis", 1)};
     const uint64_t want = k == "reduce_max_mask" ? X.rows() * X.cols() : rp.axis == 0 ? X.cols() : X.rows();
     if (val(op.outs[0]).elems() != want) return bad("output size does not match the reduction");
     if (k == "reduce_max_mask" && val(op.outs[0]).row_stride() != X.row_stride())
@@ -993,7 +1015,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
     const Value &X = val(op.ins[0]);
     if (op.ins.size() > 3 && val(op.ins[3]).row_stride() != X.row_stride())
       return bad("rmsnorm_grad: acc must have the row stride of X");
-    BwppRmsnormParams rp = {(uint32_t)X.rows(), (uint32_t)X.cols(), (uint32_t)X.row_stride(), (float)num("eps", 1e-5)};
+    BwppRmsnormParams rp = {(uint32_t)X.rows(), (uint32_t)X.cols(), (uint32_t)X.row_stride(), (float)at.num("eps", 1e-5)};
     s = BWPP_PLAN_CALL(bwpp_hip_dispatch_rmsnorm_grad_acc(
         h, f32(op.ins[0]), f32(op.ins[1]), f32(op.ins[2]), op.ins.size() > 3 ? f32(op.ins[3]) : nullptr,
         f32(op.outs[0]), op.outs.size() > 1 ? f32(op.outs[1]) : nullptr, op.outs.size() > 2 ? f32(op.outs[2]) : nullptr,
@@ -1007,7 +1029,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
     // layout=bshd (default): [batch*seq, heads*dim] row blocks, head h of a
     // row at column h*dim.  layout=bhsd: [batch, heads, seq, dim] with one
     // row per (batch, head, position).
-    const uint64_t B = (uint64_t)num("batch", 1), H = (uint64_t)num("heads", 1);
+    const uint64_t B = at.count("batch", 1), H = at.count("heads", 1);
     const std::string lay = attr(op, "layout", "bshd");
     if (lay != "bshd" && lay != "bhsd") return bad("layout must be bshd or bhsd");
     const bool bhsd = lay == "bhsd";
@@ -1038,8 +1060,8 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
     ap.o_head_stride = bhsd ? M * ap.ldo : dv;
     ap.o_batch_stride = bhsd ? H * M * ap.ldo : M * ap.ldo;
     // scale=auto: 1/sqrt(head dim), the usual choice the graph cannot state
-    ap.scale = attr(op, "scale", "") == "auto" ? (float)(1.0 / std::sqrt((double)dk)) : (float)num("scale", 0.0);
-    ap.causal = (uint32_t)num("causal", 0);
+    ap.scale = attr(op, "scale", "") == "auto" ? (float)(1.0 / std::sqrt((double)dk)) : (float)at.num("scale", 0.0);
+    ap.causal = at.count("causal", 0);
     ap.dtype = Q.dtype;
     if (!grad) {
       // A second output receives the per-query log-sum-exp ([batch, heads, seq]).
@@ -1058,6 +1080,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
   } else {
     return bad("unknown op");
   }
+  if (!at.wrong.empty()) return bad("");
   if (s != BWPP_HIP_OK) return perr(&p, s, "line %d (%s): %s", op.line, k.c_str(), bwpp_hip_last_error(h));
   return BWPP_HIP_OK;
 }
