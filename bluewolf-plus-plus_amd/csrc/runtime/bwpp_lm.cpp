@@ -141,6 +141,56 @@ const char *const bwpp_hip_lm_kernels[] = {
 const int bwpp_hip_lm_kernel_count = (int)(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]));
 static_assert(sizeof(bwpp_hip_lm_kernels) / sizeof(bwpp_hip_lm_kernels[0]) == LM_COUNT, "kernel names");
 
+// ------------------------------------- parameters, without their operands
+
+namespace {
+
+BwppHipFault invalid(const char *why) { return {BWPP_HIP_ERR_INVALID_ARG, why}; }
+BwppHipFault unsupported(const char *why) { return {BWPP_HIP_ERR_UNSUPPORTED, why}; }
+bool short_row(uint32_t ld, uint64_t cols) { return ld != 0 && ld < cols; }
+
+}  // namespace
+
+BwppHipFault bwpp_hip_check_rotary(const BwppRotaryParams &p) {
+  if (p.dtype > BWPP_HIP_BF16) return invalid("unknown dtype");
+  if (p.layout > BWPP_HIP_ROTARY_INTERLEAVED) return invalid("unknown layout");
+  if (p.scaling > BWPP_HIP_ROTARY_SCALE_BY_PARTS) return invalid("unknown scaling");
+  const uint32_t rot = p.rot_dim ? p.rot_dim : p.dim;
+  if (rot % 2 || rot > p.dim) return invalid("rot_dim must be even and at most dim");
+  if (!(p.base >= 0.0f) || !(p.factor >= 0.0f) || !std::isfinite(p.base) || !std::isfinite(p.factor) ||
+      !std::isfinite(p.magnitude))
+    return invalid("base and factor must be positive and finite, magnitude finite");
+  if (p.scaling == BWPP_HIP_ROTARY_SCALE_BY_PARTS &&
+      (p.context == 0 || !(p.high_turns > p.low_turns) || !std::isfinite(p.low_turns) || !std::isfinite(p.high_turns)))
+    return invalid("scaling by parts needs a context and low_turns < high_turns");
+  const uint64_t heads = (uint64_t)p.q_heads + p.k_heads;
+  if (p.tokens && p.dim && (rot > 4096 || heads > (1u << 24) || p.tokens > (1u << 31)))
+    return unsupported("rot_dim above 4096, or heads or tokens out of range");
+  return {BWPP_HIP_OK, nullptr};
+}
+
+BwppHipFault bwpp_hip_check_residual_norm(const BwppResidualNormParams &p) {
+  if (p.dtype > BWPP_HIP_BF16) return invalid("unknown dtype");
+  if (short_row(p.ldx, p.cols) || short_row(p.ldo, p.cols) || short_row(p.ldy, p.cols) || short_row(p.ldg, p.cols))
+    return invalid("row stride smaller than the row");
+  if (!(p.eps >= 0.0f)) return invalid("eps must not be negative");
+  return {BWPP_HIP_OK, nullptr};
+}
+
+BwppHipFault bwpp_hip_check_linear_xent(const BwppLinearXentParams &p) {
+  if (p.dtype > BWPP_HIP_BF16) return invalid("unknown dtype");
+  if (p.vocab == 0 || p.dim == 0) return invalid("empty vocabulary or dim");
+  if (!std::isfinite(p.scale)) return invalid("scale must be finite");
+  const uint64_t wcols = p.trans_w ? p.dim : p.vocab;
+  if (short_row(p.ldx, p.dim) || short_row(p.ldw, wcols) || short_row(p.lddx, p.dim) || short_row(p.lddw, wcols))
+    return invalid("row stride smaller than the row");
+  if (p.rows >= (1u << 27) || p.vocab > 0x7fffffffu || p.dim > 0x7fffffffu)
+    return unsupported("2^27 rows, or another size of 2^31, or more");
+  if (p.dtype == BWPP_HIP_BF16 && (p.dim < 8 || (!p.trans_w && p.vocab < 8)))
+    return unsupported("bf16 rows of fewer than 8 elements");
+  return {BWPP_HIP_OK, nullptr};
+}
+
 namespace {
 
 uint32_t cus_of(const BwppHip *h) {
@@ -199,24 +249,13 @@ bool disjoint_rows(const RowSet &s) {
 BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k, const int32_t *positions, void *qo,
                      void *ko, const BwppRotaryParams &p, bool grad) {
   auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
-  if (p.dtype > BWPP_HIP_BF16) return bad("unknown dtype");
-  if (p.layout > BWPP_HIP_ROTARY_INTERLEAVED) return bad("unknown layout");
-  if (p.scaling > BWPP_HIP_ROTARY_SCALE_BY_PARTS) return bad("unknown scaling");
+  const BwppHipFault fault = bwpp_hip_check_rotary(p);
+  if (fault.why) return bwpp_hip_set_error(h, fault.status, "%s: %s", what, fault.why);
   if ((p.q_heads && (!q || !qo)) || (p.k_heads && (!k || !ko))) return bad("NULL q, k or output");
-  const uint32_t rot = p.rot_dim ? p.rot_dim : p.dim;
-  if (rot % 2 || rot > p.dim) return bad("rot_dim must be even and at most dim");
-  const double base = p.base != 0.0f ? p.base : 10000.0, factor = p.factor != 0.0f ? p.factor : 1.0;
-  if (!(base > 0.0) || !(factor > 0.0) || !std::isfinite(base) || !std::isfinite(factor) ||
-      !std::isfinite(p.magnitude))
-    return bad("base and factor must be positive and finite, magnitude finite");
-  if (p.scaling == BWPP_HIP_ROTARY_SCALE_BY_PARTS &&
-      (p.context == 0 || !(p.high_turns > p.low_turns) || !std::isfinite(p.low_turns) || !std::isfinite(p.high_turns)))
-    return bad("scaling by parts needs a context and low_turns < high_turns");
-  const uint64_t B = p.batch ? p.batch : 1, T = p.tokens, d = p.dim;
   if (p.tokens == 0 || p.dim == 0 || (p.q_heads == 0 && p.k_heads == 0)) return bwpp_hip_enter(h);
-  const uint64_t heads = (uint64_t)p.q_heads + p.k_heads;
-  if (rot > 4096 || heads > (1u << 24) || T > (1u << 31))
-    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: rot_dim above 4096, or heads or tokens out of range", what);
+  const uint32_t rot = p.rot_dim ? p.rot_dim : p.dim;
+  const double base = p.base != 0.0f ? p.base : 10000.0, factor = p.factor != 0.0f ? p.factor : 1.0;
+  const uint64_t B = p.batch ? p.batch : 1, T = p.tokens, d = p.dim, heads = (uint64_t)p.q_heads + p.k_heads;
   auto rows = [&](const void *ptr, uint32_t heads, uint32_t ld, uint64_t hs, uint64_t bs) {
     RowSet r = {heads ? ptr : nullptr, ld ? ld : d, 0, 0, B, heads ? heads : 1u, T, d};
     r.hs = hs ? hs : T * r.ts;
@@ -304,17 +343,14 @@ BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k,
 
 // Checks and the arguments both directions share.
 BwppHipStatus resnorm_prepare(BwppHip *h, const char *what, const BwppResidualNormParams &p, BwppResNormArgs &a) {
-  auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
-  if (p.dtype > BWPP_HIP_BF16) return bad("unknown dtype");
+  const BwppHipFault fault = bwpp_hip_check_residual_norm(p);
+  if (fault.why) return bwpp_hip_set_error(h, fault.status, "%s: %s", what, fault.why);
   a.rows = p.rows;
   a.cols = p.cols;
   a.ldx = p.ldx ? p.ldx : p.cols;
   a.ldo = p.ldo ? p.ldo : p.cols;
   a.ldy = p.ldy ? p.ldy : p.cols;
   a.ldg = p.ldg ? p.ldg : p.cols;
-  if (a.ldx < p.cols || a.ldo < p.cols || a.ldy < p.cols || a.ldg < p.cols)
-    return bad("row stride smaller than the row");
-  if (!(p.eps >= 0.0f)) return bad("eps must not be negative");
   a.post_norm = p.post_norm ? 1u : 0u;
   a.gate_rows = p.gate_rows;
   a.eps = p.eps;
@@ -582,21 +618,14 @@ struct XentMatrices {
 };
 
 BwppHipStatus xent_prepare(BwppHip *h, const char *what, const BwppLinearXentParams &p, XentMatrices &m) {
-  auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
-  if (p.dtype > BWPP_HIP_BF16) return bad("unknown dtype");
-  if (p.vocab == 0 || p.dim == 0) return bad("empty vocabulary or dim");
-  if (!std::isfinite(p.scale)) return bad("scale must be finite");
+  const BwppHipFault fault = bwpp_hip_check_linear_xent(p);
+  if (fault.why) return bwpp_hip_set_error(h, fault.status, "%s: %s", what, fault.why);
   m.wrows = p.trans_w ? p.vocab : p.dim;
   m.wcols = p.trans_w ? p.dim : p.vocab;
   m.ldx = p.ldx ? p.ldx : p.dim;
   m.ldw = p.ldw ? p.ldw : m.wcols;
   m.lddx = p.lddx ? p.lddx : p.dim;
   m.lddw = p.lddw ? p.lddw : m.wcols;
-  if (m.ldx < p.dim || m.ldw < m.wcols || m.lddx < p.dim || m.lddw < m.wcols) return bad("row stride smaller than the row");
-  if (p.rows >= (1u << 27) || p.vocab > 0x7fffffffu || p.dim > 0x7fffffffu)
-    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: 2^27 rows, or another size of 2^31, or more", what);
-  if (p.dtype == BWPP_HIP_BF16 && (p.dim < 8 || (!p.trans_w && p.vocab < 8)))
-    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: bf16 rows of fewer than 8 elements", what);
   return BWPP_HIP_OK;
 }
 

@@ -655,6 +655,15 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     }
     return true;
   };
+  // The parameters' sizes and row strides are 32-bit.
+  auto rows32 = [&](uint64_t rows) {
+    for (const std::vector<int> *list : {&op.ins, &op.outs})
+      for (int v : *list)
+        if (val(v).cols() > UINT32_MAX || val(v).row_stride() > UINT32_MAX) return false;
+    return rows <= UINT32_MAX;
+  };
+  // Parameters that the entry point would refuse at every run.
+  auto refused = [&](const BwppHipFault &f) { return perr(&p, f.status, "line %d (%s): %s", op.line, k.c_str(), f.why); };
   const bool grad = k.size() > 5 && k.compare(k.size() - 5, 5, "_grad") == 0;
   if (op.ins.empty()) return bad("no operands");
   const uint32_t dt = val(op.ins[0]).dtype;
@@ -686,6 +695,7 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
       dim = d;
       if (!dtype({op.ins[i], op.outs[i]}, dt)) return bad("operands of different dtypes");
     }
+    if (!rows32(seq)) return bad("sizes past 32 bits");
     if (pos >= 0 && !elems(pos, B * seq) && !elems(pos, seq)) return bad("positions need batch*seq or seq elements");
     BwppRotaryParams r = {};
     r.tokens = (uint32_t)seq;
@@ -719,6 +729,8 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
       strides(grad ? op.outs[1] : op.ins[1], Hk, r.ldk, r.k_head_stride, r.k_batch_stride);
       strides(grad ? op.ins[1] : op.outs[1], Hk, r.ldko, r.ko_head_stride, r.ko_batch_stride);
     }
+    if (!at.wrong.empty()) return bad("");
+    if (const BwppHipFault f = bwpp_hip_check_rotary(r); f.why) return refused(f);
     const int ki = n > 1 ? op.ins[1] : -1, ko = n > 1 ? op.outs[1] : -1;
     s = BWPP_PLAN_CALL(grad ? bwpp_hip_dispatch_rotary_grad(h, ptr(op.ins[0]), ptr(ki), i32(pos), ptr(op.outs[0]), ptr(ko), r)
                             : bwpp_hip_dispatch_rotary(h, ptr(op.ins[0]), ptr(ki), i32(pos), ptr(op.outs[0]), ptr(ko), r));
@@ -734,6 +746,7 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     const int post = listed(op.ins, with, 2, "post"), gate = listed(op.ins, with, 2, "gate"),
               pre = listed(op.ins, with, 2, "pre");
     const uint64_t rows = val(o).rows(), cols = val(o).cols();
+    if (!rows32(rows)) return bad("sizes past 32 bits");
     BwppResidualNormParams r = {};
     r.rows = (uint32_t)rows;
     r.cols = (uint32_t)cols;
@@ -744,6 +757,8 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     r.stream_scale = (float)at.num("stream_scale", 0);
     r.branch_scale = (float)at.num("branch_scale", 0);
     r.dtype = dt;
+    if (!at.wrong.empty()) return bad("");
+    if (const BwppHipFault f = bwpp_hip_check_residual_norm(r); f.why) return refused(f);
     const uint64_t gates = r.gate_rows ? (rows + r.gate_rows - 1) / r.gate_rows : 1;
     for (const std::vector<int> *list : {&op.ins, &op.outs})
       for (int v : *list)
@@ -764,6 +779,7 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
                 dpost = listed(op.outs, gives, 0, "dpost"), dgate = listed(op.outs, gives, 0, "dgate"),
                 dpre = listed(op.outs, gives, 0, "dpre");
       if (dr < 0 && dy < 0) return bad("needs dr or dy");
+      if (dpost >= 0 && !r.post_norm) return bad("dpost without a post-norm");
       if (!shape(a1, rows, cols) || !shape(dr, rows, cols) || !shape(dy, rows, cols) || !shape(dx, rows, cols) ||
           !shape(dout, rows, cols) || !shape(dgate, gates, cols) || !elems(dpost, cols) || !elems(dpre, cols))
         return bad("operand shapes do not match");
@@ -787,6 +803,7 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
       return bad(grad ? "out=.. gives=dx,dw (those given, in order)" : "out=.. gives=loss,lse,sums (those given, in order)");
     const int x = op.ins[0], w = op.ins[1], t = op.ins[2];
     const uint64_t rows = val(x).rows(), dim = val(x).cols();
+    if (!rows32(rows) || val(w).rows() > UINT32_MAX) return bad("sizes past 32 bits");
     BwppLinearXentParams r = {};
     r.trans_w = at.count("trans_w", 0);
     r.rows = (uint32_t)rows;
@@ -797,6 +814,8 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
     r.dtype = dt;
     r.scale = (float)at.num("scale", 0);
     if ((r.trans_w ? val(w).cols() : val(w).rows()) != dim) return bad("W does not have X's columns");
+    if (!at.wrong.empty()) return bad("");
+    if (const BwppHipFault f = bwpp_hip_check_linear_xent(r); f.why) return refused(f);
     if (!dtype({w}, dt) || !dtype({t}, kI32)) return bad("W must have X's dtype, targets i32");
     if (!elems(t, rows)) return bad("targets need one element a row");
     if (!grad) {
@@ -818,7 +837,6 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
       s = BWPP_PLAN_CALL(bwpp_hip_dispatch_linear_xent_grad(h, ptr(x), ptr(w), i32(t), f32(lse), f32(dloss), ptr(dx), ptr(dw), r));
     }
   }
-  if (!at.wrong.empty()) return bad("");
   if (s != BWPP_HIP_OK) return perr(&p, s, "line %d (%s): %s", op.line, k.c_str(), bwpp_hip_last_error(h));
   return BWPP_HIP_OK;
 }

@@ -62,6 +62,16 @@ BwppHipStatus bwpp_hip_copy_strided_multi(BwppHip *h, uint32_t n, const float *c
 extern const char *const bwpp_hip_lm_kernels[];
 extern const int bwpp_hip_lm_kernel_count;
 
+// What is wrong with an operator's parameters, whatever its operands (why NULL:
+// nothing): the entry points refuse them, and so does a plan's creation.
+struct BwppHipFault {
+  BwppHipStatus status;
+  const char *why;
+};
+BwppHipFault bwpp_hip_check_rotary(const BwppRotaryParams &p);
+BwppHipFault bwpp_hip_check_residual_norm(const BwppResidualNormParams &p);
+BwppHipFault bwpp_hip_check_linear_xent(const BwppLinearXentParams &p);
+
 // Clears the last error and makes the handle's device current.
 BwppHipStatus bwpp_hip_enter(BwppHip *h);
 
