@@ -35,6 +35,19 @@ def _ptr(buf) -> int | None:
     raise TypeError(f"cannot pass {type(buf)!r} as a device buffer")
 
 
+def _int32(buf, what: str, rows_apart: bool = False) -> int | None:
+    """Address of 32-bit integers (torch's own are 64-bit) that lie side by side,
+    or of rows of them that may lie apart."""
+    if hasattr(buf, "data_ptr"):
+        import torch
+        if buf.dtype != torch.int32:
+            raise ValueError(f"{what} must be int32, not {buf.dtype}")
+        side_by_side = buf.dim() == 0 or buf.size(-1) <= 1 or buf.stride(-1) == 1
+        if not (side_by_side if rows_apart else buf.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous")
+    return _ptr(buf)
+
+
 def tensor_of(t, layout: int = 0) -> "_lib.Tensor":
     """BwppHipTensor describing a torch CUDA tensor (f32 or bf16, its own
     shape and element strides).  layout 1 (column-major) marks a rank-2
@@ -193,12 +206,12 @@ class HipBackend:
     def dispatch_rotary(self, q, k, positions, qo, ko, params):
         """qo, ko = q, k with rotary positions (in place: qo is q, ko is k)."""
         self._check(self.lib.bwpp_hip_dispatch_rotary(
-            self._h, _ptr(q), _ptr(k), _ptr(positions), _ptr(qo), _ptr(ko), params))
+            self._h, _ptr(q), _ptr(k), _int32(positions, "positions", True), _ptr(qo), _ptr(ko), params))
 
     def dispatch_rotary_grad(self, dqo, dko, positions, dq, dk, params):
         """dq, dk from the gradients of qo, ko (q's strides and qo's, as in the forward)."""
         self._check(self.lib.bwpp_hip_dispatch_rotary_grad(
-            self._h, _ptr(dqo), _ptr(dko), _ptr(positions), _ptr(dq), _ptr(dk), params))
+            self._h, _ptr(dqo), _ptr(dko), _int32(positions, "positions", True), _ptr(dq), _ptr(dk), params))
 
     def dispatch_residual_norm(self, x, o, post_gamma, gate, pre_gamma, r, y, params):
         """r = stream_scale x + branch_scale gate post_norm(o), y = pre_norm(r)."""
@@ -214,11 +227,11 @@ class HipBackend:
     def dispatch_linear_xent(self, x, w, targets, loss, lse, sums, params):
         """loss[t] = lse[t] - z[t][targets[t]], z = scale x W; sums: their sum and how many rows count."""
         self._check(self.lib.bwpp_hip_dispatch_linear_xent(
-            self._h, _ptr(x), _ptr(w), _ptr(targets), _ptr(loss), _ptr(lse), _ptr(sums), params))
+            self._h, _ptr(x), _ptr(w), _int32(targets, "targets"), _ptr(loss), _ptr(lse), _ptr(sums), params))
 
     def dispatch_linear_xent_grad(self, x, w, targets, lse, dloss, dx, dw, params):
         self._check(self.lib.bwpp_hip_dispatch_linear_xent_grad(
-            self._h, _ptr(x), _ptr(w), _ptr(targets), _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw), params))
+            self._h, _ptr(x), _ptr(w), _int32(targets, "targets"), _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw), params))
 
     # ------------------------------------------------------ tensor forms
     def tensor_matmul(self, a, b, bias, c, epilogue: int = 0):

@@ -68,6 +68,8 @@ class Plan:
         self._check(self.lib.bwpp_hip_plan_allocate(self._p))
 
     def bind(self, name: str, tensor):
+        if tensor.element_size() > 4:  # e.g. torch's own integers for an i32 value
+            raise ValueError(f"'{name}': a plan has f32, bf16 and i32 values, not {tensor.dtype}")
         self._keep = getattr(self, "_keep", {})
         self._keep[name] = tensor
         self._check(self.lib.bwpp_hip_plan_bind(self._p, name.encode(), tensor.data_ptr()))
