@@ -816,11 +816,12 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_xent_terms(const BwppXent
   }
 }
 
-// Zeros (dW of no rows).
+// Zeros (dW of no rows): 2-byte units, rows of up to 2^32 of them (64-bit columns: a
+// 32-bit one would pass the end of such a row and start again).
 extern "C" __global__ __launch_bounds__(256) void bwpp_xent_clear(const BwppXentRowArgs a) {
   for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    unsigned char *y = static_cast<unsigned char *>(a.y) + row * a.ldy;  // bytes
-    for (uint32_t c = threadIdx.x; c < a.cols; c += 256) y[c] = 0;
+    uint16_t *y = static_cast<uint16_t *>(a.y) + row * a.ldy;
+    for (uint64_t c = blockIdx.y * 256u + threadIdx.x; c < a.cols; c += gridDim.y * 256u) y[c] = 0;
   }
 }
 

@@ -1065,10 +1065,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
     if (!dw) return BWPP_HIP_OK;
     r.y = dw;
     r.rows = (uint32_t)m.wrows;
-    r.cols = (uint32_t)std::min<uint64_t>(m.wcols * es, 0xffffffffull);
-    if (m.wcols * es > 0xffffffffull) return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: rows too long", what);
-    r.ldy = m.lddw * es;
-    return bwpp_hip_launch_lm(h, LM_XENT_CLEAR, xent_grid(h, m.wrows), 1, 256, &r);
+    r.cols = (uint32_t)(m.wcols * (es / 2));  // (fewer than 2^31 columns)
+    r.ldy = m.lddw * (es / 2);
+    return bwpp_hip_launch_lm(h, LM_XENT_CLEAR, xent_grid(h, m.wrows), xent_columns(m.wrows, r.cols), 256, &r);
   }
   if (!bf16 && xent_in_terms(h, p, m, true))
     return terms_grad(h, static_cast<const float *>(x), static_cast<const float *>(w), static_cast<float *>(dx),
