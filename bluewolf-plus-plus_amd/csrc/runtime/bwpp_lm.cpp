@@ -164,8 +164,9 @@ BwppHipFault bwpp_hip_check_rotary(const BwppRotaryParams &p) {
       (p.context == 0 || !(p.high_turns > p.low_turns) || !std::isfinite(p.low_turns) || !std::isfinite(p.high_turns)))
     return invalid("scaling by parts needs a context and low_turns < high_turns");
   const uint64_t heads = (uint64_t)p.q_heads + p.k_heads;
-  if (p.tokens && p.dim && (rot > 4096 || heads > (1u << 24) || p.tokens > (1u << 31)))
-    return unsupported("rot_dim above 4096, or heads or tokens out of range");
+  // (dim: a kernel's columns are 32-bit, and so is the end of a chunk that passes it)
+  if (p.tokens && p.dim && (rot > 4096 || heads > (1u << 24) || p.tokens > (1u << 31) || p.dim > (1u << 31)))
+    return unsupported("rot_dim above 4096, or dim, heads or tokens out of range");
   return {BWPP_HIP_OK, nullptr};
 }
 
@@ -174,6 +175,7 @@ BwppHipFault bwpp_hip_check_residual_norm(const BwppResidualNormParams &p) {
   if (short_row(p.ldx, p.cols) || short_row(p.ldo, p.cols) || short_row(p.ldy, p.cols) || short_row(p.ldg, p.cols))
     return invalid("row stride smaller than the row");
   if (!(p.eps >= 0.0f)) return invalid("eps must not be negative");
+  if (p.cols >= (1u << 31)) return unsupported("2^31 columns or more");  // (32-bit columns are stepped past the row's end)
   return {BWPP_HIP_OK, nullptr};
 }
 
@@ -445,6 +447,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const 
   BwppHipStatus s = resnorm_prepare(h, what, p, a);
   if (s != BWPP_HIP_OK) return s;
   const uint64_t es = p.dtype == BWPP_HIP_BF16 ? 2 : 4, R = p.rows, C = p.cols;
+  if ((dpost_gamma || dgate || dpre_gamma) && (C + 63) / 64 * 1024 > 0xffffffffull)  // the sums' second launch
+    return bwpp_hip_set_error(h, BWPP_HIP_ERR_UNSUPPORTED, "%s: weight or gate gradients of almost 2^28 columns or more", what);
   const uint64_t gates = p.gate_rows ? (R + p.gate_rows - 1) / p.gate_rows : 1;
   const Block in[7] = {{o, R, C, a.ldo}, {r, R, C, a.ldx}, {dr, R, C, a.ldx}, {dy, R, C, a.ldy},
                        {p.post_norm ? post_gamma : nullptr, 1, C, C}, {gate, gates, C, a.ldg}, {pre_gamma, 1, C, C}};

@@ -188,7 +188,8 @@ typedef struct {
   uint32_t k_heads;
   uint32_t dim;
   uint32_t batch;   /* 0 = 1 */
-  uint32_t rot_dim; /* even, at most dim and 4096; 0 = dim */
+  uint32_t rot_dim; /* even, at most dim and 4096; 0 = dim.  dim and tokens: at most
+                       2^31, heads of q and k 2^24 */
   uint32_t layout;  /* BwppHipRotaryLayout */
   uint32_t dtype;   /* BwppHipDType, 0 = F32 */
   uint32_t ldq, ldk, ldqo, ldko; /* token strides; 0 = dim */
@@ -217,7 +218,7 @@ typedef struct {
  * gradient ldo, y and its gradient ldy, gate rows ldg. */
 typedef struct {
   uint32_t rows;
-  uint32_t cols;
+  uint32_t cols; /* fewer than 2^31, for weight and gate gradients at most 2^28 - 64 */
   uint32_t ldx, ldo, ldy, ldg; /* 0 = cols */
   uint32_t post_norm;
   uint32_t gate_rows;
