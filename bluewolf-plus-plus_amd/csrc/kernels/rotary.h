@@ -16,7 +16,7 @@
 // reduced in 64 bits, in quarter turns (position 10^6 at f = 1 keeps 2^-32 of
 // a turn; in 32 bits it would lose 2^-5), the remainder's sine and cosine come
 // from their Taylor series in 32 bits (|z| <= pi/4: terms up to z^11 and z^10
-// leave 2^-35 and 2^-28), then one rounding to the output type.
+// leave 2^-37 and 2^-33), then one rounding to the output type.
 //
 // A thread's item is a chunk of C pairs of one row: 16-byte loads of each
 // half for bf16 with C = 8 and fp32 with C = 4 (any address), two 16-byte
@@ -24,7 +24,7 @@
 // rotated widths those do not divide.
 //
 // 4 x 4096 tokens of 32 + 8 heads of 128, bf16: 71 us (335 MB, 4.7 TB/s; a copy of as
-// many bytes, not in the caches, 65).  8 x 1 tokens: 4.5 us, a launch.  3 x 1001 x 24
+// many bytes, not in the caches, 65).  8 x 1 tokens: 4.7 us, a launch.  3 x 1001 x 24
 // heads of 80, 40 turned, fp32: 11.9 us (46 MB, 3.9 TB/s).
 #pragma once
 

@@ -6,9 +6,9 @@
 //   dz_tv = g_t (exp(z_tv - lse_t) - [v = target]),   dx = scale dz W^T,
 //   dW = scale x^T dz
 //
-// Measured: 4 x 1024 x 16384 loss 11.5 us (W at 2.9 TB/s, and two launches), 2048 x
-// 4096 x 50001 loss 679 (1235 TFLOP/s), 4096 x 2048 x 32768 train 1797 and 4096 x 4096
-// x 131072 12.8 ms (1224 and 1374 TFLOP/s of the four products a call that does not
+// Measured: 4 x 1024 x 16384 loss 11.8 us (W at 2.8 TB/s, and two launches), 2048 x
+// 4096 x 50001 loss 666 (1260 TFLOP/s), 4096 x 2048 x 32768 train 1828 and 4096 x 4096
+// x 131072 13.0 ms (1203 and 1350 TFLOP/s of the four products a call that does not
 // keep the logits makes); the wide products run at the rate that the chip's power
 // allows (gemm_bf16_k32.h).
 //
@@ -32,7 +32,7 @@
 // dz as three bf16 terms each (gemm_bf16_k32.h), and all as in bf16; the gradient's
 // epilogue leaves dz's terms, and dW is fp32.  What it costs beside the products is
 // a pass over W a call (4 bytes read and 8 written an element, 17 us for 8003 x
-// 1021).  777 x 1021 x 8003 train: 604 us on fp32 matrix instructions, 428 so, and
+// 1021).  777 x 1021 x 8003 train: 604 us on fp32 matrix instructions, 424 so, and
 // off by 3e-7 of the result; 4096 x 2048 x 8000 4450 and 2630.  A dz that overflows
 // to an infinity leaves NaN where fp32 products could leave the infinity.
 //
@@ -195,8 +195,11 @@ struct DwRest {
   // own rounding, without).  Of the tokens first .. end - 1 those whose target is in
   // the tile, in order, 32 at a time as one more K step: a one-hot operand of the
   // remainders (bf16: 2^-9 of 2^-9) and the rows of x, both laid out as the main
-  // loop's K tiles.  256 T / V tokens a tile on average.  No longer at 4096 x 2048 x
-  // 32768 (440 us), 2 to 6 us at 120 x 1216 x 19298 (19 -> 24) and the like.
+  // loop's K tiles.  256 T / V tokens a tile on average: no longer at 4096 x 2048 x
+  // 32768 (465 us), 2 to 6 us at 120 x 1216 x 19298 (19 -> 24) and the like.  The steps
+  // wait for their loads, so it shows where a tile has many: dW and the logits again,
+  // targets uniform, half one id, all of one id or of 256: 8192 x 4096 x 2048 342, 469,
+  // 615 us; 8192 x 4096 x 32000 3270, 3770, 4260; 4096 x 2048 x 32768 906, 949, 945.
   template <class FR, int BM, int BN, int WM, int WN, class V, int FN, int FM>
   __device__ __forceinline__ void add_rest(V (&acc)[FN][FM], unsigned char *smem, uint32_t m0, uint32_t n0, uint32_t first,
                                            uint32_t end, int tid, int wm, int wn) const {

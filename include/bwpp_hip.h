@@ -271,7 +271,10 @@ void bwpp_hip_destroy(BwppHip *h);
  * the last one; changing the stream while the old one is being recorded
  * leaves no way to wait, and the handle then goes on without the scratch.
  * A graph that the caller records addresses the workspace as it then is: run
- * the calls once before, and record again after a call that needs more. */
+ * the calls once before, and record again after a call that needs more.  Such
+ * graphs, and the handle's other work, write the same workspace: replay them
+ * one after another (on one stream, or with events between).  The workspace
+ * grows to the largest call's and is freed by bwpp_hip_destroy. */
 BwppHipStatus bwpp_hip_set_stream(BwppHip *h, void *hip_stream);
 void *bwpp_hip_get_stream(const BwppHip *h);
 /* Waits for all work on the handle's stream. */
@@ -665,9 +668,11 @@ BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const voi
  * dz that overflows to an infinity may come out as NaN.  dx rows of left-out tokens are 0, and their x
  * (which may hold anything) has no part in dw.  Outputs must not meet inputs or
  * each other (ALIAS).  Workspace: a copy of x, dz of a piece (256 MiB or 1024
- * columns, in some cases as many again) and fp32 sums of dx, 1 to 32 planes;
- * fp32 in terms: those of x, W's and dz's piece, sums of dx and, up to 8 planes,
- * of dw's piece. */
+ * columns, in some cases as many again), a float per row, and fp32 sums of dx
+ * and of a small dw's piece, 1 to 32 planes each (the copy and a plane of dx
+ * are rows x dim: they grow with the batch, whatever the piece); fp32 in terms:
+ * those of x, W's and dz's piece, sums of dx and, up to 8 planes, of dw's
+ * piece. */
 BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const void *x, const void *w, const int32_t *targets,
                                                  const float *lse, const float *dloss, void *dx, void *dw,
                                                  BwppLinearXentParams params);
