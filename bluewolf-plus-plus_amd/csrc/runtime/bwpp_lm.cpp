@@ -262,8 +262,8 @@ BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k,
   auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
   const BwppHipFault fault = bwpp_hip_check_rotary(p);
   if (fault.why) return bwpp_hip_set_error(h, fault.status, "%s: %s", what, fault.why);
-  if ((p.q_heads && (!q || !qo)) || (p.k_heads && (!k || !ko))) return bad("NULL q, k or output");
   if (p.tokens == 0 || p.dim == 0 || (p.q_heads == 0 && p.k_heads == 0)) return bwpp_hip_enter(h);
+  if ((p.q_heads && (!q || !qo)) || (p.k_heads && (!k || !ko))) return bad("NULL q, k or output");
   const uint32_t rot = p.rot_dim ? p.rot_dim : p.dim;
   const double base = p.base != 0.0f ? p.base : 10000.0, factor = p.factor != 0.0f ? p.factor : 1.0;
   const uint64_t B = p.batch ? p.batch : 1, T = p.tokens, d = p.dim, heads = (uint64_t)p.q_heads + p.k_heads;
@@ -405,7 +405,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm(BwppHip *h, const void 
                                                          const void *post_gamma, const void *gate,
                                                          const void *pre_gamma, void *r, void *y,
                                                          BwppResidualNormParams p) {
-  if (!x || !o || !r) return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "residual_norm: NULL x, o or r");
+  if (p.rows && (!x || !o || !r)) return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "residual_norm: NULL x, o or r");
   BwppResNormArgs a = {};
   BwppHipStatus s = resnorm_prepare(h, "residual_norm", p, a);
   if (s != BWPP_HIP_OK) return s;
@@ -440,8 +440,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_residual_norm_grad(BwppHip *h, const 
                                                               void *dpre_gamma, BwppResidualNormParams p) {
   const char *what = "residual_norm_grad";
   auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
-  if (!o || !r || (!dr && !dy)) return bad("NULL o or r, or neither dr nor dy");
-  if (!dx && !dout && !dpost_gamma && !dgate && !dpre_gamma) return bad("no output");
+  if (p.rows && (!o || !r || (!dr && !dy))) return bad("NULL o or r, or neither dr nor dy");
+  if (p.rows && !dx && !dout && !dpost_gamma && !dgate && !dpre_gamma) return bad("no output");
   if (dpost_gamma && !p.post_norm) return bad("dpost_gamma without a post-norm");
   BwppResNormArgs a = {};
   BwppHipStatus s = resnorm_prepare(h, what, p, a);
@@ -948,7 +948,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x
                                                        const int32_t *targets, float *loss, float *lse, float *sums,
                                                        BwppLinearXentParams p) {
   const char *what = "linear_xent";
-  if (!x || !w || !targets || (!loss && !lse && !sums))
+  if (p.rows && (!x || !w || !targets || (!loss && !lse && !sums)))
     return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: NULL x, w or targets, or no output", what);
   XentMatrices m;
   BwppHipStatus s = xent_prepare(h, what, p, m);
@@ -1039,7 +1039,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
                                                             const float *dloss, void *dx, void *dw,
                                                             BwppLinearXentParams p) {
   const char *what = "linear_xent_grad";
-  if (!x || !w || !targets || !lse || (!dx && !dw))
+  if (p.rows && (!x || !w || !targets || !lse || (!dx && !dw)))
     return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: NULL x, w, targets or lse, or no output", what);
   XentMatrices m;
   BwppHipStatus s = xent_prepare(h, what, p, m);

@@ -611,7 +611,8 @@ BwppHipStatus bwpp_hip_dispatch_elementwise(BwppHip *h, const float *a, const fl
 
 /* ---- around the block: positions, residual joins ----
  * F32 or BF16 operands; arithmetic and sums in fp32, each output rounded
- * once.  No reference counterparts. */
+ * once.  With no rows (tokens) operands may be NULL, as empty tensors are, and
+ * sums over rows are 0.  No reference counterparts. */
 
 /* qo, ko = the rotated q, k.  positions: device int32 [batch][tokens] (row
  * stride pos_batch_stride) or NULL; any int32 is a position.  k may be NULL
