@@ -54,3 +54,42 @@ def test_targets_keep_their_bits(be, wide, T, D, V, targets, pads):
         assert any(k.startswith(("bwpp_xent_rowsums_r", "bwpp_xent_rows_r")) for k in recent), recent
         assert bool(((_vd(dw, wide).double() - want).abs() <= tol).all()), only
         assert untouched(dw, buf)
+
+
+@pytest.mark.parametrize("wide,T,D,V", [("vd", 3000, 256, 1500), ("dv", 300, 130, 516)])
+def test_recorded(be, wide, T, D, V):
+    """Its planes lie in the handle's workspace, so a recorded graph takes the same
+    kernels and gives the same bits; a smaller call runs between the replays."""
+    import bwpp
+    x, w, t = _case(T, D, V, BF16, wide, 23)
+    x2, w2, t2 = _case(40, 64, 300, BF16, "vd", 24)
+    b, side = bwpp.HipBackend(0), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    b.set_stream(side)
+    lse, lse2 = torch.empty(T, device="cuda"), torch.empty(40, device="cuda")
+    out, small = (torch.empty_like(x), torch.empty_like(w)), (torch.empty_like(x2), torch.empty_like(w2))
+    torch.cuda.synchronize()
+
+    def call(a, c, d, l, o, p):
+        b.dispatch_linear_xent(a, c, d, None, l, None, p)
+        b.dispatch_linear_xent_grad(a, c, d, l, None, *o, p)
+
+    p, p2 = _params(T, D, V, BF16, wide, x, w), _params(40, 64, 300, BF16, "vd", x2, w2)
+    call(x, w, t, lse, out, p)
+    assert any(b.recent_kernel(i).startswith(("bwpp_xent_rowsums_r", "bwpp_xent_rows_r")) for i in range(3))
+    side.synchronize()
+    want = [v.clone() for v in out]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call(x, w, t, lse, out, p)
+    for i in range(4):
+        for v in (*out, lse):
+            v.fill_(3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        call(x2, w2, t2, lse2, small, p2)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), i
+    b.close()
