@@ -1139,7 +1139,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const vo
   void *xc = base, *z = base + x_bytes;
   float *acc = reinterpret_cast<float *>(base + x_bytes + z_bytes);
   // What rounding leaves of the targets' dz, for the kernels that add it: dx from
-  // planes, dW on the wide tiles.
+  // planes, and dW's.
   float *rest = reinterpret_cast<float *>(base + x_bytes + z_bytes + sum_bytes);
   auto at = [&](const void *ptr, uint64_t elems) {
     return static_cast<const unsigned char *>(ptr) + elems * es;
