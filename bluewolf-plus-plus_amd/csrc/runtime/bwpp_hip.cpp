@@ -1202,7 +1202,10 @@ BwppHipStatus matmul_impl(BwppHip *h, const void *a, const void *b, void *c, con
   const Extent eb = extent(b, tb ? p.N : p.K, b_cols, ldb, es);
   const bool use_bias = (p.epilogue & BWPP_HIP_EPILOGUE_ADD) && bias;
   const Extent ebias = use_bias ? extent(bias, 1, p.N, p.N, es) : Extent{};
-  if (overlaps(ec, ea) || overlaps(ec, eb) || overlaps(ec, ebias))
+  // By byte range; an operator that holds the workspace has compared its operands'
+  // rows already (its output may lie between the rows of an input).
+  const bool checked = h->ws_held != 0;
+  if (!checked && (overlaps(ec, ea) || overlaps(ec, eb) || overlaps(ec, ebias)))
     return fail(h, BWPP_HIP_ERR_ALIAS, "matmul: C overlaps A, B or bias");
   // Fused tail: fp32 only; aux (residual / SiLU input) and c2 (dual output).
   const uint32_t fuse = fz.kind;

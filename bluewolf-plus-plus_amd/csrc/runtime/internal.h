@@ -90,5 +90,6 @@ bool bwpp_hip_blocks_overlap(const void *pa, uint64_t ra, uint64_t ca, uint64_t 
 
 // Keeps the first `bytes` of the workspace for the caller while it runs other
 // operators of the library (matrix products), which then split through what
-// lies behind them and never move the workspace.  0 ends it.
+// lies behind them, never move the workspace, and leave it to the caller that
+// outputs and inputs do not meet.  0 ends it.
 void bwpp_hip_hold_workspace(BwppHip *h, size_t bytes);
