@@ -294,6 +294,7 @@ def prepare(case, seed):
     if k == "rules":
         st["out"] = dict(y=new(case["rows"], case["vocab"], dtype=torch.float32))
         st["p"] = bwpp.LogitRulesParams(rows=case["rows"], vocab=case["vocab"], dtype_x=code,
+                                        history=t["history"].numel(),
                                         ld_bias=case["vocab"] if case["bias"] == "rows" else 0,
                                         ld_mask=(case["vocab"] + 31) // 32)
         return st
