@@ -5,7 +5,8 @@ objects (lib/); this package only binds them.  There is no CPU fallback:
 if the library or a code object is missing, HipBackend() raises.
 """
 from . import _lib, plan, synth
-from ._lib import (AttentionParams, CoreDType, DType, ElementwiseParams, Epilogue, Fusion,
+from ._lib import (CacheAppendParams, CacheAttentionParams, CacheKeepParams, CacheParams, LogitRulesParams,
+                   AttentionParams, CoreDType, DType, ElementwiseParams, Epilogue, Fusion,
                    FusionParams, LibraryMissing, LinearXentParams, MatmulParams, MeanSquareParams, ReduceParams,
                    ResidualNormParams, RmsnormParams, RotaryLayout, RotaryParams, RotaryScaling,
                    SoftmaxParams, Status, Tensor)
@@ -14,7 +15,8 @@ from .backend import BwppError, HipBackend, tensor_of
 __all__ = ["HipBackend", "BwppError", "LibraryMissing", "Status", "DType",
            "Epilogue", "Fusion", "FusionParams", "MatmulParams", "SoftmaxParams", "RmsnormParams",
            "MeanSquareParams", "RotaryLayout", "RotaryScaling", "RotaryParams", "ResidualNormParams",
-           "LinearXentParams",
+           "LinearXentParams", "CacheParams", "CacheAppendParams", "CacheAttentionParams", "CacheKeepParams",
+           "LogitRulesParams",
            "AttentionParams", "ReduceParams", "ElementwiseParams", "CoreDType", "Tensor",
            "tensor_of", "synth", "plan",
            "load_library"]

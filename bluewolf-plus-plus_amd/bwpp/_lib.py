@@ -132,6 +132,35 @@ class LinearXentParams(Structure):
                 ("dloss_scalar", c_uint32), ("scale", c_float)]
 
 
+class CacheParams(Structure):
+    _fields_ = [("pages", c_uint32), ("page_tokens", c_uint32), ("heads", c_uint32), ("dim", c_uint32),
+                ("batch", c_uint32), ("max_pages", c_uint32), ("ld_table", c_uint32), ("tokens", c_uint32),
+                ("q_heads", c_uint32), ("dtype", c_uint32),
+                ("page_stride", c_uint64), ("token_stride", c_uint64), ("head_stride", c_uint64)]
+
+
+class CacheAppendParams(Structure):
+    _fields_ = [("cache", CacheParams), ("ldq", c_uint32), ("ldk", c_uint32), ("ldv", c_uint32), ("ldqo", c_uint32),
+                ("q_head_stride", c_uint64), ("k_head_stride", c_uint64), ("v_head_stride", c_uint64),
+                ("qo_head_stride", c_uint64), ("no_rotation", c_uint32), ("rot_dim", c_uint32), ("layout", c_uint32),
+                ("scaling", c_uint32), ("base", c_float), ("factor", c_float), ("low_turns", c_float),
+                ("high_turns", c_float), ("context", c_uint32), ("magnitude", c_float)]
+
+
+class CacheAttentionParams(Structure):
+    _fields_ = [("cache", CacheParams), ("ldq", c_uint32), ("ldo", c_uint32), ("q_head_stride", c_uint64),
+                ("o_head_stride", c_uint64), ("mask_words", c_uint32), ("scale", c_float)]
+
+
+class CacheKeepParams(Structure):
+    _fields_ = [("cache", CacheParams), ("max_kept", c_uint32), ("ld_kept", c_uint32)]
+
+
+class LogitRulesParams(Structure):
+    _fields_ = [("rows", c_uint32), ("vocab", c_uint32), ("ldx", c_uint32), ("ldy", c_uint32), ("dtype_x", c_uint32),
+                ("dtype_y", c_uint32), ("history", c_uint32), ("ld_bias", c_uint32), ("ld_mask", c_uint32)]
+
+
 class Arena(Structure):
     _fields_ = [("buffer", c_void_p), ("capacity", c_size_t),
                 ("offset", c_size_t), ("device", c_int)]
@@ -228,6 +257,10 @@ SIGNATURES = {
     "bwpp_hip_dispatch_residual_norm_grad": (c_int, [_P] * 13 + [ResidualNormParams]),
     "bwpp_hip_dispatch_linear_xent": (c_int, [_P] * 7 + [LinearXentParams]),
     "bwpp_hip_dispatch_linear_xent_grad": (c_int, [_P] * 8 + [LinearXentParams]),
+    "bwpp_hip_dispatch_cache_append": (c_int, [_P] * 11 + [CacheAppendParams]),
+    "bwpp_hip_dispatch_cache_attention": (c_int, [_P] * 10 + [CacheAttentionParams]),
+    "bwpp_hip_dispatch_cache_keep": (c_int, [_P] * 7 + [CacheKeepParams]),
+    "bwpp_hip_dispatch_logit_rules": (c_int, [_P] * 11 + [LogitRulesParams]),
     "bwpp_synth_uniform_f32": (None, [_P, c_uint64, c_uint64, c_uint64, c_float, c_float]),
     "bwpp_synth_normal_f32": (None, [_P, c_uint64, c_uint64, c_uint64, c_float, c_float]),
     "bwpp_synth_ramp_f32": (None, [_P, c_uint32, c_uint32, c_float]),
@@ -272,6 +305,7 @@ def load():
 __all__ = ["Status", "DType", "Epilogue", "MatmulParams", "Fusion", "FusionParams", "SoftmaxParams",
            "RmsnormParams", "MeanSquareParams", "AttentionParams", "ReduceParams", "ElementwiseParams", "Arena",
            "RotaryLayout", "RotaryScaling", "RotaryParams", "ResidualNormParams",
-           "LinearXentParams", "CoreDType", "Tensor",
+           "LinearXentParams", "CacheParams", "CacheAppendParams", "CacheAttentionParams", "CacheKeepParams",
+           "LogitRulesParams", "CoreDType", "Tensor",
            "SIGNATURES", "load", "LIB_PATH", "LIB_DIR", "HEADER_PATH",
            "LibraryMissing", "byref", "c_void_p", "c_uint16"]

@@ -233,6 +233,32 @@ class HipBackend:
         self._check(self.lib.bwpp_hip_dispatch_linear_xent_grad(
             self._h, _ptr(x), _ptr(w), _int32(targets, "targets"), _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw), params))
 
+    # ------------------------------------- a paged cache, the next token
+    def dispatch_cache_append(self, q, k, v, positions, table, starts, held, qo, k_cache, v_cache, params):
+        """k, v of new tokens into their pages, k and q (to qo, or in place) with rotary positions."""
+        self._check(self.lib.bwpp_hip_dispatch_cache_append(
+            self._h, _ptr(q), _ptr(k), _ptr(v), _int32(positions, "positions"), _int32(table, "table", True),
+            _int32(starts, "starts"), _int32(held, "held"), _ptr(qo), _ptr(k_cache), _ptr(v_cache), params))
+
+    def dispatch_cache_attention(self, q, k_cache, v_cache, table, starts, held, mask, o, lse, params):
+        """o = softmax(scale q k) v of new tokens over the cache; mask: bits (as int32) of the new tokens seen,
+        or None: each sees those up to itself."""
+        self._check(self.lib.bwpp_hip_dispatch_cache_attention(
+            self._h, _ptr(q), _ptr(k_cache), _ptr(v_cache), _int32(table, "table", True), _int32(starts, "starts"),
+            _int32(held, "held"), _int32(mask, "mask"), _ptr(o), _ptr(lse), params))
+
+    def dispatch_cache_keep(self, k_cache, v_cache, table, held, kept, counts, params):
+        """Slot held + i of each sequence takes what lies in slot held + kept[i]."""
+        self._check(self.lib.bwpp_hip_dispatch_cache_keep(
+            self._h, _ptr(k_cache), _ptr(v_cache), _int32(table, "table", True), _int32(held, "held"),
+            _int32(kept, "kept", True), _int32(counts, "counts"), params))
+
+    def dispatch_logit_rules(self, x, history, starts, prompt, repetition, presence, frequency, bias, mask, y, params):
+        """y = x with penalties for tokens of the history, a bias and a mask of bits (as int32)."""
+        self._check(self.lib.bwpp_hip_dispatch_logit_rules(
+            self._h, _ptr(x), _int32(history, "history"), _int32(starts, "starts"), _int32(prompt, "prompt"),
+            _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias), _int32(mask, "mask", True), _ptr(y), params))
+
     # ------------------------------------------------------ tensor forms
     def tensor_matmul(self, a, b, bias, c, epilogue: int = 0):
         ref = lambda t: ctypes.byref(t) if t is not None else None

@@ -258,4 +258,73 @@ typedef struct {
   float scale;
 } BwppXentRowArgs;
 
+/* A paged cache of keys and values and a ragged batch of new tokens
+ * (kv_cache.h).  Strides in elements. */
+typedef struct {
+  void *k, *v;             /* pools of the same strides */
+  const int32_t *table;    /* [batch][ld_table] page numbers */
+  const int32_t *starts;   /* [batch + 1] first rows */
+  const int32_t *held;     /* [batch] tokens in the cache before the new ones */
+  uint64_t page_s, tok_s, head_s, ld_table;
+  uint32_t pages, page_shift;
+  uint32_t capacity;       /* slots of a sequence, below 2^31 */
+  uint32_t batch, tokens, heads, dim;
+} BwppCacheArgs;
+
+/* New keys and values into their pages, q and k with rotary positions
+ * (kv_append.h).  r: q, k, qo, their token and head strides, the rotation,
+ * chunks; tile and hgroup as there, heads = q's + twice the cache's. */
+typedef struct {
+  BwppCacheArgs c;
+  BwppRotaryArgs r;
+  const void *v_in;
+  uint64_t v_ts, v_hs;
+} BwppCacheAppendArgs;
+
+/* Accepted tokens moved together. */
+typedef struct {
+  BwppCacheArgs c;
+  const int32_t *kept, *counts; /* [batch][ld_kept], [batch] */
+  uint64_t ld_kept;
+  uint32_t max_kept;
+  uint32_t unit;   /* elements a chunk */
+  uint32_t chunks; /* chunks a head's row */
+} BwppCacheKeepArgs;
+
+/* Attention of the new tokens over the cache (kv_attention.h).  Row r of a
+ * sequence and key head is query head r % group of token r / group. */
+typedef struct {
+  BwppCacheArgs c;
+  const void *q;
+  void *o;
+  float *lse;           /* [tokens][group * heads], or NULL */
+  const uint32_t *mask; /* [tokens][mask_words], or NULL: causal */
+  uint64_t q_ts, q_hs, o_ts, o_hs;
+  uint32_t mask_words;
+  uint32_t group;       /* query heads per key head */
+  float scale_log2;     /* |scale| * log2(e) */
+  uint32_t flip;        /* 1: the scale is negative */
+  uint32_t blocks;      /* workers that share the keys */
+  uint32_t rows;        /* a tile's rows (the join's) */
+  uint32_t unit;        /* keys of a unit of work (the join's) */
+  uint32_t vec;         /* 1: rows of 4 elements at their natural alignment, dim a multiple of 4 */
+  float *part_o;        /* [2 blocks][rows][dim up to a multiple of 4] */
+  float *part_ml;       /* [2 blocks][rows][2] */
+} BwppCacheAttnArgs;
+
+/* Rules for the next token on logits (logit_rules.h). */
+typedef struct {
+  const void *x;
+  void *y;
+  const int32_t *history, *starts, *prompt;
+  const float *repetition, *presence, *frequency, *bias;
+  const uint32_t *mask;
+  uint64_t ldx, ldy, ld_bias, ld_mask;
+  uint32_t rows, vocab;
+  uint32_t chunk;  /* columns a block, a power of two */
+  uint32_t chunks; /* blocks a row */
+  uint32_t history_len; /* elements of the history */
+  uint32_t count;  /* 1: tokens of the history are counted */
+} BwppLogitArgs;
+
 #endif /* BWPP_KARGS_H */

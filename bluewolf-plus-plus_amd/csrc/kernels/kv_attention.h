@@ -1,0 +1,396 @@
+// Attention of new tokens over a paged cache, any head dim up to 256, fp32 or
+// bf16, any alignment; and the join of items that several blocks shared.
+//
+//   o[t][h] = sum_p w_p v_p / sum_p w_p,  w_p = e^(scale q[t][h] . k_p)
+//
+// over the held tokens and those new tokens of the sequence that token t sees
+// (its mask bits, or those up to itself).  The query heads that share a key
+// head are rows of one tile, so keys and values are read once for all.
+//
+// A wave holds 16 query rows.  Per 16 keys it computes S^T = K Q^T with fp32
+// matrix instructions (16 x 16 x 4, exact products): lane l's keys come
+// straight from memory, 4 elements of key l % 16 a load, and are the "A"
+// operand as they stand, since a product may take the head's columns in any
+// order as long as q's are in the same.  The accumulator then has row l % 16
+// against keys 4 (l / 16) .. + 3, which is how the "B" operand of
+// O^T += V^T P^T wants the probabilities, and V's rows are loaded 4 columns a
+// lane (column 64 j + 4 i + c is row i of product (j, c)).  So nothing passes
+// through LDS but the sums at the end.
+//
+// Few rows (ROWS false): the block's four waves take every fourth tile of keys
+// and their sums meet in LDS.  More rows (ROWS true): each wave has 16 rows of
+// its own and walks all keys.
+#pragma once
+
+#include "attention_common.h"
+#include "kv_cache.h"
+#include "kv_schedule.h"
+#include "rotary_math.h"
+#include "../kargs.h"
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+namespace kv {
+
+// Four elements from column c of a row of `dim`, zeros past it.
+template <class T, bool VEC>
+__device__ __forceinline__ void load4(const T *row, uint32_t c, uint32_t dim, float (&o)[4]) {
+  if (VEC || c + 4 <= dim) {
+    rotary_pos::Vec<T, 4>::load(row + c, o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float e[1] = {0.0f};
+      if (c + (uint32_t)i < dim) rotary_pos::Vec<T, 1>::load(row + c + i, e);
+      o[i] = e[0];
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T *row, uint32_t c, uint32_t dim, const float (&v)[4]) {
+  if (c + 4 <= dim) {
+    rotary_pos::Vec<T, 4>::store(row + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e[1] = {v[i]};
+      if (c + (uint32_t)i < dim) rotary_pos::Vec<T, 1>::store(row + c + i, e);
+    }
+  }
+}
+
+// Bits 0 .. 15: whether the token `i` (of a sequence that begins at row first)
+// sees the new tokens j0 .. j0 + 15 of it.
+__device__ __forceinline__ uint32_t mask_bits(const BwppCacheAttnArgs &a, uint32_t first, uint32_t i, int64_t j0) {
+  if (!a.mask) {
+    const int64_t seen = (int64_t)i + 1 - j0;  // of the 16
+    return seen <= 0 ? 0u : seen >= 16 ? 0xffffu : (1u << seen) - 1u;
+  }
+  uint64_t two = 0;
+  const uint32_t *row = a.mask + (uint64_t)(first + i) * a.mask_words;
+  const int64_t w = j0 >> 5;
+  if (w >= 0 && w < (int64_t)a.mask_words) two = row[w];
+  if (w + 1 >= 0 && w + 1 < (int64_t)a.mask_words) two |= (uint64_t)row[w + 1] << 32;
+  return (uint32_t)(two >> (j0 & 31)) & 0xffffu;
+}
+
+template <class T, int DC, bool ROWS>
+__device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
+  constexpr uint32_t kRows = ROWS ? 64 : 16, kUnit = 64, kTile = 16;
+  constexpr int KC = 4 * DC, kLd = 64 * DC + 4;
+  typedef Work<kRows, kUnit> W;
+  __shared__ uint64_t wave_sums[kThreads / 64];
+  __shared__ Share share;
+  __shared__ float os[ROWS ? 1 : 4][ROWS ? 1 : 16][ROWS ? 4 : kLd];
+  __shared__ float ml[4][16][2];
+  const BwppCacheArgs &c = a.c;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i16 = lane & 15u, grp = lane >> 4;
+  const uint32_t D = c.dim, g = a.group, Dp = (D + 3u) & ~3u;
+  find_share<kRows, kUnit>(a, blockIdx.x, &share, wave_sums);
+  const Place to = share.to;
+  Place at = share.from;
+  const uint32_t pmask = (1u << c.page_shift) - 1u;
+
+  Seq q = {};
+  if (at.s < c.batch) q = seq_at(c, at.s);
+  // A part of an item that began in another block is written even if it has no
+  // keys: the join reads it.
+  bool part = at.unit != 0;
+  for (; part || earlier(at, to); part = false) {
+    const bool same = at.s == to.s && at.head == to.head && at.tile == to.tile;
+    const uint32_t total = W::units(a, q, at.tile), u1 = same ? to.unit : total;  // (to.unit >= at.unit)
+    const bool whole = at.unit == 0 && u1 == total;
+    const uint32_t kbeg = at.unit * kUnit, kend = min(u1 * kUnit, W::keys(a, q, at.tile));
+    const uint32_t R = q.n * g, r0 = at.tile * kRows + (ROWS ? 16u * wave : 0u);
+    const uint32_t row = r0 + i16, tok = min(row, R - 1u) / g, hq = at.head * g + min(row, R - 1u) % g;
+    float qf[KC][4];
+    {
+      const T *Q = static_cast<const T *>(a.q) + (uint64_t)(q.first + tok) * a.q_ts + (uint64_t)hq * a.q_hs;
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        if (16u * j < D) load4<T, false>(Q, 16u * j + 4u * grp, D, qf[j]);
+        else qf[j][0] = qf[j][1] = qf[j][2] = qf[j][3] = 0.0f;
+      }
+    }
+    const float scale = a.flip ? -a.scale_log2 : a.scale_log2;
+    const T *K = static_cast<const T *>(c.k) + (uint64_t)at.head * c.head_s;
+    const T *V = static_cast<const T *>(c.v) + (uint64_t)at.head * c.head_s;
+    const int32_t *table = c.table + (uint64_t)at.s * c.ld_table;
+
+    f32x4_t o[DC][4];
+#pragma unroll
+    for (int j = 0; j < DC; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+
+    const uint32_t step = ROWS ? kTile : 4u * kTile;
+    uint32_t k0 = kbeg + (ROWS ? 0u : kTile * wave);
+    // A lane's key of the tile at k: its row's offset, kNoSlot past the keys or
+    // outside the pool.  Page numbers are fetched one tile ahead.
+    auto page = [&](uint32_t k) { return k + i16 < kend ? (uint32_t)table[(k + i16) >> c.page_shift] : ~0u; };
+    auto offset = [&](uint32_t k, uint32_t pg) {
+      return pg < c.pages ? (uint64_t)pg * c.page_s + (uint64_t)((k + i16) & pmask) * c.tok_s : kNoSlot;
+    };
+    float kf[KC][4];
+    auto load_keys = [&](uint64_t off) {
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        kf[j][0] = kf[j][1] = kf[j][2] = kf[j][3] = 0.0f;
+        if (16u * j < D && off != kNoSlot) load4<T, false>(K + off, 16u * j + 4u * grp, D, kf[j]);
+      }
+    };
+    uint64_t off = kNoSlot;
+    uint32_t next_page = ~0u;
+    if (k0 < kend) {
+      off = offset(k0, page(k0));
+      next_page = page(k0 + step);
+      load_keys(off);
+    }
+    for (; k0 < kend; k0 += step) {
+      float vf[4][DC][4];
+      bool live[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint64_t ov = __shfl(off, 4 * grp + r, 64);
+        live[r] = ov != kNoSlot;
+#pragma unroll
+        for (int j = 0; j < DC; ++j) {
+          vf[r][j][0] = vf[r][j][1] = vf[r][j][2] = vf[r][j][3] = 0.0f;
+          if (live[r] && 64u * j + 4u * i16 < D) load4<T, false>(V + ov, 64u * j + 4u * i16, D, vf[r][j]);
+        }
+      }
+      f32x4_t s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        if (16u * j >= D) continue;
+        s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][0], qf[j][0], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][1], qf[j][1], s1, 0, 0, 0);
+        s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][2], qf[j][2], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][3], qf[j][3], s1, 0, 0, 0);
+      }
+      off = offset(k0 + step, next_page);
+      next_page = page(k0 + 2 * step);
+      load_keys(off);
+      // Visible keys of this lane's row among its four.
+      uint32_t vis = (live[0] ? 1u : 0u) | (live[1] ? 2u : 0u) | (live[2] ? 4u : 0u) | (live[3] ? 8u : 0u);
+      const bool fresh = k0 + kTile > q.held;  // new tokens among the keys
+      if (fresh) {
+        uint32_t bits = mask_bits(a, q.first, tok, (int64_t)k0 - (int64_t)q.held);
+        if (k0 < q.held) bits |= (1u << (q.held - k0)) - 1u;  // fewer than 16
+        vis &= bits >> (4u * grp);
+      }
+      float p[4], mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[r] = vis >> r & 1u ? (s0[r] + s1[r]) * scale : -INFINITY;
+        mx = fmaxf(mx, p[r]);
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      float alpha = 1.0f;
+      if (mx > m + kLazy) {
+        alpha = __builtin_amdgcn_exp2f(m - mx);  // 0 when m is -inf
+        m = mx;
+      }
+      const float use = m == -INFINITY ? 0.0f : m;
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(p[r] - use);
+        sum += p[r];
+      }
+      l = l * alpha + sum;  // of this lane's keys: the lanes of a row are added at the end
+      if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+        for (int j = 0; j < DC; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j][e] *= alpha;
+      }
+      // 0 times an infinite or NaN v would reach rows that do not see it.
+      bool odd = false;
+      if (fresh) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < DC; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= !(fabsf(vf[r][j][e]) < INFINITY);
+      }
+      if (fresh && __ballot(odd)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          for (uint32_t k4 = 0; k4 < 4; ++k4) {  // key 4 k4 + r
+            const float pk = __shfl(p[r], 16 * k4 + i16, 64);
+            const bool see = __shfl(vis >> r & 1u, 16 * k4 + i16, 64) != 0;
+#pragma unroll
+            for (int j = 0; j < DC; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr) {
+                  const float v = __shfl(vf[r][j][e], 16 * k4 + 4 * grp + rr, 64);
+                  if (see) o[j][e][rr] += pk * v;
+                }
+          }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < DC; ++j) {
+            if (64u * j >= D) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r][j][e], p[r], o[j][e], 0, 0, 0);
+          }
+      }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // Results: row i16 has columns 64 j + 4 (4 grp + rr) + e in o[j][e][rr].
+    const uint32_t slot = 2u * blockIdx.x + (at.unit == 0 ? 1u : 0u);
+    auto put = [&](uint32_t rw, uint32_t col, const float (&v)[4], float mm, float ll, bool head) {
+      // rw: row of the tile
+      const uint32_t rr = at.tile * kRows + rw;
+      if (rr >= R || col >= D) return;
+      if (!whole) {
+        float *po = a.part_o + ((uint64_t)slot * kRows + rw) * Dp + col;
+        *reinterpret_cast<float4 *>(po) = make_float4(v[0], v[1], v[2], v[3]);
+        if (head) *reinterpret_cast<float2 *>(a.part_ml + ((uint64_t)slot * kRows + rw) * 2) = make_float2(mm, ll);
+        return;
+      }
+      const uint64_t t = q.first + rr / g, hh = at.head * g + rr % g;
+      const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+      const float u[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+      store4(static_cast<T *>(a.o) + t * a.o_ts + hh * a.o_hs, col, D, u);
+      if (head && a.lse) a.lse[t * (uint64_t)(c.heads * g) + hh] = ll == 0.0f ? -INFINITY : lse_of(mm == -INFINITY ? 0.0f : mm, ll);
+    };
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int j = 0; j < DC; ++j)
+#pragma unroll
+        for (int rr = 0; rr < 4; ++rr) {
+          const float v[4] = {o[j][0][rr], o[j][1][rr], o[j][2][rr], o[j][3][rr]};
+          put(16u * wave + i16, 64u * j + 4u * (4u * grp + rr), v, m, l, j == 0 && rr == 0 && grp == 0);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < DC; ++j)
+#pragma unroll
+        for (int rr = 0; rr < 4; ++rr)
+          *reinterpret_cast<float4 *>(&os[wave][i16][64 * j + 4 * (4 * grp + rr)]) =
+              make_float4(o[j][0][rr], o[j][1][rr], o[j][2][rr], o[j][3][rr]);
+      if (grp == 0) ml[wave][i16][0] = m, ml[wave][i16][1] = l;
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < 16u * (Dp / 4u); i += kThreads) {
+        const uint32_t rw = i / (Dp / 4u), col = 4u * (i % (Dp / 4u));
+        float mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w][rw][0]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float mw = ml[w][rw][0];
+          // no key seen (offset -inf): sums of 0 (or NaN, kept)
+          const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - mm);
+          ll += ml[w][rw][1] * f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += os[w][rw][col + e] * f;
+        }
+        put(rw, col, v, mm, ll, col == 0);
+      }
+      __syncthreads();
+    }
+
+    // The next item.
+    at.unit = 0;
+    if (++at.tile >= W::tiles(q, g)) {
+      at.tile = 0;
+      if (++at.head >= c.heads) {
+        at.head = 0;
+        do {
+          ++at.s;
+          if (at.s >= c.batch) break;
+          q = seq_at(c, at.s);
+        } while (q.n == 0);
+      }
+    }
+  }
+}
+
+// Joins the parts of the item that block b's border is the first to divide
+// (b = 1 .. G - 1, a block of this launch each).
+template <class T, uint32_t kRows, uint32_t kUnit>
+__device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
+  typedef Work<kRows, kUnit> W;
+  __shared__ uint64_t wave_sums[kThreads / 64];
+  __shared__ Place item;
+  __shared__ uint32_t last;  // block with the item's last part; 0: nothing to join
+  const BwppCacheArgs &c = a.c;
+  const Costs<kRows, kUnit> costs(a, wave_sums);
+  const uint32_t G = sharers(a, costs.total), b = blockIdx.x + 1;
+  if (b >= G) return;
+  if (threadIdx.x == 0) last = 0;
+  __syncthreads();
+  const uint64_t x = costs.total * b / G, prev = costs.total * (b - 1) / G;
+  costs.at(a, x, [&](uint32_t s, const Seq &q, uint64_t at) {
+    uint64_t begin, end;
+    const Place p = W::find(a, s, q, x - at, begin, end);
+    if (p.unit == 0) return;
+    if (prev >= at + begin && W::unit(a, q, p.tile, prev - at - begin, end - begin) != 0) return;  // not the first
+    item = p;
+    last = (uint32_t)(((at + end) * G - 1) / costs.total);
+    last = min(last, G - 1);
+  });
+  __syncthreads();
+  if (last == 0) return;
+  const Seq q = seq_at(c, item.s);
+  const uint32_t g = a.group, D = c.dim, n4 = (D + 3u) / 4u, Dp = 4u * n4;
+  const uint32_t rows = min(kRows, q.n * g - item.tile * kRows), parts = last - b + 2;
+  for (uint32_t i = threadIdx.x; i < rows * n4; i += kThreads) {
+    const uint32_t rw = i / n4, col = 4u * (i % n4);
+    // part 0 in slot 2 (b - 1) + 1, part k in slot 2 (b + k - 1)
+    auto slot_row = [&](uint32_t k) { return (uint64_t)(k == 0 ? 2 * b - 1 : 2 * (b + k - 1)) * kRows + rw; };
+    float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t k = 0; k < parts; ++k) m = fmaxf(m, a.part_ml[2 * slot_row(k)]);
+#pragma unroll 4
+    for (uint32_t k = 0; k < parts; ++k) {
+      const uint64_t sr = slot_row(k);
+      const float2 w = *reinterpret_cast<const float2 *>(a.part_ml + 2 * sr);
+      const float f = w.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.x - m);
+      const float4 u = *reinterpret_cast<const float4 *>(a.part_o + sr * Dp + col);
+      l += w.y * f;
+      v[0] += u.x * f, v[1] += u.y * f, v[2] += u.z * f, v[3] += u.w * f;
+    }
+    const uint32_t rr = item.tile * kRows + rw;
+    const uint64_t t = q.first + rr / g, hh = item.head * g + rr % g;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float u[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+    store4(static_cast<T *>(a.o) + t * a.o_ts + hh * a.o_hs, col, D, u);
+    if (col == 0 && a.lse) a.lse[t * (uint64_t)(c.heads * g) + hh] = l == 0.0f ? -INFINITY : lse_of(m == -INFINITY ? 0.0f : m, l);
+  }
+}
+
+}  // namespace kv
+
+#define BWPP_ATTEND(NAME, T, DC, ROWS)                                                                  \
+  extern "C" __global__ __launch_bounds__(256, DC <= 2 ? 2 : 1) void bwpp_cache_attend_##NAME(const BwppCacheAttnArgs a) { \
+    kv::attend<T, DC, ROWS>(a);                                                                         \
+  }
+#define BWPP_ATTEND_DIMS(NAME, T, ROWS) \
+  BWPP_ATTEND(NAME##_d64, T, 1, ROWS)   \
+  BWPP_ATTEND(NAME##_d128, T, 2, ROWS)  \
+  BWPP_ATTEND(NAME##_d192, T, 3, ROWS)  \
+  BWPP_ATTEND(NAME##_d256, T, 4, ROWS)
+BWPP_ATTEND_DIMS(f32, float, false)
+BWPP_ATTEND_DIMS(f32_rows, float, true)
+BWPP_ATTEND_DIMS(bf16, uint16_t, false)
+BWPP_ATTEND_DIMS(bf16_rows, uint16_t, true)
+
+#define BWPP_JOIN(NAME, T, ROWS, UNIT) \
+  extern "C" __global__ __launch_bounds__(256) void bwpp_cache_join_##NAME(const BwppCacheAttnArgs a) { kv::join<T, ROWS, UNIT>(a); }
+BWPP_JOIN(f32, float, 16, 64)
+BWPP_JOIN(f32_rows, float, 64, 64)
+BWPP_JOIN(bf16, uint16_t, 16, 64)
+BWPP_JOIN(bf16_rows, uint16_t, 64, 64)

@@ -1,0 +1,160 @@
+// Who computes what in the attention over a paged cache.
+//
+// Lengths lie in device memory and differ from sequence to sequence, so the
+// work is shared out on the device: a fixed number of blocks, whatever the
+// lengths, and a captured launch follows the lengths of its replay.  An item is
+// a tile of ROWS query rows of one (sequence, key head) with all the keys that
+// it sees, in units of UNIT keys.  Items stand in the order of sequences, heads
+// and tiles, each with a cost: its keys (of a causal tile up to its last
+// token) and kItem more for what an item costs by itself.  Block b of G takes
+// what lies between the costs W b / G and W (b + 1) / G of the total W, rounded
+// to whole units.  An item whose keys fall to several blocks is left by each
+// as a triple (exponent offset, sum of p, sum of p v) and joined by a second
+// launch: the block where it begins leaves it in slot 2 b + 1, the others,
+// for which it is the first item, in slot 2 b.
+//
+// Costs are whole numbers, g times keys (g query heads a key head): a block and
+// its successor find the same border.
+#pragma once
+
+#include "kv_cache.h"
+
+namespace kv {
+
+constexpr uint32_t kItem = 96;      // keys that an item costs by itself
+constexpr uint32_t kLeast = 192;    // a block's share is at least as many keys
+constexpr uint32_t kThreads = 256;  // of the blocks that find their shares
+
+// A place in the order of the work.
+struct Place {
+  uint32_t s, head, tile, unit;
+};
+__device__ __forceinline__ bool earlier(const Place &a, const Place &b) {
+  if (a.s != b.s) return a.s < b.s;
+  if (a.head != b.head) return a.head < b.head;
+  return a.tile != b.tile ? a.tile < b.tile : a.unit < b.unit;
+}
+struct Share {
+  Place from, to;
+  uint32_t blocks;  // that have a share
+};
+
+template <uint32_t ROWS, uint32_t UNIT>
+struct Work {
+  static __device__ __forceinline__ uint32_t tiles(const Seq &q, uint32_t g) { return (q.n * g + ROWS - 1) / ROWS; }
+  static __device__ __forceinline__ uint64_t before(const Seq &q, uint32_t g, uint64_t t) {  // cost of tiles 0 .. t - 1
+    return t * ((uint64_t)g * (q.held + kItem)) + ROWS * (t * (t + 1) / 2);
+  }
+  // Keys that a tile may see.
+  static __device__ __forceinline__ uint32_t keys(const BwppCacheAttnArgs &a, const Seq &q, uint32_t tile) {
+    const uint32_t g = a.group;
+    const uint32_t last = a.mask ? q.n : (min((tile + 1) * ROWS, q.n * g) - 1) / g + 1;
+    return min(q.held + last, a.c.capacity);
+  }
+  static __device__ __forceinline__ uint32_t units(const BwppCacheAttnArgs &a, const Seq &q, uint32_t tile) {
+    return (keys(a, q, tile) + UNIT - 1) / UNIT;
+  }
+  // Where cost x of sequence s (all its heads) falls, and the costs where that
+  // item begins and ends.
+  static __device__ __forceinline__ Place find(const BwppCacheAttnArgs &a, uint32_t s, const Seq &q, uint64_t x,
+                                               uint64_t &begin, uint64_t &end) {
+    const uint32_t T = tiles(q, a.group);
+    const uint64_t head_cost = before(q, a.group, T);
+    const uint32_t head = (uint32_t)(x / head_cost);
+    const uint64_t rest = x - head * head_cost;
+    uint32_t lo = 0, hi = T;  // before(lo) <= rest < before(hi)
+    while (hi - lo > 1) {
+      const uint32_t m = (lo + hi) / 2;
+      if (before(q, a.group, m) <= rest) lo = m;
+      else hi = m;
+    }
+    const uint64_t b0 = before(q, a.group, lo), b1 = before(q, a.group, lo + 1);
+    begin = head * head_cost + b0;
+    end = head * head_cost + b1;
+    return {s, head, lo, unit(a, q, lo, rest - b0, b1 - b0)};
+  }
+  static __device__ __forceinline__ uint32_t unit(const BwppCacheAttnArgs &a, const Seq &q, uint32_t tile, uint64_t off,
+                                                  uint64_t cost) {
+    return (uint32_t)(off * units(a, q, tile) / cost);
+  }
+};
+
+// Costs of the sequences that this thread adds up (a run of `per`), the costs
+// before them, and the total.
+template <uint32_t ROWS, uint32_t UNIT>
+struct Costs {
+  uint32_t s0, s1;
+  uint64_t first, total;
+
+  static __device__ __forceinline__ uint64_t of(const BwppCacheAttnArgs &a, const Seq &q) {
+    return a.c.heads * Work<ROWS, UNIT>::before(q, a.group, Work<ROWS, UNIT>::tiles(q, a.group));
+  }
+  __device__ __forceinline__ Costs(const BwppCacheAttnArgs &a, uint64_t *wave_sums) {
+    const uint32_t per = (a.c.batch + kThreads - 1) / kThreads;
+    s0 = min(threadIdx.x * per, a.c.batch);
+    s1 = min(s0 + per, a.c.batch);
+    uint64_t mine = 0;
+    for (uint32_t s = s0; s < s1; ++s) mine += of(a, seq_at(a.c, s));
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint64_t up = __shfl_up(sum, d, 64);
+      if (lane >= (uint32_t)d) sum += up;
+    }
+    if (lane == 63) wave_sums[wave] = sum;
+    __syncthreads();
+    first = sum - mine;
+    total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 64; ++w) {
+      if (w < wave) first += wave_sums[w];
+      total += wave_sums[w];
+    }
+  }
+  // Calls f(sequence, its cost range) in the thread that has the sequence of cost x.
+  template <class F>
+  __device__ __forceinline__ void at(const BwppCacheAttnArgs &a, uint64_t x, F f) const {
+    uint64_t begin = first;
+    if (x < begin) return;
+    for (uint32_t s = s0; s < s1; ++s) {
+      const Seq q = seq_at(a.c, s);
+      const uint64_t end = begin + of(a, q);
+      if (x < end) {
+        f(s, q, begin);
+        return;
+      }
+      begin = end;
+    }
+  }
+};
+
+// Blocks that share a total cost.
+__device__ __forceinline__ uint32_t sharers(const BwppCacheAttnArgs &a, uint64_t total) {
+  const uint64_t most = total / ((uint64_t)a.group * kLeast);
+  return (uint32_t)(most < 1 ? 1 : most < a.blocks ? most : a.blocks);
+}
+
+// The share of block b, the same in every thread (`share` in LDS).
+template <uint32_t ROWS, uint32_t UNIT>
+__device__ __forceinline__ void find_share(const BwppCacheAttnArgs &a, uint32_t b, Share *share, uint64_t *wave_sums) {
+  const Costs<ROWS, UNIT> costs(a, wave_sums);
+  const uint32_t G = sharers(a, costs.total);
+  if (threadIdx.x == 0) {
+    share->from = share->to = {a.c.batch, 0, 0, 0};
+    share->blocks = G;
+  }
+  __syncthreads();
+  if (b >= G) return;
+  uint64_t begin, end;
+  const uint64_t x0 = costs.total * b / G, x1 = costs.total * (b + 1) / G;
+  costs.at(a, x0, [&](uint32_t s, const Seq &q, uint64_t at) {
+    share->from = Work<ROWS, UNIT>::find(a, s, q, x0 - at, begin, end);
+  });
+  costs.at(a, x1, [&](uint32_t s, const Seq &q, uint64_t at) {
+    share->to = Work<ROWS, UNIT>::find(a, s, q, x1 - at, begin, end);
+  });
+  __syncthreads();
+}
+
+}  // namespace kv

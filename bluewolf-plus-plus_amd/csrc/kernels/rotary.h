@@ -29,6 +29,7 @@
 #pragma once
 
 #include "common.h"
+#include "rotary_math.h"
 #include "../kargs.h"
 
 using namespace bwpp;
@@ -36,94 +37,6 @@ using namespace bwpp;
 namespace rotary_pos {
 
 constexpr int kMaxAngles = 2048;  // (token, pair) angles of a block: 16 KiB of LDS
-
-// N elements of T at any address aligned to T, as floats.
-template <class T, int N>
-struct Vec;
-template <int N>
-struct Vec<float, N> {
-  typedef float V __attribute__((ext_vector_type(N), aligned(4)));
-  static __device__ __forceinline__ void load(const float *p, float (&o)[N]) {
-    const V v = *reinterpret_cast<const V *>(p);
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = v[i];
-  }
-  static __device__ __forceinline__ void store(float *p, const float (&o)[N]) {
-    V v;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = o[i];
-    *reinterpret_cast<V *>(p) = v;
-  }
-};
-template <>
-struct Vec<float, 1> {
-  static __device__ __forceinline__ void load(const float *p, float (&o)[1]) { o[0] = *p; }
-  static __device__ __forceinline__ void store(float *p, const float (&o)[1]) { *p = o[0]; }
-};
-template <int N>
-struct Vec<uint16_t, N> {
-  typedef uint32_t V __attribute__((ext_vector_type(N / 2), aligned(2)));
-  static __device__ __forceinline__ void load(const uint16_t *p, float (&o)[N]) {
-    const V v = *reinterpret_cast<const V *>(p);
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      o[2 * i] = __uint_as_float(v[i] << 16);
-      o[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ void store(uint16_t *p, const float (&o)[N]) {
-    V v;
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) v[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
-    *reinterpret_cast<V *>(p) = v;
-  }
-};
-template <>
-struct Vec<uint16_t, 2> {
-  static __device__ __forceinline__ void load(const uint16_t *p, float (&o)[2]) {
-    o[0] = bf16_bits_to_f32(p[0]);
-    o[1] = bf16_bits_to_f32(p[1]);
-  }
-  static __device__ __forceinline__ void store(uint16_t *p, const float (&o)[2]) {
-    p[0] = f32_to_bf16_bits(o[0]);
-    p[1] = f32_to_bf16_bits(o[1]);
-  }
-};
-template <>
-struct Vec<uint16_t, 1> {
-  static __device__ __forceinline__ void load(const uint16_t *p, float (&o)[1]) { o[0] = bf16_bits_to_f32(*p); }
-  static __device__ __forceinline__ void store(uint16_t *p, const float (&o)[1]) { *p = f32_to_bf16_bits(o[0]); }
-};
-
-// Frequency i in quarter turns per position.
-__device__ __forceinline__ double quarter_turns(const BwppRotaryArgs &a, uint32_t i) {
-  double f = exp2((double)i * a.log2_step);
-  if (a.scaling == 1) f *= a.inv_factor;
-  if (a.scaling == 2) {
-    const double kept = fmin(fmax((a.turns * f - a.low) * a.inv_range, 0.0), 1.0);
-    f *= kept + (1.0 - kept) * a.inv_factor;
-  }
-  return f * 0.63661977236758134308;  // 2 / pi
-}
-
-__device__ __forceinline__ float2 cos_sin(const BwppRotaryArgs &a, double u) {
-  const double k = rint(u);
-  const float z = (float)((u - k) * 1.57079632679489661923), w = z * z;
-  const int q = (int)(int64_t)k & 3;
-  // sin z and cos z for |z| <= pi / 4
-  float s = fmaf(w, -2.50521083854417e-8f, 2.75573192239859e-6f);
-  s = fmaf(w, s, -1.98412698412698e-4f);
-  s = fmaf(w, s, 8.33333333333333e-3f);
-  s = fmaf(w, s, -0.166666666666667f);
-  s = fmaf(z * w, s, z);
-  float c = fmaf(w, -2.75573192239859e-7f, 2.48015873015873e-5f);
-  c = fmaf(w, c, -1.38888888888889e-3f);
-  c = fmaf(w, c, 4.16666666666667e-2f);
-  c = fmaf(w, c, -0.5f);
-  c = fmaf(w, c, 1.0f);
-  const float cs = q & 1 ? s : c, sn = q & 1 ? c : s;
-  return make_float2((q == 1 || q == 2 ? -cs : cs) * a.cos_scale, (q >= 2 ? -sn : sn) * a.sin_scale);
-}
 
 template <class T, bool INTER, int C>
 __device__ __forceinline__ void rotary(const BwppRotaryArgs &a) {

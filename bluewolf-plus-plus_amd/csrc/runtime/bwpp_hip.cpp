@@ -33,7 +33,8 @@ thread_local std::string g_create_error;
 
 // Code objects built by the package Makefile, all required.
 const char *const kModules[] = {"bwpp_rowops.hsaco", "bwpp_gemm.hsaco", "bwpp_attention.hsaco",
-                                 "bwpp_attention_f32.hsaco", "bwpp_attention_bwd.hsaco", "bwpp_grad.hsaco"};
+                                 "bwpp_attention_f32.hsaco", "bwpp_attention_bwd.hsaco", "bwpp_grad.hsaco",
+                                 "bwpp_cache.hsaco"};
 
 // Row-op kernels: bwpp_row_<op>_v<VPT>_w<WPR>_<f|p>, see rowops.hip.
 enum RowOpId { ROW_SOFTMAX, ROW_RMSNORM, ROW_LAYERNORM, ROW_MAX, ROW_MAXGRAD, ROW_MASK, ROW_NOPS };
@@ -141,7 +142,8 @@ struct BwppHip {
   hipFunction_t silu_grad = nullptr, softmax_grad = nullptr, rmsnorm_grad = nullptr, col_partials_sum = nullptr,
                 reduce_sum_rows = nullptr, reduce_sum_cols = nullptr, elementwise = nullptr,
                 mean_square_part = nullptr, mean_square_final = nullptr, copy_multi = nullptr;
-  std::vector<hipFunction_t> lm;  // bwpp_hip_lm_kernels
+  std::vector<hipFunction_t> lm;     // bwpp_hip_lm_kernels
+  std::vector<hipFunction_t> cache;  // bwpp_hip_cache_kernels
   // Library-owned device workspace (column partials), grown on demand and
   // freed by bwpp_hip_destroy.  Calls on one handle are stream-ordered, so
   // reuse across calls is safe.
@@ -334,6 +336,9 @@ BwppHipStatus resolve_all(BwppHip *h) {
   h->lm.resize((size_t)bwpp_hip_lm_kernel_count);
   for (int i = 0; i < bwpp_hip_lm_kernel_count; ++i)
     if ((s = resolve(h, bwpp_hip_lm_kernels[i], &h->lm[(size_t)i])) != BWPP_HIP_OK) return s;
+  h->cache.resize((size_t)bwpp_hip_cache_kernel_count);
+  for (int i = 0; i < bwpp_hip_cache_kernel_count; ++i)
+    if ((s = resolve(h, bwpp_hip_cache_kernels[i], &h->cache[(size_t)i])) != BWPP_HIP_OK) return s;
   for (int c = 0; c < kGradNCfg; ++c)
     for (int vec = 0; vec < 2; ++vec) {
       const std::string n = "_v" + std::to_string(kGradCfgs[c].vpt) + "_w" + std::to_string(kGradCfgs[c].wpr) +
@@ -2219,12 +2224,26 @@ BwppHipStatus bwpp_hip_enter(BwppHip *h) {
   return enter(h);
 }
 
-BwppHipStatus bwpp_hip_launch_lm(BwppHip *h, int index, uint64_t gx, uint32_t gy, uint32_t threads, const void *args,
-                                 uint32_t shmem) {
+namespace {
+
+BwppHipStatus launch_listed(BwppHip *h, hipFunction_t f, uint64_t gx, uint32_t gy, uint32_t threads, const void *args,
+                            uint32_t shmem) {
   if (!launchable(gx, threads))
     return fail(h, BWPP_HIP_ERR_UNSUPPORTED, "launch of %llu blocks of %u threads: 2^32 threads or more",
                 (unsigned long long)gx, threads);
-  return launch_block(h, h->lm[(size_t)index], (uint32_t)gx, gy, 1, threads, args, shmem);
+  return launch_block(h, f, (uint32_t)gx, gy, 1, threads, args, shmem);
+}
+
+}  // namespace
+
+BwppHipStatus bwpp_hip_launch_lm(BwppHip *h, int index, uint64_t gx, uint32_t gy, uint32_t threads, const void *args,
+                                 uint32_t shmem) {
+  return launch_listed(h, h->lm[(size_t)index], gx, gy, threads, args, shmem);
+}
+
+BwppHipStatus bwpp_hip_launch_cache(BwppHip *h, int index, uint64_t gx, uint32_t gy, uint32_t threads,
+                                    const void *args, uint32_t shmem) {
+  return launch_listed(h, h->cache[(size_t)index], gx, gy, threads, args, shmem);
 }
 
 BwppHipStatus bwpp_hip_take_workspace(BwppHip *h, size_t bytes, void **p) {

@@ -4,6 +4,7 @@
 // kernel; the kernels are rotary.h, resnorm.h and xent.h.
 #include "bwpp_hip.h"
 #include "internal.h"
+#include "rowset.h"
 
 #include <algorithm>
 #include <cmath>
@@ -170,6 +171,22 @@ BwppHipFault bwpp_hip_check_rotary(const BwppRotaryParams &p) {
   return {BWPP_HIP_OK, nullptr};
 }
 
+void bwpp_hip_rotary_args(const BwppRotaryParams &p, uint32_t rot, BwppRotaryArgs &a) {
+  const double base = p.base != 0.0f ? p.base : 10000.0, factor = p.factor != 0.0f ? p.factor : 1.0;
+  a.log2_step = rot ? -2.0 / rot * std::log2(base) : 0.0;
+  a.inv_factor = 1.0 / factor;
+  a.turns = p.context * 0.15915494309189533577;  // 1 / (2 pi)
+  a.low = p.low_turns;
+  a.inv_range = p.scaling == BWPP_HIP_ROTARY_SCALE_BY_PARTS ? 1.0 / ((double)p.high_turns - (double)p.low_turns) : 0.0;
+  a.cos_scale = p.magnitude != 0.0f ? p.magnitude : 1.0f;
+  a.sin_scale = a.cos_scale;
+  a.tokens = p.tokens;
+  a.q_heads = p.q_heads;
+  a.dim = p.dim;
+  a.pairs = rot / 2;
+  a.scaling = p.scaling;
+}
+
 BwppHipFault bwpp_hip_check_residual_norm(const BwppResidualNormParams &p) {
   if (p.dtype > BWPP_HIP_BF16) return invalid("unknown dtype");
   if (short_row(p.ldx, p.cols) || short_row(p.ldo, p.cols) || short_row(p.ldy, p.cols) || short_row(p.ldg, p.cols))
@@ -202,61 +219,6 @@ uint32_t cus_of(const BwppHip *h) {
 
 // ---------------------------------------------------------------- rotary
 
-// Rows of one operand of a rotary call: [batch][heads][tokens] rows of dim.
-struct RowSet {
-  const void *p;
-  uint64_t ts, hs, bs;
-  uint64_t batch, heads, tokens, dim;
-
-  // A block of row stride ld that holds the set, where there is one: axes whose
-  // strides are multiples of ld go along its rows, the others into a row.
-  bool as_block(uint64_t ld, uint64_t &rows, uint64_t &cols) const {
-    rows = 1;
-    cols = dim;
-    const uint64_t n[3] = {tokens, heads, batch}, st[3] = {ts, hs, bs};
-    for (int i = 0; i < 3; ++i) {
-      if (n[i] == 1) continue;
-      if (st[i] % ld == 0) rows += (n[i] - 1) * (st[i] / ld);
-      else cols += (n[i] - 1) * st[i];
-    }
-    return cols <= ld;
-  }
-  uint64_t span() const { return (batch - 1) * bs + (heads - 1) * hs + (tokens - 1) * ts + dim; }
-};
-
-// Whether two sets may share an element: not where they lie in blocks of one row
-// stride, a token's, head's or batch's, that share none (q and k side by side in
-// each token's row, or in each batch: heads before tokens); else by byte range.
-bool meet(const RowSet &a, const RowSet &b, uint64_t es) {
-  if (!a.p || !b.p) return false;
-  for (const uint64_t ld : {a.tokens > 1 ? a.ts : 0, a.heads > 1 ? a.hs : 0, a.batch > 1 ? a.bs : 0}) {
-    uint64_t ra, ca, rb, cb;
-    if (ld && a.as_block(ld, ra, ca) && b.as_block(ld, rb, cb) &&
-        !bwpp_hip_blocks_overlap(a.p, ra, ca, ld, b.p, rb, cb, ld, es))
-      return false;
-  }
-  return bwpp_hip_blocks_overlap(a.p, 1, a.span(), 0, b.p, 1, b.span(), 0, es);
-}
-bool same_rows(const RowSet &a, const RowSet &b) {
-  return a.p == b.p && (a.tokens == 1 || a.ts == b.ts) && (a.heads == 1 || a.hs == b.hs) &&
-         (a.batch == 1 || a.bs == b.bs);
-}
-// Whether the rows of an output are disjoint: every stride passes what lies
-// inside it, in some order of the three.
-bool disjoint_rows(const RowSet &s) {
-  struct Axis {
-    uint64_t n, st;
-  } ax[3] = {{s.tokens, s.ts}, {s.heads, s.hs}, {s.batch, s.bs}};
-  std::sort(ax, ax + 3, [](const Axis &a, const Axis &b) { return a.st < b.st; });
-  uint64_t inside = s.dim;
-  for (const Axis &a : ax) {
-    if (a.n == 1) continue;
-    if (a.st < inside) return false;
-    inside += (a.n - 1) * a.st;
-  }
-  return true;
-}
-
 BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k, const int32_t *positions, void *qo,
                      void *ko, const BwppRotaryParams &p, bool grad) {
   auto bad = [&](const char *why) { return bwpp_hip_set_error(h, BWPP_HIP_ERR_INVALID_ARG, "%s: %s", what, why); };
@@ -265,7 +227,6 @@ BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k,
   if (p.tokens == 0 || p.dim == 0 || (p.q_heads == 0 && p.k_heads == 0)) return bwpp_hip_enter(h);
   if ((p.q_heads && (!q || !qo)) || (p.k_heads && (!k || !ko))) return bad("NULL q, k or output");
   const uint32_t rot = p.rot_dim ? p.rot_dim : p.dim;
-  const double base = p.base != 0.0f ? p.base : 10000.0, factor = p.factor != 0.0f ? p.factor : 1.0;
   const uint64_t B = p.batch ? p.batch : 1, T = p.tokens, d = p.dim, heads = (uint64_t)p.q_heads + p.k_heads;
   auto rows = [&](const void *ptr, uint32_t heads, uint32_t ld, uint64_t hs, uint64_t bs) {
     RowSet r = {heads ? ptr : nullptr, ld ? ld : d, 0, 0, B, heads ? heads : 1u, T, d};
@@ -315,20 +276,10 @@ BwppHipStatus rotary(BwppHip *h, const char *what, const void *q, const void *k,
   a.qo_ts = dq.ts, a.qo_hs = dq.hs, a.qo_bs = dq.bs;
   a.ko_ts = dk.ts, a.ko_hs = dk.hs, a.ko_bs = dk.bs;
   a.pos_bs = p.pos_batch_stride;
-  a.log2_step = rot ? -2.0 / rot * std::log2(base) : 0.0;
-  a.inv_factor = 1.0 / factor;
-  a.turns = p.context * 0.15915494309189533577;  // 1 / (2 pi)
-  a.low = p.low_turns;
-  a.inv_range = p.scaling == BWPP_HIP_ROTARY_SCALE_BY_PARTS ? 1.0 / ((double)p.high_turns - (double)p.low_turns) : 0.0;
-  a.cos_scale = p.magnitude != 0.0f ? p.magnitude : 1.0f;
-  a.sin_scale = grad ? -a.cos_scale : a.cos_scale;
+  bwpp_hip_rotary_args(p, rot, a);
+  if (grad) a.sin_scale = -a.sin_scale;
   a.pos0 = p.pos_offset;
-  a.tokens = p.tokens;
   a.batch = (uint32_t)B;
-  a.q_heads = p.q_heads;
-  a.dim = p.dim;
-  a.pairs = rot / 2;
-  a.scaling = p.scaling;
   a.copy = rot < p.dim ? (sq.p && !q_in_place ? 1u : 0u) | (sk.p && !k_in_place ? 2u : 0u) : 0u;
   a.heads = (uint32_t)heads;
   const bool bf16 = p.dtype == BWPP_HIP_BF16, inter = p.layout == BWPP_HIP_ROTARY_INTERLEAVED;

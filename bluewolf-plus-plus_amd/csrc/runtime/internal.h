@@ -3,6 +3,8 @@
 
 #include "bwpp_hip.h"
 
+#include "../kargs.h"
+
 // Attention backward without the hull-based aliasing test of
 // bwpp_hip_dispatch_attention_grad: for callers that place dq / dk / dv
 // themselves (the plan executor writes them as disjoint column blocks of
@@ -69,6 +71,8 @@ struct BwppHipFault {
   const char *why;
 };
 BwppHipFault bwpp_hip_check_rotary(const BwppRotaryParams &p);
+// Sizes and rotation of a rotary call as its kernels take them.
+void bwpp_hip_rotary_args(const BwppRotaryParams &p, uint32_t rot, BwppRotaryArgs &a);
 BwppHipFault bwpp_hip_check_residual_norm(const BwppResidualNormParams &p);
 BwppHipFault bwpp_hip_check_linear_xent(const BwppLinearXentParams &p);
 
@@ -78,6 +82,12 @@ BwppHipStatus bwpp_hip_enter(BwppHip *h);
 // Launches kernel `index` of bwpp_hip_lm_kernels with one argument block.
 BwppHipStatus bwpp_hip_launch_lm(BwppHip *h, int index, uint64_t gx, uint32_t gy, uint32_t threads, const void *args,
                                  uint32_t shmem = 0);
+
+// The same for bwpp_cache.cpp (a paged cache, rules on logits).
+extern const char *const bwpp_hip_cache_kernels[];
+extern const int bwpp_hip_cache_kernel_count;
+BwppHipStatus bwpp_hip_launch_cache(BwppHip *h, int index, uint64_t gx, uint32_t gy, uint32_t threads,
+                                    const void *args, uint32_t shmem = 0);
 
 // `bytes` of the handle's workspace (OUT_OF_MEMORY while the handle's stream
 // is being recorded and the workspace would have to grow).

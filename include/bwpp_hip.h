@@ -243,6 +243,78 @@ typedef struct {
   float scale;           /* 0 = 1 */
 } BwppLinearXentParams;
 
+/* A cache of keys and values in pages, and a ragged batch of new tokens over it
+ * (no reference counterpart).  The pools of keys and values have `pages` pages of
+ * page_tokens tokens and the same strides (elements); zero strides mean contiguous
+ * [pages][heads][page_tokens][dim] (token_stride 0 = dim, head_stride 0 =
+ * page_tokens token_stride, page_stride 0 = heads head_stride).  In device memory,
+ * so that a recorded launch follows them:
+ *   table   int32 [batch][max_pages], row stride ld_table: page numbers
+ *   starts  int32 [batch + 1]: new tokens of sequence s are rows starts[s] ..
+ *           starts[s + 1] - 1 of the operands' `tokens` rows; rows before the
+ *           first and behind the last sequence are left alone
+ *   held    int32 [batch]: tokens that the cache holds before the new ones, which
+ *           take the slots behind them
+ * Slot p of a sequence lies in page table[s][p / page_tokens].  Starts and lengths
+ * are cut to the operands and the table; a slot past the table, or whose page
+ * number is outside 0 .. pages - 1 (-1: no page), does not exist: nothing is
+ * written there and no query sees it. */
+typedef struct {
+  uint32_t pages;
+  uint32_t page_tokens; /* a power of two */
+  uint32_t heads;       /* key (and value) heads */
+  uint32_t dim;         /* of a key and of a value */
+  uint32_t batch;       /* sequences, at most 2^24 */
+  uint32_t max_pages;   /* columns of the table */
+  uint32_t ld_table;    /* 0 = max_pages */
+  uint32_t tokens;      /* rows of the new tokens' operands */
+  uint32_t q_heads;     /* a multiple of heads; tokens q_heads below 2^31 */
+  uint32_t dtype;       /* BwppHipDType of every operand that is not int32 or lse */
+  uint64_t page_stride, token_stride, head_stride;
+} BwppCacheParams;
+
+/* Rows of the new tokens: zero strides mean contiguous [tokens][heads][dim]
+ * (heads: v's are k's).  The rotation is BwppRotaryParams', fields as there. */
+typedef struct {
+  BwppCacheParams cache;
+  uint32_t ldq, ldk, ldv, ldqo; /* token strides; 0 = heads * dim */
+  uint64_t q_head_stride, k_head_stride, v_head_stride, qo_head_stride; /* 0 = dim */
+  uint32_t no_rotation; /* 1: q and k as they are */
+  uint32_t rot_dim;     /* 0 = dim */
+  uint32_t layout;
+  uint32_t scaling;
+  float base;
+  float factor;
+  float low_turns, high_turns;
+  uint32_t context;
+  float magnitude;
+} BwppCacheAppendParams;
+
+typedef struct {
+  BwppCacheParams cache; /* dim at most 256 */
+  uint32_t ldq, ldo;     /* token strides; 0 = q_heads * dim */
+  uint64_t q_head_stride, o_head_stride; /* 0 = dim */
+  uint32_t mask_words;   /* 32-bit words a row of the mask */
+  float scale;           /* 0 = 1 */
+} BwppCacheAttentionParams;
+
+typedef struct {
+  BwppCacheParams cache; /* tokens and q_heads are not read */
+  uint32_t max_kept;     /* columns of kept */
+  uint32_t ld_kept;      /* 0 = max_kept */
+} BwppCacheKeepParams;
+
+/* Rules for the next token on rows of logits (no reference counterpart). */
+typedef struct {
+  uint32_t rows;
+  uint32_t vocab;
+  uint32_t ldx, ldy;  /* 0 = vocab */
+  uint32_t dtype_x, dtype_y; /* BwppHipDType, 0 = F32 */
+  uint32_t history;   /* tokens of the history, all rows together */
+  uint32_t ld_bias;   /* 0: one row for all */
+  uint32_t ld_mask;   /* 32-bit words; 0: one row for all */
+} BwppLogitRulesParams;
+
 typedef struct BwppHip BwppHip;
 
 /* ---- handle ---- */
@@ -677,6 +749,61 @@ BwppHipStatus bwpp_hip_dispatch_linear_xent(BwppHip *h, const void *x, const voi
 BwppHipStatus bwpp_hip_dispatch_linear_xent_grad(BwppHip *h, const void *x, const void *w, const int32_t *targets,
                                                  const float *lse, const float *dloss, void *dx, void *dw,
                                                  BwppLinearXentParams params);
+
+/* ---- a paged cache, and the next token ----
+ * Operands and lengths of BwppCacheParams; no call reads lengths on the host.
+ * With no tokens or no sequences operands may be NULL.  No reference
+ * counterparts. */
+
+/* Appends: k and v go to their slots, k and q with rotary positions, q to qo (may
+ * be q with the same strides: in place; NULL with q_heads 0).  A token's position
+ * is positions[row] (int32 [tokens]) or, NULL, its slot.  The rows of a pool must
+ * not overlap, outputs must not meet inputs or each other otherwise (ALIAS).  Two
+ * sequences with a page in common that write the same slot of it leave either's
+ * rows. */
+BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *q, const void *k, const void *v,
+                                             const int32_t *positions, const int32_t *table, const int32_t *starts,
+                                             const int32_t *held, void *qo, void *k_cache, void *v_cache,
+                                             BwppCacheAppendParams params);
+
+/* Attention of the new tokens, whose keys are in the cache already: token i of a
+ * sequence sees the held tokens and those new tokens j whose bit j % 32 of word
+ * j / 32 of its mask row (uint32 [tokens][mask_words]; bits past the row: not
+ * seen) is set, or, without a mask, j <= i.  Query head h reads key head h /
+ * (q_heads / heads).  o = softmax(scale q k) v; lse (may be NULL) [tokens][q_heads]
+ * fp32 is the natural log-sum-exp.  A token that sees nothing gets 0 and -inf.
+ * What lies in slots that a token does not see has no part in it, infinities and
+ * NaN included.  Sums and probabilities are held in fp32.  Workspace: for
+ * 2 (bf16 of some dims: 1) partial results a block of the device, at most 128
+ * rows of dim + 2 floats each. */
+BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const void *q, const void *k_cache, const void *v_cache,
+                                                const int32_t *table, const int32_t *starts, const int32_t *held,
+                                                const uint32_t *mask, void *o, float *lse,
+                                                BwppCacheAttentionParams params);
+
+/* After a tree of drafts is verified: slot held[s] + i takes the keys and values of
+ * slot held[s] + kept[s][i] for i < counts[s] (int32 [batch], cut to max_kept), as
+ * if all were read before any is written.  kept (int32 [batch][max_kept]) must not
+ * descend where a row has more than 16 entries; entries below 0 or past the table
+ * move nothing.  held itself is the caller's to raise by counts. */
+BwppHipStatus bwpp_hip_dispatch_cache_keep(BwppHip *h, void *k_cache, void *v_cache, const int32_t *table,
+                                           const int32_t *held, const int32_t *kept, const int32_t *counts,
+                                           BwppCacheKeepParams params);
+
+/* y = x under the rules, row by row, in fp32.  Row r's history is history[starts[r]
+ * .. starts[r + 1] - 1] (int32 tokens; those outside the vocabulary do not count),
+ * its first prompt[r] (NULL: 0) given, the rest written.  In this order:
+ *   z > 0 ? z / repetition[r] : z repetition[r]   where the token occurs
+ *   z - (frequency[r] count + presence[r])        where it was written count times
+ *   z + bias                                      fp32, row r of it or its one row
+ *   -inf                                          where its mask bit (bit v % 32 of
+ *                                                 word v / 32) is 0
+ * NULL: without that rule.  y may be x (same dtype and stride), and must not meet
+ * another operand otherwise (ALIAS). */
+BwppHipStatus bwpp_hip_dispatch_logit_rules(BwppHip *h, const void *x, const int32_t *history, const int32_t *starts,
+                                            const int32_t *prompt, const float *repetition, const float *presence,
+                                            const float *frequency, const float *bias, const uint32_t *mask, void *y,
+                                            BwppLogitRulesParams params);
 
 /* ---- launch plans (compiled graphs) ----
  *
