@@ -32,6 +32,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 namespace kv {
 
+constexpr uint32_t kThreads = 256;
+
 // Four elements from column c of a row of `dim`, zeros past it.
 template <class T, bool VEC>
 __device__ __forceinline__ void load4(const T *row, uint32_t c, uint32_t dim, float (&o)[4]) {
@@ -87,7 +89,7 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
   const BwppCacheArgs &c = a.c;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i16 = lane & 15u, grp = lane >> 4;
   const uint32_t D = c.dim, g = a.group, Dp = (D + 3u) & ~3u;
-  find_share<kRows, kUnit>(a, blockIdx.x, &share, wave_sums);
+  find_share<kRows, kUnit, kThreads>(a, blockIdx.x, &share, wave_sums);
   const Place to = share.to;
   Place at = share.from;
   const uint32_t pmask = (1u << c.page_shift) - 1u;
@@ -328,7 +330,7 @@ __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
   __shared__ Place item;
   __shared__ uint32_t last;  // block with the item's last part; 0: nothing to join
   const BwppCacheArgs &c = a.c;
-  const Costs<kRows, kUnit> costs(a, wave_sums);
+  const Costs<kRows, kUnit, kThreads> costs(a, wave_sums);
   const uint32_t G = sharers(a, costs.total), b = blockIdx.x + 1;
   if (b >= G) return;
   if (threadIdx.x == 0) last = 0;
@@ -394,3 +396,5 @@ BWPP_JOIN(f32, float, 16, 64)
 BWPP_JOIN(f32_rows, float, 64, 64)
 BWPP_JOIN(bf16, uint16_t, 16, 64)
 BWPP_JOIN(bf16_rows, uint16_t, 64, 64)
+BWPP_JOIN(bf16_32, uint16_t, 32, 64)
+BWPP_JOIN(bf16_128, uint16_t, 128, 64)

@@ -1,0 +1,574 @@
+// Attention over a paged cache for bf16 rows of 16-byte chunks, head dims of
+// multiples of 16, on the bf16 matrix cores: the scheme of attention.hip
+// (S^T = K Q^T, softmax on the accumulator registers, O^T += V^T P^T with V
+// read transposed from LDS) over pages.
+//
+// A wave holds 32 query rows, which are the tokens of a tile times the query
+// heads of one key head, so a key is read once for all of them.
+//
+// Few rows (attend_few): reading K and V once bounds it.  A block of NW waves
+// has one tile of 32 rows; every wave streams key tiles of 32 of its own
+// (every NW-th of the block's) through a DMA ring of its own, and the waves'
+// triples meet in LDS at the end of an item.
+//
+// More rows (attend_rows): the matrix products bound it.  Each of a block's
+// four waves has 32 rows of a tile of 128, and key tiles of 64 come through a
+// two-stage ring that all four read.
+//
+// Page numbers of an item's keys are copied to LDS, 1024 at a time, before its
+// tiles: no load of the compiler's is outstanding beside the DMA, whose
+// completion is counted by hand.  Where a key tile lies in one page its base
+// is a scalar and the lanes' offsets in the tile never change; smaller pages
+// take an address per lane and row.
+#pragma once
+
+#include "attention_common.h"
+#include "kv_cache.h"
+#include "kv_schedule.h"
+#include "../kargs.h"
+
+namespace kv {
+
+__device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// A tile of key or value rows in LDS: dense rows of D / 8 chunks of 16 bytes,
+// chunk c of row r at c ^ swz(r).
+template <int D>
+struct Rows {
+  static constexpr uint32_t kSlots = D / 8, kRowB = 16 * kSlots;
+  static constexpr uint32_t kPow = kSlots & (~kSlots + 1);         // chunks that may change places
+  static constexpr uint32_t kMask = (kPow < 16 ? kPow : 16) - 1;
+  static constexpr uint32_t kShift = kPow >= 16 ? 0 : kPow == 8 ? 1 : kPow == 4 ? 2 : 3;  // rows that differ by their address
+  // The 16 rows of a quarter-wave's ds_read_b128 fall on distinct bank groups.
+  static __device__ __forceinline__ uint32_t k_swz(uint32_t r) { return (r >> kShift) & kMask; }
+  // Rows of a half-wave's transposing reads likewise; unchanged by steps of 8 rows.
+  static __device__ __forceinline__ uint32_t v_swz(uint32_t r) {
+    return kSlots % 16 == 0 ? 4u * (r & 3u) : kSlots % 8 == 0 ? 4u * ((r >> 1) & 1u) : 0u;
+  }
+};
+
+// A wave's 32 query rows and what it has of their results.  Lane l has row
+// l % 32; of a block of 32 keys it has the scores of keys 8 (r >> 2) + 4 (l >>
+// 5) + (r & 3) in register r.
+template <int D, int KB>
+struct Wave32 {
+  using R = Rows<D>;
+  static constexpr int KS = D / 16, DB = (D + 31) / 32, kKeys = 32 * KB;
+  static constexpr uint32_t kTile = kKeys * R::kRowB, kStage = 2 * kTile;
+  bf16x8_t q[KS];
+  f32x16_t o[DB];
+  float m, l, c;
+  uint32_t lq, lh, koff[KS], voff[DB];
+
+  __device__ __forceinline__ void place() {
+    const uint32_t lane = threadIdx.x & 63u, grp = lane >> 4, L = lane & 15u;
+    lq = lane & 31u;
+    lh = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) koff[ks] = lq * R::kRowB + 16u * ((2u * ks + lh) ^ R::k_swz(lq));
+    const uint32_t kbase = 4u * (grp >> 1) + (L >> 2);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const uint32_t col = 32u * d + 16u * (grp & 1u) + 4u * (L & 3u);
+      voff[d] = kTile + kbase * R::kRowB + 16u * ((col >> 3) ^ R::v_swz(kbase)) + (col & 7u) * 2u;
+    }
+  }
+  // Starts an item: the query row at Q (any valid row where the lane has none).
+  __device__ __forceinline__ void start(const uint16_t *Q, float scale_log2, uint32_t flip) {
+    c = scale_log2;
+    const uint32_t sign = flip ? 0x80008000u : 0u;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint4 v = *reinterpret_cast<const uint4 *>(Q + 16 * ks + 8 * lh);
+      v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
+      q[ks] = __builtin_bit_cast(bf16x8_t, v);
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    m = -INFINITY;
+    l = 0.0f;
+  }
+
+  // One key tile at `st`.  MASK: vis has bit k of word kb where this lane's row
+  // sees key 32 kb + k; elsewhere all are seen.
+  template <bool MASK>
+  __device__ __forceinline__ void tile(const unsigned char *st, const uint32_t (&vis)[KB]) {
+    f32x16_t s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4 *>(st + koff[ks] + 32u * kb * R::kRowB)), q[ks],
+            s[kb], 0, 0, 0);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const uint32_t w = MASK ? vis[kb] >> (4u * lh) : 0u;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (MASK) s[kb][r] = w >> (8 * (r >> 2) + (r & 3)) & 1u ? s[kb][r] : -INFINITY;
+        mx = fmaxf(mx, s[kb][r]);
+      }
+    }
+    {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * c;
+    }
+    float alpha = 1.0f;
+    if (mx > m + kLazy) {
+      alpha = __builtin_amdgcn_exp2f(m - mx);  // 0 when m is -inf
+      m = mx;
+    }
+    const float use = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, -use));
+        s[kb][r] = p;
+        sum += p;
+      }
+    l = l * alpha + sum;  // of this lane's keys; lane ^ 32 has the others
+    if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+    bool odd = false;  // infinite or NaN values: 0 times those would reach rows that do not see them
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int kq = 0; kq < 2; ++kq) {
+        bf16x8_t ph, pl;
+        split_bf16x8(&s[kb], 8 * kq, ph, pl);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const unsigned char *p = st + voff[d] + (32u * kb + 16u * kq) * R::kRowB;
+          const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)p);
+          const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)(p + 8u * R::kRowB));
+          v8s_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          if (MASK) {
+            const u16x2_t big = max_abs_bf16(u16x2_t{0, 0}, v);
+            if (__ballot(big[0] >= 0x7f80u || big[1] >= 0x7f80u)) {
+              odd = true;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = (v[e] & 0x7f80) == 0x7f80 ? (short)0 : v[e];
+            }
+          }
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), ph, o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), pl, o[d], 0, 0, 0);
+        }
+      }
+    if constexpr (MASK) {
+      if (odd) {  // wave-uniform: the values left out, key by key
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+          for (uint32_t k = 0; k < 32; ++k) {
+            float mine = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mine = (uint32_t)r == 4u * (k >> 3) + (k & 3u) ? s[kb][r] : mine;
+            const float pk = __shfl(mine, (int)(lq + 32u * (k >> 2 & 1u)), 64);
+            if (!(vis[kb] >> k & 1u)) continue;
+            const uint32_t row = 32u * kb + k;
+            const unsigned char *vr = st + kTile + row * R::kRowB;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                if (r % 4 == 0) asm volatile("" ::: "memory");  // few reads at a time: registers
+                const uint32_t col = 32u * d + 8u * (r >> 2) + 4u * lh + (r & 3);
+                if (col >= (uint32_t)D) continue;
+                const float v = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(
+                    vr + 16u * ((col >> 3) ^ R::v_swz(row)) + 2u * (col & 7u)));
+                if (!(fabsf(v) < INFINITY)) o[d][r] += pk * v;
+              }
+          }
+      }
+    }
+  }
+  // The row's whole sum in both of its lanes.
+  __device__ __forceinline__ void finish() {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+};
+
+// 32 bits: which of the sequence's new tokens j0 .. j0 + 31 its token i sees
+// (those below zero: none).
+__device__ __forceinline__ uint32_t mask_bits32(const BwppCacheAttnArgs &a, uint32_t first, uint32_t i, int64_t j0) {
+  if (!a.mask) {
+    const int64_t seen = (int64_t)i + 1 - j0;
+    return seen <= 0 ? 0u : seen >= 32 ? ~0u : (1u << seen) - 1u;
+  }
+  uint64_t two = 0;
+  const uint32_t *row = a.mask + (uint64_t)(first + i) * a.mask_words;
+  const int64_t w = j0 >> 5;
+  if (w >= 0 && w < (int64_t)a.mask_words) two = row[w];
+  if (w + 1 >= 0 && w + 1 < (int64_t)a.mask_words) two |= (uint64_t)row[w + 1] << 32;
+  return (uint32_t)(two >> (j0 & 31));
+}
+
+constexpr uint32_t kPages = 1024;          // page numbers in LDS
+constexpr uint32_t kNoPage = 0x80000000u;  // outside the pool: page 0 is read, and not seen
+
+// An item as a wave sees it.
+struct Item {
+  Seq q;
+  uint32_t s, head, tile, kbeg, kend, R;
+  bool whole;
+};
+
+// Page numbers of the keys from k on, as many as LDS holds; returns the end of
+// these keys (a multiple of the tiles, or kend) and whether some have no page.
+// Every thread of the block calls it.
+template <uint32_t THREADS>
+__device__ __forceinline__ uint32_t load_pages(const BwppCacheArgs &c, const Item &it, uint32_t k, uint32_t *pages, bool &bad) {
+  const uint32_t first = k >> c.page_shift, n = min(kPages, ((it.kend - 1) >> c.page_shift) - first + 1);
+  const int32_t *table = c.table + (uint64_t)it.s * c.ld_table + first;
+  int none = 0;
+  __syncthreads();  // done with the last ones
+  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+    const uint32_t p = (uint32_t)table[i];
+    none |= p >= c.pages;
+    pages[i] = p < c.pages ? p : kNoPage;
+  }
+  bad = __syncthreads_or(none) != 0;
+  const uint64_t end = (uint64_t)(first + n) << c.page_shift;
+  return (uint32_t)min(end, (uint64_t)it.kend);
+}
+
+// Which of the keys k0 .. k0 + 31 lie in a page (of those below kend), the same in every lane.
+__device__ __forceinline__ uint32_t keys_with_page(const BwppCacheArgs &c, const Item &it, uint32_t k0, uint32_t first,
+                                                   const uint32_t *pages) {
+  const uint32_t k = k0 + (threadIdx.x & 31u);
+  const bool ok = k < it.kend && !(pages[(min(k, it.kend - 1) >> c.page_shift) - first] & kNoPage);
+  return (uint32_t)__ballot(ok);
+}
+
+// Rows of keys and values from their pages to LDS: one wave's share (every
+// STEP-th from `from` on) of the DMA instructions of a tile of KEYS keys.
+template <int D, int KEYS, int FROM_WAVES>
+struct Fetch {
+  using R = Rows<D>;
+  static constexpr uint32_t kDma = KEYS * R::kSlots / 64, kMine = (kDma + FROM_WAVES - 1) / FROM_WAVES;
+  static constexpr uint32_t kTile = KEYS * R::kRowB;
+  const uint16_t *K, *V;  // the item's key head
+  uint32_t koff[kMine], voff[kMine];
+  uint32_t wave;          // of FROM_WAVES that share the tile
+
+  static __device__ __forceinline__ uint32_t slot(uint32_t i, uint32_t w) { return (i * FROM_WAVES + w) * 64u + (threadIdx.x & 63u); }
+  __device__ __forceinline__ void place(const BwppCacheArgs &c, uint32_t w) {
+    wave = w;
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+      const uint32_t q = slot(i, w), r = q / R::kSlots, pc = q % R::kSlots;
+      koff[i] = 2u * (r * (uint32_t)c.tok_s + 8u * (pc ^ R::k_swz(r)));
+      voff[i] = 2u * (r * (uint32_t)c.tok_s + 8u * (pc ^ R::v_swz(r)));
+    }
+  }
+  __device__ __forceinline__ void issue(const BwppCacheArgs &c, const Item &it, uint32_t k0, uint32_t first,
+                                        const uint32_t *pages, uint32_t lds) const {
+    const uint32_t pmask = (1u << c.page_shift) - 1u, n = min((uint32_t)KEYS, it.kend - k0);
+    if (pmask + 1u >= (uint32_t)KEYS) {
+      const uint32_t page = uni(pages[(k0 >> c.page_shift) - first]) & ~kNoPage;
+      const uint64_t base = page * c.page_s + (uint64_t)(k0 & pmask) * c.tok_s;
+      if (n == (uint32_t)KEYS) {
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+          if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
+          g2lds16_so(K + base, koff[i], lds + (i * FROM_WAVES + wave) * 1024u);
+          g2lds16_so(V + base, voff[i], lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+        }
+      } else {  // rows past the last key re-read it
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+          if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
+          const uint32_t r = slot(i, wave) / R::kSlots, back = r < n ? 0u : 2u * (r - (n - 1)) * (uint32_t)c.tok_s;
+          g2lds16_so(K + base, koff[i] - back, lds + (i * FROM_WAVES + wave) * 1024u);
+          g2lds16_so(V + base, voff[i] - back, lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kMine; ++i) {
+        if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
+        const uint32_t r = slot(i, wave) / R::kSlots, key = k0 + min(r, n - 1);
+        const uint32_t page = pages[(key >> c.page_shift) - first] & ~kNoPage;
+        // less the row's offset, which koff and voff have
+        const uint64_t row = (uint64_t)page * (uint32_t)c.page_s + (uint64_t)(key & pmask) * (uint32_t)c.tok_s;
+        const uint32_t mine = 2u * r * (uint32_t)c.tok_s;
+        g2lds16_v(reinterpret_cast<const char *>(K + row) + (koff[i] - mine), lds + (i * FROM_WAVES + wave) * 1024u);
+        g2lds16_v(reinterpret_cast<const char *>(V + row) + (voff[i] - mine), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ float4 scaled(const float4 &t, float f) { return make_float4(t.x * f, t.y * f, t.z * f, t.w * f); }
+
+// Four columns of a row of the tile: to the output or, of a part, to its slot.
+template <int D, uint32_t ROWS>
+__device__ __forceinline__ void put(const BwppCacheAttnArgs &a, const Item &it, uint32_t slot, uint32_t row, uint32_t col,
+                                    const float4 &t, float m, float l, bool head) {
+  const uint32_t rr = it.tile * ROWS + row;
+  if (rr >= it.R) return;
+  if (!it.whole) {
+    const uint64_t sr = (uint64_t)slot * ROWS + row;
+    *reinterpret_cast<float4 *>(a.part_o + sr * D + col) = t;
+    if (head) *reinterpret_cast<float2 *>(a.part_ml + 2 * sr) = make_float2(m, l);
+    return;
+  }
+  const uint64_t tok = it.q.first + rr / a.group, hh = it.head * a.group + rr % a.group;
+  const float4 u = scaled(t, l == 0.0f ? 0.0f : 1.0f / l);
+  *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.o) + tok * a.o_ts + hh * a.o_hs + col) =
+      make_uint2(pack_bf16x2(u.x, u.y), pack_bf16x2(u.z, u.w));
+  if (head && a.lse)
+    a.lse[tok * (uint64_t)(a.c.heads * a.group) + hh] = l == 0.0f ? -INFINITY : lse_of(m == -INFINITY ? 0.0f : m, l);
+}
+
+template <int D, int KB>
+__device__ __forceinline__ const uint16_t *query_row(const BwppCacheAttnArgs &a, const Item &it, uint32_t row, uint32_t &tok) {
+  const uint32_t r = min(row, it.R - 1u);
+  tok = r / a.group;
+  return static_cast<const uint16_t *>(a.q) + (uint64_t)(it.q.first + tok) * a.q_ts +
+         (uint64_t)(it.head * a.group + r % a.group) * a.q_hs;
+}
+
+// Walks a block's share: f(item, slot of its part).
+template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS, class F>
+__device__ __forceinline__ void for_items(const BwppCacheAttnArgs &a, F f) {
+  typedef Work<ROWS, UNIT> W;
+  __shared__ uint64_t wave_sums[THREADS / 64];
+  __shared__ Share share;
+  const uint32_t b = blockIdx.x;
+  find_share<ROWS, UNIT, THREADS>(a, b, &share, wave_sums);
+  Place at = {uni(share.from.s), uni(share.from.head), uni(share.from.tile), uni(share.from.unit)};
+  const Place to = {uni(share.to.s), uni(share.to.head), uni(share.to.tile), uni(share.to.unit)};
+  Item it = {};
+  auto sequence = [&]() {
+    const Seq q = seq_at(a.c, at.s);
+    it.q = {uni(q.first), uni(q.n), uni(q.held)};
+    it.s = at.s;
+    it.R = it.q.n * a.group;
+  };
+  if (at.s < a.c.batch) sequence();
+  // A part of an item that began in another block is written even if it has no
+  // keys: the join reads it.
+  bool part = at.unit != 0;
+  for (; part || earlier(at, to); part = false) {
+    const bool same = at.s == to.s && at.head == to.head && at.tile == to.tile;
+    const uint32_t keys = W::keys(a, it.q, at.tile), total = (keys + UNIT - 1) / UNIT, u1 = same ? to.unit : total;
+    it.head = at.head;
+    it.tile = at.tile;
+    it.whole = at.unit == 0 && u1 == total;
+    it.kbeg = at.unit * UNIT;
+    it.kend = min(u1 * UNIT, keys);
+    f(it, 2u * b + (at.unit == 0 ? 1u : 0u));
+    at.unit = 0;
+    if (++at.tile >= W::tiles(it.q, a.group)) {
+      at.tile = 0;
+      if (++at.head >= a.c.heads) {
+        at.head = 0;
+        do {
+          ++at.s;
+          if (at.s >= a.c.batch) break;
+          sequence();
+        } while (it.q.n == 0);
+      }
+    }
+  }
+}
+
+template <int D, int NW>
+__device__ __forceinline__ void attend_few(const BwppCacheAttnArgs &a) {
+  typedef Wave32<D, 1> W;
+  typedef Fetch<D, 32, 1> F;
+  constexpr uint32_t kStage = W::kStage, kStages = kStage * 3 <= 32768 ? 32768 / kStage : 2, kDma = 2 * F::kDma;
+  constexpr uint32_t kRing = kStages * kStage, kCld = D + 4, kMerge = NW * 32 * kCld * 4;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[(NW * kRing > kMerge ? NW * kRing : kMerge) + 64];
+  __shared__ uint32_t pages[kPages];
+  __shared__ float mls[NW][32][2];
+  const BwppCacheArgs &c = a.c;
+  const uint32_t wave = uni(threadIdx.x >> 6);
+  unsigned char *ring = smem + wave * kRing;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)ring;
+  W w;
+  w.place();
+  F fetch;
+  fetch.place(c, 0);
+
+  for_items<32, 64, 64 * NW>(a, [&](const Item &it, uint32_t slot) {
+    uint32_t tok;
+    const uint16_t *Q = query_row<D, 1>(a, it, it.tile * 32u + w.lq, tok);
+    w.start(Q, a.scale_log2, a.flip);
+    fetch.K = static_cast<const uint16_t *>(c.k) + (uint64_t)it.head * c.head_s;
+    fetch.V = static_cast<const uint16_t *>(c.v) + (uint64_t)it.head * c.head_s;
+    for (uint32_t seg = it.kbeg; seg < it.kend;) {
+      bool bad;
+      const uint32_t end = uni(load_pages<64 * NW>(c, it, seg, pages, bad)), first = seg >> c.page_shift;
+      wait_vmcnt<0>();  // no load of the compiler's outstanding beside the DMA
+      const uint32_t ntile = (end - seg + 31u) / 32u, mine = ntile > wave ? (ntile - wave + NW - 1) / NW : 0u;
+      auto key0 = [&](uint32_t j) { return seg + 32u * (NW * j + wave); };
+      auto issue = [&](uint32_t j) { fetch.issue(c, it, key0(j), first, pages, lds0 + (j % kStages) * kStage); };
+#pragma unroll
+      for (uint32_t j = 0; j < kStages - 1; ++j)
+        if (j < mine) issue(j);
+      for (uint32_t j = 0; j < mine; ++j) {
+        const uint32_t k0 = key0(j), younger = min(mine - 1 - j, kStages - 2);
+        if (kStages >= 4 && younger >= 2) wait_vmcnt<(kStages >= 4 ? 2 * kDma : 0)>();
+        else if (kStages >= 3 && younger >= 1) wait_vmcnt<(kStages >= 3 ? kDma : 0)>();
+        else wait_vmcnt<0>();
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): done reading the stage that is refilled now
+        if (j + kStages - 1 < mine) issue(j + kStages - 1);
+        const unsigned char *st = ring + uni((j % kStages) * kStage);
+        uint32_t vis[1] = {~0u};
+        if (bad || k0 + 32u > it.kend || k0 + 32u > it.q.held) {
+          if (k0 + 32u > it.q.held) {
+            vis[0] = mask_bits32(a, it.q.first, tok, (int64_t)k0 - (int64_t)it.q.held);
+            if (k0 < it.q.held) vis[0] |= (1u << (it.q.held - k0)) - 1u;  // fewer than 32
+            wait_vmcnt<0>();  // the mask's loads
+          }
+          vis[0] &= keys_with_page(c, it, k0, first, pages);
+          w.template tile<true>(st, vis);
+        } else {
+          w.template tile<false>(st, vis);
+        }
+      }
+      seg = end;
+    }
+    w.finish();
+    // The waves' triples: O (this lane's row, column 32 d + 8 (r >> 2) + 4 lh +
+    // (r & 3)) and (offset, sum).
+    __syncthreads();
+    float *os = reinterpret_cast<float *>(smem) + wave * (32 * kCld);
+#pragma unroll
+    for (int d = 0; d < W::DB; ++d)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        if (32 * d + 8 * q4 + 4 * (int)w.lh < D)
+          *reinterpret_cast<float4 *>(os + w.lq * kCld + 32 * d + 8 * q4 + 4 * (int)w.lh) =
+              make_float4(w.o[d][4 * q4], w.o[d][4 * q4 + 1], w.o[d][4 * q4 + 2], w.o[d][4 * q4 + 3]);
+    if (w.lh == 0) {
+      mls[wave][w.lq][0] = w.m;
+      mls[wave][w.lq][1] = w.l;
+    }
+    __syncthreads();
+    const uint32_t rows = min(32u, it.R - it.tile * 32u);
+    for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += 64 * NW) {
+      const uint32_t row = i / (D / 4), d4 = 4u * (i % (D / 4));
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int v = 0; v < NW; ++v) m = fmaxf(m, mls[v][row][0]);
+      float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int v = 0; v < NW; ++v) {
+        const float mw = mls[v][row][0];
+        // no key seen (offset -inf): sums of 0 (or NaN, kept)
+        const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+        const float4 u = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem) + (v * 32 + row) * kCld + d4);
+        l += mls[v][row][1] * f;
+        t.x += u.x * f, t.y += u.y * f, t.z += u.z * f, t.w += u.w * f;
+      }
+      put<D, 32>(a, it, slot, row, d4, t, m, l, d4 == 0);
+    }
+    __syncthreads();  // before the rings are filled again
+  });
+}
+
+template <int D>
+__device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
+  constexpr int NW = 4, KB = 2;
+  typedef Wave32<D, KB> W;
+  typedef Fetch<D, 32 * KB, NW> F;
+  constexpr uint32_t kStage = W::kStage;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * kStage + 64];
+  __shared__ uint32_t pages[kPages];
+  const BwppCacheArgs &c = a.c;
+  const uint32_t wave = uni(threadIdx.x >> 6);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
+  W w;
+  w.place();
+  F fetch;
+  fetch.place(c, wave);
+
+  for_items<128, 64, 64 * NW>(a, [&](const Item &it, uint32_t slot) {
+    uint32_t tok;
+    const uint32_t row0 = it.tile * 128u + 32u * wave;
+    const uint16_t *Q = query_row<D, KB>(a, it, row0 + w.lq, tok);
+    w.start(Q, a.scale_log2, a.flip);
+    fetch.K = static_cast<const uint16_t *>(c.k) + (uint64_t)it.head * c.head_s;
+    fetch.V = static_cast<const uint16_t *>(c.v) + (uint64_t)it.head * c.head_s;
+    // Keys below `all` are seen by all of the wave's rows, from `none` on by none.
+    const uint32_t t0 = min(row0, it.R - 1u) / a.group, t1 = min(row0 + 31u, it.R - 1u) / a.group;
+    const uint32_t all = a.mask ? it.q.held : it.q.held + t0 + 1u;
+    const uint32_t none = row0 >= it.R ? 0u : a.mask ? it.kend : min(it.kend, it.q.held + t1 + 1u);
+    for (uint32_t seg = it.kbeg; seg < it.kend;) {
+      bool bad;
+      const uint32_t end = uni(load_pages<64 * NW>(c, it, seg, pages, bad)), first = seg >> c.page_shift;
+      wait_vmcnt<0>();  // no load of the compiler's outstanding beside the DMA
+      const uint32_t ntile = (end - seg + 63u) / 64u;
+      fetch.issue(c, it, seg, first, pages, lds0);
+      for (uint32_t j = 0; j < ntile; ++j) {
+        const uint32_t k0 = seg + 64u * j;
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (j + 1 < ntile) fetch.issue(c, it, k0 + 64u, first, pages, lds0 + ((j + 1) & 1u) * kStage);
+        const unsigned char *st = smem + uni((j & 1u) * kStage);
+        if (k0 >= none) continue;
+        uint32_t vis[KB] = {~0u, ~0u};
+        if (bad || k0 + 64u > it.kend || k0 + 64u > all) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            const uint32_t k = k0 + 32u * kb;
+            if (k + 32u > it.q.held) {
+              vis[kb] = mask_bits32(a, it.q.first, tok, (int64_t)k - (int64_t)it.q.held);
+              if (k < it.q.held) vis[kb] |= (1u << (it.q.held - k)) - 1u;  // fewer than 32
+            }
+            vis[kb] &= keys_with_page(c, it, k, first, pages);
+          }
+          w.template tile<true>(st, vis);
+        } else {
+          w.template tile<false>(st, vis);
+        }
+      }
+      seg = end;
+      // (the next pages' first barrier comes before any stage is filled again)
+    }
+    w.finish();
+#pragma unroll
+    for (int d = 0; d < W::DB; ++d)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const uint32_t col = 32u * d + 8u * q4 + 4u * w.lh;
+        if (col < (uint32_t)D)
+          put<D, 128>(a, it, slot, 32u * wave + w.lq, col,
+                      make_float4(w.o[d][4 * q4], w.o[d][4 * q4 + 1], w.o[d][4 * q4 + 2], w.o[d][4 * q4 + 3]), w.m, w.l,
+                      d == 0 && q4 == 0 && w.lh == 0);
+      }
+  });
+}
+
+}  // namespace kv
+
+#define BWPP_ATTEND_BF16(D)                                                                                        \
+  extern "C" __global__ __launch_bounds__(128) void bwpp_cache_attend_few_d##D(const BwppCacheAttnArgs a) {         \
+    kv::attend_few<D, 2>(a);                                                                                       \
+  }                                                                                                                \
+  extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void bwpp_cache_attend_rows_d##D(const BwppCacheAttnArgs a) { \
+    kv::attend_rows<D>(a);                                                                                         \
+  }
+BWPP_ATTEND_BF16(64)
+BWPP_ATTEND_BF16(80)
+BWPP_ATTEND_BF16(96)
+BWPP_ATTEND_BF16(128)
+BWPP_ATTEND_BF16(160)
+BWPP_ATTEND_BF16(192)
+BWPP_ATTEND_BF16(256)

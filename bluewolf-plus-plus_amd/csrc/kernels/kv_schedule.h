@@ -23,7 +23,6 @@ namespace kv {
 
 constexpr uint32_t kItem = 96;      // keys that an item costs by itself
 constexpr uint32_t kLeast = 192;    // a block's share is at least as many keys
-constexpr uint32_t kThreads = 256;  // of the blocks that find their shares
 
 // A place in the order of the work.
 struct Place {
@@ -81,7 +80,7 @@ struct Work {
 
 // Costs of the sequences that this thread adds up (a run of `per`), the costs
 // before them, and the total.
-template <uint32_t ROWS, uint32_t UNIT>
+template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
 struct Costs {
   uint32_t s0, s1;
   uint64_t first, total;
@@ -90,7 +89,7 @@ struct Costs {
     return a.c.heads * Work<ROWS, UNIT>::before(q, a.group, Work<ROWS, UNIT>::tiles(q, a.group));
   }
   __device__ __forceinline__ Costs(const BwppCacheAttnArgs &a, uint64_t *wave_sums) {
-    const uint32_t per = (a.c.batch + kThreads - 1) / kThreads;
+    const uint32_t per = (a.c.batch + THREADS - 1) / THREADS;
     s0 = min(threadIdx.x * per, a.c.batch);
     s1 = min(s0 + per, a.c.batch);
     uint64_t mine = 0;
@@ -107,7 +106,7 @@ struct Costs {
     first = sum - mine;
     total = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kThreads / 64; ++w) {
+    for (uint32_t w = 0; w < THREADS / 64; ++w) {
       if (w < wave) first += wave_sums[w];
       total += wave_sums[w];
     }
@@ -136,9 +135,9 @@ __device__ __forceinline__ uint32_t sharers(const BwppCacheAttnArgs &a, uint64_t
 }
 
 // The share of block b, the same in every thread (`share` in LDS).
-template <uint32_t ROWS, uint32_t UNIT>
+template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
 __device__ __forceinline__ void find_share(const BwppCacheAttnArgs &a, uint32_t b, Share *share, uint64_t *wave_sums) {
-  const Costs<ROWS, UNIT> costs(a, wave_sums);
+  const Costs<ROWS, UNIT, THREADS> costs(a, wave_sums);
   const uint32_t G = sharers(a, costs.total);
   if (threadIdx.x == 0) {
     share->from = share->to = {a.c.batch, 0, 0, 0};

@@ -18,8 +18,9 @@ enum CacheKernel {
   CK_APPEND_F32 = CK_APPEND_BF16 + 6,  // [interleaved][chunk 4, 1]
   CK_KEEP = CK_APPEND_F32 + 4,         // chunks of 16, 4, 2 bytes
   CK_ATTEND = CK_KEEP + 3,             // [bf16][rows][dim up to 64, 128, 192, 256]
-  CK_JOIN = CK_ATTEND + 16,            // [bf16][rows]
-  CK_RULES = CK_JOIN + 4,              // [x bf16][y bf16]
+  CK_ATTEND_BF16 = CK_ATTEND + 16,     // [kFlashDims][few, rows]
+  CK_JOIN = CK_ATTEND_BF16 + 14,       // [bf16][rows], tiles of 32, of 128
+  CK_RULES = CK_JOIN + 6,              // [x bf16][y bf16]
   CK_COUNT = CK_RULES + 4
 };
 
@@ -55,10 +56,26 @@ const char *const bwpp_hip_cache_kernels[] = {
     "bwpp_cache_attend_bf16_rows_d128",
     "bwpp_cache_attend_bf16_rows_d192",
     "bwpp_cache_attend_bf16_rows_d256",
+    "bwpp_cache_attend_few_d64",
+    "bwpp_cache_attend_rows_d64",
+    "bwpp_cache_attend_few_d80",
+    "bwpp_cache_attend_rows_d80",
+    "bwpp_cache_attend_few_d96",
+    "bwpp_cache_attend_rows_d96",
+    "bwpp_cache_attend_few_d128",
+    "bwpp_cache_attend_rows_d128",
+    "bwpp_cache_attend_few_d160",
+    "bwpp_cache_attend_rows_d160",
+    "bwpp_cache_attend_few_d192",
+    "bwpp_cache_attend_rows_d192",
+    "bwpp_cache_attend_few_d256",
+    "bwpp_cache_attend_rows_d256",
     "bwpp_cache_join_f32",
     "bwpp_cache_join_f32_rows",
     "bwpp_cache_join_bf16",
     "bwpp_cache_join_bf16_rows",
+    "bwpp_cache_join_bf16_32",
+    "bwpp_cache_join_bf16_128",
     "bwpp_logit_rules_f32",
     "bwpp_logit_rules_f32_bf16",
     "bwpp_logit_rules_bf16_f32",
@@ -68,6 +85,9 @@ const int bwpp_hip_cache_kernel_count = (int)(sizeof(bwpp_hip_cache_kernels) / s
 static_assert(sizeof(bwpp_hip_cache_kernels) / sizeof(bwpp_hip_cache_kernels[0]) == CK_COUNT, "kernel names");
 
 namespace {
+
+// Head dims of the bf16 matrix-core kernels (kv_flash.h).
+const uint32_t kFlashDims[] = {64, 80, 96, 128, 160, 192, 256};
 
 BwppHipFault invalid(const char *why) { return {BWPP_HIP_ERR_INVALID_ARG, why}; }
 BwppHipFault unsupported(const char *why) { return {BWPP_HIP_ERR_UNSUPPORTED, why}; }
@@ -319,11 +339,20 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
                meet(sk, ls, es) || meet(sv, ls, es);
   for (const Span &s : small) alias = alias || meet(so, s, es) || meet(ls, s);
   if (alias) return bad(BWPP_HIP_ERR_ALIAS, "an output overlaps another operand");
-  // Tiles of 16 rows, whose waves share the keys out, or of 64, each wave 16:
-  // by the rows that a sequence and key head has on average.
+  // bf16 rows of 16-byte chunks (q, keys, values; 8-byte results) take the
+  // matrix-core kernels where the lanes' 32-bit offsets in a tile of 64 keys reach.
+  int flash = -1;
+  const uint64_t chunks = sq.ts | sq.hs | c.tok_s | c.head_s | c.page_s | (uintptr_t)q / 2 | (uintptr_t)k_cache / 2 | (uintptr_t)v_cache / 2;
+  if (cp.dtype == BWPP_HIP_BF16 && chunks % 8 == 0 && (so.ts | so.hs | (uintptr_t)o / 2) % 4 == 0 &&
+      ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)o) % 2 == 0 && c.tok_s < (1u << 24) &&
+      c.page_s < (1ull << 32))
+    for (int i = 0; i < 7; ++i)
+      if (kFlashDims[i] == cp.dim) flash = i;
+  // Tiles of few rows, whose waves share the keys out, or of more, where each wave
+  // has its own: by the rows that a sequence and key head has on average.
   const uint64_t mean = (T + cp.batch - 1) / cp.batch * g;
-  const bool many = mean > 16;
-  const uint32_t rows = many ? 64u : 16u, Dp = (cp.dim + 3) / 4 * 4;
+  const bool many = mean > (flash >= 0 ? 32u : 16u);
+  const uint32_t rows = flash >= 0 ? (many ? 128u : 32u) : many ? 64u : 16u, Dp = (cp.dim + 3) / 4 * 4;
   // Costs (kv_schedule.h) are counted in 64 bits and multiplied by the blocks.
   const long double worst = (long double)cp.heads * ((long double)T * g / rows + cp.batch) *
                             ((long double)g * (c.capacity + 256) + (long double)T * g + 2 * rows);
@@ -344,16 +373,18 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   const float scale = p.scale != 0.0f ? p.scale : 1.0f;
   a.scale_log2 = std::fabs(scale) * 1.4426950408889634f;
   a.flip = scale < 0.0f ? 1u : 0u;
-  a.blocks = 2 * cus_of(h);
+  // Blocks as many as are resident at once.
+  a.blocks = (flash >= 0 && cp.dim > 128 ? 1 : 2) * cus_of(h);
   void *ws = nullptr;
   s = bwpp_hip_take_workspace(h, (size_t)2 * a.blocks * rows * (Dp + 2) * 4, &ws);
   if (s != BWPP_HIP_OK) return s;
   a.part_o = static_cast<float *>(ws);
   a.part_ml = a.part_o + (size_t)2 * a.blocks * rows * Dp;
   const int kind = (cp.dtype == BWPP_HIP_BF16 ? 2 : 0) + (many ? 1 : 0);
-  s = bwpp_hip_launch_cache(h, CK_ATTEND + 4 * kind + (int)((cp.dim - 1) / 64), a.blocks, 1, 256, &a);
+  const int attend = flash >= 0 ? CK_ATTEND_BF16 + 2 * flash + (many ? 1 : 0) : CK_ATTEND + 4 * kind + (int)((cp.dim - 1) / 64);
+  s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, flash >= 0 && !many ? 128 : 256, &a);
   if (s != BWPP_HIP_OK) return s;
-  return bwpp_hip_launch_cache(h, CK_JOIN + kind, a.blocks - 1, 1, 256, &a);
+  return bwpp_hip_launch_cache(h, flash >= 0 ? CK_JOIN + 4 + (many ? 1 : 0) : CK_JOIN + kind, a.blocks - 1, 1, 256, &a);
 }
 
 // ------------------------------------------------------------------- rules
