@@ -304,12 +304,10 @@ typedef struct {
   uint32_t group;       /* query heads per key head */
   float scale_log2;     /* |scale| * log2(e) */
   uint32_t flip;        /* 1: the scale is negative */
-  uint32_t blocks;      /* workers that share the keys */
-  uint32_t rows;        /* a tile's rows (the join's) */
-  uint32_t unit;        /* keys of a unit of work (the join's) */
-  uint32_t vec;         /* 1: rows of 4 elements at their natural alignment, dim a multiple of 4 */
-  float *part_o;        /* [2 blocks][rows][dim up to a multiple of 4] */
-  float *part_ml;       /* [2 blocks][rows][2] */
+  uint32_t blocks;      /* blocks that share the keys */
+  double inv_blocks;    /* 1 / blocks */
+  float *part_o;        /* [2 blocks][rows of a tile][dim up to a multiple of 4] */
+  float *part_ml;       /* [2 blocks][rows of a tile][2] */
 } BwppCacheAttnArgs;
 
 /* Rules for the next token on logits (logit_rules.h). */

@@ -89,7 +89,7 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
   const BwppCacheArgs &c = a.c;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i16 = lane & 15u, grp = lane >> 4;
   const uint32_t D = c.dim, g = a.group, Dp = (D + 3u) & ~3u;
-  find_share<kRows, kUnit, kThreads>(a, blockIdx.x, &share, wave_sums);
+  find_share<kRows, kUnit, kThreads>(a, &share, wave_sums);
   const Place to = share.to;
   Place at = share.from;
   const uint32_t pmask = (1u << c.page_shift) - 1u;
@@ -252,7 +252,7 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
     l += __shfl_xor(l, 32, 64);
 
     // Results: row i16 has columns 64 j + 4 (4 grp + rr) + e in o[j][e][rr].
-    const uint32_t slot = 2u * blockIdx.x + (at.unit == 0 ? 1u : 0u);
+    const uint32_t slot = 2u * share.b + (at.unit == 0 ? 1u : 0u);
     auto put = [&](uint32_t rw, uint32_t col, const float (&v)[4], float mm, float ll, bool head) {
       // rw: row of the tile
       const uint32_t rr = at.tile * kRows + rw;
@@ -321,56 +321,97 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
   }
 }
 
-// Joins the parts of the item that block b's border is the first to divide
-// (b = 1 .. G - 1, a block of this launch each).
+// Joins the parts of the item that the border before sharer b is the first to
+// divide (b = 1 .. blocks - 1: blockIdx.x), kJoin rows of it a block.
+constexpr uint32_t kJoin = 16;
 template <class T, uint32_t kRows, uint32_t kUnit>
 __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
   typedef Work<kRows, kUnit> W;
+  constexpr uint32_t kParts = 64;  // a round of them in LDS
   __shared__ uint64_t wave_sums[kThreads / 64];
   __shared__ Place item;
-  __shared__ uint32_t last;  // block with the item's last part; 0: nothing to join
+  __shared__ uint32_t last;  // sharer with the item's last part; 0: nothing to join
+  __shared__ float top[kJoin], sum[kJoin], factor[kParts][kJoin];
   const BwppCacheArgs &c = a.c;
   const Costs<kRows, kUnit, kThreads> costs(a, wave_sums);
-  const uint32_t G = sharers(a, costs.total), b = blockIdx.x + 1;
-  if (b >= G) return;
+  const uint32_t b = blockIdx.x + 1, row0 = blockIdx.y * kJoin;
+  const uint64_t S = share_of(a, costs.total);
+  if (S * b >= costs.total) return;
   if (threadIdx.x == 0) last = 0;
   __syncthreads();
-  const uint64_t x = costs.total * b / G, prev = costs.total * (b - 1) / G;
-  costs.at(a, x, [&](uint32_t s, const Seq &q, uint64_t at) {
+  costs.at(a, S * b, [&](uint32_t s, const Seq &q, uint64_t at) {
     uint64_t begin, end;
-    const Place p = W::find(a, s, q, x - at, begin, end);
+    const Place p = W::find(a, s, q, S * b - at, begin, end);
     if (p.unit == 0) return;
+    const uint64_t prev = S * (b - 1);
     if (prev >= at + begin && W::unit(a, q, p.tile, prev - at - begin, end - begin) != 0) return;  // not the first
     item = p;
-    last = (uint32_t)(((at + end) * G - 1) / costs.total);
-    last = min(last, G - 1);
+    uint32_t e = b;  // the last border before the item's end
+    while (S * (e + 1) < at + end) ++e;
+    last = e;
   });
   __syncthreads();
   if (last == 0) return;
   const Seq q = seq_at(c, item.s);
   const uint32_t g = a.group, D = c.dim, n4 = (D + 3u) / 4u, Dp = 4u * n4;
-  const uint32_t rows = min(kRows, q.n * g - item.tile * kRows), parts = last - b + 2;
-  for (uint32_t i = threadIdx.x; i < rows * n4; i += kThreads) {
-    const uint32_t rw = i / n4, col = 4u * (i % n4);
-    // part 0 in slot 2 (b - 1) + 1, part k in slot 2 (b + k - 1)
-    auto slot_row = [&](uint32_t k) { return (uint64_t)(k == 0 ? 2 * b - 1 : 2 * (b + k - 1)) * kRows + rw; };
-    float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t k = 0; k < parts; ++k) m = fmaxf(m, a.part_ml[2 * slot_row(k)]);
-#pragma unroll 4
-    for (uint32_t k = 0; k < parts; ++k) {
-      const uint64_t sr = slot_row(k);
-      const float2 w = *reinterpret_cast<const float2 *>(a.part_ml + 2 * sr);
-      const float f = w.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.x - m);
-      const float4 u = *reinterpret_cast<const float4 *>(a.part_o + sr * Dp + col);
-      l += w.y * f;
-      v[0] += u.x * f, v[1] += u.y * f, v[2] += u.z * f, v[3] += u.w * f;
+  const uint32_t all = min(kRows, q.n * g - item.tile * kRows), parts = last - b + 2;
+  if (row0 >= all) return;
+  const uint32_t rows = min(kJoin, all - row0);
+  // part 0 in slot 2 (b - 1) + 1, part k in slot 2 (b + k - 1)
+  auto slot_row = [&](uint32_t k) { return (uint64_t)(k == 0 ? 2 * b - 1 : 2 * (b + k - 1)) * kRows + row0; };
+  // The rows' exponent offsets and sums: 16 threads a row.
+  {
+    const uint32_t r = threadIdx.x / 16u, j = threadIdx.x % 16u;
+    float m = -INFINITY;
+    if (r < rows)
+      for (uint32_t k = j; k < parts; k += 16u) m = fmaxf(m, a.part_ml[2 * (slot_row(k) + r)]);
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) m = fmaxf(m, __shfl_xor(m, d, 64));
+    float l = 0.0f;
+    if (r < rows)
+      for (uint32_t k = j; k < parts; k += 16u) {
+        const float2 w = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (slot_row(k) + r));
+        l += w.y * (w.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.x - m));
+      }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) l += __shfl_xor(l, d, 64);
+    if (j == 0) top[r] = m, sum[r] = l;
+  }
+  constexpr uint32_t kMost = kJoin * 64u / kThreads;  // float4 a thread, dim 256
+  float4 v[kMost];
+#pragma unroll
+  for (uint32_t e = 0; e < kMost; ++e) v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (uint32_t k0 = 0; k0 < parts; k0 += kParts) {
+    const uint32_t n = min(kParts, parts - k0);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n * kJoin; i += kThreads) {
+      const uint32_t k = i / kJoin, r = i % kJoin;
+      const float w = r < rows ? a.part_ml[2 * (slot_row(k0 + k) + r)] : -INFINITY;
+      factor[k][r] = w == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w - top[r]);
     }
-    const uint32_t rr = item.tile * kRows + rw;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < kMost; ++e) {
+      const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
+      if (r >= rows) continue;
+#pragma unroll 8
+      for (uint32_t k = 0; k < n; ++k) {
+        const float4 u = *reinterpret_cast<const float4 *>(a.part_o + (slot_row(k0 + k) + r) * Dp + col);
+        const float f = factor[k][r];
+        v[e].x += u.x * f, v[e].y += u.y * f, v[e].z += u.z * f, v[e].w += u.w * f;
+      }
+    }
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < kMost; ++e) {
+    const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
+    if (r >= rows) continue;
+    const uint32_t rr = item.tile * kRows + row0 + r;
     const uint64_t t = q.first + rr / g, hh = item.head * g + rr % g;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const float u[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+    const float l = sum[r], inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float u[4] = {v[e].x * inv, v[e].y * inv, v[e].z * inv, v[e].w * inv};
     store4(static_cast<T *>(a.o) + t * a.o_ts + hh * a.o_hs, col, D, u);
-    if (col == 0 && a.lse) a.lse[t * (uint64_t)(c.heads * g) + hh] = l == 0.0f ? -INFINITY : lse_of(m == -INFINITY ? 0.0f : m, l);
+    if (col == 0 && a.lse) a.lse[t * (uint64_t)(c.heads * g) + hh] = l == 0.0f ? -INFINITY : lse_of(top[r] == -INFINITY ? 0.0f : top[r], l);
   }
 }
 

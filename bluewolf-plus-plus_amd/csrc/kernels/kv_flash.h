@@ -91,11 +91,9 @@ struct Wave32 {
     l = 0.0f;
   }
 
-  // One key tile at `st`.  MASK: vis has bit k of word kb where this lane's row
-  // sees key 32 kb + k; elsewhere all are seen.
-  template <bool MASK>
-  __device__ __forceinline__ void tile(const unsigned char *st, const uint32_t (&vis)[KB]) {
-    f32x16_t s[KB];
+  // Scores and probabilities (in s) of the key tile at `st`.  masked: vis has bit k
+  // of word kb where this lane's row sees key 32 kb + k; otherwise all are seen.
+  __device__ __forceinline__ void scores(const unsigned char *st, bool masked, const uint32_t (&vis)[KB], f32x16_t (&s)[KB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -106,16 +104,27 @@ struct Wave32 {
             __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4 *>(st + koff[ks] + 32u * kb * R::kRowB)), q[ks],
             s[kb], 0, 0, 0);
     }
-    float mx = -INFINITY;
+    // Two reads of K ahead of the products: hoisted all, they would not fit the registers.
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const uint32_t w = MASK ? vis[kb] >> (4u * lh) : 0u;
+    for (int i = 0; i < KB * KS - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    if (masked) {  // wave-uniform
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if (MASK) s[kb][r] = w >> (8 * (r >> 2) + (r & 3)) & 1u ? s[kb][r] : -INFINITY;
-        mx = fmaxf(mx, s[kb][r]);
+      for (int kb = 0; kb < KB; ++kb) {
+        const uint32_t w = vis[kb] >> (4u * lh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = w >> (8 * (r >> 2) + (r & 3)) & 1u ? s[kb][r] : -INFINITY;
       }
     }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
     {
       const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
       mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * c;
@@ -142,7 +151,10 @@ struct Wave32 {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
-    bool odd = false;  // infinite or NaN values: 0 times those would reach rows that do not see them
+  }
+
+  // O^T += V^T P^T.  P enters as two bf16 terms, 2^-16 of p together.
+  __device__ __forceinline__ void products(const unsigned char *st, const f32x16_t (&s)[KB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -154,44 +166,62 @@ struct Wave32 {
           const unsigned char *p = st + voff[d] + (32u * kb + 16u * kq) * R::kRowB;
           const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)p);
           const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)(p + 8u * R::kRowB));
-          v8s_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          if (MASK) {
-            const u16x2_t big = max_abs_bf16(u16x2_t{0, 0}, v);
-            if (__ballot(big[0] >= 0x7f80u || big[1] >= 0x7f80u)) {
-              odd = true;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = (v[e] & 0x7f80) == 0x7f80 ? (short)0 : v[e];
-            }
-          }
+          const v8s_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), ph, o[d], 0, 0, 0);
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), pl, o[d], 0, 0, 0);
         }
       }
-    if constexpr (MASK) {
-      if (odd) {  // wave-uniform: the values left out, key by key
+    // Four (transposing) reads of V ahead.
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-          for (uint32_t k = 0; k < 32; ++k) {
-            float mine = 0.0f;
+    for (int i = 0; i < 2 * KB * DB - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+  }
+
+  // Infinite and NaN values of a tile with masked keys: 0 times those would reach
+  // rows that do not see them.  Where odd_values finds one, add_odd adds what the
+  // rows that see them get, key by key, and clear_odd puts zeros in their place,
+  // before the products.  `share` of `shares` that look through the tile.
+  static __device__ __forceinline__ bool odd_values(const unsigned char *st, uint32_t share, uint32_t shares) {
+    u16x2_t big = {0, 0};
+    for (uint32_t i = share * 64u + (threadIdx.x & 63u); i < kTile / 16u; i += shares * 64u)
+      big = max_abs_bf16(big, *reinterpret_cast<const v8s_t *>(st + kTile + 16u * i));
+    return __ballot(big[0] >= 0x7f80u || big[1] >= 0x7f80u) != 0;
+  }
+  __device__ __forceinline__ void add_odd(const unsigned char *st, const uint32_t (&vis)[KB], const f32x16_t (&s)[KB]) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mine = (uint32_t)r == 4u * (k >> 3) + (k & 3u) ? s[kb][r] : mine;
-            const float pk = __shfl(mine, (int)(lq + 32u * (k >> 2 & 1u)), 64);
-            if (!(vis[kb] >> k & 1u)) continue;
-            const uint32_t row = 32u * kb + k;
-            const unsigned char *vr = st + kTile + row * R::kRowB;
+    for (int kb = 0; kb < KB; ++kb)
+      for (uint32_t k = 0; k < 32; ++k) {
+        float mine = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+        for (int r = 0; r < 16; ++r) mine = (uint32_t)r == 4u * (k >> 3) + (k & 3u) ? s[kb][r] : mine;
+        const float pk = __shfl(mine, (int)(lq + 32u * (k >> 2 & 1u)), 64);
+        const bool see = vis[kb] >> k & 1u;
+        const uint32_t row = 32u * kb + k;
+        const unsigned char *vr = st + kTile + row * R::kRowB;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                if (r % 4 == 0) asm volatile("" ::: "memory");  // few reads at a time: registers
-                const uint32_t col = 32u * d + 8u * (r >> 2) + 4u * lh + (r & 3);
-                if (col >= (uint32_t)D) continue;
-                const float v = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(
-                    vr + 16u * ((col >> 3) ^ R::v_swz(row)) + 2u * (col & 7u)));
-                if (!(fabsf(v) < INFINITY)) o[d][r] += pk * v;
-              }
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            if (r % 4 == 0) asm volatile("" ::: "memory");  // few reads at a time: registers
+            const uint32_t col = 32u * d + 8u * (r >> 2) + 4u * lh + (r & 3);
+            if (col >= (uint32_t)D) continue;
+            const float v = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(
+                vr + 16u * ((col >> 3) ^ R::v_swz(row)) + 2u * (col & 7u)));
+            if (see && !(fabsf(v) < INFINITY)) o[d][r] += pk * v;
           }
       }
+  }
+  static __device__ __forceinline__ void clear_odd(unsigned char *st, uint32_t share, uint32_t shares) {
+    for (uint32_t i = share * 64u + (threadIdx.x & 63u); i < kTile / 16u; i += shares * 64u) {
+      v8s_t *p = reinterpret_cast<v8s_t *>(st + kTile + 16u * i);
+      v8s_t v = *p;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (v[e] & 0x7f80) == 0x7f80 ? (short)0 : v[e];
+      *p = v;
     }
   }
   // The row's whole sum in both of its lanes.
@@ -234,11 +264,13 @@ __device__ __forceinline__ uint32_t load_pages(const BwppCacheArgs &c, const Ite
   const uint32_t first = k >> c.page_shift, n = min(kPages, ((it.kend - 1) >> c.page_shift) - first + 1);
   const int32_t *table = c.table + (uint64_t)it.s * c.ld_table + first;
   int none = 0;
+  uint32_t p = threadIdx.x < n ? (uint32_t)table[threadIdx.x] : 0u;  // under way with the query rows
   __syncthreads();  // done with the last ones
-  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-    const uint32_t p = (uint32_t)table[i];
+  for (uint32_t i = threadIdx.x; i < n;) {
     none |= p >= c.pages;
     pages[i] = p < c.pages ? p : kNoPage;
+    i += THREADS;
+    if (i < n) p = (uint32_t)table[i];
   }
   bad = __syncthreads_or(none) != 0;
   const uint64_t end = (uint64_t)(first + n) << c.page_shift;
@@ -261,19 +293,26 @@ struct Fetch {
   static constexpr uint32_t kDma = KEYS * R::kSlots / 64, kMine = (kDma + FROM_WAVES - 1) / FROM_WAVES;
   static constexpr uint32_t kTile = KEYS * R::kRowB;
   const uint16_t *K, *V;  // the item's key head
-  uint32_t koff[kMine], voff[kMine];
-  uint32_t wave;          // of FROM_WAVES that share the tile
+  static constexpr bool kKeep = kMine <= 8;  // offsets are kept in registers, more of them made again
+  uint32_t kept[kKeep ? 2 * kMine : 1];
+  uint32_t wave, tok_s;   // wave: of FROM_WAVES that share the tile
 
   static __device__ __forceinline__ uint32_t slot(uint32_t i, uint32_t w) { return (i * FROM_WAVES + w) * 64u + (threadIdx.x & 63u); }
   __device__ __forceinline__ void place(const BwppCacheArgs &c, uint32_t w) {
     wave = w;
+    tok_s = (uint32_t)c.tok_s;
+    if constexpr (kKeep) {
 #pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) {
-      const uint32_t q = slot(i, w), r = q / R::kSlots, pc = q % R::kSlots;
-      koff[i] = 2u * (r * (uint32_t)c.tok_s + 8u * (pc ^ R::k_swz(r)));
-      voff[i] = 2u * (r * (uint32_t)c.tok_s + 8u * (pc ^ R::v_swz(r)));
+      for (uint32_t i = 0; i < kMine; ++i) kept[2 * i] = offset(i, false), kept[2 * i + 1] = offset(i, true);
     }
   }
+  // Bytes from the tile's first row to a lane's chunk.
+  __device__ __forceinline__ uint32_t offset(uint32_t i, bool values) const {
+    const uint32_t q = slot(i, wave), r = q / R::kSlots, pc = q % R::kSlots;
+    return 2u * (r * tok_s + 8u * (pc ^ (values ? R::v_swz(r) : R::k_swz(r))));
+  }
+  __device__ __forceinline__ uint32_t koff(uint32_t i) const { return kKeep ? kept[kKeep ? 2 * i : 0] : offset(i, false); }
+  __device__ __forceinline__ uint32_t voff(uint32_t i) const { return kKeep ? kept[kKeep ? 2 * i + 1 : 0] : offset(i, true); }
   __device__ __forceinline__ void issue(const BwppCacheArgs &c, const Item &it, uint32_t k0, uint32_t first,
                                         const uint32_t *pages, uint32_t lds) const {
     const uint32_t pmask = (1u << c.page_shift) - 1u, n = min((uint32_t)KEYS, it.kend - k0);
@@ -284,16 +323,16 @@ struct Fetch {
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
           if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
-          g2lds16_so(K + base, koff[i], lds + (i * FROM_WAVES + wave) * 1024u);
-          g2lds16_so(V + base, voff[i], lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+          g2lds16_so(K + base, koff(i), lds + (i * FROM_WAVES + wave) * 1024u);
+          g2lds16_so(V + base, voff(i), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
         }
       } else {  // rows past the last key re-read it
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
           if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
-          const uint32_t r = slot(i, wave) / R::kSlots, back = r < n ? 0u : 2u * (r - (n - 1)) * (uint32_t)c.tok_s;
-          g2lds16_so(K + base, koff[i] - back, lds + (i * FROM_WAVES + wave) * 1024u);
-          g2lds16_so(V + base, voff[i] - back, lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+          const uint32_t r = slot(i, wave) / R::kSlots, back = r < n ? 0u : 2u * (r - (n - 1)) * tok_s;
+          g2lds16_so(K + base, koff(i) - back, lds + (i * FROM_WAVES + wave) * 1024u);
+          g2lds16_so(V + base, voff(i) - back, lds + kTile + (i * FROM_WAVES + wave) * 1024u);
         }
       }
     } else {
@@ -303,10 +342,10 @@ struct Fetch {
         const uint32_t r = slot(i, wave) / R::kSlots, key = k0 + min(r, n - 1);
         const uint32_t page = pages[(key >> c.page_shift) - first] & ~kNoPage;
         // less the row's offset, which koff and voff have
-        const uint64_t row = (uint64_t)page * (uint32_t)c.page_s + (uint64_t)(key & pmask) * (uint32_t)c.tok_s;
-        const uint32_t mine = 2u * r * (uint32_t)c.tok_s;
-        g2lds16_v(reinterpret_cast<const char *>(K + row) + (koff[i] - mine), lds + (i * FROM_WAVES + wave) * 1024u);
-        g2lds16_v(reinterpret_cast<const char *>(V + row) + (voff[i] - mine), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+        const uint64_t row = (uint64_t)page * (uint32_t)c.page_s + (uint64_t)(key & pmask) * tok_s;
+        const uint32_t mine = 2u * r * tok_s;
+        g2lds16_v(reinterpret_cast<const char *>(K + row) + (koff(i) - mine), lds + (i * FROM_WAVES + wave) * 1024u);
+        g2lds16_v(reinterpret_cast<const char *>(V + row) + (voff(i) - mine), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
       }
     }
   }
@@ -348,8 +387,8 @@ __device__ __forceinline__ void for_items(const BwppCacheAttnArgs &a, F f) {
   typedef Work<ROWS, UNIT> W;
   __shared__ uint64_t wave_sums[THREADS / 64];
   __shared__ Share share;
-  const uint32_t b = blockIdx.x;
-  find_share<ROWS, UNIT, THREADS>(a, b, &share, wave_sums);
+  find_share<ROWS, UNIT, THREADS>(a, &share, wave_sums);
+  const uint32_t b = uni(share.b);
   Place at = {uni(share.from.s), uni(share.from.head), uni(share.from.tile), uni(share.from.unit)};
   const Place to = {uni(share.to.s), uni(share.to.head), uni(share.to.tile), uni(share.to.unit)};
   Item it = {};
@@ -428,19 +467,24 @@ __device__ __forceinline__ void attend_few(const BwppCacheAttnArgs &a) {
         else wait_vmcnt<0>();
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): done reading the stage that is refilled now
         if (j + kStages - 1 < mine) issue(j + kStages - 1);
-        const unsigned char *st = ring + uni((j % kStages) * kStage);
+        unsigned char *st = ring + uni((j % kStages) * kStage);
         uint32_t vis[1] = {~0u};
-        if (bad || k0 + 32u > it.kend || k0 + 32u > it.q.held) {
+        const bool masked = bad || k0 + 32u > it.kend || k0 + 32u > it.q.held;
+        if (masked) {
           if (k0 + 32u > it.q.held) {
             vis[0] = mask_bits32(a, it.q.first, tok, (int64_t)k0 - (int64_t)it.q.held);
             if (k0 < it.q.held) vis[0] |= (1u << (it.q.held - k0)) - 1u;  // fewer than 32
             wait_vmcnt<0>();  // the mask's loads
           }
           vis[0] &= keys_with_page(c, it, k0, first, pages);
-          w.template tile<true>(st, vis);
-        } else {
-          w.template tile<false>(st, vis);
         }
+        f32x16_t s[1];
+        w.scores(st, masked, vis, s);
+        if (masked && W::odd_values(st, 0, 1)) {
+          w.add_odd(st, vis, s);
+          W::clear_odd(st, 0, 1);
+        }
+        w.products(st, s);
       }
       seg = end;
     }
@@ -506,9 +550,10 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
     w.start(Q, a.scale_log2, a.flip);
     fetch.K = static_cast<const uint16_t *>(c.k) + (uint64_t)it.head * c.head_s;
     fetch.V = static_cast<const uint16_t *>(c.v) + (uint64_t)it.head * c.head_s;
-    // Keys below `all` are seen by all of the wave's rows, from `none` on by none.
+    // Keys below `all` are seen by all of the wave's rows (`all_block`: the block's), from `none` on by none.
     const uint32_t t0 = min(row0, it.R - 1u) / a.group, t1 = min(row0 + 31u, it.R - 1u) / a.group;
     const uint32_t all = a.mask ? it.q.held : it.q.held + t0 + 1u;
+    const uint32_t all_block = a.mask ? it.q.held : it.q.held + it.tile * 128u / a.group + 1u;
     const uint32_t none = row0 >= it.R ? 0u : a.mask ? it.kend : min(it.kend, it.q.held + t1 + 1u);
     for (uint32_t seg = it.kbeg; seg < it.kend;) {
       bool bad;
@@ -521,10 +566,11 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
         wait_vmcnt<0>();
         __syncthreads();
         if (j + 1 < ntile) fetch.issue(c, it, k0 + 64u, first, pages, lds0 + ((j + 1) & 1u) * kStage);
-        const unsigned char *st = smem + uni((j & 1u) * kStage);
-        if (k0 >= none) continue;
+        unsigned char *st = smem + uni((j & 1u) * kStage);
+        const bool none_odd = !bad && k0 + 64u <= it.kend && k0 + 64u <= all_block;  // the same in every wave
+        const bool mine = k0 < none, masked = !none_odd && (bad || k0 + 64u > it.kend || k0 + 64u > all);
         uint32_t vis[KB] = {~0u, ~0u};
-        if (bad || k0 + 64u > it.kend || k0 + 64u > all) {
+        if (masked) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
             const uint32_t k = k0 + 32u * kb;
@@ -534,10 +580,16 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
             }
             vis[kb] &= keys_with_page(c, it, k, first, pages);
           }
-          w.template tile<true>(st, vis);
-        } else {
-          w.template tile<false>(st, vis);
         }
+        f32x16_t s[KB];
+        if (mine) w.scores(st, masked, vis, s);
+        if (!none_odd && __syncthreads_or(W::odd_values(st, wave, NW))) {
+          if (mine) w.add_odd(st, vis, s);
+          __syncthreads();
+          W::clear_odd(st, wave, NW);
+          __syncthreads();
+        }
+        if (mine) w.products(st, s);
       }
       seg = end;
       // (the next pages' first barrier comes before any stage is filled again)

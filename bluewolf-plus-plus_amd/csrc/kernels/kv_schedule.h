@@ -10,11 +10,14 @@
 // what lies between the costs W b / G and W (b + 1) / G of the total W, rounded
 // to whole units.  An item whose keys fall to several blocks is left by each
 // as a triple (exponent offset, sum of p, sum of p v) and joined by a second
-// launch: the block where it begins leaves it in slot 2 b + 1, the others,
-// for which it is the first item, in slot 2 b.
+// launch: the sharer where it begins leaves it in slot 2 b + 1, the others,
+// for which it is the first item, in slot 2 b.  The sharers of one XCD are
+// neighbours: the tiles of a head meet its keys in one L2.
 //
-// Costs are whole numbers, g times keys (g query heads a key head): a block and
-// its successor find the same border.
+// Costs are whole numbers below 2^52, g times keys (g query heads a key head);
+// quotients are taken in doubles (64-bit integer ones cost a microsecond
+// here), the same in every block, so a sharer and its successor find the same
+// border.
 #pragma once
 
 #include "kv_cache.h"
@@ -35,7 +38,7 @@ __device__ __forceinline__ bool earlier(const Place &a, const Place &b) {
 }
 struct Share {
   Place from, to;
-  uint32_t blocks;  // that have a share
+  uint32_t b;  // whose it is
 };
 
 template <uint32_t ROWS, uint32_t UNIT>
@@ -59,7 +62,8 @@ struct Work {
                                                uint64_t &begin, uint64_t &end) {
     const uint32_t T = tiles(q, a.group);
     const uint64_t head_cost = before(q, a.group, T);
-    const uint32_t head = (uint32_t)(x / head_cost);
+    uint32_t head = (uint32_t)((double)x / (double)head_cost);
+    if (head * head_cost > x) --head;  // (a quotient rounded up)
     const uint64_t rest = x - head * head_cost;
     uint32_t lo = 0, hi = T;  // before(lo) <= rest < before(hi)
     while (hi - lo > 1) {
@@ -74,7 +78,8 @@ struct Work {
   }
   static __device__ __forceinline__ uint32_t unit(const BwppCacheAttnArgs &a, const Seq &q, uint32_t tile, uint64_t off,
                                                   uint64_t cost) {
-    return (uint32_t)(off * units(a, q, tile) / cost);
+    const uint32_t n = units(a, q, tile), u = (uint32_t)((double)off * (double)n / (double)cost);
+    return min(u, n ? n - 1u : 0u);
   }
 };
 
@@ -128,30 +133,32 @@ struct Costs {
   }
 };
 
-// Blocks that share a total cost.
-__device__ __forceinline__ uint32_t sharers(const BwppCacheAttnArgs &a, uint64_t total) {
-  const uint64_t most = total / ((uint64_t)a.group * kLeast);
-  return (uint32_t)(most < 1 ? 1 : most < a.blocks ? most : a.blocks);
+// The share of a total cost: as many keys for each block, kLeast at least.
+__device__ __forceinline__ uint64_t share_of(const BwppCacheAttnArgs &a, uint64_t total) {
+  const uint64_t even = (uint64_t)((double)total * a.inv_blocks) + 1, least = (uint64_t)a.group * kLeast;
+  return even < least ? least : even;
 }
 
-// The share of block b, the same in every thread (`share` in LDS).
+// The share of this block, the same in every thread (`share` in LDS).
 template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
-__device__ __forceinline__ void find_share(const BwppCacheAttnArgs &a, uint32_t b, Share *share, uint64_t *wave_sums) {
+__device__ __forceinline__ void find_share(const BwppCacheAttnArgs &a, Share *share, uint64_t *wave_sums) {
+  constexpr uint32_t kXcds = 8;  // blocks go to them in turn
   const Costs<ROWS, UNIT, THREADS> costs(a, wave_sums);
-  const uint32_t G = sharers(a, costs.total);
+  const uint64_t S = share_of(a, costs.total);
+  const uint32_t sharers = min((uint32_t)((double)costs.total / (double)S) + 1u, a.blocks), per = (sharers + kXcds - 1) / kXcds;
+  const uint32_t b = blockIdx.x % kXcds * per + blockIdx.x / kXcds;
   if (threadIdx.x == 0) {
     share->from = share->to = {a.c.batch, 0, 0, 0};
-    share->blocks = G;
+    share->b = b;
   }
   __syncthreads();
-  if (b >= G) return;
+  if (blockIdx.x / kXcds >= per || b >= a.blocks) return;
   uint64_t begin, end;
-  const uint64_t x0 = costs.total * b / G, x1 = costs.total * (b + 1) / G;
-  costs.at(a, x0, [&](uint32_t s, const Seq &q, uint64_t at) {
-    share->from = Work<ROWS, UNIT>::find(a, s, q, x0 - at, begin, end);
+  costs.at(a, S * b, [&](uint32_t s, const Seq &q, uint64_t at) {
+    share->from = Work<ROWS, UNIT>::find(a, s, q, S * b - at, begin, end);
   });
-  costs.at(a, x1, [&](uint32_t s, const Seq &q, uint64_t at) {
-    share->to = Work<ROWS, UNIT>::find(a, s, q, x1 - at, begin, end);
+  costs.at(a, S * (b + 1), [&](uint32_t s, const Seq &q, uint64_t at) {
+    share->to = Work<ROWS, UNIT>::find(a, s, q, S * (b + 1) - at, begin, end);
   });
   __syncthreads();
 }

@@ -373,8 +373,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   const float scale = p.scale != 0.0f ? p.scale : 1.0f;
   a.scale_log2 = std::fabs(scale) * 1.4426950408889634f;
   a.flip = scale < 0.0f ? 1u : 0u;
-  // Blocks as many as are resident at once.
-  a.blocks = (flash >= 0 && cp.dim > 128 ? 1 : 2) * cus_of(h);
+  // Blocks as many as are resident at once, the same number on each XCD.
+  a.blocks = ((flash >= 0 && cp.dim > 128 ? 1 : 2) * cus_of(h) + 7) / 8 * 8;
+  a.inv_blocks = 1.0 / a.blocks;
   void *ws = nullptr;
   s = bwpp_hip_take_workspace(h, (size_t)2 * a.blocks * rows * (Dp + 2) * 4, &ws);
   if (s != BWPP_HIP_OK) return s;
@@ -384,7 +385,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   const int attend = flash >= 0 ? CK_ATTEND_BF16 + 2 * flash + (many ? 1 : 0) : CK_ATTEND + 4 * kind + (int)((cp.dim - 1) / 64);
   s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, flash >= 0 && !many ? 128 : 256, &a);
   if (s != BWPP_HIP_OK) return s;
-  return bwpp_hip_launch_cache(h, flash >= 0 ? CK_JOIN + 4 + (many ? 1 : 0) : CK_JOIN + kind, a.blocks - 1, 1, 256, &a);
+  return bwpp_hip_launch_cache(h, flash >= 0 ? CK_JOIN + 4 + (many ? 1 : 0) : CK_JOIN + kind, a.blocks - 1,
+                               (rows + 15) / 16, 256, &a);
 }
 
 // ------------------------------------------------------------------- rules
