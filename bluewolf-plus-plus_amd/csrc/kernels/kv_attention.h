@@ -439,3 +439,4 @@ BWPP_JOIN(bf16, uint16_t, 16, 64)
 BWPP_JOIN(bf16_rows, uint16_t, 64, 64)
 BWPP_JOIN(bf16_32, uint16_t, 32, 64)
 BWPP_JOIN(bf16_128, uint16_t, 128, 64)
+BWPP_JOIN(bf16_256, uint16_t, 256, 64)

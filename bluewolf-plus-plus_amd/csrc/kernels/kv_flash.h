@@ -11,9 +11,14 @@
 // (every NW-th of the block's) through a DMA ring of its own, and the waves'
 // triples meet in LDS at the end of an item.
 //
-// More rows (attend_rows): the matrix products bound it.  Each of a block's
-// four waves has 32 rows of a tile of 128, and key tiles of 64 come through a
-// two-stage ring that all four read.
+// More rows (attend_rows): the matrix products and the softmax bound it.  Each
+// of a block's waves has 32 rows of the tile, and key tiles of 64 come through
+// a two-stage ring that all of them read: four waves, two blocks a CU, or, for
+// more than 128 rows and head dims up to 128, eight (2 x 2048 tokens 32 : 8
+// heads of 128: four 386 us, eight 379; 8 trees of 48 tokens 62 and 57).  Here P
+// is rounded to one bf16 term, as in attention.hip's kernel for d = 128: two
+// cost 475 and 64 us, and the result's error (rms, of its norm) is 0.0022 with
+// one, 0.0017, its own rounding, with two.
 //
 // Page numbers of an item's keys are copied to LDS, 1024 at a time, before its
 // tiles: no load of the compiler's is outstanding beside the DMA, whose
@@ -153,14 +158,22 @@ struct Wave32 {
     }
   }
 
-  // O^T += V^T P^T.  P enters as two bf16 terms, 2^-16 of p together.
+  // O^T += V^T P^T.  P enters as two bf16 terms, 2^-16 of p together, or rounded to
+  // one, 2^-8 (the sum of p has it whole).
+  template <int TERMS>
   __device__ __forceinline__ void products(const unsigned char *st, const f32x16_t (&s)[KB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int kq = 0; kq < 2; ++kq) {
         bf16x8_t ph, pl;
-        split_bf16x8(&s[kb], 8 * kq, ph, pl);
+        if constexpr (TERMS == 2) {
+          split_bf16x8(&s[kb], 8 * kq, ph, pl);
+        } else {
+          const uint4 w = make_uint4(pack_bf16x2(s[kb][8 * kq], s[kb][8 * kq + 1]), pack_bf16x2(s[kb][8 * kq + 2], s[kb][8 * kq + 3]),
+                                     pack_bf16x2(s[kb][8 * kq + 4], s[kb][8 * kq + 5]), pack_bf16x2(s[kb][8 * kq + 6], s[kb][8 * kq + 7]));
+          ph = __builtin_bit_cast(bf16x8_t, w);
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const unsigned char *p = st + voff[d] + (32u * kb + 16u * kq) * R::kRowB;
@@ -168,17 +181,18 @@ struct Wave32 {
           const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)(p + 8u * R::kRowB));
           const v8s_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), ph, o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), pl, o[d], 0, 0, 0);
+          if constexpr (TERMS == 2)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), pl, o[d], 0, 0, 0);
         }
       }
     // Four (transposing) reads of V ahead.
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
     for (int i = 0; i < 2 * KB * DB - 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, TERMS, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 2 * TERMS, 0);
   }
 
   // Infinite and NaN values of a tile with masked keys: 0 times those would reach
@@ -484,7 +498,7 @@ __device__ __forceinline__ void attend_few(const BwppCacheAttnArgs &a) {
           w.add_odd(st, vis, s);
           W::clear_odd(st, 0, 1);
         }
-        w.products(st, s);
+        w.template products<2>(st, s);
       }
       seg = end;
     }
@@ -527,9 +541,10 @@ __device__ __forceinline__ void attend_few(const BwppCacheAttnArgs &a) {
   });
 }
 
-template <int D>
+template <int D, int NW>
 __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
-  constexpr int NW = 4, KB = 2;
+  constexpr int KB = 2, TERMS = 1;
+  constexpr uint32_t kRows = 32 * NW, kKeys = 32 * KB;
   typedef Wave32<D, KB> W;
   typedef Fetch<D, 32 * KB, NW> F;
   constexpr uint32_t kStage = W::kStage;
@@ -543,9 +558,9 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
   F fetch;
   fetch.place(c, wave);
 
-  for_items<128, 64, 64 * NW>(a, [&](const Item &it, uint32_t slot) {
+  for_items<kRows, 64, 64 * NW>(a, [&](const Item &it, uint32_t slot) {
     uint32_t tok;
-    const uint32_t row0 = it.tile * 128u + 32u * wave;
+    const uint32_t row0 = it.tile * kRows + 32u * wave;
     const uint16_t *Q = query_row<D, KB>(a, it, row0 + w.lq, tok);
     w.start(Q, a.scale_log2, a.flip);
     fetch.K = static_cast<const uint16_t *>(c.k) + (uint64_t)it.head * c.head_s;
@@ -553,23 +568,25 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
     // Keys below `all` are seen by all of the wave's rows (`all_block`: the block's), from `none` on by none.
     const uint32_t t0 = min(row0, it.R - 1u) / a.group, t1 = min(row0 + 31u, it.R - 1u) / a.group;
     const uint32_t all = a.mask ? it.q.held : it.q.held + t0 + 1u;
-    const uint32_t all_block = a.mask ? it.q.held : it.q.held + it.tile * 128u / a.group + 1u;
+    const uint32_t all_block = a.mask ? it.q.held : it.q.held + it.tile * kRows / a.group + 1u;
     const uint32_t none = row0 >= it.R ? 0u : a.mask ? it.kend : min(it.kend, it.q.held + t1 + 1u);
     for (uint32_t seg = it.kbeg; seg < it.kend;) {
       bool bad;
       const uint32_t end = uni(load_pages<64 * NW>(c, it, seg, pages, bad)), first = seg >> c.page_shift;
       wait_vmcnt<0>();  // no load of the compiler's outstanding beside the DMA
-      const uint32_t ntile = (end - seg + 63u) / 64u;
+      const uint32_t ntile = (end - seg + kKeys - 1) / kKeys;
       fetch.issue(c, it, seg, first, pages, lds0);
       for (uint32_t j = 0; j < ntile; ++j) {
-        const uint32_t k0 = seg + 64u * j;
+        const uint32_t k0 = seg + kKeys * j;
         wait_vmcnt<0>();
         __syncthreads();
-        if (j + 1 < ntile) fetch.issue(c, it, k0 + 64u, first, pages, lds0 + ((j + 1) & 1u) * kStage);
+        if (j + 1 < ntile) fetch.issue(c, it, k0 + kKeys, first, pages, lds0 + ((j + 1) & 1u) * kStage);
         unsigned char *st = smem + uni((j & 1u) * kStage);
-        const bool none_odd = !bad && k0 + 64u <= it.kend && k0 + 64u <= all_block;  // the same in every wave
-        const bool mine = k0 < none, masked = !none_odd && (bad || k0 + 64u > it.kend || k0 + 64u > all);
-        uint32_t vis[KB] = {~0u, ~0u};
+        const bool none_odd = !bad && k0 + kKeys <= it.kend && k0 + kKeys <= all_block;  // the same in every wave
+        const bool mine = k0 < none, masked = !none_odd && (bad || k0 + kKeys > it.kend || k0 + kKeys > all);
+        uint32_t vis[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) vis[kb] = ~0u;
         if (masked) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
@@ -589,7 +606,7 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
           W::clear_odd(st, wave, NW);
           __syncthreads();
         }
-        if (mine) w.products(st, s);
+        if (mine) w.template products<TERMS>(st, s);
       }
       seg = end;
       // (the next pages' first barrier comes before any stage is filled again)
@@ -601,7 +618,7 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
       for (int q4 = 0; q4 < 4; ++q4) {
         const uint32_t col = 32u * d + 8u * q4 + 4u * w.lh;
         if (col < (uint32_t)D)
-          put<D, 128>(a, it, slot, 32u * wave + w.lq, col,
+          put<D, kRows>(a, it, slot, 32u * wave + w.lq, col,
                       make_float4(w.o[d][4 * q4], w.o[d][4 * q4 + 1], w.o[d][4 * q4 + 2], w.o[d][4 * q4 + 3]), w.m, w.l,
                       d == 0 && q4 == 0 && w.lh == 0);
       }
@@ -610,17 +627,29 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
 
 }  // namespace kv
 
-#define BWPP_ATTEND_BF16(D)                                                                                        \
-  extern "C" __global__ __launch_bounds__(128) void bwpp_cache_attend_few_d##D(const BwppCacheAttnArgs a) {         \
-    kv::attend_few<D, 2>(a);                                                                                       \
-  }                                                                                                                \
-  extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void bwpp_cache_attend_rows_d##D(const BwppCacheAttnArgs a) { \
-    kv::attend_rows<D>(a);                                                                                         \
+#define BWPP_ATTEND_FEW(D)                                                                                  \
+  extern "C" __global__ __launch_bounds__(128) void bwpp_cache_attend_few_d##D(const BwppCacheAttnArgs a) { \
+    kv::attend_few<D, 2>(a);                                                                                \
   }
-BWPP_ATTEND_BF16(64)
-BWPP_ATTEND_BF16(80)
-BWPP_ATTEND_BF16(96)
-BWPP_ATTEND_BF16(128)
-BWPP_ATTEND_BF16(160)
-BWPP_ATTEND_BF16(192)
-BWPP_ATTEND_BF16(256)
+#define BWPP_ATTEND_ROWS(ROWS, D, NW, BLOCKS)                                                                             \
+  extern "C" __global__ __launch_bounds__(64 * NW, BLOCKS) void bwpp_cache_attend_r##ROWS##_d##D(const BwppCacheAttnArgs a) { \
+    kv::attend_rows<D, NW>(a);                                                                                            \
+  }
+BWPP_ATTEND_FEW(64)
+BWPP_ATTEND_FEW(80)
+BWPP_ATTEND_FEW(96)
+BWPP_ATTEND_FEW(128)
+BWPP_ATTEND_FEW(160)
+BWPP_ATTEND_FEW(192)
+BWPP_ATTEND_FEW(256)
+BWPP_ATTEND_ROWS(128, 64, 4, 2)
+BWPP_ATTEND_ROWS(128, 80, 4, 2)
+BWPP_ATTEND_ROWS(128, 96, 4, 2)
+BWPP_ATTEND_ROWS(128, 128, 4, 2)
+BWPP_ATTEND_ROWS(128, 160, 4, 1)
+BWPP_ATTEND_ROWS(128, 192, 4, 1)
+BWPP_ATTEND_ROWS(128, 256, 4, 1)
+BWPP_ATTEND_ROWS(256, 64, 8, 1)
+BWPP_ATTEND_ROWS(256, 80, 8, 1)
+BWPP_ATTEND_ROWS(256, 96, 8, 1)
+BWPP_ATTEND_ROWS(256, 128, 8, 1)

@@ -18,9 +18,11 @@ enum CacheKernel {
   CK_APPEND_F32 = CK_APPEND_BF16 + 6,  // [interleaved][chunk 4, 1]
   CK_KEEP = CK_APPEND_F32 + 4,         // chunks of 16, 4, 2 bytes
   CK_ATTEND = CK_KEEP + 3,             // [bf16][rows][dim up to 64, 128, 192, 256]
-  CK_ATTEND_BF16 = CK_ATTEND + 16,     // [kFlashDims][few, rows]
-  CK_JOIN = CK_ATTEND_BF16 + 14,       // [bf16][rows], tiles of 32, of 128
-  CK_RULES = CK_JOIN + 6,              // [x bf16][y bf16]
+  CK_ATTEND_FEW = CK_ATTEND + 16,      // [kFlashDims]
+  CK_ATTEND_R128 = CK_ATTEND_FEW + 7,  // [kFlashDims]
+  CK_ATTEND_R256 = CK_ATTEND_R128 + 7, // [kFlashDims up to 128]
+  CK_JOIN = CK_ATTEND_R256 + 4,        // [bf16][rows], tiles of 32, 128, 256
+  CK_RULES = CK_JOIN + 7,              // [x bf16][y bf16]
   CK_COUNT = CK_RULES + 4
 };
 
@@ -57,25 +59,30 @@ const char *const bwpp_hip_cache_kernels[] = {
     "bwpp_cache_attend_bf16_rows_d192",
     "bwpp_cache_attend_bf16_rows_d256",
     "bwpp_cache_attend_few_d64",
-    "bwpp_cache_attend_rows_d64",
     "bwpp_cache_attend_few_d80",
-    "bwpp_cache_attend_rows_d80",
     "bwpp_cache_attend_few_d96",
-    "bwpp_cache_attend_rows_d96",
     "bwpp_cache_attend_few_d128",
-    "bwpp_cache_attend_rows_d128",
     "bwpp_cache_attend_few_d160",
-    "bwpp_cache_attend_rows_d160",
     "bwpp_cache_attend_few_d192",
-    "bwpp_cache_attend_rows_d192",
     "bwpp_cache_attend_few_d256",
-    "bwpp_cache_attend_rows_d256",
+    "bwpp_cache_attend_r128_d64",
+    "bwpp_cache_attend_r128_d80",
+    "bwpp_cache_attend_r128_d96",
+    "bwpp_cache_attend_r128_d128",
+    "bwpp_cache_attend_r128_d160",
+    "bwpp_cache_attend_r128_d192",
+    "bwpp_cache_attend_r128_d256",
+    "bwpp_cache_attend_r256_d64",
+    "bwpp_cache_attend_r256_d80",
+    "bwpp_cache_attend_r256_d96",
+    "bwpp_cache_attend_r256_d128",
     "bwpp_cache_join_f32",
     "bwpp_cache_join_f32_rows",
     "bwpp_cache_join_bf16",
     "bwpp_cache_join_bf16_rows",
     "bwpp_cache_join_bf16_32",
     "bwpp_cache_join_bf16_128",
+    "bwpp_cache_join_bf16_256",
     "bwpp_logit_rules_f32",
     "bwpp_logit_rules_f32_bf16",
     "bwpp_logit_rules_bf16_f32",
@@ -351,8 +358,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // Tiles of few rows, whose waves share the keys out, or of more, where each wave
   // has its own: by the rows that a sequence and key head has on average.
   const uint64_t mean = (T + cp.batch - 1) / cp.batch * g;
-  const bool many = mean > (flash >= 0 ? 32u : 16u);
-  const uint32_t rows = flash >= 0 ? (many ? 128u : 32u) : many ? 64u : 16u, Dp = (cp.dim + 3) / 4 * 4;
+  const uint32_t rows = flash < 0 ? (mean > 16 ? 64u : 16u) : mean <= 32 ? 32u : mean <= 128 || cp.dim > 128 ? 128u : 256u;
+  const uint32_t Dp = (cp.dim + 3) / 4 * 4;
   // Costs (kv_schedule.h) are counted in 64 bits and multiplied by the blocks.
   const long double worst = (long double)cp.heads * ((long double)T * g / rows + cp.batch) *
                             ((long double)g * (c.capacity + 256) + (long double)T * g + 2 * rows);
@@ -374,19 +381,25 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   a.scale_log2 = std::fabs(scale) * 1.4426950408889634f;
   a.flip = scale < 0.0f ? 1u : 0u;
   // Blocks as many as are resident at once, the same number on each XCD.
-  a.blocks = ((flash >= 0 && cp.dim > 128 ? 1 : 2) * cus_of(h) + 7) / 8 * 8;
+  a.blocks = ((rows == 256 || (flash >= 0 && cp.dim > 128) ? 1 : 2) * cus_of(h) + 7) / 8 * 8;
   a.inv_blocks = 1.0 / a.blocks;
   void *ws = nullptr;
   s = bwpp_hip_take_workspace(h, (size_t)2 * a.blocks * rows * (Dp + 2) * 4, &ws);
   if (s != BWPP_HIP_OK) return s;
   a.part_o = static_cast<float *>(ws);
   a.part_ml = a.part_o + (size_t)2 * a.blocks * rows * Dp;
-  const int kind = (cp.dtype == BWPP_HIP_BF16 ? 2 : 0) + (many ? 1 : 0);
-  const int attend = flash >= 0 ? CK_ATTEND_BF16 + 2 * flash + (many ? 1 : 0) : CK_ATTEND + 4 * kind + (int)((cp.dim - 1) / 64);
-  s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, flash >= 0 && !many ? 128 : 256, &a);
+  int attend, join;
+  if (flash >= 0) {
+    attend = flash + (rows == 32 ? CK_ATTEND_FEW : rows == 128 ? CK_ATTEND_R128 : CK_ATTEND_R256);
+    join = CK_JOIN + (rows == 32 ? 4 : rows == 128 ? 5 : 6);
+  } else {
+    const int kind = (cp.dtype == BWPP_HIP_BF16 ? 2 : 0) + (rows == 64 ? 1 : 0);
+    attend = CK_ATTEND + 4 * kind + (int)((cp.dim - 1) / 64);
+    join = CK_JOIN + kind;
+  }
+  s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, rows == 32 ? 128 : rows == 256 ? 512 : 256, &a);
   if (s != BWPP_HIP_OK) return s;
-  return bwpp_hip_launch_cache(h, flash >= 0 ? CK_JOIN + 4 + (many ? 1 : 0) : CK_JOIN + kind, a.blocks - 1,
-                               (rows + 15) / 16, 256, &a);
+  return bwpp_hip_launch_cache(h, join, a.blocks - 1, (rows + 15) / 16, 256, &a);
 }
 
 // ------------------------------------------------------------------- rules

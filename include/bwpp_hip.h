@@ -773,9 +773,12 @@ BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *q, const vo
  * (q_heads / heads).  o = softmax(scale q k) v; lse (may be NULL) [tokens][q_heads]
  * fp32 is the natural log-sum-exp.  A token that sees nothing gets 0 and -inf.
  * What lies in slots that a token does not see has no part in it, infinities and
- * NaN included.  Sums and probabilities are held in fp32.  Workspace: for
- * 2 (bf16 of some dims: 1) partial results a block of the device, at most 128
- * rows of dim + 2 floats each. */
+ * NaN included.  Scores, sums and the probabilities that lse has are fp32; bf16
+ * probabilities enter the product with v as two bf16 terms, or, for more than 32
+ * rows (tokens times q_heads / heads, on average) of dims 64, 80, 96, 128, 160, 192
+ * and 256, rounded to one.  Workspace: two partial results for each of one or two
+ * blocks a compute unit, 16 to 256 rows of dim + 2 floats each (at most 128 MiB on
+ * 256 of them), whatever the lengths. */
 BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const void *q, const void *k_cache, const void *v_cache,
                                                 const int32_t *table, const int32_t *starts, const int32_t *held,
                                                 const uint32_t *mask, void *o, float *lse,

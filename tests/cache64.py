@@ -111,16 +111,20 @@ def attention64(c, q, scale, sees=None):
     Bounds, u = 2^-24.  A score is a sum of d products in fp32, off by at most
     (d + 4) u S, S = |scale| sum |q k|; its exponential is off by that, by 2 u
     for the instruction and 2 u |score| for its scaling and offset: e.  bf16
-    kernels may hold a probability in two bf16 terms, 2^-16.  A sum over n keys
+    kernels hold a probability in two bf16 terms, 2^-16, or, where a key head has
+    more than 32 rows on average, rounded to one bf16 (half a step of 8 significant
+    bits: 2^-8 of it) for the weighted sum alone: r.  A sum over n keys
     adds n u to the weights' sum and to the weighted sum (running maxima,
     partial sums and joins rescale: 8 u and u for every 16 keys more, inside n u
-    + 64 u).  So o is off by (2 e + (2 n + 64) u) sum w |v| and its own
-    rounding, lse by e + (n + 64) u and 2 u |lse|."""
+    + 64 u).  So o is off by (2 e + r + (2 n + 64) u) sum w |v| and its own
+    rounding (e enters twice, by the weights and their sum, r once), lse by e +
+    (n + 64) u and 2 u |lse|."""
     T, Hq, d = q.shape
     o = torch.full((T, Hq, d), float("nan"), dtype=torch.float64, device="cuda")
     lse = torch.full((T, Hq), float("nan"), dtype=torch.float64, device="cuda")
     to, tl = torch.zeros_like(o), torch.zeros_like(lse)
     g = Hq // c.Hk
+    one = q.dtype == BF16 and -(-T // len(c.held)) * g > 32
     for s, (held, n) in enumerate(zip(c.held, c.new)):
         if n == 0:
             continue
@@ -146,7 +150,7 @@ def attention64(c, q, scale, sees=None):
             lse[r, h] = torch.where(total == 0, torch.full_like(total, -math.inf), total.log() + top[:, 0])
             e = (d + 4) * U * S + 2 * U + 2 * U * S + (2.0 ** -16 if q.dtype == BF16 else 0.0)
             size = (p[:, :, None] * vis.abs()).sum(dim=1)
-            to[r, h] = (2 * e + (2 * L + 64) * U)[:, None] * size + HALF_STEP[q.dtype] * o[r, h].abs()
+            to[r, h] = (2 * e + (2.0 ** -8 if one else 0.0) + (2 * L + 64) * U)[:, None] * size + HALF_STEP[q.dtype] * o[r, h].abs()
             tl[r, h] = e + (L + 64) * U + 2 * U * lse[r, h].abs().nan_to_num(0, 0, 0)
     return o, lse, to, tl
 
