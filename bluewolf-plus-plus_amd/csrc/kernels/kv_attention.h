@@ -82,20 +82,17 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
   constexpr uint32_t kRows = ROWS ? 64 : 16, kUnit = 64, kTile = 16;
   constexpr int KC = 4 * DC, kLd = 64 * DC + 4;
   typedef Work<kRows, kUnit> W;
-  __shared__ uint64_t wave_sums[kThreads / 64];
-  __shared__ Share share;
   __shared__ float os[ROWS ? 1 : 4][ROWS ? 1 : 16][ROWS ? 4 : kLd];
   __shared__ float ml[4][16][2];
   const BwppCacheArgs &c = a.c;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i16 = lane & 15u, grp = lane >> 4;
   const uint32_t D = c.dim, g = a.group, Dp = (D + 3u) & ~3u;
-  find_share<kRows, kUnit, kThreads>(a, &share, wave_sums);
+  const Share share = find_share<kRows, kUnit>(a);
   const Place to = share.to;
   Place at = share.from;
   const uint32_t pmask = (1u << c.page_shift) - 1u;
 
-  Seq q = {};
-  if (at.s < c.batch) q = seq_at(c, at.s);
+  Seq q = share.q;
   // A part of an item that began in another block is written even if it has no
   // keys: the join reads it.
   bool part = at.unit != 0;
@@ -328,31 +325,20 @@ template <class T, uint32_t kRows, uint32_t kUnit>
 __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
   typedef Work<kRows, kUnit> W;
   constexpr uint32_t kParts = 64;  // a round of them in LDS
-  __shared__ uint64_t wave_sums[kThreads / 64];
-  __shared__ Place item;
-  __shared__ uint32_t last;  // sharer with the item's last part; 0: nothing to join
   __shared__ float top[kJoin], sum[kJoin], factor[kParts][kJoin];
   const BwppCacheArgs &c = a.c;
-  const Costs<kRows, kUnit, kThreads> costs(a, wave_sums);
+  const Costs<kRows, kUnit> costs(a);
   const uint32_t b = blockIdx.x + 1, row0 = blockIdx.y * kJoin;
-  const uint64_t S = share_of(a, costs.total);
-  if (S * b >= costs.total) return;
-  if (threadIdx.x == 0) last = 0;
-  __syncthreads();
-  costs.at(a, S * b, [&](uint32_t s, const Seq &q, uint64_t at) {
-    uint64_t begin, end;
-    const Place p = W::find(a, s, q, S * b - at, begin, end);
-    if (p.unit == 0) return;
-    const uint64_t prev = S * (b - 1);
-    if (prev >= at + begin && W::unit(a, q, p.tile, prev - at - begin, end - begin) != 0) return;  // not the first
-    item = p;
-    uint32_t e = b;  // the last border before the item's end
-    while (S * (e + 1) < at + end) ++e;
-    last = e;
-  });
-  __syncthreads();
-  if (last == 0) return;
-  const Seq q = seq_at(c, item.s);
+  const uint64_t S = share_of(a, costs.total), x = S * b;
+  if (x >= costs.total) return;
+  Seq q;
+  uint64_t before, begin, end;
+  const uint32_t seq = costs.at(a, x, q, before);
+  const Place item = W::find(a, seq, q, x - before, begin, end);
+  if (item.unit == 0) return;
+  if (x - S >= before + begin && W::unit(a, q, item.tile, x - S - before - begin, end - begin) != 0) return;  // not the first
+  uint32_t last = b;  // the last border before the item's end
+  while (S * (last + 1) < before + end) ++last;
   const uint32_t g = a.group, D = c.dim, n4 = (D + 3u) / 4u, Dp = 4u * n4;
   const uint32_t all = min(kRows, q.n * g - item.tile * kRows), parts = last - b + 2;
   if (row0 >= all) return;

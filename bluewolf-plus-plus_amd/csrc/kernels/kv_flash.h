@@ -396,23 +396,20 @@ __device__ __forceinline__ const uint16_t *query_row(const BwppCacheAttnArgs &a,
 }
 
 // Walks a block's share: f(item, slot of its part).
-template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS, class F>
+template <uint32_t ROWS, uint32_t UNIT, class F>
 __device__ __forceinline__ void for_items(const BwppCacheAttnArgs &a, F f) {
   typedef Work<ROWS, UNIT> W;
-  __shared__ uint64_t wave_sums[THREADS / 64];
-  __shared__ Share share;
-  find_share<ROWS, UNIT, THREADS>(a, &share, wave_sums);
+  const Share share = find_share<ROWS, UNIT>(a);
   const uint32_t b = uni(share.b);
   Place at = {uni(share.from.s), uni(share.from.head), uni(share.from.tile), uni(share.from.unit)};
   const Place to = {uni(share.to.s), uni(share.to.head), uni(share.to.tile), uni(share.to.unit)};
   Item it = {};
-  auto sequence = [&]() {
-    const Seq q = seq_at(a.c, at.s);
+  auto sequence = [&](const Seq &q) {
     it.q = {uni(q.first), uni(q.n), uni(q.held)};
     it.s = at.s;
     it.R = it.q.n * a.group;
   };
-  if (at.s < a.c.batch) sequence();
+  sequence(share.q);
   // A part of an item that began in another block is written even if it has no
   // keys: the join reads it.
   bool part = at.unit != 0;
@@ -433,7 +430,7 @@ __device__ __forceinline__ void for_items(const BwppCacheAttnArgs &a, F f) {
         do {
           ++at.s;
           if (at.s >= a.c.batch) break;
-          sequence();
+          sequence(seq_at(a.c, at.s));
         } while (it.q.n == 0);
       }
     }
@@ -458,7 +455,7 @@ __device__ __forceinline__ void attend_few(const BwppCacheAttnArgs &a) {
   F fetch;
   fetch.place(c, 0);
 
-  for_items<32, 64, 64 * NW>(a, [&](const Item &it, uint32_t slot) {
+  for_items<32, 64>(a, [&](const Item &it, uint32_t slot) {
     uint32_t tok;
     const uint16_t *Q = query_row<D, 1>(a, it, it.tile * 32u + w.lq, tok);
     w.start(Q, a.scale_log2, a.flip);
@@ -558,7 +555,7 @@ __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
   F fetch;
   fetch.place(c, wave);
 
-  for_items<kRows, 64, 64 * NW>(a, [&](const Item &it, uint32_t slot) {
+  for_items<kRows, 64>(a, [&](const Item &it, uint32_t slot) {
     uint32_t tok;
     const uint32_t row0 = it.tile * kRows + 32u * wave;
     const uint16_t *Q = query_row<D, KB>(a, it, row0 + w.lq, tok);

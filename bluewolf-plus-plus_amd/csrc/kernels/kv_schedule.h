@@ -24,8 +24,8 @@
 
 namespace kv {
 
-constexpr uint32_t kItem = 96;      // keys that an item costs by itself
-constexpr uint32_t kLeast = 192;    // a block's share is at least as many keys
+constexpr uint32_t kItem = 96;   // keys that an item costs by itself
+constexpr uint32_t kLeast = 64;  // a block's share is at least as many keys
 
 // A place in the order of the work.
 struct Place {
@@ -38,6 +38,7 @@ __device__ __forceinline__ bool earlier(const Place &a, const Place &b) {
 }
 struct Share {
   Place from, to;
+  Seq q;       // from's sequence
   uint32_t b;  // whose it is
 };
 
@@ -83,53 +84,53 @@ struct Work {
   }
 };
 
-// Costs of the sequences that this thread adds up (a run of `per`), the costs
-// before them, and the total.
-template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 | lo;
+}
+
+// Costs of all sequences, in every wave by itself (no barrier: a short call is
+// a chain of latencies): a lane adds up a run of `per` sequences.
+template <uint32_t ROWS, uint32_t UNIT>
 struct Costs {
-  uint32_t s0, s1;
-  uint64_t first, total;
+  uint32_t per;
+  Seq q;           // of the lane's first sequence
+  uint64_t first;  // costs before the lane's
+  uint64_t mine, total;
 
   static __device__ __forceinline__ uint64_t of(const BwppCacheAttnArgs &a, const Seq &q) {
     return a.c.heads * Work<ROWS, UNIT>::before(q, a.group, Work<ROWS, UNIT>::tiles(q, a.group));
   }
-  __device__ __forceinline__ Costs(const BwppCacheAttnArgs &a, uint64_t *wave_sums) {
-    const uint32_t per = (a.c.batch + THREADS - 1) / THREADS;
-    s0 = min(threadIdx.x * per, a.c.batch);
-    s1 = min(s0 + per, a.c.batch);
-    uint64_t mine = 0;
-    for (uint32_t s = s0; s < s1; ++s) mine += of(a, seq_at(a.c, s));
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __device__ __forceinline__ Costs(const BwppCacheAttnArgs &a) {
+    const uint32_t lane = threadIdx.x & 63u;
+    per = (a.c.batch + 63u) / 64u;
+    const uint32_t s0 = min(lane * per, a.c.batch), s1 = min(s0 + per, a.c.batch);
+    q = {0, 0, 0};
+    if (s0 < s1) q = seq_at(a.c, s0);
+    mine = of(a, q);
+#pragma unroll 4
+    for (uint32_t s = s0 + 1; s < s1; ++s) mine += of(a, seq_at(a.c, s));
     uint64_t sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const uint64_t up = __shfl_up(sum, d, 64);
       if (lane >= (uint32_t)d) sum += up;
     }
-    if (lane == 63) wave_sums[wave] = sum;
-    __syncthreads();
     first = sum - mine;
-    total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < THREADS / 64; ++w) {
-      if (w < wave) first += wave_sums[w];
-      total += wave_sums[w];
-    }
+    total = lane_of(sum, 63);
   }
-  // Calls f(sequence, its cost range) in the thread that has the sequence of cost x.
-  template <class F>
-  __device__ __forceinline__ void at(const BwppCacheAttnArgs &a, uint64_t x, F f) const {
-    uint64_t begin = first;
-    if (x < begin) return;
-    for (uint32_t s = s0; s < s1; ++s) {
-      const Seq q = seq_at(a.c, s);
-      const uint64_t end = begin + of(a, q);
-      if (x < end) {
-        f(s, q, begin);
-        return;
-      }
-      begin = end;
+  // The sequence of cost x < total, and the costs before it.
+  __device__ __forceinline__ uint32_t at(const BwppCacheAttnArgs &a, uint64_t x, Seq &at, uint64_t &begin) const {
+    const int lane = __builtin_ctzll(__ballot(x >= first && x - first < mine));
+    uint32_t s = (uint32_t)lane * per;
+    begin = lane_of(first, lane);
+    at = {(uint32_t)__builtin_amdgcn_readlane((int)q.first, lane), (uint32_t)__builtin_amdgcn_readlane((int)q.n, lane),
+          (uint32_t)__builtin_amdgcn_readlane((int)q.held, lane)};
+    for (uint64_t c = of(a, at); x - begin >= c; c = of(a, at)) {
+      begin += c;
+      at = seq_at(a.c, ++s);  // (the run's last sequence ends past x)
     }
+    return s;
   }
 };
 
@@ -139,28 +140,26 @@ __device__ __forceinline__ uint64_t share_of(const BwppCacheAttnArgs &a, uint64_
   return even < least ? least : even;
 }
 
-// The share of this block, the same in every thread (`share` in LDS).
-template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
-__device__ __forceinline__ void find_share(const BwppCacheAttnArgs &a, Share *share, uint64_t *wave_sums) {
+// The share of this block.
+template <uint32_t ROWS, uint32_t UNIT>
+__device__ __forceinline__ Share find_share(const BwppCacheAttnArgs &a) {
+  typedef Work<ROWS, UNIT> W;
   constexpr uint32_t kXcds = 8;  // blocks go to them in turn
-  const Costs<ROWS, UNIT, THREADS> costs(a, wave_sums);
+  const Costs<ROWS, UNIT> costs(a);
   const uint64_t S = share_of(a, costs.total);
   const uint32_t sharers = min((uint32_t)((double)costs.total / (double)S) + 1u, a.blocks), per = (sharers + kXcds - 1) / kXcds;
-  const uint32_t b = blockIdx.x % kXcds * per + blockIdx.x / kXcds;
-  if (threadIdx.x == 0) {
-    share->from = share->to = {a.c.batch, 0, 0, 0};
-    share->b = b;
+  Share share = {{a.c.batch, 0, 0, 0}, {a.c.batch, 0, 0, 0}, {0, 0, 0}, blockIdx.x % kXcds * per + blockIdx.x / kXcds};
+  const uint64_t x0 = S * share.b, x1 = x0 + S;
+  if (blockIdx.x / kXcds >= per || x0 >= costs.total) return share;
+  uint64_t begin, end, before;
+  uint32_t s = costs.at(a, x0, share.q, before);
+  share.from = W::find(a, s, share.q, x0 - before, begin, end);
+  if (x1 < costs.total) {
+    Seq q;
+    s = costs.at(a, x1, q, before);
+    share.to = W::find(a, s, q, x1 - before, begin, end);
   }
-  __syncthreads();
-  if (blockIdx.x / kXcds >= per || b >= a.blocks) return;
-  uint64_t begin, end;
-  costs.at(a, S * b, [&](uint32_t s, const Seq &q, uint64_t at) {
-    share->from = Work<ROWS, UNIT>::find(a, s, q, S * b - at, begin, end);
-  });
-  costs.at(a, S * (b + 1), [&](uint32_t s, const Seq &q, uint64_t at) {
-    share->to = Work<ROWS, UNIT>::find(a, s, q, S * (b + 1) - at, begin, end);
-  });
-  __syncthreads();
+  return share;
 }
 
 }  // namespace kv
