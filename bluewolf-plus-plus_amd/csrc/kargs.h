@@ -306,6 +306,7 @@ typedef struct {
   uint32_t flip;        /* 1: the scale is negative */
   uint32_t blocks;      /* blocks that share the keys */
   double inv_blocks;    /* 1 / blocks */
+  uint32_t whole_keys;  /* sequences up to here have whole items */
   float *part_o;        /* [2 blocks][rows of a tile][dim up to a multiple of 4] */
   float *part_ml;       /* [2 blocks][rows of a tile][2] */
 } BwppCacheAttnArgs;

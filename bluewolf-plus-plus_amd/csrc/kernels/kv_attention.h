@@ -319,72 +319,86 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
 }
 
 // Joins the parts of the item that the border before sharer b is the first to
-// divide (b = 1 .. blocks - 1: blockIdx.x), kJoin rows of it a block.
-constexpr uint32_t kJoin = 16;
+// divide (b = 1 .. blocks - 1), kJoin rows of it a block: blockIdx.y's.  A chain of
+// latencies, so the parts' pairs and first sums are fetched at once, and every
+// thread makes its row's factors by itself.
 template <class T, uint32_t kRows, uint32_t kUnit>
 __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
   typedef Work<kRows, kUnit> W;
-  constexpr uint32_t kParts = 64;  // a round of them in LDS
-  __shared__ float top[kJoin], sum[kJoin], factor[kParts][kJoin];
+  constexpr uint32_t kJoin = 16;                       // rows a block
+  constexpr uint32_t kParts = 64;                      // a round of them in LDS
+  constexpr uint32_t kMost = kJoin * 64u / kThreads;   // float4 a thread, dim 256
+  constexpr uint32_t kAhead = 16;                      // sums on the way at once; the first with the pairs
+  __shared__ float2 pair[kParts][kJoin];
   const BwppCacheArgs &c = a.c;
   const Costs<kRows, kUnit> costs(a);
   const uint32_t b = blockIdx.x + 1, row0 = blockIdx.y * kJoin;
   const uint64_t S = share_of(a, costs.total), x = S * b;
-  if (x >= costs.total) return;
+  if (costs.whole || x >= costs.total) return;
   Seq q;
   uint64_t before, begin, end;
   const uint32_t seq = costs.at(a, x, q, before);
-  const Place item = W::find(a, seq, q, x - before, begin, end);
+  const Place item = W::find(a, false, seq, q, x - before, begin, end);
   if (item.unit == 0) return;
   if (x - S >= before + begin && W::unit(a, q, item.tile, x - S - before - begin, end - begin) != 0) return;  // not the first
-  uint32_t last = b;  // the last border before the item's end
-  while (S * (last + 1) < before + end) ++last;
   const uint32_t g = a.group, D = c.dim, n4 = (D + 3u) / 4u, Dp = 4u * n4;
-  const uint32_t all = min(kRows, q.n * g - item.tile * kRows), parts = last - b + 2;
+  const uint32_t all = min(kRows, q.n * g - item.tile * kRows);
   if (row0 >= all) return;
-  const uint32_t rows = min(kJoin, all - row0);
+  uint32_t last = (uint32_t)((double)(before + end - 1) / (double)S);  // the last border before the item's end
+  if (S * last >= before + end) --last;  // (a quotient rounded up)
+  const uint32_t rows = min(kJoin, all - row0), parts = last - b + 2;
   // part 0 in slot 2 (b - 1) + 1, part k in slot 2 (b + k - 1)
   auto slot_row = [&](uint32_t k) { return (uint64_t)(k == 0 ? 2 * b - 1 : 2 * (b + k - 1)) * kRows + row0; };
-  // The rows' exponent offsets and sums: 16 threads a row.
-  {
-    const uint32_t r = threadIdx.x / 16u, j = threadIdx.x % 16u;
-    float m = -INFINITY;
-    if (r < rows)
-      for (uint32_t k = j; k < parts; k += 16u) m = fmaxf(m, a.part_ml[2 * (slot_row(k) + r)]);
+  auto sums = [&](uint32_t k, uint32_t r, uint32_t col) {
+    return *reinterpret_cast<const float4 *>(a.part_o + (slot_row(k) + r) * Dp + col);
+  };
+  float4 v[kMost], u[kAhead];
+  float m[kMost], l[kMost];
 #pragma unroll
-    for (int d = 1; d < 16; d *= 2) m = fmaxf(m, __shfl_xor(m, d, 64));
-    float l = 0.0f;
-    if (r < rows)
-      for (uint32_t k = j; k < parts; k += 16u) {
-        const float2 w = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (slot_row(k) + r));
-        l += w.y * (w.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.x - m));
-      }
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) l += __shfl_xor(l, d, 64);
-    if (j == 0) top[r] = m, sum[r] = l;
+  for (uint32_t e = 0; e < kMost; ++e) {
+    const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
+    v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    m[e] = -INFINITY;
+    l[e] = 0.0f;
   }
-  constexpr uint32_t kMost = kJoin * 64u / kThreads;  // float4 a thread, dim 256
-  float4 v[kMost];
+  auto fetch = [&](uint32_t k, uint32_t n, uint32_t r, uint32_t col) {  // parts k .. below n
 #pragma unroll
-  for (uint32_t e = 0; e < kMost; ++e) v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t j = 0; j < kAhead; ++j)
+      u[j] = k + j < n ? sums(k + j, r, col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  if (threadIdx.x / n4 < rows) fetch(0, parts, threadIdx.x / n4, 4u * (threadIdx.x % n4));
   for (uint32_t k0 = 0; k0 < parts; k0 += kParts) {
     const uint32_t n = min(kParts, parts - k0);
-    __syncthreads();
+    if (k0) __syncthreads();
     for (uint32_t i = threadIdx.x; i < n * kJoin; i += kThreads) {
       const uint32_t k = i / kJoin, r = i % kJoin;
-      const float w = r < rows ? a.part_ml[2 * (slot_row(k0 + k) + r)] : -INFINITY;
-      factor[k][r] = w == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w - top[r]);
+      if (r < rows) pair[k][r] = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (slot_row(k0 + k) + r));
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t e = 0; e < kMost; ++e) {
       const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
       if (r >= rows) continue;
-#pragma unroll 8
-      for (uint32_t k = 0; k < n; ++k) {
-        const float4 u = *reinterpret_cast<const float4 *>(a.part_o + (slot_row(k0 + k) + r) * Dp + col);
-        const float f = factor[k][r];
-        v[e].x += u.x * f, v[e].y += u.y * f, v[e].z += u.z * f, v[e].w += u.w * f;
+      float top = m[e];
+      for (uint32_t k = 0; k < n; ++k) top = fmaxf(top, pair[k][r].x);
+      // no key seen (offset -inf): sums of 0 (or NaN, kept)
+      auto factor = [&](float o) { return o == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(o - top); };
+      if (k0) {
+        const float f = factor(m[e]);
+        l[e] *= f;
+        v[e].x *= f, v[e].y *= f, v[e].z *= f, v[e].w *= f;
+      }
+      m[e] = top;
+      for (uint32_t k = 0; k < n; k += kAhead) {
+        if (e || k0 || k) fetch(k0 + k, k0 + n, r, col);
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+          if (k + j >= n) break;
+          const float2 w = pair[k + j][r];
+          const float f = factor(w.x);
+          l[e] += w.y * f;
+          v[e].x += u[j].x * f, v[e].y += u[j].y * f, v[e].z += u[j].z * f, v[e].w += u[j].w * f;
+        }
       }
     }
   }
@@ -394,10 +408,11 @@ __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
     if (r >= rows) continue;
     const uint32_t rr = item.tile * kRows + row0 + r;
     const uint64_t t = q.first + rr / g, hh = item.head * g + rr % g;
-    const float l = sum[r], inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
     const float u[4] = {v[e].x * inv, v[e].y * inv, v[e].z * inv, v[e].w * inv};
     store4(static_cast<T *>(a.o) + t * a.o_ts + hh * a.o_hs, col, D, u);
-    if (col == 0 && a.lse) a.lse[t * (uint64_t)(c.heads * g) + hh] = l == 0.0f ? -INFINITY : lse_of(top[r] == -INFINITY ? 0.0f : top[r], l);
+    if (col == 0 && a.lse)
+      a.lse[t * (uint64_t)(c.heads * g) + hh] = l[e] == 0.0f ? -INFINITY : lse_of(m[e] == -INFINITY ? 0.0f : m[e], l[e]);
   }
 }
 

@@ -11,7 +11,9 @@
 // to whole units.  An item whose keys fall to several blocks is left by each
 // as a triple (exponent offset, sum of p, sum of p v) and joined by a second
 // launch: the sharer where it begins leaves it in slot 2 b + 1, the others,
-// for which it is the first item, in slot 2 b.  The sharers of one XCD are
+// for which it is the first item, in slot 2 b.  Where all sequences are short
+// items are left whole, since parts cost more than an even share gains (and
+// where the table's width says so, there is no second launch).  The sharers of one XCD are
 // neighbours: the tiles of a head meet its keys in one L2.
 //
 // Costs are whole numbers below 2^52, g times keys (g query heads a key head);
@@ -59,7 +61,7 @@ struct Work {
   }
   // Where cost x of sequence s (all its heads) falls, and the costs where that
   // item begins and ends.
-  static __device__ __forceinline__ Place find(const BwppCacheAttnArgs &a, uint32_t s, const Seq &q, uint64_t x,
+  static __device__ __forceinline__ Place find(const BwppCacheAttnArgs &a, bool whole, uint32_t s, const Seq &q, uint64_t x,
                                                uint64_t &begin, uint64_t &end) {
     const uint32_t T = tiles(q, a.group);
     const uint64_t head_cost = before(q, a.group, T);
@@ -75,7 +77,7 @@ struct Work {
     const uint64_t b0 = before(q, a.group, lo), b1 = before(q, a.group, lo + 1);
     begin = head * head_cost + b0;
     end = head * head_cost + b1;
-    return {s, head, lo, unit(a, q, lo, rest - b0, b1 - b0)};
+    return {s, head, lo, whole ? 0u : unit(a, q, lo, rest - b0, b1 - b0)};
   }
   static __device__ __forceinline__ uint32_t unit(const BwppCacheAttnArgs &a, const Seq &q, uint32_t tile, uint64_t off,
                                                   uint64_t cost) {
@@ -97,6 +99,7 @@ struct Costs {
   Seq q;           // of the lane's first sequence
   uint64_t first;  // costs before the lane's
   uint64_t mine, total;
+  bool whole;      // every sequence is so short that its items are not shared
 
   static __device__ __forceinline__ uint64_t of(const BwppCacheAttnArgs &a, const Seq &q) {
     return a.c.heads * Work<ROWS, UNIT>::before(q, a.group, Work<ROWS, UNIT>::tiles(q, a.group));
@@ -108,8 +111,14 @@ struct Costs {
     q = {0, 0, 0};
     if (s0 < s1) q = seq_at(a.c, s0);
     mine = of(a, q);
+    uint32_t most = q.n ? q.held + q.n : 0u;
 #pragma unroll 4
-    for (uint32_t s = s0 + 1; s < s1; ++s) mine += of(a, seq_at(a.c, s));
+    for (uint32_t s = s0 + 1; s < s1; ++s) {
+      const Seq t = seq_at(a.c, s);
+      mine += of(a, t);
+      most = max(most, t.n ? t.held + t.n : 0u);
+    }
+    whole = __ballot(most > a.whole_keys) == 0;
     uint64_t sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -153,11 +162,11 @@ __device__ __forceinline__ Share find_share(const BwppCacheAttnArgs &a) {
   if (blockIdx.x / kXcds >= per || x0 >= costs.total) return share;
   uint64_t begin, end, before;
   uint32_t s = costs.at(a, x0, share.q, before);
-  share.from = W::find(a, s, share.q, x0 - before, begin, end);
+  share.from = W::find(a, costs.whole, s, share.q, x0 - before, begin, end);
   if (x1 < costs.total) {
     Seq q;
     s = costs.at(a, x1, q, before);
-    share.to = W::find(a, s, q, x1 - before, begin, end);
+    share.to = W::find(a, costs.whole, s, q, x1 - before, begin, end);
   }
   return share;
 }

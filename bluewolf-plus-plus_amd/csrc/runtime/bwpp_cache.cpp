@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "../kargs.h"
 
@@ -358,7 +359,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // Tiles of few rows, whose waves share the keys out, or of more, where each wave
   // has its own: by the rows that a sequence and key head has on average.
   const uint64_t mean = (T + cp.batch - 1) / cp.batch * g;
-  const uint32_t rows = flash < 0 ? (mean > 16 ? 64u : 16u) : mean <= 32 ? 32u : mean <= 128 || cp.dim > 128 ? 128u : 256u;
+  const uint32_t r256 = getenv("W_R") ? (uint32_t)atoi(getenv("W_R")) : 128;
+  const uint32_t rows = flash < 0 ? (mean > 16 ? 64u : 16u) : mean <= 32 ? 32u : mean <= r256 || cp.dim > 128 ? 128u : 256u;
   const uint32_t Dp = (cp.dim + 3) / 4 * 4;
   // Costs (kv_schedule.h) are counted in 64 bits and multiplied by the blocks.
   const long double worst = (long double)cp.heads * ((long double)T * g / rows + cp.batch) *
@@ -383,11 +385,15 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // Blocks as many as are resident at once, the same number on each XCD.
   a.blocks = ((rows == 256 || (flash >= 0 && cp.dim > 128) ? 1 : 2) * cus_of(h) + 7) / 8 * 8;
   a.inv_blocks = 1.0 / a.blocks;
-  void *ws = nullptr;
-  s = bwpp_hip_take_workspace(h, (size_t)2 * a.blocks * rows * (Dp + 2) * 4, &ws);
-  if (s != BWPP_HIP_OK) return s;
-  a.part_o = static_cast<float *>(ws);
-  a.part_ml = a.part_o + (size_t)2 * a.blocks * rows * Dp;
+  a.whole_keys = getenv("W_K") ? (uint32_t)atoi(getenv("W_K")) : flash >= 0 ? 512 : rows == 64 ? 128 : 256;
+  const bool parts = c.capacity > a.whole_keys;
+  if (parts) {
+    void *ws = nullptr;
+    s = bwpp_hip_take_workspace(h, (size_t)2 * a.blocks * rows * (Dp + 2) * 4, &ws);
+    if (s != BWPP_HIP_OK) return s;
+    a.part_o = static_cast<float *>(ws);
+    a.part_ml = a.part_o + (size_t)2 * a.blocks * rows * Dp;
+  }
   int attend, join;
   if (flash >= 0) {
     attend = flash + (rows == 32 ? CK_ATTEND_FEW : rows == 128 ? CK_ATTEND_R128 : CK_ATTEND_R256);
@@ -398,7 +404,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
     join = CK_JOIN + kind;
   }
   s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, rows == 32 ? 128 : rows == 256 ? 512 : 256, &a);
-  if (s != BWPP_HIP_OK) return s;
+  if (s != BWPP_HIP_OK || !parts) return s;
   return bwpp_hip_launch_cache(h, join, a.blocks - 1, (rows + 15) / 16, 256, &a);
 }
 
