@@ -2,4 +2,5 @@
 // attention) and rules on logits.
 #include "kv_append.h"
 #include "kv_attention.h"
+#include "kv_rows.h"
 #include "logit_rules.h"

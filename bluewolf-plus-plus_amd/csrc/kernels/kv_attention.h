@@ -17,14 +17,13 @@
 // lane (column 64 j + 4 i + c is row i of product (j, c)).  So nothing passes
 // through LDS but the sums at the end.
 //
-// Few rows (ROWS false): the block's four waves take every fourth tile of keys
-// and their sums meet in LDS.  More rows (ROWS true): each wave has 16 rows of
-// its own and walks all keys.
+// A block's four waves take every fourth tile of its 16 rows' keys, and their
+// sums meet in LDS.  More rows are kv_rows.h's.
 #pragma once
 
 #include "attention_common.h"
 #include "kv_cache.h"
-#include "kv_schedule.h"
+#include "kv_items.h"
 #include "rotary_math.h"
 #include "../kargs.h"
 
@@ -35,9 +34,9 @@ namespace kv {
 constexpr uint32_t kThreads = 256;
 
 // Four elements from column c of a row of `dim`, zeros past it.
-template <class T, bool VEC>
+template <class T>
 __device__ __forceinline__ void load4(const T *row, uint32_t c, uint32_t dim, float (&o)[4]) {
-  if (VEC || c + 4 <= dim) {
+  if (c + 4 <= dim) {
     rotary_pos::Vec<T, 4>::load(row + c, o);
   } else {
 #pragma unroll
@@ -62,60 +61,31 @@ __device__ __forceinline__ void store4(T *row, uint32_t c, uint32_t dim, const f
   }
 }
 
-// Bits 0 .. 15: whether the token `i` (of a sequence that begins at row first)
-// sees the new tokens j0 .. j0 + 15 of it.
-__device__ __forceinline__ uint32_t mask_bits(const BwppCacheAttnArgs &a, uint32_t first, uint32_t i, int64_t j0) {
-  if (!a.mask) {
-    const int64_t seen = (int64_t)i + 1 - j0;  // of the 16
-    return seen <= 0 ? 0u : seen >= 16 ? 0xffffu : (1u << seen) - 1u;
-  }
-  uint64_t two = 0;
-  const uint32_t *row = a.mask + (uint64_t)(first + i) * a.mask_words;
-  const int64_t w = j0 >> 5;
-  if (w >= 0 && w < (int64_t)a.mask_words) two = row[w];
-  if (w + 1 >= 0 && w + 1 < (int64_t)a.mask_words) two |= (uint64_t)row[w + 1] << 32;
-  return (uint32_t)(two >> (j0 & 31)) & 0xffffu;
-}
-
-template <class T, int DC, bool ROWS>
-__device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
-  constexpr uint32_t kRows = ROWS ? 64 : 16, kUnit = 64, kTile = 16;
+template <class T, int DC>
+__device__ __forceinline__ void attend_split(const BwppCacheAttnArgs &a) {
+  constexpr uint32_t kRows = 16, kUnit = 64, kTile = 16, kStep = 4 * kTile;
   constexpr int KC = 4 * DC, kLd = 64 * DC + 4;
-  typedef Work<kRows, kUnit> W;
-  __shared__ float os[ROWS ? 1 : 4][ROWS ? 1 : 16][ROWS ? 4 : kLd];
+  __shared__ float os[4][16][kLd];
   __shared__ float ml[4][16][2];
   const BwppCacheArgs &c = a.c;
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, i16 = lane & 15u, grp = lane >> 4;
-  const uint32_t D = c.dim, g = a.group, Dp = (D + 3u) & ~3u;
-  const Share share = find_share<kRows, kUnit>(a);
-  const Place to = share.to;
-  Place at = share.from;
-  const uint32_t pmask = (1u << c.page_shift) - 1u;
+  const uint32_t lane = threadIdx.x & 63u, wave = uni(threadIdx.x >> 6), i16 = lane & 15u, grp = lane >> 4;
+  const uint32_t D = c.dim, g = a.group, Dp = (D + 3u) & ~3u, pmask = (1u << c.page_shift) - 1u;
+  const float scale = a.flip ? -a.scale_log2 : a.scale_log2;
 
-  Seq q = share.q;
-  // A part of an item that began in another block is written even if it has no
-  // keys: the join reads it.
-  bool part = at.unit != 0;
-  for (; part || earlier(at, to); part = false) {
-    const bool same = at.s == to.s && at.head == to.head && at.tile == to.tile;
-    const uint32_t total = W::units(a, q, at.tile), u1 = same ? to.unit : total;  // (to.unit >= at.unit)
-    const bool whole = at.unit == 0 && u1 == total;
-    const uint32_t kbeg = at.unit * kUnit, kend = min(u1 * kUnit, W::keys(a, q, at.tile));
-    const uint32_t R = q.n * g, r0 = at.tile * kRows + (ROWS ? 16u * wave : 0u);
-    const uint32_t row = r0 + i16, tok = min(row, R - 1u) / g, hq = at.head * g + min(row, R - 1u) % g;
+  for_items<kRows, kUnit>(a, [&](const Item &it, uint32_t slot) {
+    const uint32_t row = min(it.tile * kRows + i16, it.R - 1u), tok = row / g, hq = it.head * g + row % g;
     float qf[KC][4];
     {
-      const T *Q = static_cast<const T *>(a.q) + (uint64_t)(q.first + tok) * a.q_ts + (uint64_t)hq * a.q_hs;
+      const T *Q = static_cast<const T *>(a.q) + (uint64_t)(it.q.first + tok) * a.q_ts + (uint64_t)hq * a.q_hs;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
-        if (16u * j < D) load4<T, false>(Q, 16u * j + 4u * grp, D, qf[j]);
+        if (16u * j < D) load4(Q, 16u * j + 4u * grp, D, qf[j]);
         else qf[j][0] = qf[j][1] = qf[j][2] = qf[j][3] = 0.0f;
       }
     }
-    const float scale = a.flip ? -a.scale_log2 : a.scale_log2;
-    const T *K = static_cast<const T *>(c.k) + (uint64_t)at.head * c.head_s;
-    const T *V = static_cast<const T *>(c.v) + (uint64_t)at.head * c.head_s;
-    const int32_t *table = c.table + (uint64_t)at.s * c.ld_table;
+    const T *K = static_cast<const T *>(c.k) + (uint64_t)it.head * c.head_s;
+    const T *V = static_cast<const T *>(c.v) + (uint64_t)it.head * c.head_s;
+    const int32_t *table = c.table + (uint64_t)it.s * c.ld_table;
 
     f32x4_t o[DC][4];
 #pragma unroll
@@ -124,11 +94,10 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
       for (int e = 0; e < 4; ++e) o[j][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
 
-    const uint32_t step = ROWS ? kTile : 4u * kTile;
-    uint32_t k0 = kbeg + (ROWS ? 0u : kTile * wave);
+    uint32_t k0 = it.kbeg + kTile * wave;
     // A lane's key of the tile at k: its row's offset, kNoSlot past the keys or
     // outside the pool.  Page numbers are fetched one tile ahead.
-    auto page = [&](uint32_t k) { return k + i16 < kend ? (uint32_t)table[(k + i16) >> c.page_shift] : ~0u; };
+    auto page = [&](uint32_t k) { return k + i16 < it.kend ? (uint32_t)table[(k + i16) >> c.page_shift] : ~0u; };
     auto offset = [&](uint32_t k, uint32_t pg) {
       return pg < c.pages ? (uint64_t)pg * c.page_s + (uint64_t)((k + i16) & pmask) * c.tok_s : kNoSlot;
     };
@@ -137,17 +106,17 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
         kf[j][0] = kf[j][1] = kf[j][2] = kf[j][3] = 0.0f;
-        if (16u * j < D && off != kNoSlot) load4<T, false>(K + off, 16u * j + 4u * grp, D, kf[j]);
+        if (16u * j < D && off != kNoSlot) load4(K + off, 16u * j + 4u * grp, D, kf[j]);
       }
     };
     uint64_t off = kNoSlot;
     uint32_t next_page = ~0u;
-    if (k0 < kend) {
+    if (k0 < it.kend) {
       off = offset(k0, page(k0));
-      next_page = page(k0 + step);
+      next_page = page(k0 + kStep);
       load_keys(off);
     }
-    for (; k0 < kend; k0 += step) {
+    for (; k0 < it.kend; k0 += kStep) {
       float vf[4][DC][4];
       bool live[4];
 #pragma unroll
@@ -157,7 +126,7 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
 #pragma unroll
         for (int j = 0; j < DC; ++j) {
           vf[r][j][0] = vf[r][j][1] = vf[r][j][2] = vf[r][j][3] = 0.0f;
-          if (live[r] && 64u * j + 4u * i16 < D) load4<T, false>(V + ov, 64u * j + 4u * i16, D, vf[r][j]);
+          if (live[r] && 64u * j + 4u * i16 < D) load4(V + ov, 64u * j + 4u * i16, D, vf[r][j]);
         }
       }
       f32x4_t s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
@@ -169,15 +138,15 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
         s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][2], qf[j][2], s0, 0, 0, 0);
         s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][3], qf[j][3], s1, 0, 0, 0);
       }
-      off = offset(k0 + step, next_page);
-      next_page = page(k0 + 2 * step);
+      off = offset(k0 + kStep, next_page);
+      next_page = page(k0 + 2 * kStep);
       load_keys(off);
       // Visible keys of this lane's row among its four.
       uint32_t vis = (live[0] ? 1u : 0u) | (live[1] ? 2u : 0u) | (live[2] ? 4u : 0u) | (live[3] ? 8u : 0u);
-      const bool fresh = k0 + kTile > q.held;  // new tokens among the keys
+      const bool fresh = k0 + kTile > it.q.held;  // new tokens among the keys
       if (fresh) {
-        uint32_t bits = mask_bits(a, q.first, tok, (int64_t)k0 - (int64_t)q.held);
-        if (k0 < q.held) bits |= (1u << (q.held - k0)) - 1u;  // fewer than 16
+        uint32_t bits = mask_bits32(a, it.q.first, tok, (int64_t)k0 - (int64_t)it.q.held);
+        if (k0 < it.q.held) bits |= (1u << (it.q.held - k0)) - 1u;  // fewer than 16
         vis &= bits >> (4u * grp);
       }
       float p[4], mx = -INFINITY;
@@ -249,32 +218,23 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
     l += __shfl_xor(l, 32, 64);
 
     // Results: row i16 has columns 64 j + 4 (4 grp + rr) + e in o[j][e][rr].
-    const uint32_t slot = 2u * share.b + (at.unit == 0 ? 1u : 0u);
     auto put = [&](uint32_t rw, uint32_t col, const float (&v)[4], float mm, float ll, bool head) {
       // rw: row of the tile
-      const uint32_t rr = at.tile * kRows + rw;
-      if (rr >= R || col >= D) return;
-      if (!whole) {
+      const uint32_t rr = it.tile * kRows + rw;
+      if (rr >= it.R || col >= D) return;
+      if (!it.whole) {
         float *po = a.part_o + ((uint64_t)slot * kRows + rw) * Dp + col;
         *reinterpret_cast<float4 *>(po) = make_float4(v[0], v[1], v[2], v[3]);
         if (head) *reinterpret_cast<float2 *>(a.part_ml + ((uint64_t)slot * kRows + rw) * 2) = make_float2(mm, ll);
         return;
       }
-      const uint64_t t = q.first + rr / g, hh = at.head * g + rr % g;
+      const uint64_t t = it.q.first + rr / g, hh = it.head * g + rr % g;
       const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
       const float u[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
       store4(static_cast<T *>(a.o) + t * a.o_ts + hh * a.o_hs, col, D, u);
       if (head && a.lse) a.lse[t * (uint64_t)(c.heads * g) + hh] = ll == 0.0f ? -INFINITY : lse_of(mm == -INFINITY ? 0.0f : mm, ll);
     };
-    if constexpr (ROWS) {
-#pragma unroll
-      for (int j = 0; j < DC; ++j)
-#pragma unroll
-        for (int rr = 0; rr < 4; ++rr) {
-          const float v[4] = {o[j][0][rr], o[j][1][rr], o[j][2][rr], o[j][3][rr]};
-          put(16u * wave + i16, 64u * j + 4u * (4u * grp + rr), v, m, l, j == 0 && rr == 0 && grp == 0);
-        }
-    } else {
+    {
 #pragma unroll
       for (int j = 0; j < DC; ++j)
 #pragma unroll
@@ -301,21 +261,7 @@ __device__ __forceinline__ void attend(const BwppCacheAttnArgs &a) {
       }
       __syncthreads();
     }
-
-    // The next item.
-    at.unit = 0;
-    if (++at.tile >= W::tiles(q, g)) {
-      at.tile = 0;
-      if (++at.head >= c.heads) {
-        at.head = 0;
-        do {
-          ++at.s;
-          if (at.s >= c.batch) break;
-          q = seq_at(c, at.s);
-        } while (q.n == 0);
-      }
-    }
-  }
+  });
 }
 
 // Joins the parts of the item that the border before sharer b is the first to
@@ -380,6 +326,7 @@ __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
       const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
       if (r >= rows) continue;
       float top = m[e];
+#pragma unroll 16
       for (uint32_t k = 0; k < n; ++k) top = fmaxf(top, pair[k][r].x);
       // no key seen (offset -inf): sums of 0 (or NaN, kept)
       auto factor = [&](float o) { return o == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(o - top); };
@@ -418,26 +365,24 @@ __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
 
 }  // namespace kv
 
-#define BWPP_ATTEND(NAME, T, DC, ROWS)                                                                  \
+#define BWPP_ATTEND(NAME, T, DC)                                                                                    \
   extern "C" __global__ __launch_bounds__(256, DC <= 2 ? 2 : 1) void bwpp_cache_attend_##NAME(const BwppCacheAttnArgs a) { \
-    kv::attend<T, DC, ROWS>(a);                                                                         \
+    kv::attend_split<T, DC>(a);                                                                                     \
   }
-#define BWPP_ATTEND_DIMS(NAME, T, ROWS) \
-  BWPP_ATTEND(NAME##_d64, T, 1, ROWS)   \
-  BWPP_ATTEND(NAME##_d128, T, 2, ROWS)  \
-  BWPP_ATTEND(NAME##_d192, T, 3, ROWS)  \
-  BWPP_ATTEND(NAME##_d256, T, 4, ROWS)
-BWPP_ATTEND_DIMS(f32, float, false)
-BWPP_ATTEND_DIMS(f32_rows, float, true)
-BWPP_ATTEND_DIMS(bf16, uint16_t, false)
-BWPP_ATTEND_DIMS(bf16_rows, uint16_t, true)
+BWPP_ATTEND(f32_d64, float, 1)
+BWPP_ATTEND(f32_d128, float, 2)
+BWPP_ATTEND(f32_d192, float, 3)
+BWPP_ATTEND(f32_d256, float, 4)
+BWPP_ATTEND(bf16_d64, uint16_t, 1)
+BWPP_ATTEND(bf16_d128, uint16_t, 2)
+BWPP_ATTEND(bf16_d192, uint16_t, 3)
+BWPP_ATTEND(bf16_d256, uint16_t, 4)
 
-#define BWPP_JOIN(NAME, T, ROWS, UNIT) \
-  extern "C" __global__ __launch_bounds__(256) void bwpp_cache_join_##NAME(const BwppCacheAttnArgs a) { kv::join<T, ROWS, UNIT>(a); }
-BWPP_JOIN(f32, float, 16, 64)
-BWPP_JOIN(f32_rows, float, 64, 64)
-BWPP_JOIN(bf16, uint16_t, 16, 64)
-BWPP_JOIN(bf16_rows, uint16_t, 64, 64)
-BWPP_JOIN(bf16_32, uint16_t, 32, 64)
-BWPP_JOIN(bf16_128, uint16_t, 128, 64)
-BWPP_JOIN(bf16_256, uint16_t, 256, 64)
+#define BWPP_JOIN(NAME, T, ROWS) \
+  extern "C" __global__ __launch_bounds__(256) void bwpp_cache_join_##NAME(const BwppCacheAttnArgs a) { kv::join<T, ROWS, 64>(a); }
+BWPP_JOIN(f32_16, float, 16)
+BWPP_JOIN(f32_128, float, 128)
+BWPP_JOIN(bf16_16, uint16_t, 16)
+BWPP_JOIN(bf16_32, uint16_t, 32)
+BWPP_JOIN(bf16_128, uint16_t, 128)
+BWPP_JOIN(bf16_256, uint16_t, 256)

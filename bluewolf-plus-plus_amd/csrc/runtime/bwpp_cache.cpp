@@ -22,8 +22,9 @@ enum CacheKernel {
   CK_ATTEND_FEW = CK_ATTEND + 16,      // [kFlashDims]
   CK_ATTEND_R128 = CK_ATTEND_FEW + 7,  // [kFlashDims]
   CK_ATTEND_R256 = CK_ATTEND_R128 + 7, // [kFlashDims up to 128]
-  CK_JOIN = CK_ATTEND_R256 + 4,        // [bf16][rows], tiles of 32, 128, 256
-  CK_RULES = CK_JOIN + 7,              // [x bf16][y bf16]
+  CK_JOIN_F32 = CK_ATTEND_R256 + 4,    // tiles of 16, 128 rows
+  CK_JOIN_BF16 = CK_JOIN_F32 + 2,      // of 16, 32, 128, 256
+  CK_RULES = CK_JOIN_BF16 + 4,         // [x bf16][y bf16]
   CK_COUNT = CK_RULES + 4
 };
 
@@ -77,10 +78,9 @@ const char *const bwpp_hip_cache_kernels[] = {
     "bwpp_cache_attend_r256_d80",
     "bwpp_cache_attend_r256_d96",
     "bwpp_cache_attend_r256_d128",
-    "bwpp_cache_join_f32",
-    "bwpp_cache_join_f32_rows",
-    "bwpp_cache_join_bf16",
-    "bwpp_cache_join_bf16_rows",
+    "bwpp_cache_join_f32_16",
+    "bwpp_cache_join_f32_128",
+    "bwpp_cache_join_bf16_16",
     "bwpp_cache_join_bf16_32",
     "bwpp_cache_join_bf16_128",
     "bwpp_cache_join_bf16_256",
@@ -360,7 +360,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // has its own: by the rows that a sequence and key head has on average.
   const uint64_t mean = (T + cp.batch - 1) / cp.batch * g;
   const uint32_t r256 = getenv("W_R") ? (uint32_t)atoi(getenv("W_R")) : 128;
-  const uint32_t rows = flash < 0 ? (mean > 16 ? 64u : 16u) : mean <= 32 ? 32u : mean <= r256 || cp.dim > 128 ? 128u : 256u;
+  const uint32_t rows = flash < 0 ? (mean > (getenv("W_F") ? (uint64_t)atoi(getenv("W_F")) : 48) ? 128u : 16u) : mean <= 32 ? 32u : mean <= r256 || cp.dim > 128 ? 128u : 256u;
   const uint32_t Dp = (cp.dim + 3) / 4 * 4;
   // Costs (kv_schedule.h) are counted in 64 bits and multiplied by the blocks.
   const long double worst = (long double)cp.heads * ((long double)T * g / rows + cp.batch) *
@@ -383,9 +383,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   a.scale_log2 = std::fabs(scale) * 1.4426950408889634f;
   a.flip = scale < 0.0f ? 1u : 0u;
   // Blocks as many as are resident at once, the same number on each XCD.
-  a.blocks = ((rows == 256 || (flash >= 0 && cp.dim > 128) ? 1 : 2) * cus_of(h) + 7) / 8 * 8;
+  a.blocks = ((rows == 256 || (rows != 16 && cp.dim > 128) ? 1 : 2) * cus_of(h) + 7) / 8 * 8;
   a.inv_blocks = 1.0 / a.blocks;
-  a.whole_keys = getenv("W_K") ? (uint32_t)atoi(getenv("W_K")) : flash >= 0 ? 512 : rows == 64 ? 128 : 256;
+  a.whole_keys = getenv("W_K") ? (uint32_t)atoi(getenv("W_K")) : flash >= 0 ? (rows == 32 ? 512 : 1024) : 256;
   const bool parts = c.capacity > a.whole_keys;
   if (parts) {
     void *ws = nullptr;
@@ -394,15 +394,11 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
     a.part_o = static_cast<float *>(ws);
     a.part_ml = a.part_o + (size_t)2 * a.blocks * rows * Dp;
   }
-  int attend, join;
-  if (flash >= 0) {
-    attend = flash + (rows == 32 ? CK_ATTEND_FEW : rows == 128 ? CK_ATTEND_R128 : CK_ATTEND_R256);
-    join = CK_JOIN + (rows == 32 ? 4 : rows == 128 ? 5 : 6);
-  } else {
-    const int kind = (cp.dtype == BWPP_HIP_BF16 ? 2 : 0) + (rows == 64 ? 1 : 0);
-    attend = CK_ATTEND + 4 * kind + (int)((cp.dim - 1) / 64);
-    join = CK_JOIN + kind;
-  }
+  const bool bf16 = cp.dtype == BWPP_HIP_BF16;
+  const int attend = flash < 0       ? CK_ATTEND + (bf16 ? 8 : 0) + (rows == 128 ? 4 : 0) + (int)((cp.dim - 1) / 64)
+                     : flash + (rows == 32 ? CK_ATTEND_FEW : rows == 128 ? CK_ATTEND_R128 : CK_ATTEND_R256);
+  const int join = bf16 ? CK_JOIN_BF16 + (rows == 16 ? 0 : rows == 32 ? 1 : rows == 128 ? 2 : 3)
+                        : CK_JOIN_F32 + (rows == 16 ? 0 : 1);
   s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, rows == 32 ? 128 : rows == 256 ? 512 : 256, &a);
   if (s != BWPP_HIP_OK || !parts) return s;
   return bwpp_hip_launch_cache(h, join, a.blocks - 1, (rows + 15) / 16, 256, &a);
