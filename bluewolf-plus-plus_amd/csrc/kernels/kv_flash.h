@@ -58,6 +58,7 @@ struct Wave32 {
   using R = Rows<D>;
   static constexpr int KS = D / 16, DB = (D + 31) / 32, kKeys = 32 * KB;
   static constexpr uint32_t kTile = kKeys * R::kRowB, kStage = 2 * kTile;
+  static constexpr int kAhead = 4;  // operands read ahead of their products
   bf16x8_t q[KS];
   f32x16_t o[DB];
   float m, l, c;
@@ -97,24 +98,24 @@ struct Wave32 {
   // Scores and probabilities (in s) of the key tile at `st`.  masked: vis has bit k
   // of word kb where this lane's row sees key 32 kb + k; otherwise all are seen.
   __device__ __forceinline__ void scores(const unsigned char *st, bool masked, const uint32_t (&vis)[KB], f32x16_t (&s)[KB]) {
+    // kAhead reads of K on the way; the order is held by hand (left to itself the
+    // compiler reads each operand right before its product and waits for it).
+    constexpr int N = KB * KS, A = N < kAhead ? N : kAhead;
+    uint4 kf[kAhead];
+    auto read = [&](int i) { return *reinterpret_cast<const uint4 *>(st + koff[i % KS] + 32u * (i / KS) * R::kRowB); };
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
+    for (int i = 0; i < A; ++i) kf[i] = read(i);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4 *>(st + koff[ks] + 32u * kb * R::kRowB)), q[ks],
-            s[kb], 0, 0, 0);
+    for (int i = 0; i < N; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      s[i / KS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf[i % kAhead]), q[i % KS], s[i / KS], 0, 0, 0);
+      if (i + A < N) kf[i % kAhead] = read(i + A);
     }
-    // Two reads of K ahead of the products: hoisted all, they would not fit the registers.
-    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-    for (int i = 0; i < KB * KS - 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    __builtin_amdgcn_sched_barrier(0);
     if (masked) {  // wave-uniform
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
@@ -160,37 +161,36 @@ struct Wave32 {
   // one, 2^-8 (the sum of p has it whole).
   template <int TERMS>
   __device__ __forceinline__ void products(const unsigned char *st, const f32x16_t (&s)[KB]) {
+    constexpr int N = KB * 2 * DB, A = N < kAhead ? N : kAhead;
+    v8s_t vf[kAhead];
+    auto read = [&](int i) {  // block i % DB of 32 columns, keys 16 (i / DB) ..
+      const unsigned char *p = st + voff[i % DB] + 16u * (i / DB) * R::kRowB;
+      const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)p);
+      const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)(p + 8u * R::kRowB));
+      return v8s_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int i = 0; i < A; ++i) vf[i] = read(i);
+    bf16x8_t ph, pl;
 #pragma unroll
-      for (int kq = 0; kq < 2; ++kq) {
-        bf16x8_t ph, pl;
+    for (int i = 0; i < N; ++i) {
+      const int d = i % DB, kb = i / DB / 2, r0 = 8 * (i / DB % 2);
+      if (d == 0) {
         if constexpr (TERMS == 2) {
-          split_bf16x8(&s[kb], 8 * kq, ph, pl);
+          split_bf16x8(&s[kb], r0, ph, pl);
         } else {
-          const uint4 w = make_uint4(pack_bf16x2(s[kb][8 * kq], s[kb][8 * kq + 1]), pack_bf16x2(s[kb][8 * kq + 2], s[kb][8 * kq + 3]),
-                                     pack_bf16x2(s[kb][8 * kq + 4], s[kb][8 * kq + 5]), pack_bf16x2(s[kb][8 * kq + 6], s[kb][8 * kq + 7]));
+          const uint4 w = make_uint4(pack_bf16x2(s[kb][r0], s[kb][r0 + 1]), pack_bf16x2(s[kb][r0 + 2], s[kb][r0 + 3]),
+                                     pack_bf16x2(s[kb][r0 + 4], s[kb][r0 + 5]), pack_bf16x2(s[kb][r0 + 6], s[kb][r0 + 7]));
           ph = __builtin_bit_cast(bf16x8_t, w);
         }
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const unsigned char *p = st + voff[d] + (32u * kb + 16u * kq) * R::kRowB;
-          const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)p);
-          const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t *)(p + 8u * R::kRowB));
-          const v8s_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), ph, o[d], 0, 0, 0);
-          if constexpr (TERMS == 2)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), pl, o[d], 0, 0, 0);
-        }
       }
-    // Four (transposing) reads of V ahead.
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-    for (int i = 0; i < 2 * KB * DB - 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, TERMS, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[i % kAhead]), ph, o[d], 0, 0, 0);
+      if constexpr (TERMS == 2)
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[i % kAhead]), pl, o[d], 0, 0, 0);
+      if (i + A < N) vf[i % kAhead] = read(i + A);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2 * TERMS, 0);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   // Infinite and NaN values of a tile with masked keys: 0 times those would reach

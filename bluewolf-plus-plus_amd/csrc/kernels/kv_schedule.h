@@ -143,7 +143,7 @@ struct Costs {
   }
 };
 
-// The share of a total cost: as many keys for each block, kLeast at least.
+// The share of a total cost: as much for each block, kLeast at least.
 __device__ __forceinline__ uint64_t share_of(const BwppCacheAttnArgs &a, uint64_t total) {
   const uint64_t even = (uint64_t)((double)total * a.inv_blocks) + 1, least = (uint64_t)a.group * kLeast;
   return even < least ? least : even;
