@@ -343,7 +343,7 @@ template <int D, int NW>
 __device__ __forceinline__ void attend_few(const BwppCacheAttnArgs &a) {
   typedef Wave32<D, 1> W;
   typedef Fetch<D, 32, 1> F;
-  constexpr uint32_t kStage = W::kStage, kStages = kStage * 3 <= 32768 ? 32768 / kStage : 2, kDma = 2 * F::kDma;
+  constexpr uint32_t kStage = W::kStage, kStages = kStage * 3 <= 36864 ? 36864 / kStage : 2, kDma = 2 * F::kDma;
   constexpr uint32_t kRing = kStages * kStage, kCld = D + 4, kMerge = NW * 32 * kCld * 4;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[(NW * kRing > kMerge ? NW * kRing : kMerge) + 64];
   __shared__ uint32_t pages[kPages];

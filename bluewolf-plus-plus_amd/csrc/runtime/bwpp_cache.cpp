@@ -8,7 +8,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "../kargs.h"
 
@@ -357,10 +356,13 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
     for (int i = 0; i < 7; ++i)
       if (kFlashDims[i] == cp.dim) flash = i;
   // Tiles of few rows, whose waves share the keys out, or of more, where each wave
-  // has its own: by the rows that a sequence and key head has on average.
+  // has its own: by the rows that a sequence and key head has on average.  16 trees
+  // over up to 8000 tokens, 8 key heads of 128: bf16 32 rows 44 us on tiles of 32,
+  // 42 of 128, 40 rows 60 and 44; fp32 64 rows 165 on tiles of 16, 179 of 128, 96
+  // rows 243 and 187.  bf16, 256 rows over 30000 tokens 52 us on tiles of 128, 43 of
+  // 256; 4 x 2000 rows without a past 38 and 30.
   const uint64_t mean = (T + cp.batch - 1) / cp.batch * g;
-  const uint32_t r256 = getenv("W_R") ? (uint32_t)atoi(getenv("W_R")) : 128;
-  const uint32_t rows = flash < 0 ? (mean > (getenv("W_F") ? (uint64_t)atoi(getenv("W_F")) : 48) ? 128u : 16u) : mean <= 32 ? 32u : mean <= r256 || cp.dim > 128 ? 128u : 256u;
+  const uint32_t rows = flash < 0 ? (mean > 64 ? 128u : 16u) : mean <= 32 ? 32u : mean <= 128 || cp.dim > 128 ? 128u : 256u;
   const uint32_t Dp = (cp.dim + 3) / 4 * 4;
   // Costs (kv_schedule.h) are counted in 64 bits and multiplied by the blocks.
   const long double worst = (long double)cp.heads * ((long double)T * g / rows + cp.batch) *
@@ -385,7 +387,11 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // Blocks as many as are resident at once, the same number on each XCD.
   a.blocks = ((rows == 256 || (rows != 16 && cp.dim > 128) ? 1 : 2) * cus_of(h) + 7) / 8 * 8;
   a.inv_blocks = 1.0 / a.blocks;
-  a.whole_keys = getenv("W_K") ? (uint32_t)atoi(getenv("W_K")) : flash >= 0 ? (rows == 32 ? 512 : 1024) : 256;
+  // Up to here an item's keys cost less than its parts and their join: 24
+  // sequences of 200 tokens 16.9 us in parts, 11.2 whole, one of 204 12.8 and
+  // 10.7, 3 x 550 tokens of 64 : 8 heads 68 and 45 (past 1024 keys parts win: one
+  // sequence of 1000 tokens 12.8 in parts, 16 whole; fp32 4 x 416 tokens 300 and 393).
+  a.whole_keys = flash < 0 ? 256 : rows == 32 ? 512 : 1024;
   const bool parts = c.capacity > a.whole_keys;
   if (parts) {
     void *ws = nullptr;
