@@ -320,7 +320,7 @@ typedef struct {
   const uint32_t *mask;
   uint64_t ldx, ldy, ld_bias, ld_mask;
   uint32_t rows, vocab;
-  uint32_t chunk;  /* columns a block, a power of two */
+  uint32_t chunk;  /* columns a block, a power of two, at most 16 a thread */
   uint32_t chunks; /* blocks a row */
   uint32_t history_len; /* elements of the history */
   uint32_t count;  /* 1: tokens of the history are counted */

@@ -57,7 +57,8 @@ __device__ __forceinline__ void append(const BwppCacheAppendArgs &a) {
     const uint32_t t = t0 + tid, s = find_seq(c, samples, step, t);
     const Seq q = seq_at(c, s);
     const bool in = t >= q.first && t - q.first < q.n;
-    const uint64_t slot = (uint64_t)q.held + (t - q.first);
+    const int32_t held = c.held[s];  // not cut to the table: the position goes on past it
+    const uint64_t slot = (uint64_t)(held < 0 ? 0 : held) + (t - q.first);
     live[tid] = in;
     place[tid] = in ? slot_row(c, s, slot) : kNoSlot;
     pos[tid] = r.positions ? (int64_t)r.positions[t] : (int64_t)slot;
@@ -147,8 +148,9 @@ __device__ __forceinline__ void append(const BwppCacheAppendArgs &a) {
 
 // Slot held + i of a sequence takes what lies at held + kept[i].  A thread owns
 // a chunk of one head's keys or values and reads kRound of its rows before it
-// writes any, so within a round the order of kept does not matter; beyond a
-// round kept must not descend (then no row is overwritten before it is read).
+// writes any, so within a round the order of kept does not matter; in later
+// rounds an entry must not be below its index (then no row is overwritten
+// before it is read).
 template <class U>
 __device__ __forceinline__ void keep(const BwppCacheKeepArgs &a) {
   constexpr uint32_t kRound = 16;

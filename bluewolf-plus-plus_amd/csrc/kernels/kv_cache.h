@@ -46,7 +46,7 @@ __device__ __forceinline__ uint64_t row_at(const BwppCacheArgs &c, uint32_t page
 }
 
 __device__ __forceinline__ uint64_t slot_row(const BwppCacheArgs &c, uint32_t s, uint64_t slot) {
-  if (slot >= c.capacity) return kNoSlot;
+  if (slot >= c.capacity || c.pages == 0) return kNoSlot;  // (without pages there may be no table)
   return row_at(c, page_of(c, s, (uint32_t)slot), (uint32_t)slot);
 }
 

@@ -8,7 +8,7 @@
 // Bound by HBM: a logit is read and written once.  A block takes a chunk of
 // one row's columns, counts the row's history in LDS (bit 31: v occurs, below
 // it c; whole numbers, so the order of the additions does not matter) and then
-// streams the chunk.
+// goes over its chunk, which it has fetched meanwhile.
 #pragma once
 
 #include "common.h"
@@ -19,29 +19,37 @@ using namespace bwpp;
 
 namespace logits {
 
+constexpr uint32_t kPer = 4;  // 4-element chunks a thread
+
 template <class TX, class TY>
 __device__ __forceinline__ void rules(const BwppLogitArgs &a) {
   using rotary_pos::Vec;
   extern __shared__ uint32_t seen[];
   const uint32_t row = blockIdx.x / a.chunks, c0 = blockIdx.x % a.chunks * a.chunk, NT = blockDim.x;
-  const uint32_t nc = min(a.chunk, a.vocab - c0);
-  uint32_t n = 0, prompt = 0;
-  const int32_t *past = a.history;
+  const uint32_t nc = min(a.chunk, a.vocab - c0), n4 = nc / 4u;
+  const TX *x = static_cast<const TX *>(a.x) + row * a.ldx + c0;
+  TY *y = static_cast<TY *>(a.y) + row * a.ldy + c0;
+  float v[kPer][4];  // on the way while the history is counted
+#pragma unroll
+  for (uint32_t j = 0; j < kPer; ++j)
+    if (threadIdx.x + j * NT < n4) Vec<TX, 4>::load(x + 4u * (threadIdx.x + j * NT), v[j]);
+
+  uint32_t n = 0;
   if (a.count) {
     const int32_t s0 = a.starts[row], s1 = a.starts[row + 1];
     const uint32_t b = s0 < 0 ? 0u : min((uint32_t)s0, a.history_len), e = s1 < 0 ? 0u : min((uint32_t)s1, a.history_len);
     n = e > b ? e - b : 0u;
-    past += b;
+    const int32_t *past = a.history + b;
     const int32_t p = a.prompt ? a.prompt[row] : 0;
-    prompt = p < 0 ? 0u : (uint32_t)p;
+    const uint32_t prompt = p < 0 ? 0u : (uint32_t)p;
     if (n) {  // uniform in the block
       for (uint32_t i = threadIdx.x; i < nc; i += NT) seen[i] = 0u;
       __syncthreads();
       for (uint32_t i = threadIdx.x; i < n; i += NT) {
-        const uint32_t v = (uint32_t)past[i] - c0;
-        if (v < nc) {
-          if (i >= prompt) atomicAdd(&seen[v], 1u);
-          atomicOr(&seen[v], 0x80000000u);
+        const uint32_t t = (uint32_t)past[i] - c0;
+        if (t < nc) {
+          if (i >= prompt) atomicAdd(&seen[t], 1u);
+          atomicOr(&seen[t], 0x80000000u);
         }
       }
       __syncthreads();
@@ -49,8 +57,6 @@ __device__ __forceinline__ void rules(const BwppLogitArgs &a) {
   }
   const float rho = a.repetition ? a.repetition[row] : 1.0f;
   const float pres = a.presence ? a.presence[row] : 0.0f, freq = a.frequency ? a.frequency[row] : 0.0f;
-  const TX *x = static_cast<const TX *>(a.x) + row * a.ldx + c0;
-  TY *y = static_cast<TY *>(a.y) + row * a.ldy + c0;
   const float *bias = a.bias ? a.bias + row * a.ld_bias + c0 : nullptr;
   const uint32_t *mask = a.mask ? a.mask + row * a.ld_mask + c0 / 32u : nullptr;  // chunks are multiples of 32
 
@@ -66,21 +72,22 @@ __device__ __forceinline__ void rules(const BwppLogitArgs &a) {
     if (bias) z += b;
     return mask && !((bits >> (i & 31u)) & 1u) ? -INFINITY : z;
   };
-  const uint32_t n4 = nc / 4u;
-  for (uint32_t i = threadIdx.x; i < n4; i += NT) {
-    float v[4], b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    Vec<TX, 4>::load(x + 4u * i, v);
+#pragma unroll
+  for (uint32_t j = 0; j < kPer; ++j) {
+    const uint32_t i = threadIdx.x + j * NT;
+    if (i >= n4) break;
+    float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (bias) Vec<float, 4>::load(bias + 4u * i, b);
     const uint32_t bits = mask ? mask[i / 8u] : 0u;
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) v[e] = rule(v[e], 4u * i + e, b[e], bits);
-    Vec<TY, 4>::store(y + 4u * i, v);
+    for (uint32_t e = 0; e < 4; ++e) v[j][e] = rule(v[j][e], 4u * i + e, b[e], bits);
+    Vec<TY, 4>::store(y + 4u * i, v[j]);
   }
   for (uint32_t i = 4u * n4 + threadIdx.x; i < nc; i += NT) {
-    float v[1];
-    Vec<TX, 1>::load(x + i, v);
-    v[0] = rule(v[0], i, bias ? bias[i] : 0.0f, mask ? mask[i / 32u] : 0u);
-    Vec<TY, 1>::store(y + i, v);
+    float w[1];
+    Vec<TX, 1>::load(x + i, w);
+    w[0] = rule(w[0], i, bias ? bias[i] : 0.0f, mask ? mask[i / 32u] : 0u);
+    Vec<TY, 1>::store(y + i, w);
   }
 }
 

@@ -236,7 +236,6 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *
 
   BwppCacheAppendArgs a = {};
   fill(a.c, cp, c, k_cache, v_cache, table, starts, held);
-  if (!pool) a.c.capacity = 0;
   const uint32_t rot = p.no_rotation ? 0u : p.rot_dim ? p.rot_dim : cp.dim;
   bwpp_hip_rotary_args(rp, rot, a.r);
   a.r.q = sq.p;

@@ -250,13 +250,13 @@ typedef struct {
  * page_tokens token_stride, page_stride 0 = heads head_stride).  In device memory,
  * so that a recorded launch follows them:
  *   table   int32 [batch][max_pages], row stride ld_table: page numbers
- *   starts  int32 [batch + 1]: new tokens of sequence s are rows starts[s] ..
- *           starts[s + 1] - 1 of the operands' `tokens` rows; rows before the
- *           first and behind the last sequence are left alone
+ *   starts  int32 [batch + 1], not descending: new tokens of sequence s are rows
+ *           starts[s] .. starts[s + 1] - 1 of the operands' `tokens` rows; rows
+ *           before the first and behind the last sequence are left alone
  *   held    int32 [batch]: tokens that the cache holds before the new ones, which
  *           take the slots behind them
- * Slot p of a sequence lies in page table[s][p / page_tokens].  Starts and lengths
- * are cut to the operands and the table; a slot past the table, or whose page
+ * Slot p of a sequence lies in page table[s][p / page_tokens].  Starts are cut to
+ * the operands, lengths below zero are none; a slot past the table, or whose page
  * number is outside 0 .. pages - 1 (-1: no page), does not exist: nothing is
  * written there and no query sees it. */
 typedef struct {
@@ -786,9 +786,10 @@ BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const void *q, const
 
 /* After a tree of drafts is verified: slot held[s] + i takes the keys and values of
  * slot held[s] + kept[s][i] for i < counts[s] (int32 [batch], cut to max_kept), as
- * if all were read before any is written.  kept (int32 [batch][max_kept]) must not
- * descend where a row has more than 16 entries; entries below 0 or past the table
- * move nothing.  held itself is the caller's to raise by counts. */
+ * if all were read before any is written.  Of kept (int32 [batch][max_kept])
+ * entries past the 16th must not be below their index (ascending ones are not);
+ * entries below 0 or past the table move nothing.  held itself is the caller's to
+ * raise by counts. */
 BwppHipStatus bwpp_hip_dispatch_cache_keep(BwppHip *h, void *k_cache, void *v_cache, const int32_t *table,
                                            const int32_t *held, const int32_t *kept, const int32_t *counts,
                                            BwppCacheKeepParams params);

@@ -77,6 +77,7 @@ def test_slots_that_do_not_exist(be, dtype):
     zero and starts past the operands: nothing leaves the pools."""
     c = Cache([30, 14], [10, 10], 2, 64, 16, dtype, max_pages=2)
     _check(be, c, 2)
+    _check(be, Cache([40, 14], [10, 10], 2, 64, 16, dtype, max_pages=2), 2)  # longer than the table: q goes on
     c = Cache([30, 14, 0], [10, 10, 5], 2, 64, 16, dtype)
     c.table[0, 2], c.table[1, 1], c.table[2, 0] = -1, c.pages, 2 ** 31 - 1
     _check(be, c, 2)
@@ -126,3 +127,29 @@ def test_page_past_32_bits(be):
     assert bool((k_cache[last, 0, 252:] == k[:, 0]).all()) and bool((k_cache[last, 0, :252] == 5.0).all())
     assert bool((v_cache[last, 0, 252:] == v[:, 0]).all())
     assert bool((k_cache[last - (1 << 32) // (256 * 128)] == 5.0).all())
+
+
+def test_no_pool(be):
+    """No pages: nothing is appended, q is turned as with them."""
+    c = Cache([3], [4], 2, 64, 16, F32)
+    q, k, v = c.normal(4, 4, 64), c.normal(4, 2, 64), c.normal(4, 2, 64)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    be.dispatch_cache_append(q, k, v, None, c.table, c.starts, c.held_t, a, c.k, c.v, bwpp.CacheAppendParams(cache=c.params(4)))
+    be.dispatch_cache_append(q, k, v, None, None, c.starts, c.held_t, b, None, None,
+                             bwpp.CacheAppendParams(cache=c.params(4, pages=0)))
+    assert bool((a == b).all())
+
+
+def test_pools_side_by_side(be):
+    """Keys and values in one buffer: of a page one behind the other, and of a token."""
+    for shape, at in (((5, 2, 2, 16, 64), lambda t, i: t[:, i]), ((5, 2, 16, 2, 64), lambda t, i: t[:, :, :, i])):
+        buf = torch.full(shape, 5.0, device="cuda")
+        kc, vc = at(buf, 0), at(buf, 1)  # [page, head, token, d]
+        k, v = torch.randn(2, 20, 2, 64, device="cuda")
+        cp = bwpp.CacheParams(pages=5, page_tokens=16, heads=2, dim=64, batch=1, max_pages=2, tokens=20,
+                              page_stride=kc.stride(0), head_stride=kc.stride(1), token_stride=kc.stride(2))
+        be.dispatch_cache_append(None, k, v, None, i32([[4, 1]]), i32([0, 20]), i32([6]), None, kc, vc,
+                                 bwpp.CacheAppendParams(cache=cp, no_rotation=1))
+        for c, x in ((kc, k), (vc, v)):
+            assert bool((c[4, :, 6:].transpose(0, 1) == x[:10]).all()) and bool((c[1, :, :10].transpose(0, 1) == x[10:]).all())
+            assert bool((c[4, :, :6] == 5.0).all()) and bool((c[[0, 2, 3]] == 5.0).all()) and bool((c[1, :, 10:] == 5.0).all())

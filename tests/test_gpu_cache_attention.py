@@ -228,6 +228,37 @@ def test_starts_and_lengths_are_cut(be, dtype, d):
 
 
 @DTYPES
+@pytest.mark.parametrize("d", [64, 80, 100])
+def test_no_pool(be, dtype, d):
+    """No pages, or a table without columns: nothing is seen."""
+    c = Cache([0, 0], [1, 40], 2, d, 16, dtype)
+    q = c.normal(41, 4, d)
+    for kw in (dict(pages=0), dict(max_pages=0)):
+        o, l = torch.full_like(q, 5.0), torch.full((41, 4), 5.0, device="cuda")
+        be.dispatch_cache_attention(q, None, None, None, c.starts, c.held_t, None, o, l,
+                                    bwpp.CacheAttentionParams(cache=c.params(4, **kw)))
+        assert bool((o == 0).all()) and bool((l == -math.inf).all())
+
+
+@DTYPES
+@pytest.mark.parametrize("d", [64, 72, 128])
+@pytest.mark.parametrize("Hq,n", [(96, 1), (33, 1), (64, 7), (100, 3), (300, 1)])
+def test_many_query_heads_a_key_head(be, dtype, d, Hq, n):
+    """More rows of one token than a tile has, and tokens that end inside one."""
+    _check(be, Cache([70, 1300, 0], [n, n, n], 1, d, 16, dtype), Hq)
+    c = Cache([70, 600], [n, n], 1, d, 16, dtype)
+    _check(be, c, Hq, [tree(n, c.g) for _ in range(2)])
+
+
+@DTYPES
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("page", [1, 2, 16])
+def test_more_pages_than_are_kept_in_lds(be, dtype, d, page):
+    _check(be, Cache([1100 * page, 2500, 70], [1, 1, 1], 1, d, page, dtype, seed=page), 2)
+    _check(be, Cache([1100 * page, 2500], [70, 3], 1, d, page, dtype, seed=page), 2)
+
+
+@DTYPES
 @pytest.mark.parametrize("d", [64, 80])
 def test_same_bits_every_time(be, dtype, d):
     c = Cache([4000, 100, 9], [1, 1, 1], 2, d, 16, dtype)
