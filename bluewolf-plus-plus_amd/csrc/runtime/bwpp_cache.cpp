@@ -146,6 +146,51 @@ BwppHipFault check_cache(const BwppCacheParams &p, Cache &c) {
   return {BWPP_HIP_OK, nullptr};
 }
 
+BwppRotaryParams rotation(const BwppCacheAppendParams &p) {
+  BwppRotaryParams r = {};
+  r.tokens = p.cache.tokens;
+  r.q_heads = p.cache.q_heads;
+  r.k_heads = p.cache.heads;
+  r.dim = p.cache.dim;
+  r.rot_dim = p.rot_dim;
+  r.layout = p.layout;
+  r.dtype = p.cache.dtype;
+  r.scaling = p.scaling;
+  r.base = p.base;
+  r.factor = p.factor;
+  r.low_turns = p.low_turns;
+  r.high_turns = p.high_turns;
+  r.context = p.context;
+  r.magnitude = p.magnitude;
+  return r;
+}
+
+BwppHipFault check_append(const BwppCacheAppendParams &p, Cache &c) {
+  const BwppHipFault f = check_cache(p.cache, c);
+  if (f.why || p.no_rotation) return f;
+  return bwpp_hip_check_rotary(rotation(p));
+}
+
+BwppHipFault check_attention(const BwppCacheAttentionParams &p, bool mask, Cache &c) {
+  const BwppHipFault f = check_cache(p.cache, c);
+  if (f.why) return f;
+  if (p.cache.q_heads == 0) return invalid("no query heads");
+  if (!std::isfinite(p.scale)) return invalid("scale must be finite");
+  if (mask && p.mask_words == 0) return invalid("a mask without words");
+  if (p.cache.dim > 256) return unsupported("dim above 256");
+  return f;
+}
+
+BwppHipFault check_keep(const BwppCacheKeepParams &p, Cache &c) {
+  BwppCacheParams cp = p.cache;
+  cp.tokens = 0;
+  cp.q_heads = 0;
+  const BwppHipFault f = check_cache(cp, c);
+  if (f.why) return f;
+  if (p.ld_kept != 0 && p.ld_kept < p.max_kept) return invalid("ld_kept smaller than max_kept");
+  return f;
+}
+
 void fill(BwppCacheArgs &a, const BwppCacheParams &p, const Cache &c, const void *k, const void *v,
           const int32_t *table, const int32_t *starts, const int32_t *held) {
   a.k = const_cast<void *>(k);
@@ -180,6 +225,27 @@ bool bad_rows(const RowSet &r, bool written) {
 
 }  // namespace
 
+BwppHipFault bwpp_hip_check_cache_append(const BwppCacheAppendParams &p) {
+  Cache c = {};
+  return check_append(p, c);
+}
+BwppHipFault bwpp_hip_check_cache_attention(const BwppCacheAttentionParams &p, bool mask) {
+  Cache c = {};
+  return check_attention(p, mask, c);
+}
+BwppHipFault bwpp_hip_check_cache_keep(const BwppCacheKeepParams &p) {
+  Cache c = {};
+  return check_keep(p, c);
+}
+BwppHipFault bwpp_hip_check_logit_rules(const BwppLogitRulesParams &p) {
+  if (p.dtype_x > BWPP_HIP_BF16 || p.dtype_y > BWPP_HIP_BF16) return invalid("unknown dtype");
+  if ((p.ldx && p.ldx < p.vocab) || (p.ldy && p.ldy < p.vocab) || (p.ld_bias && p.ld_bias < p.vocab) ||
+      (p.ld_mask && p.ld_mask < ((uint64_t)p.vocab + 31) / 32))
+    return invalid("row stride smaller than the row");
+  if (p.vocab > 0x7fffffffu || p.history > 0x7fffffffu) return unsupported("vocab or history of 2^31 or more");
+  return {BWPP_HIP_OK, nullptr};
+}
+
 // ------------------------------------------------------------------ append
 
 extern "C" BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *q, const void *k, const void *v,
@@ -189,24 +255,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *
   auto bad = [&](BwppHipStatus s, const char *why) { return bwpp_hip_set_error(h, s, "cache_append: %s", why); };
   const BwppCacheParams &cp = p.cache;
   Cache c = {};
-  BwppHipFault fault = check_cache(cp, c);
+  const BwppHipFault fault = check_append(p, c);
   if (fault.why) return bad(fault.status, fault.why);
-  BwppRotaryParams rp = {};
-  rp.tokens = cp.tokens;
-  rp.q_heads = cp.q_heads;
-  rp.k_heads = cp.heads;
-  rp.dim = cp.dim;
-  rp.rot_dim = p.rot_dim;
-  rp.layout = p.layout;
-  rp.dtype = cp.dtype;
-  rp.scaling = p.scaling;
-  rp.base = p.base;
-  rp.factor = p.factor;
-  rp.low_turns = p.low_turns;
-  rp.high_turns = p.high_turns;
-  rp.context = p.context;
-  rp.magnitude = p.magnitude;
-  if (!p.no_rotation && (fault = bwpp_hip_check_rotary(rp)).why) return bad(fault.status, fault.why);
   if (cp.tokens == 0 || cp.batch == 0) return bwpp_hip_enter(h);
   const bool pool = cp.pages && cp.max_pages;  // somewhere to write
   if ((cp.q_heads && (!q || !qo)) || !k || !v || !starts || !held || (pool && (!table || !k_cache || !v_cache)))
@@ -237,7 +287,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *
   BwppCacheAppendArgs a = {};
   fill(a.c, cp, c, k_cache, v_cache, table, starts, held);
   const uint32_t rot = p.no_rotation ? 0u : p.rot_dim ? p.rot_dim : cp.dim;
-  bwpp_hip_rotary_args(rp, rot, a.r);
+  bwpp_hip_rotary_args(rotation(p), rot, a.r);
   a.r.q = sq.p;
   a.r.k = k;
   a.r.qo = qo;
@@ -272,13 +322,10 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_keep(BwppHip *h, void *k_cache,
                                                       const int32_t *held, const int32_t *kept, const int32_t *counts,
                                                       BwppCacheKeepParams p) {
   auto bad = [&](BwppHipStatus s, const char *why) { return bwpp_hip_set_error(h, s, "cache_keep: %s", why); };
-  BwppCacheParams cp = p.cache;
-  cp.tokens = 0;
-  cp.q_heads = 0;
+  const BwppCacheParams &cp = p.cache;
   Cache c = {};
-  const BwppHipFault fault = check_cache(cp, c);
+  const BwppHipFault fault = check_keep(p, c);
   if (fault.why) return bad(fault.status, fault.why);
-  if (p.ld_kept != 0 && p.ld_kept < p.max_kept) return bad(BWPP_HIP_ERR_INVALID_ARG, "ld_kept smaller than max_kept");
   if (cp.batch == 0 || p.max_kept == 0 || cp.pages == 0 || cp.max_pages == 0) return bwpp_hip_enter(h);
   if (!k_cache || !v_cache || !table || !held || !kept || !counts) return bad(BWPP_HIP_ERR_INVALID_ARG, "NULL operand");
   const RowSet dk = c.pool(k_cache, cp), dv = c.pool(v_cache, cp);
@@ -320,12 +367,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   auto bad = [&](BwppHipStatus s, const char *why) { return bwpp_hip_set_error(h, s, "cache_attention: %s", why); };
   const BwppCacheParams &cp = p.cache;
   Cache c = {};
-  const BwppHipFault fault = check_cache(cp, c);
+  const BwppHipFault fault = check_attention(p, mask != nullptr, c);
   if (fault.why) return bad(fault.status, fault.why);
-  if (cp.q_heads == 0) return bad(BWPP_HIP_ERR_INVALID_ARG, "no query heads");
-  if (!std::isfinite(p.scale)) return bad(BWPP_HIP_ERR_INVALID_ARG, "scale must be finite");
-  if (mask && p.mask_words == 0) return bad(BWPP_HIP_ERR_INVALID_ARG, "a mask without words");
-  if (cp.dim > 256) return bad(BWPP_HIP_ERR_UNSUPPORTED, "dim above 256");
   if (cp.tokens == 0 || cp.batch == 0) return bwpp_hip_enter(h);
   const bool pool = cp.pages && cp.max_pages;
   if (!q || !o || !starts || !held || (pool && (!table || !k_cache || !v_cache)))
@@ -417,11 +460,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_logit_rules(BwppHip *h, const void *x
                                                        const float *frequency, const float *bias, const uint32_t *mask,
                                                        void *y, BwppLogitRulesParams p) {
   auto bad = [&](BwppHipStatus s, const char *why) { return bwpp_hip_set_error(h, s, "logit_rules: %s", why); };
-  if (p.dtype_x > BWPP_HIP_BF16 || p.dtype_y > BWPP_HIP_BF16) return bad(BWPP_HIP_ERR_INVALID_ARG, "unknown dtype");
+  const BwppHipFault fault = bwpp_hip_check_logit_rules(p);
+  if (fault.why) return bad(fault.status, fault.why);
   const uint64_t R = p.rows, V = p.vocab, ldx = p.ldx ? p.ldx : V, ldy = p.ldy ? p.ldy : V, words = (V + 31) / 32;
-  if (ldx < V || ldy < V || (p.ld_bias && p.ld_bias < V) || (p.ld_mask && p.ld_mask < words))
-    return bad(BWPP_HIP_ERR_INVALID_ARG, "row stride smaller than the row");
-  if (V > 0x7fffffffull || p.history > 0x7fffffffu) return bad(BWPP_HIP_ERR_UNSUPPORTED, "vocab or history of 2^31 or more");
   if (R == 0 || V == 0) return bwpp_hip_enter(h);
   if (!x || !y) return bad(BWPP_HIP_ERR_INVALID_ARG, "NULL x or y");
   const bool penalties = repetition || presence || frequency;

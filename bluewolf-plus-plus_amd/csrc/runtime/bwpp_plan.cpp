@@ -33,6 +33,15 @@
 //   residual_norm_grad    in=O,R with=post,gate,pre,dr,dy gives=dx,do,dpost,dgate,dpre
 //   linear_xent           in=X,W,TARGETS gives=loss,lse,sums  (trans_w, scale)
 //   linear_xent_grad      in=X,W,TARGETS,LSE[,DLOSS] gives=dx,dw
+//   cache_append          in=Q,K,V,KC,VC,TABLE,STARTS,HELD[,POSITIONS] out=QO,KC,VC
+//                         (rotate=0: as they are; rot, pairs, base, scaling, factor,
+//                         context, low, high, magnitude as rotary); QO may be Q
+//   cache_attention       in=Q,KC,VC,TABLE,STARTS,HELD[,MASK] out=O[,LSE]  (scale)
+//   cache_keep            in=KC,VC,TABLE,HELD,KEPT,COUNTS out=KC,VC
+//                         KC, VC: [pages, heads, page, dim] or, cache=pthd, [pages,
+//                         page, heads, dim] inputs or params, written in place
+//   logit_rules           in=X,.. with=history,starts,prompt,repetition,presence,
+//                         frequency,bias,mask out=Y
 // Tensors are row-major; row operators see [rows, cols] with cols the last
 // dim and rows the product of the others; a view is a 2-D strided window
 // (offset and row stride ld in elements) into another tensor's storage.
@@ -46,6 +55,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <initializer_list>
+#include <iterator>
 #include <map>
 #include <sstream>
 #include <string>
@@ -619,7 +629,8 @@ int listed(const std::vector<int> &ops, const std::vector<std::string> &names, s
 
 bool checks_own_dtypes(const std::string &k) {
   return k == "rotary" || k == "rotary_grad" || k == "residual_norm" || k == "residual_norm_grad" ||
-         k == "linear_xent" || k == "linear_xent_grad";
+         k == "linear_xent" || k == "linear_xent_grad" || k == "cache_append" || k == "cache_attention" ||
+         k == "cache_keep" || k == "logit_rules";
 }
 
 // In check-only mode (plan creation) each op validates its arguments and
@@ -835,6 +846,171 @@ BwppHipStatus run_lm_op(BwppHipPlan &p, const Op &op) {
       if (dx >= 0) r.lddx = (uint32_t)val(dx).row_stride();
       if (dw >= 0) r.lddw = (uint32_t)val(dw).row_stride();
       s = BWPP_PLAN_CALL(bwpp_hip_dispatch_linear_xent_grad(h, ptr(x), ptr(w), i32(t), f32(lse), f32(dloss), ptr(dx), ptr(dw), r));
+    }
+  }
+  if (s != BWPP_HIP_OK) return perr(&p, s, "line %d (%s): %s", op.line, k.c_str(), bwpp_hip_last_error(h));
+  return BWPP_HIP_OK;
+}
+
+// cache_append, cache_attention, cache_keep, logit_rules.
+BwppHipStatus run_cache_op(BwppHipPlan &p, const Op &op) {
+  BwppHip *h = p.h;
+  const std::string &k = op.kind;
+  auto val = [&](int i) -> const Value & { return p.values[i]; };
+  auto ptr = [&](int i) { return i < 0 ? nullptr : bwpp_hip_plan_value_ptr(&p, p.values[i].name.c_str()); };
+  auto f32 = [&](int i) { return static_cast<float *>(ptr(i)); };
+  auto i32 = [&](int i) { return static_cast<const int32_t *>(ptr(i)); };
+  Numbers at{p, op, {}};
+  auto bad = [&](const char *what) {  // (a wrong number is named before what followed from its default)
+    return perr(&p, BWPP_HIP_ERR_INVALID_ARG, "line %d (%s): %s", op.line, k.c_str(), at.wrong.empty() ? what : at.wrong.c_str());
+  };
+  auto refused = [&](const BwppHipFault &f) { return perr(&p, f.status, "line %d (%s): %s", op.line, k.c_str(), f.why); };
+  auto whole = [&](int i, uint32_t dt, uint64_t n) {  // a value by itself of n elements (-1: absent)
+    return i < 0 || (val(i).kind != Kind::kView && val(i).dtype == dt && val(i).elems() == n);
+  };
+  for (const std::vector<int> *list : {&op.ins, &op.outs})
+    for (int v : *list)
+      if (val(v).rows() > UINT32_MAX || val(v).cols() > UINT32_MAX || val(v).row_stride() > UINT32_MAX) return bad("sizes past 32 bits");
+  if (op.ins.empty()) return bad("no operands");
+  BwppHipStatus s = BWPP_HIP_OK;
+  if (k == "logit_rules") {
+    const std::vector<std::string> with = name_list(op, "with");
+    const char *const all[] = {"history", "starts", "prompt", "repetition", "presence", "frequency", "bias", "mask"};
+    bool ok = with.size() == op.ins.size() - 1 && op.outs.size() == 1;
+    for (size_t i = 0; ok && i < with.size(); ++i) {
+      ok = std::find(std::begin(all), std::end(all), with[i]) != std::end(all);
+      for (size_t j = 0; ok && j < i; ++j) ok = with[i] != with[j];
+    }
+    if (!ok) return bad("in=X,.. with=history,starts,prompt,repetition,presence,frequency,bias,mask (those given, in order) out=Y");
+    const int x = op.ins[0], y = op.outs[0];
+    const uint64_t rows = val(x).rows(), cols = val(x).cols(), words = (cols + 31) / 32;
+    if (val(x).dtype > BWPP_HIP_BF16 || val(y).dtype > BWPP_HIP_BF16) return bad("X and Y must be f32 or bf16");
+    if (val(y).rows() != rows || val(y).cols() != cols) return bad("Y must have X's shape");
+    auto get = [&](const char *name) { return listed(op.ins, with, 1, name); };
+    const int history = get("history"), starts = get("starts"), prompt = get("prompt"), rep = get("repetition"),
+              pres = get("presence"), freq = get("frequency"), bias = get("bias"), mask = get("mask");
+    if ((history < 0) != (starts < 0)) return bad("history and starts go together");
+    if ((history >= 0 && !whole(history, kI32, val(history).elems())) || !whole(starts, kI32, rows + 1) || !whole(prompt, kI32, rows))
+      return bad("history, starts [rows + 1] and prompt [rows] are i32");
+    if (!whole(rep, BWPP_HIP_F32, rows) || !whole(pres, BWPP_HIP_F32, rows) || !whole(freq, BWPP_HIP_F32, rows))
+      return bad("repetition, presence and frequency are f32, one element a row");
+    if (!whole(bias, BWPP_HIP_F32, cols) && !whole(bias, BWPP_HIP_F32, rows * cols)) return bad("bias is f32, a row or X's shape");
+    if (!whole(mask, kI32, words) && !whole(mask, kI32, rows * words)) return bad("mask is i32, a row of words or one for each row");
+    if (history >= 0 && val(history).elems() > UINT32_MAX) return bad("sizes past 32 bits");
+    BwppLogitRulesParams r = {};
+    r.rows = (uint32_t)rows;
+    r.vocab = (uint32_t)cols;
+    r.ldx = (uint32_t)val(x).row_stride();
+    r.ldy = (uint32_t)val(y).row_stride();
+    r.dtype_x = val(x).dtype;
+    r.dtype_y = val(y).dtype;
+    r.history = history >= 0 ? (uint32_t)val(history).elems() : 0;
+    r.ld_bias = bias >= 0 && rows > 1 && val(bias).elems() == rows * cols ? (uint32_t)cols : 0;
+    r.ld_mask = mask >= 0 && rows > 1 && val(mask).elems() == rows * words ? (uint32_t)words : 0;
+    if (const BwppHipFault f = bwpp_hip_check_logit_rules(r); f.why) return refused(f);
+    s = BWPP_PLAN_CALL(bwpp_hip_dispatch_logit_rules(h, ptr(x), i32(history), i32(starts), i32(prompt), f32(rep), f32(pres), f32(freq),
+                                                     f32(bias), static_cast<const uint32_t *>(ptr(mask)), ptr(y), r));
+    if (s != BWPP_HIP_OK) return perr(&p, s, "line %d (%s): %s", op.line, k.c_str(), bwpp_hip_last_error(h));
+    return BWPP_HIP_OK;
+  }
+  const bool append = k == "cache_append", keep = k == "cache_keep";
+  const size_t first = append ? 3 : keep ? 0 : 1;  // of the pools among the inputs
+  const size_t nin = append ? 8 : 6;
+  if (append ? (op.ins.size() != nin && op.ins.size() != nin + 1) || op.outs.size() != 3
+             : keep ? op.ins.size() != nin || op.outs.size() != 2
+                    : (op.ins.size() != nin && op.ins.size() != nin + 1) || op.outs.empty() || op.outs.size() > 2)
+    return bad(append ? "in=Q,K,V,KC,VC,TABLE,STARTS,HELD[,POSITIONS] out=QO,KC,VC"
+                      : keep ? "in=KC,VC,TABLE,HELD,KEPT,COUNTS out=KC,VC" : "in=Q,KC,VC,TABLE,STARTS,HELD[,MASK] out=O[,LSE]");
+  const int kc = op.ins[first], vc = op.ins[first + 1], table = op.ins[first + 2];
+  const std::string order = attr(op, "cache", "phtd");
+  if (order != "phtd" && order != "pthd") return bad("cache must be phtd or pthd");
+  const bool phtd = order == "phtd";
+  for (int v : {kc, vc})
+    if ((val(v).kind != Kind::kInput && val(v).kind != Kind::kParam) || val(v).dims.size() != 4 || val(v).dims != val(kc).dims ||
+        val(v).dtype > BWPP_HIP_BF16 || val(v).dtype != val(kc).dtype)
+      return bad("KC and VC are f32 or bf16 inputs or params of one 4-D shape");
+  if (append || keep)
+    if (op.outs[append ? 1 : 0] != kc || op.outs[append ? 2 : 1] != vc) return bad("the pools are written in place: name them in out= too");
+  const std::vector<uint64_t> &kd = val(kc).dims;
+  for (uint64_t d : kd)
+    if (d > UINT32_MAX) return bad("sizes past 32 bits");
+  if (val(table).dims.size() != 2 || val(table).dtype != kI32 || val(table).kind == Kind::kView) return bad("TABLE is i32 [batch, pages]");
+  BwppCacheParams c = {};
+  c.dtype = val(kc).dtype;
+  c.pages = (uint32_t)kd[0];
+  c.heads = (uint32_t)kd[phtd ? 1 : 2];
+  c.page_tokens = (uint32_t)kd[phtd ? 2 : 1];
+  c.dim = (uint32_t)kd[3];
+  c.token_stride = phtd ? kd[3] : kd[2] * kd[3];
+  c.head_stride = phtd ? kd[2] * kd[3] : kd[3];
+  c.page_stride = kd[1] * kd[2] * kd[3];
+  c.batch = (uint32_t)val(table).dims[0];
+  c.max_pages = (uint32_t)val(table).dims[1];
+  if (keep) {
+    const int held = op.ins[3], kept = op.ins[4], counts = op.ins[5];
+    if (!whole(held, kI32, c.batch) || !whole(counts, kI32, c.batch) || val(kept).dtype != kI32 || val(kept).kind == Kind::kView ||
+        val(kept).rows() != c.batch)
+      return bad("HELD and COUNTS are i32 [batch], KEPT i32 [batch, most]");
+    BwppCacheKeepParams r = {};
+    r.cache = c;
+    r.max_kept = (uint32_t)val(kept).cols();
+    if (const BwppHipFault f = bwpp_hip_check_cache_keep(r); f.why) return refused(f);
+    s = BWPP_PLAN_CALL(bwpp_hip_dispatch_cache_keep(h, ptr(kc), ptr(vc), i32(table), i32(held), i32(kept), i32(counts), r));
+  } else {
+    const int q = op.ins[0], o = op.outs[0], starts = op.ins[first + 3], held = op.ins[first + 4];
+    const int extra = op.ins.size() > nin ? op.ins[nin] : -1;
+    if (!whole(starts, kI32, (uint64_t)c.batch + 1) || !whole(held, kI32, c.batch)) return bad("STARTS is i32 [batch + 1], HELD i32 [batch]");
+    if (val(q).dtype != c.dtype || val(o).dtype != c.dtype) return bad("operands of different dtypes");
+    const uint64_t T = val(q).rows(), cols = val(q).cols();
+    if (c.dim == 0 || cols % c.dim) return bad("Q's rows are heads of the pools' dim");
+    if (val(o).rows() != T || val(o).cols() != cols) return bad("the output must have Q's shape");
+    c.tokens = (uint32_t)T;
+    c.q_heads = (uint32_t)(cols / c.dim);
+    if (append) {
+      const int kk = op.ins[1], vv = op.ins[2];
+      for (int v : {kk, vv})
+        if (val(v).dtype != c.dtype || val(v).rows() != T || val(v).cols() != (uint64_t)c.heads * c.dim)
+          return bad("K and V need a row of the pools' heads for each of Q's");
+      if (!whole(extra, kI32, T)) return bad("POSITIONS are i32, one a row");
+      const std::string pairs = attr(op, "pairs", "half"), sc = attr(op, "scaling", "none");
+      if (pairs != "half" && pairs != "interleaved") return bad("pairs must be half or interleaved");
+      if (sc != "none" && sc != "linear" && sc != "parts") return bad("scaling must be none, linear or parts");
+      BwppCacheAppendParams r = {};
+      r.cache = c;
+      r.ldq = (uint32_t)val(q).row_stride();
+      r.ldk = (uint32_t)val(kk).row_stride();
+      r.ldv = (uint32_t)val(vv).row_stride();
+      r.ldqo = (uint32_t)val(o).row_stride();
+      r.no_rotation = at.count("rotate", 1) ? 0 : 1;
+      r.rot_dim = at.count("rot", 0);
+      r.layout = pairs == "half" ? BWPP_HIP_ROTARY_HALF : BWPP_HIP_ROTARY_INTERLEAVED;
+      r.scaling = sc == "none" ? BWPP_HIP_ROTARY_SCALE_NONE : sc == "linear" ? BWPP_HIP_ROTARY_SCALE_LINEAR
+                                                                         : BWPP_HIP_ROTARY_SCALE_BY_PARTS;
+      r.base = (float)at.num("base", 0);
+      r.factor = (float)at.num("factor", 0);
+      r.context = at.count("context", 0);
+      r.low_turns = (float)at.num("low", 0);
+      r.high_turns = (float)at.num("high", 0);
+      r.magnitude = (float)at.num("magnitude", 0);
+      if (!at.wrong.empty()) return bad("");
+      if (const BwppHipFault f = bwpp_hip_check_cache_append(r); f.why) return refused(f);
+      s = BWPP_PLAN_CALL(bwpp_hip_dispatch_cache_append(h, ptr(q), ptr(kk), ptr(vv), i32(extra), i32(table), i32(starts), i32(held), ptr(o),
+                                                        ptr(kc), ptr(vc), r));
+    } else {
+      const int lse = op.outs.size() > 1 ? op.outs[1] : -1;
+      if (!whole(lse, BWPP_HIP_F32, T * c.q_heads)) return bad("LSE is f32 [tokens, heads]");
+      if (extra >= 0 && (val(extra).dtype != kI32 || val(extra).kind == Kind::kView || val(extra).rows() != T))
+        return bad("MASK is i32, a row of words for each of Q's");
+      BwppCacheAttentionParams r = {};
+      r.cache = c;
+      r.ldq = (uint32_t)val(q).row_stride();
+      r.ldo = (uint32_t)val(o).row_stride();
+      r.mask_words = extra >= 0 ? (uint32_t)val(extra).cols() : 0;
+      r.scale = attr(op, "scale", "") == "auto" ? 1.0f / std::sqrt((float)c.dim) : (float)at.num("scale", 0);
+      if (!at.wrong.empty()) return bad("");
+      if (const BwppHipFault f = bwpp_hip_check_cache_attention(r, extra >= 0); f.why) return refused(f);
+      s = BWPP_PLAN_CALL(bwpp_hip_dispatch_cache_attention(h, ptr(q), ptr(kc), ptr(vc), i32(table), i32(starts), i32(held),
+                                                           static_cast<const uint32_t *>(ptr(extra)), ptr(o), f32(lse), r));
     }
   }
   if (s != BWPP_HIP_OK) return perr(&p, s, "line %d (%s): %s", op.line, k.c_str(), bwpp_hip_last_error(h));
@@ -1094,7 +1270,7 @@ BwppHipStatus run_op(BwppHipPlan &p, const Op &op) {
                                           ptr(op.outs[2]), ap));
     }
   } else if (checks_own_dtypes(k)) {
-    return run_lm_op(p, op);
+    return k.compare(0, 6, "cache_") == 0 || k == "logit_rules" ? run_cache_op(p, op) : run_lm_op(p, op);
   } else {
     return bad("unknown op");
   }

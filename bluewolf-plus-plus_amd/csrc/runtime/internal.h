@@ -75,6 +75,10 @@ BwppHipFault bwpp_hip_check_rotary(const BwppRotaryParams &p);
 void bwpp_hip_rotary_args(const BwppRotaryParams &p, uint32_t rot, BwppRotaryArgs &a);
 BwppHipFault bwpp_hip_check_residual_norm(const BwppResidualNormParams &p);
 BwppHipFault bwpp_hip_check_linear_xent(const BwppLinearXentParams &p);
+BwppHipFault bwpp_hip_check_cache_append(const BwppCacheAppendParams &p);
+BwppHipFault bwpp_hip_check_cache_attention(const BwppCacheAttentionParams &p, bool mask);
+BwppHipFault bwpp_hip_check_cache_keep(const BwppCacheKeepParams &p);
+BwppHipFault bwpp_hip_check_logit_rules(const BwppLogitRulesParams &p);
 
 // Clears the last error and makes the handle's device current.
 BwppHipStatus bwpp_hip_enter(BwppHip *h);
