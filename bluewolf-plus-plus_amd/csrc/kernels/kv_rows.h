@@ -34,10 +34,7 @@ __device__ __forceinline__ void attend_rows_f32(const BwppCacheAttnArgs &a) {
     {
       const T *Q = static_cast<const T *>(a.q) + (uint64_t)(it.q.first + tok) * a.q_ts + (uint64_t)(it.head * g + row % g) * a.q_hs;
 #pragma unroll
-      for (int j = 0; j < 4 * DB; ++j) {
-        qf[j][0] = qf[j][1] = qf[j][2] = qf[j][3] = 0.0f;
-        if (8u * j < D) load4(Q, 8u * j + 4u * lh, D, qf[j]);
-      }
+      for (int j = 0; j < 4 * DB; ++j) load4(Q, 8u * j + 4u * lh, D, qf[j]);  // zeros past the head's columns
     }
     const T *K = static_cast<const T *>(c.k) + (uint64_t)it.head * c.head_s;
     const T *V = static_cast<const T *>(c.v) + (uint64_t)it.head * c.head_s;
@@ -98,15 +95,19 @@ __device__ __forceinline__ void attend_rows_f32(const BwppCacheAttnArgs &a) {
         if (mine) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+          // Operands are read ahead of their products; the order is held by hand.
+          auto read = [&](int j) { return *reinterpret_cast<const float4 *>(&ks[lq][8u * j + 4u * lh]); };
+          float4 k4[2] = {read(0), read(1)};
 #pragma unroll
           for (int j = 0; j < 4 * DB; ++j) {
-            if (8u * j >= D) continue;
-            const float4 k4 = *reinterpret_cast<const float4 *>(&ks[lq][8u * j + 4u * lh]);
-            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.x, qf[j][0], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.y, qf[j][1], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.z, qf[j][2], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4.w, qf[j][3], s, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4[j % 2].x, qf[j][0], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4[j % 2].y, qf[j][1], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4[j % 2].z, qf[j][2], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(k4[j % 2].w, qf[j][3], s, 0, 0, 0);
+            if (j + 2 < 4 * DB) k4[j % 2] = read(j + 2);
           }
+          __builtin_amdgcn_sched_barrier(0);
           const uint32_t w = vis >> (4u * lh);
           float mx = -INFINITY;
 #pragma unroll
@@ -161,13 +162,18 @@ __device__ __forceinline__ void attend_rows_f32(const BwppCacheAttnArgs &a) {
           __syncthreads();
         }
         if (mine) {
+          constexpr int N = 16 * DB, kAhead = 6;
+          auto read = [&](int i) { return vs[8 * (i / DB >> 2) + 4 * lh + (i / DB & 3)][32 * (i % DB) + lq]; };
+          float v[kAhead];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float *v = vs[8 * (r >> 2) + 4 * lh + (r & 3)] + lq;
+          for (int i = 0; i < kAhead; ++i) v[i] = read(i);
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
-              if (32u * d < D) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * d], s[r], o[d], 0, 0, 0);
+          for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            o[i % DB] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[i % kAhead], s[i / DB], o[i % DB], 0, 0, 0);
+            if (i + kAhead < N) v[i % kAhead] = read(i + kAhead);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
       seg = end;
@@ -204,11 +210,19 @@ __device__ __forceinline__ void attend_rows_f32(const BwppCacheAttnArgs &a) {
   extern "C" __global__ __launch_bounds__(256, DB <= 4 ? 2 : 1) void bwpp_cache_attend_##NAME(const BwppCacheAttnArgs a) { \
     kv::attend_rows_f32<T, DB>(a);                                                                                    \
   }
+BWPP_ATTEND_ROWS_F32(f32_rows_d32, float, 1)
 BWPP_ATTEND_ROWS_F32(f32_rows_d64, float, 2)
+BWPP_ATTEND_ROWS_F32(f32_rows_d96, float, 3)
 BWPP_ATTEND_ROWS_F32(f32_rows_d128, float, 4)
+BWPP_ATTEND_ROWS_F32(f32_rows_d160, float, 5)
 BWPP_ATTEND_ROWS_F32(f32_rows_d192, float, 6)
+BWPP_ATTEND_ROWS_F32(f32_rows_d224, float, 7)
 BWPP_ATTEND_ROWS_F32(f32_rows_d256, float, 8)
+BWPP_ATTEND_ROWS_F32(bf16_rows_d32, uint16_t, 1)
 BWPP_ATTEND_ROWS_F32(bf16_rows_d64, uint16_t, 2)
+BWPP_ATTEND_ROWS_F32(bf16_rows_d96, uint16_t, 3)
 BWPP_ATTEND_ROWS_F32(bf16_rows_d128, uint16_t, 4)
+BWPP_ATTEND_ROWS_F32(bf16_rows_d160, uint16_t, 5)
 BWPP_ATTEND_ROWS_F32(bf16_rows_d192, uint16_t, 6)
+BWPP_ATTEND_ROWS_F32(bf16_rows_d224, uint16_t, 7)
 BWPP_ATTEND_ROWS_F32(bf16_rows_d256, uint16_t, 8)

@@ -17,8 +17,9 @@ enum CacheKernel {
   CK_APPEND_BF16,                      // [interleaved][chunk 8, 4, 1]
   CK_APPEND_F32 = CK_APPEND_BF16 + 6,  // [interleaved][chunk 4, 1]
   CK_KEEP = CK_APPEND_F32 + 4,         // chunks of 16, 4, 2 bytes
-  CK_ATTEND = CK_KEEP + 3,             // [bf16][rows][dim up to 64, 128, 192, 256]
-  CK_ATTEND_FEW = CK_ATTEND + 16,      // [kFlashDims]
+  CK_ATTEND = CK_KEEP + 3,             // [bf16][dim up to 64, 128, 192, 256]
+  CK_ATTEND_ROWS = CK_ATTEND + 8,      // [bf16][dim up to 32, 64, .. 256]
+  CK_ATTEND_FEW = CK_ATTEND_ROWS + 16, // [kFlashDims]
   CK_ATTEND_R128 = CK_ATTEND_FEW + 7,  // [kFlashDims]
   CK_ATTEND_R256 = CK_ATTEND_R128 + 7, // [kFlashDims up to 128]
   CK_JOIN_F32 = CK_ATTEND_R256 + 4,    // tiles of 16, 128 rows
@@ -47,17 +48,25 @@ const char *const bwpp_hip_cache_kernels[] = {
     "bwpp_cache_attend_f32_d128",
     "bwpp_cache_attend_f32_d192",
     "bwpp_cache_attend_f32_d256",
-    "bwpp_cache_attend_f32_rows_d64",
-    "bwpp_cache_attend_f32_rows_d128",
-    "bwpp_cache_attend_f32_rows_d192",
-    "bwpp_cache_attend_f32_rows_d256",
     "bwpp_cache_attend_bf16_d64",
     "bwpp_cache_attend_bf16_d128",
     "bwpp_cache_attend_bf16_d192",
     "bwpp_cache_attend_bf16_d256",
+    "bwpp_cache_attend_f32_rows_d32",
+    "bwpp_cache_attend_f32_rows_d64",
+    "bwpp_cache_attend_f32_rows_d96",
+    "bwpp_cache_attend_f32_rows_d128",
+    "bwpp_cache_attend_f32_rows_d160",
+    "bwpp_cache_attend_f32_rows_d192",
+    "bwpp_cache_attend_f32_rows_d224",
+    "bwpp_cache_attend_f32_rows_d256",
+    "bwpp_cache_attend_bf16_rows_d32",
     "bwpp_cache_attend_bf16_rows_d64",
+    "bwpp_cache_attend_bf16_rows_d96",
     "bwpp_cache_attend_bf16_rows_d128",
+    "bwpp_cache_attend_bf16_rows_d160",
     "bwpp_cache_attend_bf16_rows_d192",
+    "bwpp_cache_attend_bf16_rows_d224",
     "bwpp_cache_attend_bf16_rows_d256",
     "bwpp_cache_attend_few_d64",
     "bwpp_cache_attend_few_d80",
@@ -443,8 +452,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
     a.part_ml = a.part_o + (size_t)2 * a.blocks * rows * Dp;
   }
   const bool bf16 = cp.dtype == BWPP_HIP_BF16;
-  const int attend = flash < 0       ? CK_ATTEND + (bf16 ? 8 : 0) + (rows == 128 ? 4 : 0) + (int)((cp.dim - 1) / 64)
-                     : flash + (rows == 32 ? CK_ATTEND_FEW : rows == 128 ? CK_ATTEND_R128 : CK_ATTEND_R256);
+  const int attend = flash >= 0    ? flash + (rows == 32 ? CK_ATTEND_FEW : rows == 128 ? CK_ATTEND_R128 : CK_ATTEND_R256)
+                     : rows == 128 ? CK_ATTEND_ROWS + (bf16 ? 8 : 0) + (int)((cp.dim - 1) / 32)
+                                   : CK_ATTEND + (bf16 ? 4 : 0) + (int)((cp.dim - 1) / 64);
   const int join = bf16 ? CK_JOIN_BF16 + (rows == 16 ? 0 : rows == 32 ? 1 : rows == 128 ? 2 : 3)
                         : CK_JOIN_F32 + (rows == 16 ? 0 : 1);
   s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, rows == 32 ? 128 : rows == 256 ? 512 : 256, &a);

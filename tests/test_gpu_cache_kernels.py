@@ -40,10 +40,10 @@ def test_every_kernel_is_reached(be):
             assert k == [f"bwpp_cache_attend_{kernel}_d{d}"]
             seen.update(k)
     for dtype, name, pad in ((F32, "f32", 0), (BF16, "bf16", 1)):
-        for d in (64, 128, 192, 256):
-            for n, rows in ((64, ""), (65, "_rows")):
+        for d in range(32, 257, 32):
+            for n, kernel in ((64, f"d{-(-d // 64) * 64}"), (65, f"rows_d{d}")):
                 k = _attend(be, dtype, d, n, pad=pad)
-                assert k == [f"bwpp_cache_attend_{name}{rows}_d{d}"]
+                assert k == [f"bwpp_cache_attend_{name}_{kernel}"]
                 seen.update(k)
     for dtype, d, n, join in ((F32, 64, 1, "f32_16"), (F32, 64, 65, "f32_128"), (BF16, 63, 1, "bf16_16"),
                               (BF16, 64, 1, "bf16_32"), (BF16, 64, 128, "bf16_128"), (BF16, 64, 129, "bf16_256")):
