@@ -81,10 +81,6 @@ __device__ __forceinline__ void g2lds16_so(const void *sbase, uint32_t voff, uin
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase)
                : "memory");
 }
-// The same from a 64-bit address per lane.
-__device__ __forceinline__ void g2lds16_v(const void *addr, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_addr), "v"(addr) : "memory");
-}
 
 template <int D>
 struct AttnTile {

@@ -926,3 +926,9 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_attn_conv_f32_to_bf16(con
     }
   }
 }
+
+// Attention over a paged cache shares this code object (and its form of matrix
+// instructions).
+#include "kv_attention.h"
+#include "kv_flash.h"
+#include "kv_rows.h"

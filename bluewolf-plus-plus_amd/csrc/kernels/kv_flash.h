@@ -34,6 +34,17 @@
 
 namespace kv {
 
+// 16 bytes a lane from memory to LDS (see g2lds16_so), from a scalar base or a
+// 64-bit address a lane.  The LDS address passes through a scalar register by
+// name: one chosen by the compiler may be VCC, and the code objects' check of M0
+// takes plain ones.
+__device__ __forceinline__ void dma16_so(const void *sbase, uint32_t voff, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{s33}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+}
+__device__ __forceinline__ void dma16_v(const void *addr, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"{s33}"(lds_addr), "v"(addr) : "memory");
+}
+
 // A tile of key or value rows in LDS: dense rows of D / 8 chunks of 16 bytes,
 // chunk c of row r at c ^ swz(r).
 template <int D>
@@ -281,16 +292,16 @@ struct Fetch {
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
           if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
-          g2lds16_so(K + base, koff(i), lds + (i * FROM_WAVES + wave) * 1024u);
-          g2lds16_so(V + base, voff(i), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so(K + base, koff(i), lds + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so(V + base, voff(i), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
         }
       } else {  // rows past the last key re-read it
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
           if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
           const uint32_t r = slot(i, wave) / R::kSlots, back = r < n ? 0u : 2u * (r - (n - 1)) * tok_s;
-          g2lds16_so(K + base, koff(i) - back, lds + (i * FROM_WAVES + wave) * 1024u);
-          g2lds16_so(V + base, voff(i) - back, lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so(K + base, koff(i) - back, lds + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so(V + base, voff(i) - back, lds + kTile + (i * FROM_WAVES + wave) * 1024u);
         }
       }
     } else {
@@ -302,8 +313,8 @@ struct Fetch {
         // less the row's offset, which koff and voff have
         const uint64_t row = (uint64_t)page * (uint32_t)c.page_s + (uint64_t)(key & pmask) * tok_s;
         const uint32_t mine = 2u * r * tok_s;
-        g2lds16_v(reinterpret_cast<const char *>(K + row) + (koff(i) - mine), lds + (i * FROM_WAVES + wave) * 1024u);
-        g2lds16_v(reinterpret_cast<const char *>(V + row) + (voff(i) - mine), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+        dma16_v(reinterpret_cast<const char *>(K + row) + (koff(i) - mine), lds + (i * FROM_WAVES + wave) * 1024u);
+        dma16_v(reinterpret_cast<const char *>(V + row) + (voff(i) - mine), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
       }
     }
   }

@@ -830,6 +830,9 @@ extern "C" __global__ __launch_bounds__(256) void bwpp_col_mask(const BwppRowArg
   }
 }
 
-// Row kernels of the operators around a block share this code object.
+// Row kernels of the operators around a block, of a paged cache and of logits
+// share this code object.
+#include "kv_append.h"
+#include "logit_rules.h"
 #include "resnorm.h"
 #include "rotary.h"

@@ -1,6 +1,6 @@
-"""The code objects of the paged cache and the rules on logits hold the kernels
-that the runtime names and no others, their direct-to-LDS loads follow the rule
-for M0, and they have no packed fp32 instructions."""
+"""The code objects that hold the paged cache's and the rules' kernels hold those
+that the runtime names and no others of them, their direct-to-LDS loads follow the
+rule for M0, and they have no packed fp32 instructions."""
 import os
 import re
 import shutil
@@ -9,9 +9,10 @@ import subprocess
 import pytest
 
 from bwpp import _lib
-from test_codeobj_m0 import IMPLICIT, LIB, LLVM, _asm
+from test_codeobj_m0 import LIB, LLVM, _asm
+from test_codeobj_m0 import test_m0_written_only_by_lds_dma_asm as check_m0
 
-OBJECTS = ("cache", "cache_bf16")
+OBJECTS = ("rowops", "attention_f32")
 
 
 def kernel_names():
@@ -21,17 +22,9 @@ def kernel_names():
 
 @pytest.mark.parametrize("kernel", OBJECTS)
 def test_instructions(kernel, tmp_path):
+    check_m0(kernel, tmp_path)
     lines = _asm(kernel, tmp_path)
-    assert len(lines) > 100
-    for i, ins in enumerate(lines):
-        assert not IMPLICIT.search(ins), f"instruction reads M0 implicitly: {ins}"
-        after = lines[i + 1] if i + 1 < len(lines) else ""
-        if re.search(r"\bm0\b", ins):  # from a scalar register (VCC is one), right before its load
-            assert re.match(r"s_mov_b32 m0, (s\d+|vcc_lo|vcc_hi)$", ins) and after.startswith("global_load_lds_dwordx4"), (ins, after)
-        if ins.startswith("global_load_lds_dwordx4"):
-            assert i > 0 and lines[i - 1].startswith("s_mov_b32 m0,"), ins
     assert not [ln for ln in lines if ln.startswith(("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32"))]
-    assert any(ln.startswith("global_load_lds_dwordx4") for ln in lines) == (kernel == "cache_bf16")
 
 
 def test_kernels_are_in_their_code_objects(tmp_path):
@@ -45,5 +38,6 @@ def test_kernels_are_in_their_code_objects(tmp_path):
         subprocess.run([os.path.join(LLVM, "clang-offload-bundler"), "--unbundle", "--type=o", f"--input={bundle}",
                         "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", f"--output={obj}"], check=True)
         out = subprocess.run([dump, "--syms", str(obj)], check=True, capture_output=True, text=True).stdout
-        have += [ln.split()[-1] for ln in out.splitlines() if " F .text" in ln]
+        have += [n for n in (ln.split()[-1] for ln in out.splitlines() if " F .text" in ln)
+                 if n.startswith(("bwpp_cache", "bwpp_logit"))]
     assert sorted(have) == sorted(names)
