@@ -264,21 +264,64 @@ __device__ __forceinline__ void attend_split(const BwppCacheAttnArgs &a) {
   });
 }
 
-// Joins the parts of the item that the border before sharer b is the first to
-// divide (b = 1 .. blocks - 1), kJoin rows of it a block: blockIdx.y's.  A chain of
-// latencies, so the parts' pairs and first sums are fetched at once, and every
-// thread makes its row's factors by itself.
+// Four columns at E places of an item's tile, joined from its parts, P of which
+// are fetched at once.
+template <int E, int P, class Sums, class Pair, class Put>
+__device__ __forceinline__ void join_columns(uint32_t i0, uint32_t end, uint32_t parts, Sums sums, Pair pair, Put put) {
+  float4 u[E][P], v[E];
+  float2 w[E][P];
+  float m[E], l[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    m[e] = -INFINITY;
+    l[e] = 0.0f;
+  }
+  for (uint32_t k = 0; k < parts; k += P) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t i = i0 + e * kThreads;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const bool there = i < end && k + j < parts;
+        w[e][j] = there ? pair(k + j, i) : make_float2(-INFINITY, 0.0f);
+        u[e][j] = there ? sums(k + j, i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float top = m[e];
+#pragma unroll
+      for (int j = 0; j < P; ++j) top = fmaxf(top, w[e][j].x);
+      // no key seen (offset -inf): sums of 0 (or NaN, kept)
+      auto factor = [&](float o) { return o == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(o - top); };
+      const float f = factor(m[e]);
+      l[e] *= f;
+      v[e] = make_float4(v[e].x * f, v[e].y * f, v[e].z * f, v[e].w * f);
+      m[e] = top;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float fj = factor(w[e][j].x);
+        l[e] += w[e][j].y * fj;
+        v[e].x += u[e][j].x * fj, v[e].y += u[e][j].y * fj, v[e].z += u[e][j].z * fj, v[e].w += u[e][j].w * fj;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (i0 + e * kThreads < end) put(i0 + e * kThreads, v[e], m[e], l[e]);
+}
+
+// Joins the parts of divided items.  The blocks of a border (blockIdx.x + 1, a
+// column of the grid) work on the item that it divides, with those of the other
+// borders inside it, each on an even share of its tile's places (a row's four
+// columns): parts times places of a block are much the same for any lengths.
 template <class T, uint32_t kRows, uint32_t kUnit>
 __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
   typedef Work<kRows, kUnit> W;
-  constexpr uint32_t kJoin = 16;                       // rows a block
-  constexpr uint32_t kParts = 64;                      // a round of them in LDS
-  constexpr uint32_t kMost = kJoin * 64u / kThreads;   // float4 a thread, dim 256
-  constexpr uint32_t kAhead = 16;                      // sums on the way at once; the first with the pairs
-  __shared__ float2 pair[kParts][kJoin];
   const BwppCacheArgs &c = a.c;
   const Costs<kRows, kUnit> costs(a);
-  const uint32_t b = blockIdx.x + 1, row0 = blockIdx.y * kJoin;
+  const uint32_t b = blockIdx.x + 1;
   const uint64_t S = share_of(a, costs.total), x = S * b;
   if (costs.whole || x >= costs.total) return;
   Seq q;
@@ -286,80 +329,37 @@ __device__ __forceinline__ void join(const BwppCacheAttnArgs &a) {
   const uint32_t seq = costs.at(a, x, q, before);
   const Place item = W::find(a, false, seq, q, x - before, begin, end);
   if (item.unit == 0) return;
-  if (x - S >= before + begin && W::unit(a, q, item.tile, x - S - before - begin, end - begin) != 0) return;  // not the first
-  const uint32_t g = a.group, D = c.dim, n4 = (D + 3u) / 4u, Dp = 4u * n4;
-  const uint32_t all = min(kRows, q.n * g - item.tile * kRows);
-  if (row0 >= all) return;
-  uint32_t last = (uint32_t)((double)(before + end - 1) / (double)S);  // the last border before the item's end
+  // Its borders first .. last; before them one may lie in it and divide nothing (unit 0).
+  uint32_t first = (uint32_t)((double)(before + begin) / (double)S);
+  if (S * first < before + begin) ++first;
+  first = min(max(first, 1u), b);
+  while (first < b && W::unit(a, q, item.tile, S * first - before - begin, end - begin) == 0) ++first;
+  uint32_t last = (uint32_t)((double)(before + end - 1) / (double)S);
   if (S * last >= before + end) --last;  // (a quotient rounded up)
-  const uint32_t rows = min(kJoin, all - row0), parts = last - b + 2;
-  // part 0 in slot 2 (b - 1) + 1, part k in slot 2 (b + k - 1)
-  auto slot_row = [&](uint32_t k) { return (uint64_t)(k == 0 ? 2 * b - 1 : 2 * (b + k - 1)) * kRows + row0; };
-  auto sums = [&](uint32_t k, uint32_t r, uint32_t col) {
-    return *reinterpret_cast<const float4 *>(a.part_o + (slot_row(k) + r) * Dp + col);
-  };
-  float4 v[kMost], u[kAhead];
-  float m[kMost], l[kMost];
-#pragma unroll
-  for (uint32_t e = 0; e < kMost; ++e) {
-    const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
-    v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    m[e] = -INFINITY;
-    l[e] = 0.0f;
-  }
-  auto fetch = [&](uint32_t k, uint32_t n, uint32_t r, uint32_t col) {  // parts k .. below n
-#pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j)
-      u[j] = k + j < n ? sums(k + j, r, col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  };
-  if (threadIdx.x / n4 < rows) fetch(0, parts, threadIdx.x / n4, 4u * (threadIdx.x % n4));
-  for (uint32_t k0 = 0; k0 < parts; k0 += kParts) {
-    const uint32_t n = min(kParts, parts - k0);
-    if (k0) __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n * kJoin; i += kThreads) {
-      const uint32_t k = i / kJoin, r = i % kJoin;
-      if (r < rows) pair[k][r] = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (slot_row(k0 + k) + r));
-    }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t e = 0; e < kMost; ++e) {
-      const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
-      if (r >= rows) continue;
-      float top = m[e];
-#pragma unroll 16
-      for (uint32_t k = 0; k < n; ++k) top = fmaxf(top, pair[k][r].x);
-      // no key seen (offset -inf): sums of 0 (or NaN, kept)
-      auto factor = [&](float o) { return o == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(o - top); };
-      if (k0) {
-        const float f = factor(m[e]);
-        l[e] *= f;
-        v[e].x *= f, v[e].y *= f, v[e].z *= f, v[e].w *= f;
-      }
-      m[e] = top;
-      for (uint32_t k = 0; k < n; k += kAhead) {
-        if (e || k0 || k) fetch(k0 + k, k0 + n, r, col);
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; ++j) {
-          if (k + j >= n) break;
-          const float2 w = pair[k + j][r];
-          const float f = factor(w.x);
-          l[e] += w.y * f;
-          v[e].x += u[j].x * f, v[e].y += u[j].y * f, v[e].z += u[j].z * f, v[e].w += u[j].w * f;
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (uint32_t e = 0; e < kMost; ++e) {
-    const uint32_t i = threadIdx.x + e * kThreads, r = i / n4, col = 4u * (i % n4);
-    if (r >= rows) continue;
-    const uint32_t rr = item.tile * kRows + row0 + r;
+  last = min(max(last, b), a.blocks - 1u);  // (costs past 2^52: only sequences that overlap have them)
+  const uint32_t g = a.group, D = c.dim, n4 = (D + 3u) / 4u, Dp = 4u * n4;
+  const uint32_t places = min(kRows, q.n * g - item.tile * kRows) * n4, parts = last - first + 2;
+  const uint32_t sharers = (last - first + 1) * gridDim.y, per = (places + sharers - 1) / sharers;
+  const uint32_t i0 = per * ((b - first) * gridDim.y + blockIdx.y), i1 = min(i0 + per, places);
+  // part 0 in slot 2 (first - 1) + 1, part k in slot 2 (first + k - 1)
+  auto slot_row = [&](uint32_t k) { return (uint64_t)(k == 0 ? 2 * first - 1 : 2 * (first + k - 1)) * kRows; };
+  auto sums = [&](uint32_t k, uint32_t i) { return *reinterpret_cast<const float4 *>(a.part_o + slot_row(k) * Dp + 4u * i); };
+  auto pair = [&](uint32_t k, uint32_t i) { return *reinterpret_cast<const float2 *>(a.part_ml + 2 * (slot_row(k) + i / n4)); };
+  auto put = [&](uint32_t i, const float4 &v, float m, float l) {
+    const uint32_t r = i / n4, col = 4u * (i % n4), rr = item.tile * kRows + r;
     const uint64_t t = q.first + rr / g, hh = item.head * g + rr % g;
-    const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
-    const float u[4] = {v[e].x * inv, v[e].y * inv, v[e].z * inv, v[e].w * inv};
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float u[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
     store4(static_cast<T *>(a.o) + t * a.o_ts + hh * a.o_hs, col, D, u);
-    if (col == 0 && a.lse)
-      a.lse[t * (uint64_t)(c.heads * g) + hh] = l[e] == 0.0f ? -INFINITY : lse_of(m[e] == -INFINITY ? 0.0f : m[e], l[e]);
+    if (col == 0 && a.lse) a.lse[t * (uint64_t)(c.heads * g) + hh] = l == 0.0f ? -INFINITY : lse_of(m == -INFINITY ? 0.0f : m, l);
+  };
+  const uint32_t i = i0 + threadIdx.x;
+  if (per <= kThreads) {
+    if (i < i1) join_columns<1, 16>(i, i1, parts, sums, pair, put);
+  } else if (parts <= 4) {
+    for (uint32_t e = i; e < i1; e += 4 * kThreads) join_columns<4, 4>(e, i1, parts, sums, pair, put);
+  } else {
+    for (uint32_t e = i; e < i1; e += 2 * kThreads) join_columns<2, 8>(e, i1, parts, sums, pair, put);
   }
 }
 
@@ -379,7 +379,7 @@ BWPP_ATTEND(bf16_d192, uint16_t, 3)
 BWPP_ATTEND(bf16_d256, uint16_t, 4)
 
 #define BWPP_JOIN(NAME, T, ROWS) \
-  extern "C" __global__ __launch_bounds__(256) void bwpp_cache_join_##NAME(const BwppCacheAttnArgs a) { kv::join<T, ROWS, 64>(a); }
+  extern "C" __global__ __launch_bounds__(256, 4) void bwpp_cache_join_##NAME(const BwppCacheAttnArgs a) { kv::join<T, ROWS, 64>(a); }
 BWPP_JOIN(f32_16, float, 16)
 BWPP_JOIN(f32_128, float, 128)
 BWPP_JOIN(bf16_16, uint16_t, 16)

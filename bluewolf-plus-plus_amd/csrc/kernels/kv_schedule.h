@@ -19,7 +19,8 @@
 // Costs are whole numbers below 2^52, g times keys (g query heads a key head);
 // quotients are taken in doubles (64-bit integer ones cost a microsecond
 // here), the same in every block, so a sharer and its successor find the same
-// border.
+// border.  Only starts that descend can bring more, up to 2^62: then quotients
+// may be off, and are cut to what there is.
 #pragma once
 
 #include "kv_cache.h"
@@ -65,7 +66,7 @@ struct Work {
                                                uint64_t &begin, uint64_t &end) {
     const uint32_t T = tiles(q, a.group);
     const uint64_t head_cost = before(q, a.group, T);
-    uint32_t head = (uint32_t)((double)x / (double)head_cost);
+    uint32_t head = min((uint32_t)((double)x / (double)head_cost), a.c.heads - 1u);
     if (head * head_cost > x) --head;  // (a quotient rounded up)
     const uint64_t rest = x - head * head_cost;
     uint32_t lo = 0, hi = T;  // before(lo) <= rest < before(hi)

@@ -415,10 +415,12 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   const uint64_t mean = (T + cp.batch - 1) / cp.batch * g;
   const uint32_t rows = flash < 0 ? (mean > 64 ? 128u : 16u) : mean <= 32 ? 32u : mean <= 128 || cp.dim > 128 ? 128u : 256u;
   const uint32_t Dp = (cp.dim + 3) / 4 * 4;
-  // Costs (kv_schedule.h) are counted in 64 bits and multiplied by the blocks.
-  const long double worst = (long double)cp.heads * ((long double)T * g / rows + cp.batch) *
-                            ((long double)g * (c.capacity + 256) + (long double)T * g + 2 * rows);
-  if (worst > 4503599627370496.0L) return bad(BWPP_HIP_ERR_UNSUPPORTED, "tokens times the longest sequence out of range");
+  // Costs (kv_schedule.h) are taken in doubles too: below 2^52; and, whatever starts
+  // holds (sequences that overlap each count all rows), in 64 bits with a share more.
+  const long double item = (long double)cp.heads * ((long double)g * (c.capacity + 256) + (long double)T * g + 2 * rows);
+  if (item * ((long double)T * g / rows + cp.batch) > 4503599627370496.0L ||
+      item * ((long double)T * g / rows + 1) * cp.batch > 4611686018427387904.0L)
+    return bad(BWPP_HIP_ERR_UNSUPPORTED, "tokens times the longest sequence out of range");
   BwppHipStatus s = bwpp_hip_enter(h);
   if (s != BWPP_HIP_OK) return s;
 
@@ -459,7 +461,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
                         : CK_JOIN_F32 + (rows == 16 ? 0 : 1);
   s = bwpp_hip_launch_cache(h, attend, a.blocks, 1, rows == 32 ? 128 : rows == 256 ? 512 : 256, &a);
   if (s != BWPP_HIP_OK || !parts) return s;
-  return bwpp_hip_launch_cache(h, join, a.blocks - 1, (rows + 15) / 16, 256, &a);
+  return bwpp_hip_launch_cache(h, join, a.blocks - 1, rows <= 32 ? 1 : rows / 64, 256, &a);
 }
 
 // ------------------------------------------------------------------- rules

@@ -777,7 +777,7 @@ BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *q, const vo
  * probabilities enter the product with v as two bf16 terms, or, for more than 32
  * rows (tokens times q_heads / heads, on average) of dims 64, 80, 96, 128, 160, 192
  * and 256, rounded to one.  Workspace: two partial results for each of one or two
- * blocks a compute unit, 16 to 256 rows of dim + 2 floats each (at most 128 MiB on
+ * blocks a compute unit, 16 to 256 rows of dim + 2 floats each (at most 65 MiB on
  * 256 of them), whatever the lengths. */
 BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const void *q, const void *k_cache, const void *v_cache,
                                                 const int32_t *table, const int32_t *starts, const int32_t *held,

@@ -119,6 +119,9 @@ def test_attention_refusals():
     assert _taken(name, args={6: I}, mask_words=1)
     assert _op(name, dict(dim=257))[0] == S.UNSUPPORTED
     assert _op(name, dict(tokens=1 << 28, max_pages=1 << 26))[0] == S.UNSUPPORTED
+    # sequences of which each could, by its starts, count all rows
+    assert _op(name, dict(tokens=1 << 24, max_pages=1 << 12, batch=1 << 24))[0] == S.UNSUPPORTED
+    assert _taken(name, dict(tokens=1 << 24, max_pages=1 << 12, batch=1 << 10))
     for args in ({7: A}, {7: B + 4}, {7: C}, {8: A}, {8: B}, {8: G}, {7: D}, {8: E}, {7: F - 4}):
         assert _op(name, args=args)[0] == S.ALIAS, args
     assert _op(name, args={6: G + 4}, mask_words=2)[0] == S.ALIAS
