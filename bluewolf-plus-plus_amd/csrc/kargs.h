@@ -307,6 +307,7 @@ typedef struct {
   uint32_t blocks;      /* blocks that share the keys */
   double inv_blocks;    /* 1 / blocks */
   uint32_t whole_keys;  /* sequences up to here have whole items */
+  uint32_t item_keys;   /* keys that an item costs by itself */
   float *part_o;        /* [2 blocks][rows of a tile][dim up to a multiple of 4] */
   float *part_ml;       /* [2 blocks][rows of a tile][2] */
 } BwppCacheAttnArgs;

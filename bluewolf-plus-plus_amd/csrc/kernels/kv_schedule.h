@@ -6,7 +6,7 @@
 // a tile of ROWS query rows of one (sequence, key head) with all the keys that
 // it sees, in units of UNIT keys.  Items stand in the order of sequences, heads
 // and tiles, each with a cost: its keys (of a causal tile up to its last
-// token) and kItem more for what an item costs by itself.  Block b of G takes
+// token) and item_keys more for what an item costs by itself.  Block b of G takes
 // what lies between the costs W b / G and W (b + 1) / G of the total W, rounded
 // to whole units.  An item whose keys fall to several blocks is left by each
 // as a triple (exponent offset, sum of p, sum of p v) and joined by a second
@@ -27,7 +27,6 @@
 
 namespace kv {
 
-constexpr uint32_t kItem = 96;   // keys that an item costs by itself
 constexpr uint32_t kLeast = 64;  // a block's share is at least as many keys
 
 // A place in the order of the work.
@@ -48,8 +47,8 @@ struct Share {
 template <uint32_t ROWS, uint32_t UNIT>
 struct Work {
   static __device__ __forceinline__ uint32_t tiles(const Seq &q, uint32_t g) { return (q.n * g + ROWS - 1) / ROWS; }
-  static __device__ __forceinline__ uint64_t before(const Seq &q, uint32_t g, uint64_t t) {  // cost of tiles 0 .. t - 1
-    return t * ((uint64_t)g * (q.held + kItem)) + ROWS * (t * (t + 1) / 2);
+  static __device__ __forceinline__ uint64_t before(const BwppCacheAttnArgs &a, const Seq &q, uint64_t t) {  // cost of tiles 0 .. t - 1
+    return t * ((uint64_t)a.group * (q.held + a.item_keys)) + ROWS * (t * (t + 1) / 2);
   }
   // Keys that a tile may see.
   static __device__ __forceinline__ uint32_t keys(const BwppCacheAttnArgs &a, const Seq &q, uint32_t tile) {
@@ -65,17 +64,17 @@ struct Work {
   static __device__ __forceinline__ Place find(const BwppCacheAttnArgs &a, bool whole, uint32_t s, const Seq &q, uint64_t x,
                                                uint64_t &begin, uint64_t &end) {
     const uint32_t T = tiles(q, a.group);
-    const uint64_t head_cost = before(q, a.group, T);
+    const uint64_t head_cost = before(a, q, T);
     uint32_t head = min((uint32_t)((double)x / (double)head_cost), a.c.heads - 1u);
     if (head * head_cost > x) --head;  // (a quotient rounded up)
     const uint64_t rest = x - head * head_cost;
     uint32_t lo = 0, hi = T;  // before(lo) <= rest < before(hi)
     while (hi - lo > 1) {
       const uint32_t m = (lo + hi) / 2;
-      if (before(q, a.group, m) <= rest) lo = m;
+      if (before(a, q, m) <= rest) lo = m;
       else hi = m;
     }
-    const uint64_t b0 = before(q, a.group, lo), b1 = before(q, a.group, lo + 1);
+    const uint64_t b0 = before(a, q, lo), b1 = before(a, q, lo + 1);
     begin = head * head_cost + b0;
     end = head * head_cost + b1;
     return {s, head, lo, whole ? 0u : unit(a, q, lo, rest - b0, b1 - b0)};
@@ -103,7 +102,7 @@ struct Costs {
   bool whole;      // every sequence is so short that its items are not shared
 
   static __device__ __forceinline__ uint64_t of(const BwppCacheAttnArgs &a, const Seq &q) {
-    return a.c.heads * Work<ROWS, UNIT>::before(q, a.group, Work<ROWS, UNIT>::tiles(q, a.group));
+    return a.c.heads * Work<ROWS, UNIT>::before(a, q, Work<ROWS, UNIT>::tiles(q, a.group));
   }
   __device__ __forceinline__ Costs(const BwppCacheAttnArgs &a) {
     const uint32_t lane = threadIdx.x & 63u;

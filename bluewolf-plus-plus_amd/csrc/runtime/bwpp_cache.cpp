@@ -417,7 +417,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   const uint32_t Dp = (cp.dim + 3) / 4 * 4;
   // Costs (kv_schedule.h) are taken in doubles too: below 2^52; and, whatever starts
   // holds (sequences that overlap each count all rows), in 64 bits with a share more.
-  const long double item = (long double)cp.heads * ((long double)g * (c.capacity + 256) + (long double)T * g + 2 * rows);
+  const long double item = (long double)cp.heads * ((long double)g * (c.capacity + 512) + (long double)T * g + 2 * rows);
   if (item * ((long double)T * g / rows + cp.batch) > 4503599627370496.0L ||
       item * ((long double)T * g / rows + 1) * cp.batch > 4611686018427387904.0L)
     return bad(BWPP_HIP_ERR_UNSUPPORTED, "tokens times the longest sequence out of range");
@@ -445,6 +445,10 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // 10.7, 3 x 550 tokens of 64 : 8 heads 68 and 45 (past 1024 keys parts win: one
   // sequence of 1000 tokens 12.8 in parts, 16 whole; fp32 4 x 416 tokens 300 and 393).
   a.whole_keys = flash < 0 ? 256 : rows == 32 ? 512 : 1024;
+  // What starting and ending an item takes, in keys: 128 sequences of up to 2000
+  // tokens 57 us with 96, 48 with 192, 49 with 384; 2 x 2048 tokens of prompts 386,
+  // 376, 378, those of d = 256 95, 89, 83; fp32 2 x 1024 tokens 257, 268, 284.
+  a.item_keys = flash < 0 ? 96 : rows == 32 ? 192 : 384;
   const bool parts = c.capacity > a.whole_keys;
   if (parts) {
     void *ws = nullptr;
