@@ -6,7 +6,7 @@
 //   v forbidden by the mask (its bit 0): z = -inf
 //
 // Bound by HBM: a logit is read and written once.  A block takes a chunk of
-// one row's columns, counts the row's history in LDS (bit 31: v occurs, below
+// one row's columns, counts the row's history in LDS (bit 31: v was given, below
 // it c; whole numbers, so the order of the additions does not matter) and then
 // goes over its chunk, which it has fetched meanwhile.
 #pragma once
@@ -19,7 +19,8 @@ using namespace bwpp;
 
 namespace logits {
 
-constexpr uint32_t kPer = 4;  // 4-element chunks a thread
+constexpr uint32_t kPer = 4;   // 4-element chunks a thread
+constexpr uint32_t kPast = 8;  // tokens of the history on the way at once
 
 template <class TX, class TY>
 __device__ __forceinline__ void rules(const BwppLogitArgs &a) {
@@ -45,12 +46,16 @@ __device__ __forceinline__ void rules(const BwppLogitArgs &a) {
     if (n) {  // uniform in the block
       for (uint32_t i = threadIdx.x; i < nc; i += NT) seen[i] = 0u;
       __syncthreads();
-      for (uint32_t i = threadIdx.x; i < n; i += NT) {
-        const uint32_t t = (uint32_t)past[i] - c0;
-        if (t < nc) {
-          if (i >= prompt) atomicAdd(&seen[t], 1u);
-          atomicOr(&seen[t], 0x80000000u);
-        }
+      for (uint32_t i = threadIdx.x; i < n; i += kPast * NT) {
+        uint32_t t[kPast];
+#pragma unroll
+        for (uint32_t j = 0; j < kPast; ++j) t[j] = i + j * NT < n ? (uint32_t)past[i + j * NT] - c0 : ~0u;
+#pragma unroll
+        for (uint32_t j = 0; j < kPast; ++j)
+          if (t[j] < nc) {
+            if (i + j * NT >= prompt) atomicAdd(&seen[t[j]], 1u);
+            else atomicOr(&seen[t[j]], 0x80000000u);
+          }
       }
       __syncthreads();
     }
