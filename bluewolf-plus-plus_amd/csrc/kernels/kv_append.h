@@ -1,6 +1,13 @@
 // New tokens into a paged cache: q and k turned by their positions (the
 // rotation of rotary.h), k and v written to their pages, q to its output; and
 // the accepted tokens of a drafted tree moved together.
+//
+// Append is bound by HBM: a row is read and written once, cosines and sines are
+// made once a tile of tokens, whose sequences are found by bisection over starts
+// sampled in LDS (four prompts of up to 4096 tokens, 32 : 8 heads of 128, bf16:
+// 48 us, 4.7 TB/s; a copy reaches 5.15).  Few tokens have a block for each eight
+// heads, and cost a launch and a chain of latencies (8 tokens 6.8 us); so does
+// keep (64 sequences, 6 of 48 tokens: 6.4 us).
 #pragma once
 
 #include "common.h"

@@ -9,16 +9,21 @@
 // Few rows (attend_few): reading K and V once bounds it.  A block of NW waves
 // has one tile of 32 rows; every wave streams key tiles of 32 of its own
 // (every NW-th of the block's) through a DMA ring of its own, and the waves'
-// triples meet in LDS at the end of an item.
+// triples meet in LDS at the end of an item.  64 sequences of up to 32768
+// tokens, 32 : 8 heads of 128: 334 us, 5.8 TB/s; of up to 16000, d = 64 4.6 TB/s,
+// pages of 16 tokens 187 us (5.4).  Four waves a block measured no better.
 //
-// More rows (attend_rows): the matrix products and the softmax bound it.  Each
-// of a block's waves has 32 rows of the tile, and key tiles of 64 come through
-// a two-stage ring that all of them read: four waves, two blocks a CU, or, for
-// more than 128 rows and head dims up to 128, eight (2 x 2048 tokens 32 : 8
-// heads of 128: four 386 us, eight 379; 8 trees of 48 tokens 62 and 57).  Here P
-// is rounded to one bf16 term, as in attention.hip's kernel for d = 128: two
-// cost 475 and 64 us, and the result's error (rms, of its norm) is 0.0022 with
-// one, 0.0017, its own rounding, with two.
+// More rows (attend_rows): the matrix products and the softmax bound it, and
+// with them power (2 x 2048 tokens over up to 32000, 32 : 8 heads of 128: 378 us
+// with the join, 880 TFLOP/s, the matrix pipe busy in 49 % of the cycles at 1.7 to
+// 2.0 GHz; a large library product reaches 1215).  Each of a block's waves has
+// 32 rows of the tile, and key tiles of 64 come through a two-stage ring that all
+// of them read (four stages: the same times): four waves, two blocks a CU, or, for
+// more than 128 rows and head dims up to 128, eight (of the attention alone: four
+// 386 us, eight 379; 8 trees of 48 tokens 62 and 57).  Here P is rounded to one
+// bf16 term, as in attention.hip's kernel for d = 128: two cost 475 and 64 us,
+// and the result's error (rms, of its norm) is 0.0022 with one, 0.0017, its own
+// rounding, with two.
 //
 // Page numbers of an item's keys are copied to LDS, 1024 at a time, before its
 // tiles: no load of the compiler's is outstanding beside the DMA, whose

@@ -8,7 +8,9 @@
 // a quarter-wave's 16-byte read fall on distinct banks.  S^T = K Q^T takes 4
 // columns a lane from LDS; of its result lane l has row l % 32 against keys
 // 8 (r >> 2) + 4 (l / 32) + (r & 3), which is how O^T += V^T P^T takes its "B"
-// operand, 2 keys a product.  The matrix products bound it.
+// operand, 2 keys a product.  The matrix products bound it: 2 x 1024 tokens of
+// prompts, 32 : 8 heads of 128, fp32 257 us, 99 TFLOP/s (a large library product
+// reaches 137).  On the 16-row tiles, which read keys for every 16 rows: 461 us.
 #pragma once
 
 #include "attention_common.h"

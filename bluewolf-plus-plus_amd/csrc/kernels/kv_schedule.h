@@ -13,8 +13,10 @@
 // launch: the sharer where it begins leaves it in slot 2 b + 1, the others,
 // for which it is the first item, in slot 2 b.  Where all sequences are short
 // items are left whole, since parts cost more than an even share gains (and
-// where the table's width says so, there is no second launch).  The sharers of one XCD are
-// neighbours: the tiles of a head meet its keys in one L2.
+// where the table's width says so, there is no second launch).  The sharers of
+// one XCD are neighbours: the tiles of a head meet its keys in one L2.  Finding
+// the share takes a block 2.4 us, its first pages and rows of q as much (8 trees
+// of 48 tokens over up to 16384, tiles of 256 rows: of 54 us 33 are key tiles).
 //
 // Costs are whole numbers below 2^52, g times keys (g query heads a key head);
 // quotients are taken in doubles (64-bit integer ones cost a microsecond
