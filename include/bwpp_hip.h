@@ -788,8 +788,9 @@ BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const void *q, const
  * slot held[s] + kept[s][i] for i < counts[s] (int32 [batch], cut to max_kept), as
  * if all were read before any is written.  Of kept (int32 [batch][max_kept])
  * entries past the 16th must not be below their index (ascending ones are not);
- * entries below 0 or past the table move nothing.  held itself is the caller's to
- * raise by counts. */
+ * entries below 0 or past the table move nothing.  Two sequences with a page in
+ * common that write the same slot of it leave either's rows.  held itself is the
+ * caller's to raise by counts. */
 BwppHipStatus bwpp_hip_dispatch_cache_keep(BwppHip *h, void *k_cache, void *v_cache, const int32_t *table,
                                            const int32_t *held, const int32_t *kept, const int32_t *counts,
                                            BwppCacheKeepParams params);
