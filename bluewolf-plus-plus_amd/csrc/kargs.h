@@ -308,6 +308,7 @@ typedef struct {
   double inv_blocks;    /* 1 / blocks */
   uint32_t whole_keys;  /* sequences up to here have whole items */
   uint32_t item_keys;   /* keys that an item costs by itself */
+  uint64_t large_cost;  /* more is of more keys and values than the caches hold */
   float *part_o;        /* [2 blocks][rows of a tile][dim up to a multiple of 4] */
   float *part_ml;       /* [2 blocks][rows of a tile][2] */
 } BwppCacheAttnArgs;

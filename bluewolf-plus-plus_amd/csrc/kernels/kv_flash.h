@@ -10,8 +10,9 @@
 // has one tile of 32 rows; every wave streams key tiles of 32 of its own
 // (every NW-th of the block's) through a DMA ring of its own, and the waves'
 // triples meet in LDS at the end of an item.  64 sequences of up to 32768
-// tokens, 32 : 8 heads of 128: 334 us, 5.8 TB/s; of up to 16000, d = 64 4.6 TB/s,
-// pages of 16 tokens 187 us (5.4).  Four waves a block measured no better.
+// tokens, 32 : 8 heads of 128: 300 us, 6.5 TB/s (through the caches 334); of up to
+// 16000, pages of 16 tokens 164 us (6.2), d = 64 92 us (5.5).  Four waves a block
+// measured no better.
 //
 // More rows (attend_rows): the matrix products and the softmax bound it, and
 // with them power (2 x 2048 tokens over up to 32000, 32 : 8 heads of 128: 378 us
@@ -42,12 +43,20 @@ namespace kv {
 // 16 bytes a lane from memory to LDS (see g2lds16_so), from a scalar base or a
 // 64-bit address a lane.  The LDS address passes through a scalar register by
 // name: one chosen by the compiler may be VCC, and the code objects' check of M0
-// takes plain ones.
+// takes plain ones.  ONCE: past the caches (Item::once).
+template <bool ONCE>
 __device__ __forceinline__ void dma16_so(const void *sbase, uint32_t voff, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{s33}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"{s33}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{s33}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
 }
+template <bool ONCE>
 __device__ __forceinline__ void dma16_v(const void *addr, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"{s33}"(lds_addr), "v"(addr) : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"{s33}"(lds_addr), "v"(addr) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"{s33}"(lds_addr), "v"(addr) : "memory");
 }
 
 // A tile of key or value rows in LDS: dense rows of D / 8 chunks of 16 bytes,
@@ -289,6 +298,12 @@ struct Fetch {
   __device__ __forceinline__ uint32_t voff(uint32_t i) const { return kKeep ? kept[kKeep ? 2 * i + 1 : 0] : offset(i, true); }
   __device__ __forceinline__ void issue(const BwppCacheArgs &c, const Item &it, uint32_t k0, uint32_t first,
                                         const uint32_t *pages, uint32_t lds) const {
+    if (it.once) rows<true>(c, it, k0, first, pages, lds);
+    else rows<false>(c, it, k0, first, pages, lds);
+  }
+  template <bool ONCE>
+  __device__ __forceinline__ void rows(const BwppCacheArgs &c, const Item &it, uint32_t k0, uint32_t first,
+                                       const uint32_t *pages, uint32_t lds) const {
     const uint32_t pmask = (1u << c.page_shift) - 1u, n = min((uint32_t)KEYS, it.kend - k0);
     if (pmask + 1u >= (uint32_t)KEYS) {
       const uint32_t page = uni(pages[(k0 >> c.page_shift) - first]) & ~kNoPage;
@@ -297,16 +312,16 @@ struct Fetch {
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
           if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
-          dma16_so(K + base, koff(i), lds + (i * FROM_WAVES + wave) * 1024u);
-          dma16_so(V + base, voff(i), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so<ONCE>(K + base, koff(i), lds + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so<ONCE>(V + base, voff(i), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
         }
       } else {  // rows past the last key re-read it
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
           if (kDma % FROM_WAVES && i * FROM_WAVES + wave >= kDma) break;
           const uint32_t r = slot(i, wave) / R::kSlots, back = r < n ? 0u : 2u * (r - (n - 1)) * tok_s;
-          dma16_so(K + base, koff(i) - back, lds + (i * FROM_WAVES + wave) * 1024u);
-          dma16_so(V + base, voff(i) - back, lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so<ONCE>(K + base, koff(i) - back, lds + (i * FROM_WAVES + wave) * 1024u);
+          dma16_so<ONCE>(V + base, voff(i) - back, lds + kTile + (i * FROM_WAVES + wave) * 1024u);
         }
       }
     } else {
@@ -318,8 +333,8 @@ struct Fetch {
         // less the row's offset, which koff and voff have
         const uint64_t row = (uint64_t)page * (uint32_t)c.page_s + (uint64_t)(key & pmask) * tok_s;
         const uint32_t mine = 2u * r * tok_s;
-        dma16_v(reinterpret_cast<const char *>(K + row) + (koff(i) - mine), lds + (i * FROM_WAVES + wave) * 1024u);
-        dma16_v(reinterpret_cast<const char *>(V + row) + (voff(i) - mine), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
+        dma16_v<ONCE>(reinterpret_cast<const char *>(K + row) + (koff(i) - mine), lds + (i * FROM_WAVES + wave) * 1024u);
+        dma16_v<ONCE>(reinterpret_cast<const char *>(V + row) + (voff(i) - mine), lds + kTile + (i * FROM_WAVES + wave) * 1024u);
       }
     }
   }

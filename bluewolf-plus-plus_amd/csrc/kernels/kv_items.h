@@ -33,6 +33,7 @@ struct Item {
   Seq q;
   uint32_t s, head, tile, kbeg, kend, R;
   bool whole;
+  bool once;  // its keys and values are read by no other tile, and of more than the caches hold
 };
 
 // Page numbers of the keys from k on, as many as LDS holds; returns the end of
@@ -69,7 +70,7 @@ template <uint32_t ROWS, uint32_t UNIT, class F>
 __device__ __forceinline__ void for_items(const BwppCacheAttnArgs &a, F f) {
   typedef Work<ROWS, UNIT> W;
   const Share share = find_share<ROWS, UNIT>(a);
-  const uint32_t b = uni(share.b);
+  const uint32_t b = uni(share.b), large = uni(share.large);
   Place at = {uni(share.from.s), uni(share.from.head), uni(share.from.tile), uni(share.from.unit)};
   const Place to = {uni(share.to.s), uni(share.to.head), uni(share.to.tile), uni(share.to.unit)};
   Item it = {};
@@ -77,6 +78,7 @@ __device__ __forceinline__ void for_items(const BwppCacheAttnArgs &a, F f) {
     it.q = {uni(q.first), uni(q.n), uni(q.held)};
     it.s = at.s;
     it.R = it.q.n * a.group;
+    it.once = large && it.R <= ROWS;
   };
   sequence(share.q);
   // A part of an item that began in another block is written even if it has no

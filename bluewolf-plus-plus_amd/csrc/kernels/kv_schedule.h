@@ -44,6 +44,7 @@ struct Share {
   Place from, to;
   Seq q;       // from's sequence
   uint32_t b;  // whose it is
+  bool large;  // the sequences' keys and values are more than the caches hold
 };
 
 template <uint32_t ROWS, uint32_t UNIT>
@@ -159,7 +160,8 @@ __device__ __forceinline__ Share find_share(const BwppCacheAttnArgs &a) {
   const Costs<ROWS, UNIT> costs(a);
   const uint64_t S = share_of(a, costs.total);
   const uint32_t sharers = min((uint32_t)((double)costs.total / (double)S) + 1u, a.blocks), per = (sharers + kXcds - 1) / kXcds;
-  Share share = {{a.c.batch, 0, 0, 0}, {a.c.batch, 0, 0, 0}, {0, 0, 0}, blockIdx.x % kXcds * per + blockIdx.x / kXcds};
+  Share share = {{a.c.batch, 0, 0, 0}, {a.c.batch, 0, 0, 0}, {0, 0, 0}, blockIdx.x % kXcds * per + blockIdx.x / kXcds,
+                 costs.total > a.large_cost};
   const uint64_t x0 = S * share.b, x1 = x0 + S;
   if (blockIdx.x / kXcds >= per || x0 >= costs.total) return share;
   uint64_t begin, end, before;

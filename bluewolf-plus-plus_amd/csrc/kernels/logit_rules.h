@@ -9,8 +9,9 @@
 // one row's columns, counts the row's history in LDS (bit 31: v was given, below
 // it c; whole numbers, so the order of the additions does not matter) and then
 // goes over its chunk, which it has fetched meanwhile.  256 rows of 131072, fp32,
-// histories of up to 8192 tokens: 64 us, 4.3 TB/s (chunks of 8192 the same); 4 of
-// 32000: 6.4, a launch and a chain of latencies.
+// histories of up to 8192 tokens: 63 us, 4.4 TB/s (chunks of 8192 the same); 4 of
+// 32000: 6.4, a launch and a chain of latencies.  x is read past the caches (62.8 us for
+// 63.8).
 #pragma once
 
 #include "common.h"
@@ -35,7 +36,7 @@ __device__ __forceinline__ void rules(const BwppLogitArgs &a) {
   float v[kPer][4];  // on the way while the history is counted
 #pragma unroll
   for (uint32_t j = 0; j < kPer; ++j)
-    if (threadIdx.x + j * NT < n4) Vec<TX, 4>::load(x + 4u * (threadIdx.x + j * NT), v[j]);
+    if (threadIdx.x + j * NT < n4) Vec<TX, 4>::load_once(x + 4u * (threadIdx.x + j * NT), v[j]);
 
   uint32_t n = 0;
   if (a.count) {
@@ -92,7 +93,7 @@ __device__ __forceinline__ void rules(const BwppLogitArgs &a) {
   }
   for (uint32_t i = 4u * n4 + threadIdx.x; i < nc; i += NT) {
     float w[1];
-    Vec<TX, 1>::load(x + i, w);
+    Vec<TX, 1>::load_once(x + i, w);
     w[0] = rule(w[0], i, bias ? bias[i] : 0.0f, mask ? mask[i / 32u] : 0u);
     Vec<TY, 1>::store(y + i, w);
   }

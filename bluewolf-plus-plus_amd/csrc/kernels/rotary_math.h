@@ -9,7 +9,7 @@ using namespace bwpp;
 
 namespace rotary_pos {
 
-// N elements of T at any address aligned to T, as floats.
+// N elements of T at any address aligned to T, as floats; load_once: past the caches.
 template <class T, int N>
 struct Vec;
 template <int N>
@@ -17,6 +17,11 @@ struct Vec<float, N> {
   typedef float V __attribute__((ext_vector_type(N), aligned(4)));
   static __device__ __forceinline__ void load(const float *p, float (&o)[N]) {
     const V v = *reinterpret_cast<const V *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = v[i];
+  }
+  static __device__ __forceinline__ void load_once(const float *p, float (&o)[N]) {
+    const V v = __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = v[i];
   }
@@ -30,6 +35,7 @@ struct Vec<float, N> {
 template <>
 struct Vec<float, 1> {
   static __device__ __forceinline__ void load(const float *p, float (&o)[1]) { o[0] = *p; }
+  static __device__ __forceinline__ void load_once(const float *p, float (&o)[1]) { o[0] = __builtin_nontemporal_load(p); }
   static __device__ __forceinline__ void store(float *p, const float (&o)[1]) { *p = o[0]; }
 };
 template <int N>
@@ -37,6 +43,14 @@ struct Vec<uint16_t, N> {
   typedef uint32_t V __attribute__((ext_vector_type(N / 2), aligned(2)));
   static __device__ __forceinline__ void load(const uint16_t *p, float (&o)[N]) {
     const V v = *reinterpret_cast<const V *>(p);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      o[2 * i] = __uint_as_float(v[i] << 16);
+      o[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ void load_once(const uint16_t *p, float (&o)[N]) {
+    const V v = __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
       o[2 * i] = __uint_as_float(v[i] << 16);
@@ -64,6 +78,9 @@ struct Vec<uint16_t, 2> {
 template <>
 struct Vec<uint16_t, 1> {
   static __device__ __forceinline__ void load(const uint16_t *p, float (&o)[1]) { o[0] = bf16_bits_to_f32(*p); }
+  static __device__ __forceinline__ void load_once(const uint16_t *p, float (&o)[1]) {
+    o[0] = bf16_bits_to_f32(__builtin_nontemporal_load(p));
+  }
   static __device__ __forceinline__ void store(uint16_t *p, const float (&o)[1]) { *p = f32_to_bf16_bits(o[0]); }
 };
 

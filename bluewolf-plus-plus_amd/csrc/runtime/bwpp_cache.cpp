@@ -449,6 +449,11 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // tokens 57 us with 96, 48 with 192, 49 with 384; 2 x 2048 tokens of prompts 386,
   // 376, 378, those of d = 256 95, 89, 83; fp32 2 x 1024 tokens 257, 268, 284.
   a.item_keys = flash < 0 ? 96 : rows == 32 ? 192 : 384;
+  // 256 MiB of keys and values fill the Infinity Cache (costs count some more than the
+  // keys).  What is more, and read once, goes past it: 64 steps over 1.9 GB 327 us,
+  // past it 293, over 0.5 GB (d = 64) 103 and 91; what it could keep for the next
+  // call: 128 steps over 245 MB 48 and 50, 16 trees over 250 MB 60 and 64.
+  a.large_cost = (320ull << 20) * g / (2 * cp.dim * es);
   const bool parts = c.capacity > a.whole_keys;
   if (parts) {
     void *ws = nullptr;

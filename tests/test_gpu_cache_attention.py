@@ -292,3 +292,20 @@ def test_page_past_32_bits(be):
         z = z.masked_fill(torch.arange(700 + n, device="cuda")[None, None] > 700 + torch.arange(n, device="cuda")[:, None, None], -math.inf)
         want = torch.softmax(z, dim=2) @ v
         assert float((o.double() - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max()) + 1e-4
+
+
+@pytest.mark.parametrize("d,page", [(64, 64), (128, 16), (128, 64), (256, 64)])
+@pytest.mark.parametrize("n", [1, 16, 48])
+def test_more_keys_than_the_caches_hold(be, d, page, n):
+    """Sequences that share their pages: 2500 tokens, 8 key heads, often enough
+    that keys and values count for more than 400 MB; each has the same result."""
+    Hk, Hq, N = 8, 32, 400_000_000 // (2500 * 8 * d * 4) + 1
+    c = Cache([2500], [n], Hk, d, page, BF16)
+    q = c.normal(n, Hq, d, std=2.5)
+    want, wl, to, tl = attention64(c, q, d ** -0.5)
+    o, l = torch.empty(N, n, Hq, d, dtype=BF16, device="cuda"), torch.empty(N, n, Hq, device="cuda")
+    p = bwpp.CacheAttentionParams(cache=c.params(Hq, batch=N, tokens=N * n), scale=d ** -0.5)
+    be.dispatch_cache_attention(q.expand(N, n, Hq, d).contiguous(), c.k, c.v, c.table.expand(N, -1).contiguous(),
+                                i32([s * n for s in range(N + 1)]), i32([2500] * N), None, o, l, p)
+    torch.cuda.synchronize()
+    assert bool(((o.double() - want).abs() <= to).all()) and bool(((l.double() - wl).abs() <= tl).all())
