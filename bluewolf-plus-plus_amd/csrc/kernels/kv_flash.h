@@ -15,8 +15,8 @@
 // measured no better.
 //
 // More rows (attend_rows): the matrix products and the softmax bound it, and
-// with them power (2 x 2048 tokens over up to 32000, 32 : 8 heads of 128: 378 us
-// with the join, 880 TFLOP/s, the matrix pipe busy in 49 % of the cycles at 1.7 to
+// with them power (2 x 2048 tokens over up to 32000, 32 : 8 heads of 128: 362 to 379 us
+// with the join, 880 to 920 TFLOP/s, the matrix pipe busy in 49 % of the cycles at 1.7 to
 // 2.0 GHz; a large library product reaches 1215).  Each of a block's waves has
 // 32 rows of the tile, and key tiles of 64 come through a two-stage ring that all
 // of them read (four stages: the same times): four waves, two blocks a CU, or, for

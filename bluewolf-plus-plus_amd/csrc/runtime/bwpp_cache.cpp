@@ -452,7 +452,8 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // 256 MiB of keys and values fill the Infinity Cache (costs count some more than the
   // keys).  What is more, and read once, goes past it: 64 steps over 1.9 GB 327 us,
   // past it 293, over 0.5 GB (d = 64) 103 and 91; what it could keep for the next
-  // call: 128 steps over 245 MB 48 and 50, 16 trees over 250 MB 60 and 64.
+  // call: 128 steps over 245 MB 48 and 50, 16 trees over 250 MB 60 and 64.  Of one row
+  // of pages for all 64, 278 and 280.
   a.large_cost = (320ull << 20) * g / (2 * cp.dim * es);
   const bool parts = c.capacity > a.whole_keys;
   if (parts) {
