@@ -309,3 +309,21 @@ def test_more_keys_than_the_caches_hold(be, d, page, n):
                                 i32([s * n for s in range(N + 1)]), i32([2500] * N), None, o, l, p)
     torch.cuda.synchronize()
     assert bool(((o.double() - want).abs() <= to).all()) and bool(((l.double() - wl).abs() <= tl).all())
+
+
+@DTYPES
+@pytest.mark.parametrize("d,n", [(64, 2), (80, 30), (128, 60)])
+def test_starts_that_descend(be, dtype, d, n):
+    """Sequences whose rows overlap: rows of one sequence alone have its results,
+    shared ones are written by either, the others stay as they were."""
+    c = Cache([900, 70, 1300], [n, n, n], 2, d, 16, dtype)
+    q = c.normal(3 * n, 8, d)
+    c.starts = i32([0, n, n // 2, n // 2 + n])  # the second has none, the third overlaps the first
+    o, l = _run(be, c, q)
+    half = n // 2
+    one = Cache([900, 70, 1300], [n, n, n], 2, d, 16, dtype)
+    want, wl, to, tl = attention64(one, q, d ** -0.5)
+    assert bool(((o[:half].double() - want[:half]).abs() <= to[:half]).all())
+    assert bool(((l[:half].double() - wl[:half]).abs() <= tl[:half]).all())
+    assert bool(torch.isfinite(o[:n + half].double()).all())
+    assert bool((o[n + half:] == 5.0).all()) and bool((l[n + half:] == 5.0).all())
