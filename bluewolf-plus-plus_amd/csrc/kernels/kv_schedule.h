@@ -107,6 +107,11 @@ struct Costs {
   static __device__ __forceinline__ uint64_t of(const BwppCacheAttnArgs &a, const Seq &q) {
     return a.c.heads * Work<ROWS, UNIT>::before(a, q, Work<ROWS, UNIT>::tiles(q, a.group));
   }
+  // Keys of a sequence that its table holds: a table of at most whole_keys slots
+  // leaves every item whole, and such a call has no workspace for parts.
+  static __device__ __forceinline__ uint32_t keys_of(const BwppCacheAttnArgs &a, const Seq &q) {
+    return q.n ? min(q.held + q.n, a.c.capacity) : 0u;
+  }
   __device__ __forceinline__ Costs(const BwppCacheAttnArgs &a) {
     const uint32_t lane = threadIdx.x & 63u;
     per = (a.c.batch + 63u) / 64u;
@@ -114,12 +119,12 @@ struct Costs {
     q = {0, 0, 0};
     if (s0 < s1) q = seq_at(a.c, s0);
     mine = of(a, q);
-    uint32_t most = q.n ? q.held + q.n : 0u;
+    uint32_t most = keys_of(a, q);
 #pragma unroll 4
     for (uint32_t s = s0 + 1; s < s1; ++s) {
       const Seq t = seq_at(a.c, s);
       mine += of(a, t);
-      most = max(most, t.n ? t.held + t.n : 0u);
+      most = max(most, keys_of(a, t));
     }
     whole = __ballot(most > a.whole_keys) == 0;
     uint64_t sum = mine;

@@ -455,6 +455,7 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // call: 128 steps over 245 MB 48 and 50, 16 trees over 250 MB 60 and 64.  Of one row
   // of pages for all 64, 278 and 280.
   a.large_cost = (320ull << 20) * g / (2 * cp.dim * es);
+  // (kv_schedule.h leaves every item whole where no sequence has more keys in its table.)
   const bool parts = c.capacity > a.whole_keys;
   if (parts) {
     void *ws = nullptr;
