@@ -21,10 +21,14 @@
 // 32 rows of the tile, and key tiles of 64 come through a two-stage ring that all
 // of them read (four stages: the same times): four waves, two blocks a CU, or, for
 // more than 128 rows and head dims up to 128, eight (of the attention alone: four
-// 386 us, eight 379; 8 trees of 48 tokens 62 and 57).  Here P is rounded to one
-// bf16 term, as in attention.hip's kernel for d = 128: two cost 475 and 64 us,
-// and the result's error (rms, of its norm) is 0.0022 with one, 0.0017, its own
-// rounding, with two.
+// 386 us, eight 379; 8 trees of 48 tokens 62 and 57).  P enters its product as two
+// bf16 terms, except for d = 128, where it is rounded to one: so do attention.hip's
+// kernels for many queries (two terms or fp32 for every other dim).  For d = 128 two
+// would cost 475 and 64 us, and the result's error (rms, of its norm) is 0.0022 with
+// one, 0.0017, its own rounding, with two.  For the other dims the second term costs
+// 26 to 33 % of prompts and 7 to 20 % of trees (2 x 2048 tokens over 32000 d = 64 1102
+// -> 1458 us, d = 256 4398 -> 5559; 8 trees of 48 54 -> 64 and 176 -> 197), and one
+// term was off by up to nine times the bound of two.
 //
 // Page numbers of an item's keys are copied to LDS, 1024 at a time, before its
 // tiles: no load of the compiler's is outstanding beside the DMA, whose
@@ -473,7 +477,7 @@ __device__ __forceinline__ void attend_few(const BwppCacheAttnArgs &a) {
 
 template <int D, int NW>
 __device__ __forceinline__ void attend_rows(const BwppCacheAttnArgs &a) {
-  constexpr int KB = 2, TERMS = 1;
+  constexpr int KB = 2, TERMS = D == 128 ? 1 : 2;  // of P
   constexpr uint32_t kRows = 32 * NW, kKeys = 32 * KB;
   typedef Wave32<D, KB> W;
   typedef Fetch<D, 32 * KB, NW> F;

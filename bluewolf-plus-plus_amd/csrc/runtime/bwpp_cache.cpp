@@ -446,8 +446,9 @@ extern "C" BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const voi
   // sequence of 1000 tokens 12.8 in parts, 16 whole; fp32 4 x 416 tokens 300 and 393).
   a.whole_keys = flash < 0 ? 256 : rows == 32 ? 512 : 1024;
   // What starting and ending an item takes, in keys: 128 sequences of up to 2000
-  // tokens 57 us with 96, 48 with 192, 49 with 384; 2 x 2048 tokens of prompts 386,
-  // 376, 378, those of d = 256 95, 89, 83; fp32 2 x 1024 tokens 257, 268, 284.
+  // tokens 57 us with 96, 48 with 192, 49 with 384; 2 x 2048 tokens of prompts over
+  // 4000 and 1000 of d = 128 293, 289, 280, of 256 740, 728, 725; fp32 2 x 1024 tokens
+  // 257, 268, 284.
   a.item_keys = flash < 0 ? 96 : rows == 32 ? 192 : 384;
   // 256 MiB of keys and values fill the Infinity Cache (costs count some more than the
   // keys).  What is more, and read once, goes past it: 64 steps over 1.9 GB 327 us,

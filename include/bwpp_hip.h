@@ -773,12 +773,15 @@ BwppHipStatus bwpp_hip_dispatch_cache_append(BwppHip *h, const void *q, const vo
  * (q_heads / heads).  o = softmax(scale q k) v; lse (may be NULL) [tokens][q_heads]
  * fp32 is the natural log-sum-exp.  A token that sees nothing gets 0 and -inf.
  * What lies in slots that a token does not see has no part in it, infinities and
- * NaN included.  Scores, sums and the probabilities that lse has are fp32; bf16
- * probabilities enter the product with v as two bf16 terms, or, for more than 32
- * rows (tokens times q_heads / heads, on average) of dims 64, 80, 96, 128, 160, 192
- * and 256, rounded to one.  Workspace: two partial results for each of one or two
- * blocks a compute unit, 16 to 256 rows of dim + 2 floats each (at most 65 MiB on
- * 256 of them), whatever the lengths. */
+ * NaN included.  Scores, sums and the probabilities that lse has are fp32.  With bf16
+ * operands the probabilities enter the product with v as two bf16 terms (2^-16 of
+ * each) or in fp32; for dim 128 and more than 32 rows rounded to one term (2^-8), as
+ * attention's of that dim and as many queries are.  Rows are those of a sequence and
+ * key head on average: `tokens` (rows of no sequence too) by `batch` (idle sequences
+ * too), rounded up, times q_heads / heads; they also choose the kernel, one for all
+ * sequences of a call.  Workspace: two partial results for each of one or two blocks a
+ * compute unit, 16 to 256 rows of dim + 2 floats each (at most 65 MiB on 256 of them),
+ * whatever the lengths. */
 BwppHipStatus bwpp_hip_dispatch_cache_attention(BwppHip *h, const void *q, const void *k_cache, const void *v_cache,
                                                 const int32_t *table, const int32_t *starts, const int32_t *held,
                                                 const uint32_t *mask, void *o, float *lse,
