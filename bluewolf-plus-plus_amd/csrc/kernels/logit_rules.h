@@ -10,8 +10,14 @@
 // it c; whole numbers, so the order of the additions does not matter) and then
 // goes over its chunk, which it has fetched meanwhile.  256 rows of 131072, fp32,
 // histories of up to 8192 tokens: 63 us, 4.4 TB/s (chunks of 8192 the same); 4 of
-// 32000: 6.4, a launch and a chain of latencies.  x is read past the caches (62.8 us for
-// 63.8).
+// 32000: 6.8, a launch and a chain of latencies.
+//
+// x, read once, goes past the caches at every size: never slower than 3 % (the noise of
+// small calls), 16 % faster at best.  500 tokens of history a row, fp32, past them and
+// through them, x in memory: 4 rows of 32000 5.9 and 5.8 us, 64 of 131072 12.9 and 13.6, 256
+// of 32000 12.8 and 14.8, 256 of 131072 52.0 and 52.5; with the copy that writes x right
+// before: 9.8 and 9.9, 23.4 and 23.6, 24.0 and 23.3, 92.6 and 93.8 (bf16 512 of 131072
+// 132 and 139).
 #pragma once
 
 #include "common.h"
