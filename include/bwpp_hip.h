@@ -256,9 +256,9 @@ typedef struct {
  *   held    int32 [batch]: tokens that the cache holds before the new ones, which
  *           take the slots behind them
  * Slot p of a sequence lies in page table[s][p / page_tokens].  Starts are cut to
- * the operands, lengths below zero are none; a slot past the table, or whose page
- * number is outside 0 .. pages - 1 (-1: no page), does not exist: nothing is
- * written there and no query sees it. */
+ * the operands, lengths below zero are none; a slot past the table (or from 2^31 - 1
+ * on), or whose page number is outside 0 .. pages - 1 (-1: no page), does not exist:
+ * nothing is written there and no query sees it. */
 typedef struct {
   uint32_t pages;
   uint32_t page_tokens; /* a power of two */
@@ -844,8 +844,9 @@ BwppHipStatus bwpp_hip_plan_run(BwppHipPlan *plan);
  * loops that replay one plan and should not pay the host cost of each
  * launch).  Runs the plan once eagerly first, so every workspace reaches its
  * final size, then captures one run on the handle's stream, which must not
- * be the default (null) stream (UNSUPPORTED).  Binding a different address
- * afterwards drops the graph; capture again. */
+ * be the default (null) stream (UNSUPPORTED).  The eager run is a run like any
+ * other: cache_keep moves tokens on it, and what is written in place stays so.
+ * Binding a different address afterwards drops the graph; capture again. */
 BwppHipStatus bwpp_hip_plan_capture(BwppHipPlan *plan);
 /* Launches the captured graph on the handle's current stream (INVALID_ARG
  * when there is none).  Results equal bwpp_hip_plan_run's.  Where the graph
